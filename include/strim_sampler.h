@@ -240,6 +240,75 @@ int strim_head_greedy(strim_ctx* ctx, void* stream, const void* hidden, int64_t 
                       const void* lm_head, int64_t lm_head_stride, int32_t V, void* out_logits,
                       int64_t out_stride, int32_t* out_ids, int32_t* out_status);
 
+/* ---- loss over the vocabulary ------------------------------------------------------
+ * Cross entropy of the projection's logits x[n][v] = sum_k hidden[n][k] lm_head[v][k], over
+ * the whole vocabulary, without keeping the logits:
+ *   out_lse[n] = log sum_v exp(x[n][v]),   out_loss[n] = out_lse[n] - x[n][targets[n]]
+ * (minus the target's log-probability), and its gradients. Training (or distilling) a draft
+ * head over its truncated vocabulary, and the log-probabilities of given tokens. No
+ * counterpart in the reference, which trains nothing.
+ *   hidden      bf16 [N][hidden_stride], lm_head bf16 [V][lm_head_stride]: K a multiple of 8,
+ *               16-byte aligned, strides multiples of 8 of at most STRIM_LOSS_MAX_STRIDE.
+ *   targets     device [N]. ignore_index: the row counts for nothing (loss 0, no gradient,
+ *               whatever its hidden row holds). Another id outside [0, V): the same, with
+ *               STRIM_EINVAL in out_status.
+ *   workspace   device, 16-byte aligned, of strim_head_loss_workspace's bytes (want_*: 0 for
+ *               the loss alone), else STRIM_ECAPACITY; free again when the call's work ends.
+ *   out_lse, out_status  [N] or NULL (status STRIM_OK, STRIM_EINVAL or STRIM_ENONFINITE: a
+ *               NaN or infinite loss).
+ * strim_head_loss_grad: lse as strim_head_loss wrote it; grad_loss [N] and grad_lse [N] (NULL:
+ * none) the gradients with respect to out_loss and out_lse (an ignored row's are not read;
+ * its out_lse takes none). It computes the logits again, in pieces of the vocabulary whose
+ * probabilities fit 512 MB:
+ *   p[n][v] = (grad_loss[n] + grad_lse[n]) exp(x[n][v] - lse[n]) - grad_loss[n] [v = targets[n]]
+ *   d_hidden[n] = sum_v p[n][v] lm_head[v],   d_lm_head[v] = sum_n p[n][v] hidden[n]
+ * p is rounded to bf16, sums are float32, results bf16; either result may be NULL (a frozen
+ * projection). Sums are added in an order that the sizes alone fix. N = 0: nothing is
+ * launched but for d_lm_head, which is zeroed. */
+#define STRIM_LOSS_MAX_ROWS (1 << 22)
+#define STRIM_LOSS_MAX_STRIDE (1 << 20)
+int64_t strim_head_loss_workspace(int32_t N, int32_t K, int32_t V, int32_t want_d_hidden,
+                                  int32_t want_d_lm_head);
+int strim_head_loss(void* stream, const void* hidden, int64_t hidden_stride, int32_t N, int32_t K,
+                    const void* lm_head, int64_t lm_head_stride, int32_t V, const int32_t* targets,
+                    int32_t ignore_index, void* workspace, int64_t workspace_bytes, float* out_loss,
+                    float* out_lse, int32_t* out_status);
+int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride, int32_t N,
+                         int32_t K, const void* lm_head, int64_t lm_head_stride, int32_t V,
+                         const int32_t* targets, int32_t ignore_index, const float* lse,
+                         const float* grad_loss, const float* grad_lse, void* workspace,
+                         int64_t workspace_bytes, void* d_hidden, int64_t d_hidden_stride,
+                         void* d_lm_head, int64_t d_lm_head_stride);
+
+/* ---- projections in 4 bits ----------------------------------------------------------
+ * [V, K] as words uint32 [V][K / 8] (eight codes a word, the lowest four bits first), and per
+ * group of 32, 64 or 128 elements of a row a bf16 scale s and bias b, [V][K / group]: the
+ * element is s q + b; biases NULL: s (q - 8). The layout of the reference's 4-bit groupwise
+ * weights (QGEMV.swift:14-15,68-69). K a multiple of the group.
+ *
+ * strim_pack_weights fills words, scales and biases (contiguous; biases NULL: symmetric) from a
+ * bf16 or float32 weight: s = bf16((max - min) / 15), b = bf16(min), q = rint((w - b) / s), or
+ * s = bf16(max|w| / 7), q = rint(w / s) + 8, clamped to [0, 15]; s = 0 gives the group's
+ * minimum (0) back. strim_unpack_weights writes s q + b, rounded once, as dtype (rows 16-byte
+ * aligned).
+ * strim_head_logits_packed is strim_head_logits over such a projection: hidden, norm_weight, eps
+ * and xn as there, any B >= 1 (the weights are read once per 64 rows), logits as dtype (bf16 or
+ * float32, what strim_sample takes), accumulated in float32 from the exact s q + b. words and
+ * its stride 16-byte aligned; workspace device, 16-byte aligned, of
+ * strim_head_logits_packed_workspace's bytes (else STRIM_ECAPACITY). */
+int strim_pack_weights(void* stream, const void* weight, int32_t dtype, int64_t weight_stride, int32_t V,
+                  int32_t K, int32_t group, uint32_t* words, void* scales, void* biases);
+int strim_unpack_weights(void* stream, const uint32_t* words, int64_t words_stride, const void* scales,
+                    const void* biases, int64_t scales_stride, int32_t V, int32_t K, int32_t group,
+                    void* out, int32_t dtype, int64_t out_stride);
+int64_t strim_head_logits_packed_workspace(int32_t B, int32_t K);
+int strim_head_logits_packed(void* stream, const void* hidden, int64_t hidden_stride, int32_t B,
+                         int32_t K, const void* norm_weight, float eps, void* xn,
+                         const uint32_t* words, int64_t words_stride, const void* scales,
+                         const void* biases, int64_t scales_stride, int32_t group, int32_t V,
+                         void* workspace, int64_t workspace_bytes, void* out_logits, int32_t dtype,
+                         int64_t out_stride);
+
 /* ---- per-kernel timing -------------------------------------------------------------
  * Counterpart of the reference's fenced per-region GPU timer OpTimer
  * (Sources/StrimCore/OpTimer.swift:1-60). While profiling is on, every kernel a call

@@ -41,6 +41,8 @@ UNITS = [
     ("qres_kernels.hip", []),
     ("aux_kernels.hip", []),
     ("head_kernels.hip", []),
+    ("loss_kernels.hip", []),
+    ("q4_kernels.hip", []),
     ("grammar_kernels.hip", []),
     ("capi.hip", []),
 ]

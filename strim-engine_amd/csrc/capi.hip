@@ -19,6 +19,26 @@ hipError_t launch_head(const void* hidden, int64_t hidden_stride, int B, int K,
                        const void* norm_w, float eps, void* xn, const void* W, int64_t w_stride,
                        int V, void* out, int64_t out_stride, bool vo, hipStream_t st,
                        uint2* tbest, int32_t* out_ids, int32_t* out_status);
+void launch_head_norm(const void* hidden, int64_t hidden_stride, int B, int K, const void* norm_w,
+                      float eps, void* xn, hipStream_t st);
+int64_t loss_workspace(int N, int K, int V, bool hid, bool head);
+hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws, int V,
+                       const int32_t* targets, int ignore_index, void* workspace, float* loss,
+                       float* lse, int32_t* status, hipStream_t st);
+hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws,
+                            int V, const int32_t* targets, int ignore_index, const float* lse,
+                            const float* grad_loss, const float* grad_lse, void* workspace,
+                            void* d_hidden, int64_t dhs, void* d_head, int64_t dws, hipStream_t st);
+int64_t q4_workspace(int B, int K);
+hipError_t launch_q4_logits(const void* x, int64_t x_stride, int B, int K, const uint32_t* words,
+                            int64_t words_stride, const uint16_t* scales, const uint16_t* biases,
+                            int64_t scales_stride, int group, int V, void* workspace, void* out,
+                            bool out_f32, int64_t out_stride, hipStream_t st);
+hipError_t launch_q4_pack(const void* w, bool f32, int64_t w_stride, int V, int K, int group,
+                          uint32_t* words, uint16_t* scales, uint16_t* biases, hipStream_t st);
+hipError_t launch_q4_unpack(const uint32_t* words, int64_t words_stride, const uint16_t* scales,
+                            const uint16_t* biases, int64_t scales_stride, int group, int V, int K,
+                            void* out, bool out_f32, int64_t out_stride, hipStream_t st);
 __global__ void k_final(Args a);
 __global__ void k_probs(Args a);
 __global__ void k_verify_combine(Args a);
@@ -723,6 +743,121 @@ int strim_draft_argmax(void* stream, const void* draft_logits, int32_t dtype, in
   const bool vec = vec_ok(draft_logits, R > 1 ? row_stride : 0, dtype) != 0;
   const hipError_t e = launch_draft_argmax(draft_logits, dtype == STRIM_DTYPE_BF16, vec, R, Vd,
                                            row_stride, draft_to_full, out, (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+namespace {
+bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+// one bf16 operand of the loss: rows of K elements, 16-byte aligned, within a tile's 32-bit offsets
+bool loss_rows_ok(const void* p, int64_t stride, int32_t K) {
+  return p && al16(p) && stride >= K && stride % 8 == 0 && stride <= STRIM_LOSS_MAX_STRIDE;
+}
+bool loss_sizes_ok(int32_t N, int32_t K, int32_t V) {
+  return N >= 0 && N <= STRIM_LOSS_MAX_ROWS && K > 0 && K % 8 == 0 && K <= STRIM_LOSS_MAX_STRIDE &&
+         V > 0 && V <= STRIM_LOSS_MAX_STRIDE;
+}
+bool group_ok(int32_t K, int32_t group) {
+  return (group == 32 || group == 64 || group == 128) && K > 0 && K % group == 0 &&
+         K <= STRIM_LOSS_MAX_STRIDE;
+}
+}  // namespace
+
+int64_t strim_head_loss_workspace(int32_t N, int32_t K, int32_t V, int32_t want_d_hidden,
+                                  int32_t want_d_lm_head) {
+  if (!loss_sizes_ok(N, K, V)) return STRIM_EINVAL;
+  return N == 0 ? 0 : loss_workspace(N, K, V, want_d_hidden != 0, want_d_lm_head != 0);
+}
+
+int strim_head_loss(void* stream, const void* hidden, int64_t hidden_stride, int32_t N, int32_t K,
+                    const void* lm_head, int64_t lm_head_stride, int32_t V, const int32_t* targets,
+                    int32_t ignore_index, void* workspace, int64_t workspace_bytes, float* out_loss,
+                    float* out_lse, int32_t* out_status) {
+  if (!loss_sizes_ok(N, K, V) || !loss_rows_ok(lm_head, lm_head_stride, K)) return STRIM_EINVAL;
+  if (N == 0) return STRIM_OK;
+  if (!loss_rows_ok(hidden, hidden_stride, K) || !targets || !out_loss || !workspace ||
+      !al16(workspace))
+    return STRIM_EINVAL;
+  if (workspace_bytes < loss_workspace(N, K, V, false, false)) return STRIM_ECAPACITY;
+  const hipError_t e = launch_loss(hidden, hidden_stride, N, K, lm_head, lm_head_stride, V, targets,
+                                   ignore_index, workspace, out_loss, out_lse, out_status,
+                                   (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride, int32_t N,
+                         int32_t K, const void* lm_head, int64_t lm_head_stride, int32_t V,
+                         const int32_t* targets, int32_t ignore_index, const float* lse,
+                         const float* grad_loss, const float* grad_lse, void* workspace,
+                         int64_t workspace_bytes, void* d_hidden, int64_t d_hidden_stride,
+                         void* d_lm_head, int64_t d_lm_head_stride) {
+  if (!loss_sizes_ok(N, K, V) || !loss_rows_ok(lm_head, lm_head_stride, K) ||
+      (!d_hidden && !d_lm_head && N > 0) ||
+      (d_lm_head && !loss_rows_ok(d_lm_head, d_lm_head_stride, K)))
+    return STRIM_EINVAL;
+  if (N > 0 && (!loss_rows_ok(hidden, hidden_stride, K) ||
+                (d_hidden && !loss_rows_ok(d_hidden, d_hidden_stride, K)) || !targets || !lse ||
+                !grad_loss || !workspace || !al16(workspace)))
+    return STRIM_EINVAL;
+  if (N > 0 && workspace_bytes < loss_workspace(N, K, V, d_hidden != nullptr, d_lm_head != nullptr))
+    return STRIM_ECAPACITY;
+  const hipError_t e = launch_loss_grad(hidden, hidden_stride, N, K, lm_head, lm_head_stride, V,
+                                        targets, ignore_index, lse, grad_loss, grad_lse, workspace,
+                                        d_hidden, d_hidden_stride, d_lm_head, d_lm_head_stride,
+                                        (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_pack_weights(void* stream, const void* weight, int32_t dtype, int64_t weight_stride, int32_t V,
+                  int32_t K, int32_t group, uint32_t* words, void* scales, void* biases) {
+  if (!weight || !words || !scales || !dtype_ok(dtype) || V <= 0 || !group_ok(K, group) ||
+      weight_stride < K || !al16(weight) || weight_stride % (dtype == STRIM_DTYPE_BF16 ? 8 : 4) != 0)
+    return STRIM_EINVAL;
+  const hipError_t e = launch_q4_pack(weight, dtype == STRIM_DTYPE_F32, weight_stride, V, K, group,
+                                      words, (uint16_t*)scales, (uint16_t*)biases,
+                                      (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_unpack_weights(void* stream, const uint32_t* words, int64_t words_stride, const void* scales,
+                    const void* biases, int64_t scales_stride, int32_t V, int32_t K, int32_t group,
+                    void* out, int32_t dtype, int64_t out_stride) {
+  if (!words || !scales || !out || !dtype_ok(dtype) || V <= 0 || !group_ok(K, group) ||
+      words_stride < K / 8 || scales_stride < K / group || out_stride < K || !al16(out) ||
+      out_stride % (dtype == STRIM_DTYPE_BF16 ? 8 : 4) != 0)
+    return STRIM_EINVAL;
+  const hipError_t e = launch_q4_unpack(words, words_stride, (const uint16_t*)scales,
+                                        (const uint16_t*)biases, scales_stride, group, V, K, out,
+                                        dtype == STRIM_DTYPE_F32, out_stride, (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int64_t strim_head_logits_packed_workspace(int32_t B, int32_t K) {
+  return B < 1 || K <= 0 || K > STRIM_LOSS_MAX_STRIDE ? STRIM_EINVAL : q4_workspace(B, K);
+}
+
+int strim_head_logits_packed(void* stream, const void* hidden, int64_t hidden_stride, int32_t B,
+                         int32_t K, const void* norm_weight, float eps, void* xn,
+                         const uint32_t* words, int64_t words_stride, const void* scales,
+                         const void* biases, int64_t scales_stride, int32_t group, int32_t V,
+                         void* workspace, int64_t workspace_bytes, void* out_logits, int32_t dtype,
+                         int64_t out_stride) {
+  if (!hidden || !words || !scales || !out_logits || !workspace || B < 1 || V <= 0 ||
+      !group_ok(K, group) || !dtype_ok(dtype) || hidden_stride < K || hidden_stride % 8 != 0 ||
+      !al16(hidden) || words_stride < K / 8 || words_stride % 4 != 0 || !al16(words) ||
+      scales_stride < K / group || out_stride < V || !(eps >= 0.0f) || !al16(workspace))
+    return STRIM_EINVAL;
+  if (norm_weight && (!xn || !al16(xn) || !al16(norm_weight))) return STRIM_EINVAL;
+  if (workspace_bytes < q4_workspace(B, K)) return STRIM_ECAPACITY;
+  if (norm_weight) {
+    launch_head_norm(hidden, hidden_stride, B, K, norm_weight, eps, xn, (hipStream_t)stream);
+    hidden = xn;
+    hidden_stride = K;
+  }
+  const hipError_t e = launch_q4_logits(hidden, hidden_stride, B, K, words, words_stride,
+                                        (const uint16_t*)scales, (const uint16_t*)biases,
+                                        scales_stride, group, V, workspace, out_logits,
+                                        dtype == STRIM_DTYPE_F32, out_stride, (hipStream_t)stream);
   return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
 }
 

@@ -525,6 +525,12 @@ __global__ __launch_bounds__(HP_T) void k_head_pick(const uint2* tbest, int ntil
   }
 }
 
+void launch_head_norm(const void* hidden, int64_t hidden_stride, int B, int K, const void* norm_w,
+                      float eps, void* xn, hipStream_t st) {
+  hipLaunchKernelGGL(k_head_norm, dim3((unsigned)B), dim3(HN_T), 0, st, (const uint16_t*)hidden,
+                     hidden_stride, K, (const uint16_t*)norm_w, eps, (uint16_t*)xn);
+}
+
 hipError_t launch_head(const void* hidden, int64_t hidden_stride, int B, int K,
                        const void* norm_w, float eps, void* xn, const void* W, int64_t w_stride,
                        int V, void* out, int64_t out_stride, bool vo, hipStream_t st,
@@ -532,8 +538,7 @@ hipError_t launch_head(const void* hidden, int64_t hidden_stride, int B, int K,
   const uint16_t* src = (const uint16_t*)hidden;
   int64_t src_stride = hidden_stride;
   if (norm_w) {
-    hipLaunchKernelGGL(k_head_norm, dim3((unsigned)B), dim3(HN_T), 0, st, (const uint16_t*)hidden,
-                       hidden_stride, K, (const uint16_t*)norm_w, eps, (uint16_t*)xn);
+    launch_head_norm(hidden, hidden_stride, B, K, norm_w, eps, xn, st);
     src = (const uint16_t*)xn;
     src_stride = K;
   }

@@ -1,0 +1,586 @@
+// loss_kernels.hip — cross entropy of the vocabulary projection's logits, without keeping the
+// logits, and its gradients, for bf16 hidden states [N, K] and a bf16 lm_head [V, K].
+//
+//   x[n][v] = sum_k hidden[n][k] lm_head[v][k]          (float32 accumulation)
+//   lse[n]  = log sum_v exp(x[n][v]),  loss[n] = lse[n] - x[n][target[n]]
+//   p[n][v] = (g[n] + z[n]) exp(x[n][v] - lse[n]) - g[n] [v = target[n]]
+//   d_hidden[n][k]  = sum_v p[n][v] lm_head[v][k]
+//   d_lm_head[v][k] = sum_n p[n][v] hidden[n][k]
+// with g = dL/dloss and z = dL/dlse.
+//
+// Four products of 2 N V K operations: the logits twice (once for their row statistics, once
+// more for p), and one for each gradient. What is kept between them is a (max, sum) pair per
+// row and 128-row vocabulary slice, and p of one piece of the vocabulary, rounded to bf16 for
+// the two gradient products (the gradients are bf16 themselves; their sums are float32).
+//
+// k_loss_gemm is all four: a tile of C = A B^T on v_mfma_f32_16x16x32_bf16, its operands
+// brought by 16-byte loads straight into LDS, one stage of 64 along the reduction ahead of
+// the multiplies. An operand whose rows run along the reduction is read from LDS 8 elements
+// a lane; one whose rows run across it (both of d_lm_head's, the projection in d_hidden) is
+// transposed on its way from LDS to the registers (ds_read_b64_tr_b16), so nothing is laid
+// out anew in memory.
+#include "kernels.hpp"
+
+namespace strim {
+
+typedef __bf16 lbf16x8 __attribute__((ext_vector_type(8)));
+typedef float lf32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t lu32x4 __attribute__((ext_vector_type(4)));
+typedef short ls16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) ls16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) lu32x4 lds_u32x4;
+
+constexpr int LG_BK = 64;                 // reduction elements a stage
+constexpr uint32_t LG_RANGE = 0x40000000u;  // bytes a buffer descriptor spans; a lane that has
+                                            // nothing to load points past it and gets zeros
+
+enum LossMode { LM_STATS = 0, LM_PROB = 1, LM_DHID = 2, LM_DHEAD = 3 };
+
+// One operand: `rows` valid rows (of the tile dimension) from `p`, `red` valid elements along
+// the reduction. TR false: element (row, k) at p[row stride + k]; true: p[k stride + row].
+struct LossOperand {
+  const uint16_t* p;
+  int64_t stride;
+  int32_t rows;
+};
+
+struct LossGemm {
+  LossOperand a, b;        // a: the tile's M side, b: its N side
+  int32_t red;             // reduction length
+  int32_t split_red;       // reduction elements a split (a multiple of LG_BK)
+  int32_t tiles_m, tiles_n, splits;
+  // LM_STATS, LM_PROB: M = vocabulary rows from v0, N = tokens
+  int32_t v0, ignore_index;
+  int32_t V;
+  const int32_t* targets;
+  float2* part;            // LM_STATS [slice][N]: max, sum exp(x - max) of a vocabulary slice
+  float* tlogit;           // LM_STATS [N]: the target's logit
+  const float *lse, *grad_loss, *grad_lse;
+  uint16_t* out16;         // LM_PROB p [N][out_stride]; LM_DHEAD [v][out_stride]
+  int64_t out_stride;
+  float* out32;            // LM_DHID [split][N][out_stride]
+  int32_t accumulate;      // LM_DHID: add to what out32 holds
+};
+
+__device__ __forceinline__ uint32_t loss_bf16(float f) {
+  const uint32_t u = __float_as_uint(f);
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x0040u;
+  return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+__device__ __forceinline__ uint2 loss_pack4(const float* f) {
+  return make_uint2(loss_bf16(f[0]) | (loss_bf16(f[1]) << 16),
+                    loss_bf16(f[2]) | (loss_bf16(f[3]) << 16));
+}
+
+__device__ __forceinline__ float loss_exp(float x) {
+  return __builtin_amdgcn_exp2f(x * 1.44269504088896340736f);
+}
+
+// 64 lanes' 16 bytes each, to LDS from `dst` (the same in every lane) in lane order.
+__device__ __forceinline__ void loss_load_lds(uint32_t dst, uint32_t voff, lu32x4 rsrc) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               ::"s"(dst), "v"(voff), "s"(rsrc) : "memory");
+}
+
+// The part of an operand's stage that one wave loads, and its fragments' places in LDS.
+// A stage holds, TR false, ROWS rows of 64 elements (128 bytes, 16-byte piece c at place
+// c ^ (row & 7)); TR true, 64 rows of ROWS elements (32-byte piece c at place c ^ f(row)):
+// with these orders the lanes of one LDS read meet all banks evenly.
+template <bool TR, int ROWS, int NW>
+struct LossTile {
+  static constexpr int BYTES = ROWS * 2 * LG_BK;
+  static constexpr int NI = BYTES / 1024 / NW;         // load instructions a wave
+  static constexpr int RPI = TR ? 512 / ROWS : 8;      // rows an instruction covers
+  static constexpr int LPR = 64 / RPI;                 // lanes a row
+  static_assert(NI >= 1 && NI * NW * 1024 == BYTES, "whole instructions");
+  uint32_t voff[NI];
+  int kofs;
+  const uint16_t* base;
+  int64_t step;
+  uint32_t lds0;
+
+  static __device__ __forceinline__ int f(int row) { return (row & 3) | ((row >> 1) & 4); }
+
+  __device__ __forceinline__ void init(const LossOperand& o, int row0, int red0, int wv, int lane) {
+    const int r0 = wv * NI * RPI + lane / LPR;
+    if constexpr (TR) {
+      base = o.p + (int64_t)red0 * o.stride + row0;
+      step = (int64_t)LG_BK * o.stride;
+      kofs = r0;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int r = r0 + j * RPI, c = lane % LPR;
+        const int col = (((c >> 1) ^ f(r)) << 4) + ((c & 1) << 3);
+        voff[j] = row0 + col < o.rows ? (uint32_t)(2 * (r * (int)o.stride + col)) : LG_RANGE;
+      }
+    } else {
+      base = o.p + (int64_t)row0 * o.stride + red0;
+      step = LG_BK;
+      const int c = (lane & 7) ^ (lane >> 3);
+      kofs = 8 * c;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const int r = r0 + j * RPI;
+        voff[j] = row0 + r < o.rows ? (uint32_t)(2 * (r * (int)o.stride + 8 * c)) : LG_RANGE;
+      }
+    }
+    lds0 = (uint32_t)(wv * NI * 1024);
+  }
+
+  // requests stage `s` (elements s * 64 onwards of a reduction of `red`) into LDS at `lds`
+  __device__ __forceinline__ void load(uint32_t lds, int s, int red) const {
+    const uint64_t at = (uint64_t)(base + (int64_t)s * step);
+    lu32x4 rsrc;
+    rsrc[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+    rsrc[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32) & 0xFFFF);
+    rsrc[2] = LG_RANGE;
+    rsrc[3] = 0x00020000u;
+    const int left = red - s * LG_BK - kofs;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const bool in = left > (TR ? j * RPI : 0);
+      loss_load_lds(__builtin_amdgcn_readfirstlane((int)(lds + lds0 + j * 1024)),
+                    in ? voff[j] : LG_RANGE, rsrc);
+    }
+  }
+};
+
+// Fragment reads: lane l holds elements 8 (l / 16) .. + 7 along the reduction of row l % 16
+// of the 16-row tile t0 + i, half kk (32 of the stage's 64 elements).
+template <bool TR, int ROWS>
+struct LossFrag {
+  uint32_t at0, at1;  // TR: at0 the row part, at1 the piece's xor
+  __device__ __forceinline__ void init(int t0, int lane) {
+    const int h = lane >> 4, j = lane & 15;
+    if constexpr (TR) {
+      at0 = (uint32_t)((8 * h + (j >> 2)) * (2 * ROWS) + 8 * (j & 3));
+      at1 = (uint32_t)(t0 * 32) ^ (uint32_t)(((j >> 2) | ((h & 1) << 2)) * 32);
+    } else {
+      at0 = (uint32_t)((t0 * 16 + j) * 128 + ((h ^ (j & 7)) << 4));
+      at1 = at0 ^ 64u;
+    }
+  }
+  __device__ __forceinline__ lbf16x8 get(uint32_t lds, int i, int kk) const {
+    if constexpr (TR) {
+      const uint32_t a = lds + at0 + (at1 ^ (uint32_t)(i * 32)) + (uint32_t)(kk * 32 * 2 * ROWS);
+      const ls16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)a);
+      const ls16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(a + 4 * 2 * ROWS));
+      return __builtin_bit_cast(lbf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const uint32_t a = lds + (kk ? at1 : at0) + (uint32_t)(i * 2048);
+      return __builtin_bit_cast(lbf16x8, *(const lds_u32x4*)(uintptr_t)a);
+    }
+  }
+};
+
+// Workgroup -> tile: each XCD (workgroups are dealt to the eight in turn) takes a run of
+// neighbouring tiles, eight of the N side by as many of the M side as are in flight, so that
+// its L2 serves each operand slab to several workgroups.
+__device__ __forceinline__ void loss_tile(int tiles_m, int tiles_n, int splits, int& tm, int& tn,
+                                          int& split) {
+  const int tiles = tiles_m * tiles_n, total = tiles * splits, b = blockIdx.x;
+  const int x = b & 7, per = total >> 3, rem = total & 7;
+  int id = x * per + min(x, rem) + (b >> 3);
+  split = id / tiles;
+  id -= split * tiles;
+  const int g = id / (8 * tiles_m), r = id - g * 8 * tiles_m;
+  const int wide = min(8, tiles_n - 8 * g);
+  tn = 8 * g + r % wide;
+  tm = r / wide;
+}
+
+template <int MODE, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g) {
+  constexpr bool ATR = MODE == LM_DHID || MODE == LM_DHEAD, BTR = MODE == LM_DHEAD;
+  constexpr int NW = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
+  typedef LossTile<ATR, BM, NW> TileA;
+  typedef LossTile<BTR, BN, NW> TileB;
+  constexpr int STAGE = TileA::BYTES + TileB::BYTES;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_buf[2 * STAGE];
+  const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)s_buf;
+  const int lane = threadIdx.x & (WAVE - 1), wv = wave_id();
+  const int wm = wv / WN, wn = wv % WN;
+  int tm, tn, split;
+  loss_tile(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
+  const int red0 = split * g.split_red;
+  const int red = max(0, min(g.split_red, g.red - red0));
+  const int steps = (red + LG_BK - 1) / LG_BK;
+
+  TileA ta;
+  TileB tb;
+  ta.init(g.a, tm * BM, red0, wv, lane);
+  tb.init(g.b, tn * BN, red0, wv, lane);
+  LossFrag<ATR, BM> fa;
+  LossFrag<BTR, BN> fb;
+  fa.init(wm * TM, lane);
+  fb.init(wn * TN, lane);
+
+  lf32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (steps > 0) {
+    ta.load(lds, 0, red);
+    tb.load(lds + TileA::BYTES, 0, red);
+  }
+  for (int s = 0; s < steps; ++s) {
+    const uint32_t cur = lds + (uint32_t)((s & 1) * STAGE);
+    const uint32_t nxt = lds + (uint32_t)(((s & 1) ^ 1) * STAGE);
+    // this stage has arrived, and every wave has read the other one
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (s + 1 < steps) {
+      ta.load(nxt, s + 1, red);
+      tb.load(nxt + TileA::BYTES, s + 1, red);
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      lbf16x8 bf[TN], af[TM];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) bf[j] = fb.get(cur + TileA::BYTES, j, kk);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) af[i] = fa.get(cur, i, kk);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[i], bf[j], acc[i][j], 0, 0, 0);
+    }
+  }
+
+  // lane l holds C[row 4 (l / 16) + r][column l % 16] of each 16 x 16 tile
+  const int h = lane >> 4, c16 = lane & 15;
+  const int m0 = tm * BM + wm * TM * 16 + 4 * h;
+  const int n0 = tn * BN + wn * TN * 16 + c16;
+  if constexpr (MODE == LM_STATS) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + 16 * j;
+      const int t = n < g.b.rows ? g.targets[n] : -1;
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int v = m0 + 16 * i + r;
+          if (v == t && v < g.V) g.tlogit[n] = acc[i][j][r];
+          if (v >= g.V) acc[i][j][r] = -INFINITY;
+          mx = fmaxf(mx, acc[i][j][r]);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float ref = mx == -INFINITY ? 0.0f : mx;  // a slice of -inf alone adds nothing
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += loss_exp(acc[i][j][r] - ref);
+      sum += __shfl_xor(sum, 16);
+      sum += __shfl_xor(sum, 32);
+      if (h == 0 && n < g.b.rows)
+        g.part[(int64_t)(tm * WM + wm) * g.b.rows + n] = make_float2(mx, sum);
+    }
+  } else if constexpr (MODE == LM_PROB) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + 16 * j;
+      if (n >= g.b.rows) continue;
+      const int t = g.targets[n];
+      const bool live = t != g.ignore_index && t >= 0 && t < g.V;
+      const float gl = live ? g.grad_loss[n] : 0.0f;
+      const float top = live && g.grad_lse ? gl + g.grad_lse[n] : gl;
+      const float lse = g.lse[n];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int v = g.v0 + m0 + 16 * i + r;
+          const float y = top * loss_exp(acc[i][j][r] - lse) - (v == t ? gl : 0.0f);
+          p[r] = live && v < g.V ? y : 0.0f;
+        }
+        *(uint2*)(g.out16 + (int64_t)n * g.out_stride + m0 + 16 * i) = loss_pack4(p);
+      }
+    }
+  } else if constexpr (MODE == LM_DHID) {
+    float* out = g.out32 + (int64_t)split * g.b.rows * g.out_stride;
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + 16 * j;
+      if (n >= g.b.rows) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int k = m0 + 16 * i;
+        if (k >= g.a.rows) continue;
+        lf32x4* at = (lf32x4*)(out + (int64_t)n * g.out_stride + k);
+        *at = g.accumulate ? *at + acc[i][j] : acc[i][j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int v = n0 + 16 * j;
+      if (v >= g.b.rows) continue;
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        const int k = m0 + 16 * i;
+        if (k >= g.a.rows) continue;
+        const float f[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        *(uint2*)(g.out16 + (int64_t)v * g.out_stride + k) = loss_pack4(f);
+      }
+    }
+  }
+}
+
+
+// Merges two (max, sum exp(x - max)) pairs; a max of -inf carries no sum.
+__device__ __forceinline__ void loss_merge(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2), ref = top == -INFINITY ? 0.0f : top;
+  s = s * loss_exp(m - ref) + s2 * loss_exp(m2 - ref);
+  m = top;
+}
+
+// The rows' results from their slices' pairs: TOK tokens a workgroup of 256, the slices of a
+// token dealt to 256 / TOK threads in a fixed order.
+template <int TOK>
+__global__ __launch_bounds__(256) void k_loss_rows(const float2* part, int slices, int N,
+                                                   const float* tlogit, const int32_t* targets,
+                                                   int ignore_index, int V, float* out_loss,
+                                                   float* out_lse, int32_t* out_status) {
+  constexpr int W = 256 / TOK;
+  __shared__ float2 s_p[W][TOK];
+  const int tok = threadIdx.x % TOK, w = threadIdx.x / TOK;
+  const int n = blockIdx.x * TOK + tok;
+  float m = -INFINITY, s = 0.0f;
+  if (n < N)
+    for (int q = w; q < slices; q += W) {
+      const float2 p = part[(int64_t)q * N + n];
+      loss_merge(m, s, p.x, p.y);
+    }
+  s_p[w][tok] = make_float2(m, s);
+  for (int d = W / 2; d > 0; d >>= 1) {
+    __syncthreads();
+    if (w < d) {
+      const float2 p = s_p[w + d][tok];
+      loss_merge(m, s, p.x, p.y);
+      s_p[w][tok] = make_float2(m, s);
+    }
+  }
+  if (w != 0 || n >= N) return;
+  const int t = targets[n];
+  const float lse = m + logf(s);
+  const bool known = t >= 0 && t < V, live = known && t != ignore_index;
+  const float loss = live ? lse - tlogit[n] : 0.0f;
+  if (out_lse) out_lse[n] = lse;
+  out_loss[n] = loss;
+  if (out_status)
+    out_status[n] = t == ignore_index ? STRIM_OK
+                    : !known          ? STRIM_EINVAL
+                    : fabsf(loss) < INFINITY ? STRIM_OK
+                                             : STRIM_ENONFINITE;
+}
+
+// Hidden rows for the projection's gradient, contiguous: a row without a target is zeroed, so
+// that what its padding holds (a NaN too) meets no weight.
+__global__ __launch_bounds__(256) void k_loss_rows_in(const uint16_t* x, int64_t stride, int N,
+                                                      int K, const int32_t* targets,
+                                                      int ignore_index, int V, uint16_t* out) {
+  const int n = blockIdx.x;
+  const int t = targets[n];
+  const bool live = t != ignore_index && t >= 0 && t < V;
+  for (int k = 8 * threadIdx.x; k < K; k += 8 * 256) {
+    const uint4 q = *(const uint4*)(x + (int64_t)n * stride + k);
+    *(uint4*)(out + (int64_t)n * K + k) = live ? q : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// d_hidden from the splits' sums, added in order and rounded once.
+__global__ __launch_bounds__(256) void k_loss_join(const float* acc, int splits, int N, int K,
+                                                   uint16_t* out, int64_t out_stride) {
+  const int64_t total = (int64_t)N * K;
+  const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+  if (i >= total) return;
+  lf32x4 s = *(const lf32x4*)(acc + i);
+  for (int q = 1; q < splits; ++q) s += *(const lf32x4*)(acc + q * total + i);
+  const float f[4] = {s[0], s[1], s[2], s[3]};
+  const int64_t n = i / K;
+  *(uint2*)(out + n * out_stride + (i - n * K)) = loss_pack4(f);
+}
+
+// ---- host --------------------------------------------------------------------------------
+constexpr int LG_CUS = 256;
+constexpr int64_t LOSS_P_BYTES = (int64_t)512 << 20;  // p of one vocabulary piece
+
+static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+static inline int64_t up256(int64_t b) { return (b + 255) & ~(int64_t)255; }
+
+struct LossPlan {
+  int bn;          // tokens a tile: 64, 128 or 256
+  int piece;       // vocabulary rows a piece (a multiple of 256)
+  int splits;      // d_hidden: parts of a piece's vocabulary
+  int64_t part, tlogit, p, acc, rows, bytes;  // offsets into the workspace
+};
+
+static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
+  LossPlan q{};
+  q.bn = N <= 64 ? 64 : N <= 128 ? 128 : 256;
+  const int64_t tn = ceil_div(N, q.bn);
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t at = off;
+    off += up256(bytes);
+    return at;
+  };
+  if (!hid && !head) {
+    q.part = take(ceil_div(V, 256) * 8 * N * (int64_t)sizeof(float2));
+    q.tlogit = take(4 * (int64_t)N);
+    q.bytes = off;
+    return q;
+  }
+  // pieces of the vocabulary whose tiles fill the CUs best
+  const int64_t vt = ceil_div(V, 256);
+  const int64_t most = LOSS_P_BYTES / (512 * (int64_t)N) > 1 ? LOSS_P_BYTES / (512 * (int64_t)N) : 1;
+  int64_t best = -1, tiles = vt;
+  for (int64_t np = ceil_div(vt, most), e = np + 4; np < e; ++np) {
+    const int64_t t = ceil_div(vt, np), last = vt - t * (ceil_div(vt, t) - 1);
+    const int64_t rounds = (ceil_div(vt, t) - 1) * ceil_div(t * tn, LG_CUS) + ceil_div(last * tn, LG_CUS);
+    if (best < 0 || rounds < best) best = rounds, tiles = t;
+  }
+  q.piece = (int)(tiles * 256);
+  // d_hidden's reduction is split until its tiles fill the CUs; each split costs a pass over
+  // its float32 sums
+  const int64_t dt = ceil_div(K, 256) * tn, steps = ceil_div(q.piece, LG_BK);
+  q.splits = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 64 && s <= steps; ++s) {
+    const double us = 0.9 * q.bn / 256 * (double)(ceil_div(dt * s, LG_CUS) * ceil_div(steps, s)) +
+                      8.0 * s * N * (double)K / 4e6;
+    if (us < least) least = us, q.splits = s;
+  }
+  q.p = take((int64_t)N * q.piece * 2);
+  if (hid) q.acc = take((int64_t)q.splits * N * K * 4);
+  if (head) q.rows = take((int64_t)N * K * 2);
+  q.bytes = off;
+  return q;
+}
+
+int64_t loss_workspace(int N, int K, int V, bool hid, bool head) {
+  return loss_plan(N, K, V, hid, head).bytes;
+}
+
+template <int MODE>
+static void loss_gemm(const LossGemm& g0, int bn, int64_t m, int64_t n, hipStream_t st) {
+  LossGemm g = g0;
+  g.tiles_m = (int)ceil_div(m, 256);
+  g.tiles_n = (int)ceil_div(n, bn);
+  const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.splits));
+  if (bn == 256)
+    hipLaunchKernelGGL((k_loss_gemm<MODE, 2, 4, 8, 4>), grid, dim3(512), 0, st, g);
+  else if constexpr (MODE != LM_DHEAD) {
+    if (bn == 128)
+      hipLaunchKernelGGL((k_loss_gemm<MODE, 4, 2, 4, 4>), grid, dim3(512), 0, st, g);
+    else
+      hipLaunchKernelGGL((k_loss_gemm<MODE, 8, 1, 2, 4>), grid, dim3(512), 0, st, g);
+  }
+}
+
+hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws, int V,
+                       const int32_t* targets, int ignore_index, void* workspace, float* loss,
+                       float* lse, int32_t* status, hipStream_t st) {
+  const LossPlan q = loss_plan(N, K, V, false, false);
+  uint8_t* w8 = (uint8_t*)workspace;
+  LossGemm g{};
+  g.a = LossOperand{(const uint16_t*)W, ws, V};
+  g.b = LossOperand{(const uint16_t*)hidden, hs, N};
+  g.red = K;
+  g.split_red = (int)(ceil_div(K, LG_BK) * LG_BK);
+  g.splits = 1;
+  g.V = V;
+  g.ignore_index = ignore_index;
+  g.targets = targets;
+  g.part = (float2*)(w8 + q.part);
+  g.tlogit = (float*)(w8 + q.tlogit);
+  loss_gemm<LM_STATS>(g, q.bn, V, N, st);
+  const int slices = (int)ceil_div(V, 256) * (q.bn == 256 ? 2 : q.bn == 128 ? 4 : 8);
+  if (N >= 1024)
+    hipLaunchKernelGGL(k_loss_rows<16>, dim3((unsigned)ceil_div(N, 16)), dim3(256), 0, st, g.part,
+                       slices, N, g.tlogit, targets, ignore_index, V, loss, lse, status);
+  else
+    hipLaunchKernelGGL(k_loss_rows<1>, dim3((unsigned)N), dim3(256), 0, st, g.part, slices, N,
+                       g.tlogit, targets, ignore_index, V, loss, lse, status);
+  return hipGetLastError();
+}
+
+hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws,
+                            int V, const int32_t* targets, int ignore_index, const float* lse,
+                            const float* grad_loss, const float* grad_lse, void* workspace,
+                            void* d_hidden, int64_t dhs, void* d_head, int64_t dws,
+                            hipStream_t st) {
+  if (N == 0) {  // no reduction: the projection's gradient is zero
+    LossGemm z{};
+    z.a.rows = K;
+    z.b.rows = V;
+    z.splits = 1;
+    z.out16 = (uint16_t*)d_head;
+    z.out_stride = dws;
+    if (d_head) loss_gemm<LM_DHEAD>(z, 256, K, V, st);
+    return hipGetLastError();
+  }
+  const LossPlan q = loss_plan(N, K, V, d_hidden != nullptr, d_head != nullptr);
+  uint8_t* w8 = (uint8_t*)workspace;
+  uint16_t *p = (uint16_t*)(w8 + q.p), *rows = (uint16_t*)(w8 + q.rows);
+  if (d_head)
+    hipLaunchKernelGGL(k_loss_rows_in, dim3((unsigned)N), dim3(256), 0, st, (const uint16_t*)hidden,
+                       hs, N, K, targets, ignore_index, V, rows);
+  for (int v0 = 0; v0 < V; v0 += q.piece) {
+    const int vn = min(q.piece, V - v0);
+    const uint16_t* wv = (const uint16_t*)W + (int64_t)v0 * ws;
+    LossGemm g{};
+    g.a = LossOperand{wv, ws, vn};
+    g.b = LossOperand{(const uint16_t*)hidden, hs, N};
+    g.red = K;
+    g.split_red = (int)(ceil_div(K, LG_BK) * LG_BK);
+    g.splits = 1;
+    g.v0 = v0;
+    g.V = V;
+    g.ignore_index = ignore_index;
+    g.targets = targets;
+    g.lse = lse;
+    g.grad_loss = grad_loss;
+    g.grad_lse = grad_lse;
+    g.out16 = p;
+    g.out_stride = q.piece;
+    loss_gemm<LM_PROB>(g, q.bn, vn, N, st);
+    if (d_hidden) {
+      LossGemm h{};
+      h.a = LossOperand{wv, ws, K};
+      h.b = LossOperand{p, q.piece, N};
+      h.red = vn;
+      h.splits = q.splits;
+      h.split_red = (int)(ceil_div(ceil_div(vn, LG_BK), q.splits) * LG_BK);
+      h.out32 = (float*)(w8 + q.acc);
+      h.out_stride = K;
+      h.accumulate = v0 > 0;
+      loss_gemm<LM_DHID>(h, q.bn, K, N, st);
+    }
+    if (d_head) {
+      LossGemm h{};
+      h.a = LossOperand{rows, K, K};
+      h.b = LossOperand{p, q.piece, vn};
+      h.red = N;
+      h.splits = 1;
+      h.split_red = (int)(ceil_div(N, LG_BK) * LG_BK);
+      h.out16 = (uint16_t*)d_head + (int64_t)v0 * dws;
+      h.out_stride = dws;
+      loss_gemm<LM_DHEAD>(h, 256, K, vn, st);
+    }
+  }
+  if (d_hidden)
+    hipLaunchKernelGGL(k_loss_join, dim3((unsigned)ceil_div((int64_t)N * K, 1024)), dim3(256), 0, st,
+                       (const float*)(w8 + q.acc), q.splits, N, K, (uint16_t*)d_hidden, dhs);
+  return hipGetLastError();
+}
+
+}  // namespace strim

@@ -1,0 +1,397 @@
+// q4_kernels.hip — a vocabulary projection held in 4 bits with group scales: packing, reading
+// back, and the logits of a few rows.
+//
+// Row v of [V, K] is K / 8 words of eight 4-bit codes, the lowest bits first, and per group of
+// G consecutive elements (32, 64 or 128) a bf16 scale s and, unless the weights are symmetric,
+// a bf16 bias b: the element is s q + b (symmetric: s (q - 8)).
+//
+//   logits[r][v] = sum over groups g of  s[v][g] T + (b[v][g] - 16 s[v][g]) X
+//   T = sum over k in g of (16 + q[v][k]) x[r][k],   X = sum over k in g of x[r][k]
+//
+// 16 + q is made in place: a code moved to bits 3 .. 6 of a half word under the bits of 16.0
+// in bf16, two codes an instruction pair (the shift, and an AND-OR), exact; no conversion, no
+// scaling of weights before the product, so T is a bf16 MFMA's sum in float32, and a group
+// costs two multiply-adds a result. The offset 16 (and not 128, which would save one of the
+// four shifts) keeps what cancels between T and 16 X to a few bits.
+#include "kernels.hpp"
+
+namespace strim {
+
+typedef __bf16 qbf16x8 __attribute__((ext_vector_type(8)));
+typedef float qf32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t qu32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ uint32_t q4_bf16(float f) {
+  const uint32_t u = __float_as_uint(f);
+  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x0040u;
+  return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+
+// ---- packing ------------------------------------------------------------------------------
+// Eight elements a thread, G / 8 neighbouring lanes a group.
+//   biased:    s = bf16((max - min) / 15), b = bf16(min), q = clamp(rint((w - b) / s), 0, 15)
+//   symmetric: s = bf16(max|w| / 7),                      q = clamp(rint(w / s) + 8, 0, 15)
+// s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). The divisions by 15 and 7
+// are products with their float32 reciprocals. A group with a NaN or an infinity gets NaN for
+// its scale and its bias.
+struct Q4Pack {
+  const void* w;
+  int64_t w_stride;
+  int32_t V, K;
+  uint32_t* words;
+  uint16_t *scales, *biases;
+};
+
+template <int G, bool F32, bool SYM>
+__global__ __launch_bounds__(256) void k_q4_pack(const Q4Pack a) {
+  const int per_row = a.K / 8;
+  const int64_t total = (int64_t)a.V * per_row;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  // whole groups: total and the stride are multiples of G / 8, which divides a wave
+  for (int64_t i = first; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t v = i / per_row;
+    const int c = (int)(i - v * per_row);
+    float x[8];
+    if constexpr (F32) {
+      const float4* p = (const float4*)((const float*)a.w + v * a.w_stride + 8 * c);
+      const float4 lo = p[0], hi = p[1];
+      x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+      x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+    } else {
+      const uint4 q = *(const uint4*)((const uint16_t*)a.w + v * a.w_stride + 8 * c);
+      const uint32_t d[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = __uint_as_float(d[e] << 16);
+        x[2 * e + 1] = __uint_as_float(d[e] & 0xFFFF0000u);
+      }
+    }
+    float hi = SYM ? fabsf(x[0]) : x[0], lo = x[0], bad = 0.0f * x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+      hi = fmaxf(hi, SYM ? fabsf(x[e]) : x[e]);
+      lo = fminf(lo, x[e]);
+      bad += 0.0f * x[e];  // NaN where an element is not finite
+    }
+#pragma unroll
+    for (int d = 1; d < G / 8; d <<= 1) {
+      hi = fmaxf(hi, __shfl_xor(hi, d));
+      if constexpr (!SYM) lo = fminf(lo, __shfl_xor(lo, d));
+      bad += __shfl_xor(bad, d);
+    }
+    const uint32_t s16 = q4_bf16((SYM ? hi * (1.0f / 7.0f) : (hi - lo) * (1.0f / 15.0f)) + bad);
+    const uint32_t b16 = SYM ? 0u : q4_bf16(lo + bad);
+    const float s = __uint_as_float(s16 << 16), b = __uint_as_float(b16 << 16);
+    uint32_t word = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float q = s > 0.0f ? rintf((SYM ? x[e] : x[e] - b) / s) : 0.0f;
+      if constexpr (SYM) q += 8.0f;
+      word |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * e);
+    }
+    a.words[i] = word;
+    if (c % (G / 8) == 0) {
+      const int64_t g = v * (a.K / G) + c / (G / 8);
+      a.scales[g] = (uint16_t)s16;
+      if constexpr (!SYM) a.biases[g] = (uint16_t)b16;
+    }
+  }
+}
+
+// ---- reading back -------------------------------------------------------------------------
+struct Q4Weights {
+  const uint32_t* words;
+  int64_t words_stride;  // words a row
+  const uint16_t *scales, *biases;
+  int64_t scales_stride;
+  int32_t V, K;
+};
+
+template <int G, bool F32>
+__global__ __launch_bounds__(256) void k_q4_unpack(const Q4Weights a, void* out, int64_t out_stride) {
+  const int per_row = a.K / 8;
+  const int64_t total = (int64_t)a.V * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t v = i / per_row;
+    const int c = (int)(i - v * per_row);
+    const uint32_t word = a.words[v * a.words_stride + c];
+    const int64_t g = v * a.scales_stride + c / (G / 8);
+    const float s = __uint_as_float((uint32_t)a.scales[g] << 16);
+    const float b = a.biases ? __uint_as_float((uint32_t)a.biases[g] << 16) : 0.0f;
+    const float z = a.biases ? 0.0f : 8.0f;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = ((float)((word >> (4 * e)) & 15u) - z) * s + b;
+    if constexpr (F32) {
+      float4* p = (float4*)((float*)out + v * out_stride + 8 * c);
+      p[0] = make_float4(x[0], x[1], x[2], x[3]);
+      p[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+      uint32_t d[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[e] = q4_bf16(x[2 * e]) | (q4_bf16(x[2 * e + 1]) << 16);
+      *(uint4*)((uint16_t*)out + v * out_stride + 8 * c) = make_uint4(d[0], d[1], d[2], d[3]);
+    }
+  }
+}
+
+// ---- logits -------------------------------------------------------------------------------
+// A step is 128 elements of K: a 16-row weight tile's 16 lanes of row r each load 16 bytes (4
+// words) in each quarter of the wave. An MFMA sums over the four quarters, so its four words
+// must be of one group: wide groups (128) are as loaded, narrower ones are exchanged between
+// the quarters (v_permlane32_swap; 32 also v_permlane16_swap), one or half an instruction a
+// word. q4_koff says which elements of the step quarter h of MFMA t then holds.
+template <int G>
+__device__ __forceinline__ constexpr int q4_koff(int t, int h) {
+  return G == 128 ? 32 * h + 8 * t
+         : G == 64 ? 32 * (2 * (t >> 1) + (h & 1)) + 8 * (2 * (t & 1) + (h >> 1))
+                   : 32 * t + 8 * h;
+}
+
+__device__ __forceinline__ void q4_swap32(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+__device__ __forceinline__ void q4_swap16(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0], b = r[1];
+}
+
+// the words of MFMAs 0 .. 3 from a lane's four
+template <int G>
+__device__ __forceinline__ void q4_order(const qu32x4& w, uint32_t* o) {
+  if constexpr (G == 128) {
+    o[0] = w[0], o[1] = w[1], o[2] = w[2], o[3] = w[3];
+  } else if constexpr (G == 64) {
+    o[0] = w[0], o[2] = w[1], o[1] = w[2], o[3] = w[3];
+    q4_swap32(o[0], o[2]);
+    q4_swap32(o[1], o[3]);
+  } else {
+    uint32_t a = w[0], b = w[2], c = w[1], d = w[3];
+    q4_swap32(a, b);
+    q4_swap32(c, d);
+    q4_swap16(a, c);
+    q4_swap16(b, d);
+    o[0] = a, o[1] = c, o[2] = b, o[3] = d;
+  }
+}
+
+// 16 + q of a word's codes, in the order 0 4 1 5 2 6 3 7
+__device__ __forceinline__ qbf16x8 q4_codes(uint32_t w) {
+  constexpr uint32_t M = 0x00780078u, O = 0x41804180u;
+  const qu32x4 r = {((w << 3) & M) | O, ((w >> 1) & M) | O, ((w >> 5) & M) | O, ((w >> 9) & M) | O};
+  return __builtin_bit_cast(qbf16x8, r);
+}
+
+// eight elements of a hidden row in that order
+__device__ __forceinline__ qu32x4 q4_xfrag(const uint16_t* p) {
+  const qu32x4 d = *(const qu32x4*)p;
+  return qu32x4{__builtin_amdgcn_perm(d[2], d[0], 0x05040100u), __builtin_amdgcn_perm(d[2], d[0], 0x07060302u),
+                __builtin_amdgcn_perm(d[3], d[1], 0x05040100u), __builtin_amdgcn_perm(d[3], d[1], 0x07060302u)};
+}
+
+struct Q4Args {
+  Q4Weights w;
+  const uint16_t* x;   // hidden [B][x_stride]
+  int64_t x_stride;
+  int32_t B;
+  uint8_t* blocks;     // k_q4_stage: the hidden rows' fragments and group sums, by steps
+  void* out;
+  int64_t out_stride;
+  int32_t out_f32;
+};
+
+// Row of the batch at place m of an MFMA's 16: rows 0 .. 3 at places 0, 4, 8, 12, so that
+// the results of up to 4 rows are one register a lane, of up to 8 two.
+__device__ __forceinline__ int q4_row(int m) { return (m >> 2) + 4 * (m & 3); }
+
+__device__ __forceinline__ void q4_store(const Q4Args& a, int b, int v, float y) {
+  if (a.out_f32) ((float*)a.out)[(int64_t)b * a.out_stride + v] = y;
+  else ((uint16_t*)a.out)[(int64_t)b * a.out_stride + v] = (uint16_t)q4_bf16(y);
+}
+
+// Sums X of a 16-place tile's fragments over a group: the product with ones.
+__device__ __forceinline__ qf32x4 q4_sum(qu32x4 x, qf32x4 acc) {
+  const qu32x4 one = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x),
+                                                 __builtin_bit_cast(qbf16x8, one), acc, 0, 0, 0);
+}
+
+// The hidden rows by steps: per step 4 NT fragments of 1 KB (MFMA t of batch tile nt at t NT +
+// nt, 16 bytes a lane), then the sums X [group][NT][16 places], padded to 1 KB.
+template <int G, int NT>
+__global__ __launch_bounds__(WAVE) void k_q4_blocks(const Q4Args a) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
+  const int lane = threadIdx.x, h = lane >> 4, m = lane & 15, step = blockIdx.x;
+  uint8_t* blk = a.blocks + (int64_t)step * BLOCK;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int b = 16 * nt + q4_row(m);
+#pragma unroll
+    for (int g = 0; g < GPS; ++g) {
+      qf32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < MPG; ++q) {
+        const int t = g * MPG + q, k = step * 128 + q4_koff<G>(t, h);
+        qu32x4 x = {0u, 0u, 0u, 0u};
+        if (b < a.B && k < a.w.K) x = q4_xfrag(a.x + (int64_t)b * a.x_stride + k);
+        *(qu32x4*)(blk + (t * NT + nt) * 1024 + lane * 16) = x;
+        s = q4_sum(x, s);
+      }
+      if (m == 0) *(qf32x4*)(blk + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4) = s;
+    }
+  }
+}
+
+// NT batch tiles; NW waves a workgroup, each RT 16-row weight tiles over the whole of K.
+template <int G, int NT, int RT, int NW>
+__global__ __launch_bounds__(NW* WAVE) void k_q4_stage(const Q4Args a) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_x[2][BLOCK];
+  const int lane = threadIdx.x & (WAVE - 1), wv = wave_id(), h = lane >> 4, r16 = lane & 15;
+  const int v0 = (blockIdx.x * NW + wv) * RT * 16;
+  const int steps = (a.w.K + 127) / 128, groups = a.w.K / G, pieces = a.w.K / 32;
+  const uint32_t* wrow[RT];
+  const uint16_t *srow[RT], *brow[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int v = min(v0 + 16 * i + r16, a.w.V - 1);
+    wrow[i] = a.w.words + (int64_t)v * a.w.words_stride;
+    srow[i] = a.w.scales + (int64_t)v * a.w.scales_stride;
+    brow[i] = a.w.biases ? a.w.biases + (int64_t)v * a.w.scales_stride : nullptr;
+  }
+  qf32x4 acc[RT][NT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[i][nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < steps; ++s) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < BLOCK / 16; e += NW * WAVE)
+      *(qu32x4*)&s_x[0][e * 16] = *(const qu32x4*)(a.blocks + (int64_t)s * BLOCK + e * 16);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      uint32_t w[4];
+      q4_order<G>(*(const qu32x4*)(wrow[i] + 4 * min(4 * s + h, pieces - 1)), w);
+#pragma unroll
+      for (int g = 0; g < GPS; ++g) {
+        const int gi = s * GPS + g;
+        if (gi >= groups) break;
+        const float sc = __uint_as_float((uint32_t)srow[i][gi] << 16);
+        const float bi = brow[i] ? __uint_as_float((uint32_t)brow[i][gi] << 16) : -8.0f * sc;
+        const float off = bi - 16.0f * sc;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          qf32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < MPG; ++q) {
+            const int m = g * MPG + q;
+            const qu32x4 x = *(const qu32x4*)&s_x[0][(m * NT + nt) * 1024 + lane * 16];
+            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), q4_codes(w[m]), t, 0, 0, 0);
+          }
+          const qf32x4 xs = *(const qf32x4*)&s_x[0][4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            acc[i][nt][r] = __builtin_fmaf(sc, t[r], __builtin_fmaf(off, xs[r], acc[i][nt][r]));
+        }
+      }
+    }
+  }
+  // lane: weight row r16, places 4 h + r of each batch tile
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int v = v0 + 16 * i + r16;
+    if (v >= a.w.V) continue;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int b = 16 * nt + q4_row(4 * h + r);
+        if (b < a.B) q4_store(a, b, v, acc[i][nt][r]);
+      }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------
+int64_t q4_workspace(int B, int K) {
+  const int64_t nt = ((B < 64 ? B : 64) + 15) / 16;
+  return ((K + 127) / 128) * (4 * nt + 1) * 1024;
+}
+
+template <int G>
+static void q4_logits(const Q4Args& a, hipStream_t st) {
+  const dim3 steps((unsigned)((a.w.K + 127) / 128)), grid((unsigned)((a.w.V + 127) / 128));
+#define STRIM_Q4(NT_)                                                            \
+  do {                                                                           \
+    hipLaunchKernelGGL((k_q4_blocks<G, NT_>), steps, dim3(WAVE), 0, st, a);      \
+    hipLaunchKernelGGL((k_q4_stage<G, NT_, 2, 4>), grid, dim3(4 * WAVE), 0, st, a); \
+  } while (0)
+  if (a.B <= 16) STRIM_Q4(1);
+  else if (a.B <= 32) STRIM_Q4(2);
+  else if (a.B <= 48) STRIM_Q4(3);
+  else STRIM_Q4(4);
+#undef STRIM_Q4
+}
+
+hipError_t launch_q4_logits(const void* x, int64_t x_stride, int B, int K, const uint32_t* words,
+                            int64_t words_stride, const uint16_t* scales, const uint16_t* biases,
+                            int64_t scales_stride, int group, int V, void* workspace, void* out,
+                            bool out_f32, int64_t out_stride, hipStream_t st) {
+  for (int b = 0; b < B; b += 64) {  // the weights are read once per 64 rows
+    Q4Args a{};
+    a.w = Q4Weights{words, words_stride, scales, biases, scales_stride, V, K};
+    a.x = (const uint16_t*)x + (int64_t)b * x_stride;
+    a.x_stride = x_stride;
+    a.B = B - b < 64 ? B - b : 64;
+    a.blocks = (uint8_t*)workspace;
+    a.out = (uint8_t*)out + (int64_t)b * out_stride * (out_f32 ? 4 : 2);
+    a.out_stride = out_stride;
+    a.out_f32 = out_f32;
+    if (group == 32) q4_logits<32>(a, st);
+    else if (group == 64) q4_logits<64>(a, st);
+    else q4_logits<128>(a, st);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_q4_pack(const void* w, bool f32, int64_t w_stride, int V, int K, int group,
+                          uint32_t* words, uint16_t* scales, uint16_t* biases, hipStream_t st) {
+  const Q4Pack a{w, w_stride, V, K, words, scales, biases};
+  const int64_t blocks = ((int64_t)V * (K / 8) + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
+#define STRIM_PACK(G_, F_, S_) hipLaunchKernelGGL((k_q4_pack<G_, F_, S_>), grid, dim3(256), 0, st, a)
+#define STRIM_PACK_G(F_, S_)                \
+  do {                                      \
+    if (group == 32) STRIM_PACK(32, F_, S_); \
+    else if (group == 64) STRIM_PACK(64, F_, S_); \
+    else STRIM_PACK(128, F_, S_);           \
+  } while (0)
+  if (f32 && biases) STRIM_PACK_G(true, false);
+  else if (f32) STRIM_PACK_G(true, true);
+  else if (biases) STRIM_PACK_G(false, false);
+  else STRIM_PACK_G(false, true);
+#undef STRIM_PACK_G
+#undef STRIM_PACK
+  return hipGetLastError();
+}
+
+hipError_t launch_q4_unpack(const uint32_t* words, int64_t words_stride, const uint16_t* scales,
+                            const uint16_t* biases, int64_t scales_stride, int group, int V, int K,
+                            void* out, bool out_f32, int64_t out_stride, hipStream_t st) {
+  const Q4Weights a{words, words_stride, scales, biases, scales_stride, V, K};
+  const int64_t blocks = ((int64_t)V * (K / 8) + 255) / 256;
+  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
+#define STRIM_UNPACK(G_)                                                                          \
+  do {                                                                                            \
+    if (out_f32) hipLaunchKernelGGL((k_q4_unpack<G_, true>), grid, dim3(256), 0, st, a, out, out_stride); \
+    else hipLaunchKernelGGL((k_q4_unpack<G_, false>), grid, dim3(256), 0, st, a, out, out_stride); \
+  } while (0)
+  if (group == 32) STRIM_UNPACK(32);
+  else if (group == 64) STRIM_UNPACK(64);
+  else STRIM_UNPACK(128);
+#undef STRIM_UNPACK
+  return hipGetLastError();
+}
+
+}  // namespace strim

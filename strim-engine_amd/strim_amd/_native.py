@@ -36,6 +36,13 @@ EXPORTS = (
     "strim_head_logits",
     "strim_head_greedy",
     "strim_draft_argmax",
+    "strim_head_loss_workspace",
+    "strim_head_loss",
+    "strim_head_loss_grad",
+    "strim_pack_weights",
+    "strim_unpack_weights",
+    "strim_head_logits_packed_workspace",
+    "strim_head_logits_packed",
     "strim_profile_begin",
     "strim_profile_end",
     "strim_kernel_name",
@@ -52,6 +59,7 @@ EXPORTS = (
     "strim_request_advance",
 )
 KERNEL_COUNT = 8
+LOSS_MAX_ROWS, LOSS_MAX_STRIDE = 1 << 22, 1 << 20  # strim_head_loss limits
 NOALLOC_MAX_ROWS, NOALLOC_MAX_VOCAB = 32, 262144  # strim_sample_noalloc limits
 
 
@@ -141,6 +149,22 @@ def lib() -> ctypes.CDLL:
                                         I32, P, I64, P, P]
         L.strim_draft_argmax.restype = ctypes.c_int
         L.strim_draft_argmax.argtypes = [P, P, I32, I32, I32, I64, P, P]
+        L.strim_head_loss_workspace.restype = I64
+        L.strim_head_loss_workspace.argtypes = [I32, I32, I32, I32, I32]
+        L.strim_head_loss.restype = ctypes.c_int
+        L.strim_head_loss.argtypes = [P, P, I64, I32, I32, P, I64, I32, P, I32, P, I64, P, P, P]
+        L.strim_head_loss_grad.restype = ctypes.c_int
+        L.strim_head_loss_grad.argtypes = [P, P, I64, I32, I32, P, I64, I32, P, I32, P, P, P, P,
+                                           I64, P, I64, P, I64]
+        L.strim_pack_weights.restype = ctypes.c_int
+        L.strim_pack_weights.argtypes = [P, P, I32, I64, I32, I32, I32, P, P, P]
+        L.strim_unpack_weights.restype = ctypes.c_int
+        L.strim_unpack_weights.argtypes = [P, P, I64, P, P, I64, I32, I32, I32, P, I32, I64]
+        L.strim_head_logits_packed_workspace.restype = I64
+        L.strim_head_logits_packed_workspace.argtypes = [I32, I32]
+        L.strim_head_logits_packed.restype = ctypes.c_int
+        L.strim_head_logits_packed.argtypes = [P, P, I64, I32, I32, P, ctypes.c_float, P, P, I64, P, P,
+                                           I64, I32, I32, P, I64, P, I32, I64]
         L.strim_profile_begin.restype = ctypes.c_int
         L.strim_profile_begin.argtypes = [P, I32]
         L.strim_profile_end.restype = ctypes.c_int

@@ -317,6 +317,186 @@ def head_greedy(ctx: "Context", hidden: torch.Tensor, lm_head: torch.Tensor,
     return ids, status
 
 
+def _check_bf16_rows(name: str, t: torch.Tensor) -> None:
+    """A bf16 operand of the loss: [R, K] with contiguous rows, 16-byte aligned."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError("every tensor argument must be on the GPU")
+    if t.dim() != 2 or (t.shape[0] > 0 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be [rows, K] with contiguous rows")
+
+
+def _same_device(*ts):
+    if len({t.device for t in ts if t is not None}) > 1:
+        raise ValueError("every tensor argument must be on the same GPU")
+
+
+def _loss_args(hidden, lm_head, targets):
+    _check_bf16_rows("hidden", hidden)
+    _check_bf16_rows("lm_head", lm_head)
+    _check_cuda(targets)
+    _same_device(hidden, lm_head, targets)
+    N_, K = hidden.shape
+    V = lm_head.shape[0]
+    if lm_head.shape[1] != K:
+        raise ValueError(f"lm_head is [{V}, {lm_head.shape[1]}], hidden K={K}")
+    if targets.dtype != torch.int32 or tuple(targets.shape) != (N_,):
+        raise ValueError(f"targets must be int32 [{N_}]")
+    return N_, K, V
+
+
+def _workspace(workspace, need: int, device) -> torch.Tensor:
+    if need < 0:
+        raise N.StrimError(need, "workspace size")
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    _check_cuda(workspace)
+    if workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace must hold {need} bytes")
+    return workspace
+
+
+def head_loss_workspace(rows: int, K: int, V: int, want_hidden: bool = False,
+                        want_lm_head: bool = False) -> int:
+    """Bytes of workspace that head_loss (no gradient wanted) or head_loss_grad takes."""
+    need = N.lib().strim_head_loss_workspace(rows, K, V, int(want_hidden), int(want_lm_head))
+    if need < 0:
+        raise N.StrimError(need, "strim_head_loss_workspace")
+    return need
+
+
+def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor,
+              ignore_index: int = -100, workspace: torch.Tensor | None = None, stream=None):
+    """Cross entropy of hidden bf16 [N, K] projected by lm_head bf16 [V, K] against targets
+    int32 [N], without keeping the logits. Returns (loss float32 [N], lse float32 [N], status
+    int32 [N]): minus the targets' log-probabilities, the logits' log-sum-exp, and OK, EINVAL
+    (a target outside [0, V) that is not ignore_index) or ENONFINITE. Ignored rows have loss
+    0. strim_amd.loss has the differentiable form."""
+    R, K, V = _loss_args(hidden, lm_head, targets)
+    dev = hidden.device
+    loss, lse = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
+    status = torch.empty(R, dtype=torch.int32, device=dev)
+    ws = _workspace(workspace, N.lib().strim_head_loss_workspace(R, K, V, 0, 0), dev)
+    N.check(N.lib().strim_head_loss(_stream(stream), _ptr(hidden), _row_stride(hidden), R, K,
+                                    _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
+                                    ignore_index, _ptr(ws), ws.numel() * ws.element_size(),
+                                    _ptr(loss), _ptr(lse), _ptr(status)), "strim_head_loss")
+    return loss, lse, status
+
+
+def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor,
+                   lse: torch.Tensor, grad_loss: torch.Tensor,
+                   grad_lse: torch.Tensor | None = None, want_hidden: bool = True,
+                   want_lm_head: bool = True, ignore_index: int = -100,
+                   workspace: torch.Tensor | None = None, stream=None):
+    """Gradients of head_loss: (d_hidden bf16 [N, K] or None, d_lm_head bf16 [V, K] or None)
+    from lse as head_loss gave it and the float32 [N] gradients of its loss and (optional)
+    its lse."""
+    R, K, V = _loss_args(hidden, lm_head, targets)
+    _check_cuda(lse, grad_loss, grad_lse)
+    _same_device(hidden, lse, grad_loss, grad_lse)
+    for t in (lse, grad_loss, grad_lse):
+        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (R,)):
+            raise ValueError(f"lse and the gradients must be float32 [{R}]")
+    dev = hidden.device
+    dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
+    dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
+    if not (want_hidden or want_lm_head):
+        return None, None
+    ws = _workspace(workspace, N.lib().strim_head_loss_workspace(R, K, V, int(want_hidden),
+                                                                 int(want_lm_head)), dev)
+    N.check(N.lib().strim_head_loss_grad(_stream(stream), _ptr(hidden), _row_stride(hidden), R, K,
+                                         _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
+                                         ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(grad_lse),
+                                         _ptr(ws), ws.numel() * ws.element_size(), _ptr(dh), K,
+                                         _ptr(dw), K), "strim_head_loss_grad")
+    return dh, dw
+
+
+class Q4Weight:
+    """A projection [V, K] in 4 bits: words int32 [V, K / 8] (eight codes a word, the lowest
+    bits first), scales bf16 [V, K / group], biases alike or None (symmetric); the element is
+    scale q + bias, or scale (q - 8). The layout of the reference's 4-bit groupwise weights
+    (QGEMV.swift:14-15,68-69)."""
+
+    def __init__(self, words: torch.Tensor, scales: torch.Tensor,
+                 biases: torch.Tensor | None = None, group: int = 64):
+        if words.dtype != torch.int32 or words.dim() != 2:
+            raise ValueError("words must be int32 [V, K / 8]")
+        V, K = words.shape[0], 8 * words.shape[1]
+        if group not in (32, 64, 128) or K % group:
+            raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
+        for t in (scales, biases):
+            if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (V, K // group)):
+                raise ValueError(f"scales and biases must be bfloat16 [{V}, {K // group}]")
+        _check_cuda(words, scales, biases)
+        _same_device(words, scales, biases)
+        self.words, self.scales, self.biases, self.group = words, scales, biases, group
+        self.V, self.K = V, K
+
+
+def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
+            stream=None) -> Q4Weight:
+    """weight [V, K] (bf16 or float32) in 4 bits with a scale (and, unless symmetric, a bias)
+    for every `group` elements of a row."""
+    code = _dtype_code(weight)
+    _check_rows(weight)
+    V, K = weight.shape
+    if group not in (32, 64, 128) or K % group:
+        raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
+    dev = weight.device
+    words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
+    scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
+    biases = None if symmetric else torch.empty_like(scales)
+    N.check(N.lib().strim_pack_weights(_stream(stream), _ptr(weight), code, _row_stride(weight), V,
+                                       K, group, _ptr(words), _ptr(scales), _ptr(biases)),
+            "strim_pack_weights")
+    return Q4Weight(words, scales, biases, group)
+
+
+def q4_unpack(q: Q4Weight, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
+    """The values [V, K] that a packed projection stands for, as bf16 or float32."""
+    out = torch.empty(q.V, q.K, dtype=dtype, device=q.words.device)
+    N.check(N.lib().strim_unpack_weights(_stream(stream), _ptr(q.words), q.K // 8, _ptr(q.scales),
+                                         _ptr(q.biases), q.K // q.group, q.V, q.K, q.group,
+                                         _ptr(out), _dtype_code(out), q.K),
+            "strim_unpack_weights")
+    return out
+
+
+def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor | None = None,
+                   eps: float = 1e-6, out: torch.Tensor | None = None,
+                   out_dtype: torch.dtype = torch.bfloat16, xn: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """head_logits over a projection held in 4 bits: logits [B, V] in bf16 or float32 (or
+    `out`), the layout sample / verify take. Any number of rows."""
+    if hidden.dim() == 1:
+        hidden = hidden.unsqueeze(0)
+    _check_bf16_rows("hidden", hidden)
+    _check_cuda(norm_weight, out, xn)
+    _same_device(hidden, q.words, norm_weight, out, xn)
+    B, K = hidden.shape
+    if K != q.K:
+        raise ValueError(f"the projection has K={q.K}, hidden K={K}")
+    if norm_weight is not None:
+        if norm_weight.dtype != torch.bfloat16 or tuple(norm_weight.shape) != (K,):
+            raise ValueError(f"norm_weight must be bfloat16 [{K}]")
+        if xn is None:
+            xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
+    if out is None:
+        out = torch.empty(B, q.V, dtype=out_dtype, device=hidden.device)
+    elif tuple(out.shape) != (B, q.V):
+        raise ValueError(f"out must be [{B}, {q.V}]")
+    ws = _workspace(workspace, N.lib().strim_head_logits_packed_workspace(B, K), hidden.device)
+    N.check(N.lib().strim_head_logits_packed(
+        _stream(stream), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), float(eps),
+        _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
+        q.V, _ptr(ws), ws.numel() * ws.element_size(), _ptr(out), _dtype_code(out), q.V),
+        "strim_head_logits_packed")
+    return out
+
+
 def draft_argmax(draft_logits: torch.Tensor, draft_to_full: torch.Tensor | None = None,
                  stream=None):
     """MTP.nextTokenIndex (MTP.swift:104-111): table[argmax(draft logits)] per row."""
