@@ -293,9 +293,10 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
  * aligned).
  * strim_head_logits_packed is strim_head_logits over such a projection: hidden, norm_weight, eps
  * and xn as there, any B >= 1 (the weights are read once per 64 rows), logits as dtype (bf16 or
- * float32, what strim_sample takes), accumulated in float32 from the exact s q + b. words and
+ * float32, what strim_sample takes), V up to STRIM_PACKED_MAX_VOCAB, accumulated in float32 from the exact s q + b. words and
  * its stride 16-byte aligned; workspace device, 16-byte aligned, of
  * strim_head_logits_packed_workspace's bytes (else STRIM_ECAPACITY). */
+#define STRIM_PACKED_MAX_VOCAB (1 << 24)
 int strim_pack_weights(void* stream, const void* weight, int32_t dtype, int64_t weight_stride, int32_t V,
                   int32_t K, int32_t group, uint32_t* words, void* scales, void* biases);
 int strim_unpack_weights(void* stream, const uint32_t* words, int64_t words_stride, const void* scales,

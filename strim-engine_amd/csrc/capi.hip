@@ -842,7 +842,7 @@ int strim_head_logits_packed(void* stream, const void* hidden, int64_t hidden_st
                          const void* biases, int64_t scales_stride, int32_t group, int32_t V,
                          void* workspace, int64_t workspace_bytes, void* out_logits, int32_t dtype,
                          int64_t out_stride) {
-  if (!hidden || !words || !scales || !out_logits || !workspace || B < 1 || V <= 0 ||
+  if (!hidden || !words || !scales || !out_logits || !workspace || B < 1 || V <= 0 || V > STRIM_PACKED_MAX_VOCAB ||
       !group_ok(K, group) || !dtype_ok(dtype) || hidden_stride < K || hidden_stride % 8 != 0 ||
       !al16(hidden) || words_stride < K / 8 || words_stride % 4 != 0 || !al16(words) ||
       scales_stride < K / group || out_stride < V || !(eps >= 0.0f) || !al16(workspace))

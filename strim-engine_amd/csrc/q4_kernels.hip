@@ -176,16 +176,25 @@ __device__ __forceinline__ void q4_order(const qu32x4& w, uint32_t* o) {
   }
 }
 
+// The masks of q4_codes, in registers that the compiler does not know the values of: an
+// instruction takes one literal, so that with known ones it makes two of each AND-OR.
+struct Q4Masks {
+  uint32_t codes, sixteen;
+  __device__ __forceinline__ Q4Masks() {
+    asm volatile("s_mov_b32 %0, 0x00780078" : "=s"(codes));
+    asm volatile("v_mov_b32 %0, 0x41804180" : "=v"(sixteen));
+  }
+};
+
 // 16 + q of a word's codes, in the order 0 4 1 5 2 6 3 7
-__device__ __forceinline__ qbf16x8 q4_codes(uint32_t w) {
-  constexpr uint32_t M = 0x00780078u, O = 0x41804180u;
-  const qu32x4 r = {((w << 3) & M) | O, ((w >> 1) & M) | O, ((w >> 5) & M) | O, ((w >> 9) & M) | O};
+__device__ __forceinline__ qbf16x8 q4_codes(uint32_t w, const Q4Masks& k) {
+  const qu32x4 r = {((w << 3) & k.codes) | k.sixteen, ((w >> 1) & k.codes) | k.sixteen,
+                    ((w >> 5) & k.codes) | k.sixteen, ((w >> 9) & k.codes) | k.sixteen};
   return __builtin_bit_cast(qbf16x8, r);
 }
 
 // eight elements of a hidden row in that order
-__device__ __forceinline__ qu32x4 q4_xfrag(const uint16_t* p) {
-  const qu32x4 d = *(const qu32x4*)p;
+__device__ __forceinline__ qu32x4 q4_interleave(const qu32x4& d) {
   return qu32x4{__builtin_amdgcn_perm(d[2], d[0], 0x05040100u), __builtin_amdgcn_perm(d[2], d[0], 0x07060302u),
                 __builtin_amdgcn_perm(d[3], d[1], 0x05040100u), __builtin_amdgcn_perm(d[3], d[1], 0x07060302u)};
 }
@@ -234,12 +243,420 @@ __global__ __launch_bounds__(WAVE) void k_q4_blocks(const Q4Args a) {
       for (int q = 0; q < MPG; ++q) {
         const int t = g * MPG + q, k = step * 128 + q4_koff<G>(t, h);
         qu32x4 x = {0u, 0u, 0u, 0u};
-        if (b < a.B && k < a.w.K) x = q4_xfrag(a.x + (int64_t)b * a.x_stride + k);
+        if (b < a.B && k < a.w.K) x = q4_interleave(*(const qu32x4*)(a.x + (int64_t)b * a.x_stride + k));
         *(qu32x4*)(blk + (t * NT + nt) * 1024 + lane * 16) = x;
         s = q4_sum(x, s);
       }
       if (m == 0) *(qf32x4*)(blk + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4) = s;
     }
+  }
+}
+
+// Few rows: every workgroup keeps the hidden rows' fragments and sums X in LDS, whole, and its
+// waves read their weights without meeting. A unit is four steps of a row tile; the workgroup's
+// row tiles are one run of units, cut evenly between the waves, so a wave has whole tiles and at
+// most a piece at either end. The pieces are added through LDS at the end, in the order of the
+// waves. RB: result registers a lane that hold rows (1, 2 or 4 for up to 4, 8, 16 rows). D:
+// units in flight. WHOLE: K a multiple of a unit's 512; otherwise K of 8 groups or more.
+//
+// What bounds it is the address unit: lanes of one 16-byte load that are neighbours are in
+// different rows, so each lane's piece is looked up by itself, 16 bytes a cycle. A unit's scales
+// and biases therefore come by one such load (even quarters the scales, odd ones the biases,
+// exchanged between the quarters afterwards) and not by one a step: with those this kernel took
+// 178 us for one row at V = 151,936, K = 5,120, groups of 64.
+constexpr int QS_NW = 16;
+constexpr size_t QS_LDS = 160 * 1024;
+
+template <int G, int RB>
+constexpr int q4_step_bytes() {
+  return 4 * 4 * 4 * RB * 16 + (128 / G) * 4 * RB * 4;  // fragments, then the sums
+}
+
+typedef uint32_t qu32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t qu32x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int G, int RB, int D, bool WHOLE>
+__global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_stream(const Q4Args a, int tiles) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, ROWS = 4 * RB;
+  constexpr int SW = G == 128 ? 2 : 4;  // words of scales a lane loads
+  extern __shared__ __attribute__((aligned(16))) uint8_t s_all[];
+  const int lane = threadIdx.x & (WAVE - 1), wv = wave_id(), h = lane >> 4, r16 = lane & 15;
+  const int units = (a.w.K + 511) / 512, groups = a.w.K / G, pieces = a.w.K / 32;
+  uint8_t* s_x = s_all;                                        // [step][MFMA][quarter][row] 16 B
+  float* s_xs = (float*)(s_all + units * 4 * (16 * ROWS * 16));  // [group][row]
+  float* s_part = s_xs + units * 4 * GPS * ROWS;               // [wave][2][RB][64]
+  // this workgroup's tiles, and this wave's units of their run
+  const int t0 = (int)((int64_t)blockIdx.x * tiles / gridDim.x);
+  const int run = ((int)((int64_t)(blockIdx.x + 1) * tiles / gridDim.x) - t0) * units;
+  const int first = run * wv / QS_NW, last = run * (wv + 1) / QS_NW;
+
+  struct Unit {
+    qu32x4 w[4];
+    uint32_t s[SW];
+  } buf[D];
+  const bool sym = a.w.biases == nullptr;
+  const uint16_t* side = (h & 1) && !sym ? a.w.biases : a.w.scales;
+  // groups of 32: the upper quarters take a unit's second eight
+  const int sofs = G == 32 ? 8 * (h >> 1) : 0;
+  int lt = t0 + first / units, lu = first % units, at = first;  // the next request
+  const uint32_t* wp;
+  const uint16_t* sp;
+  auto row = [&]() {
+    const int v = min(lt * 16 + r16, a.w.V - 1);
+    wp = a.w.words + (int64_t)v * a.w.words_stride + 64 * lu + 4 * h;
+    sp = side + (int64_t)v * a.w.scales_stride + lu * 4 * GPS + sofs;
+  };
+  auto load = [&](Unit& u) {  // past the run's end: the last unit again
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      u.w[p] = *(const qu32x4*)(wp + (WHOLE ? 16 * p : min(16 * p, 4 * (pieces - 1 - 16 * lu - h))));
+    const uint16_t* from = sp;
+    // not past the row: an earlier run of scales, moved into place
+    const int back = WHOLE ? 0 : max(0, lu * 4 * GPS + sofs + 2 * SW - groups);
+    if constexpr (!WHOLE) from -= back;
+    if constexpr (SW == 2) {
+      const qu32x2u v = *(const qu32x2u*)from;
+      u.s[0] = v[0], u.s[1] = v[1];
+    } else {
+      const qu32x4u v = *(const qu32x4u*)from;
+      u.s[0] = v[0], u.s[1] = v[1], u.s[2] = v[2], u.s[3] = v[3];
+    }
+    if (++at < last) {
+      wp += 64, sp += 4 * GPS;
+      if (++lu == units) lu = 0, ++lt, row();
+    }
+  };
+  row();
+  if (first < last) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(buf[d]);
+  }
+
+  // the hidden rows: lane = (quarter, place) of a step's four MFMAs
+  for (int st = wv; st < units * 4; st += QS_NW) {
+    const int m = r16, b = (m >> 2) + 4 * (m & (RB - 1));  // (the other places repeat these)
+    const uint16_t* xr = a.x + (int64_t)min(b, a.B - 1) * a.x_stride;
+    qu32x4 x[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = *(const qu32x4*)(xr + min(st * 128 + q4_koff<G>(t, h), a.w.K - 8));
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bool in = b < a.B && st * 128 + q4_koff<G>(t, h) < a.w.K;
+      x[t] = q4_interleave(x[t]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = in ? x[t][e] : 0u;
+      if ((m & 3) < RB) *(qu32x4*)(s_x + ((st * 4 + t) * 4 + h) * ROWS * 16 + b * 16) = x[t];
+    }
+#pragma unroll
+    for (int g = 0; g < GPS; ++g) {
+      qf32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < MPG; ++q) s = q4_sum(x[g * MPG + q], s);
+      if (r16 == 0)
+#pragma unroll
+        for (int r = 0; r < RB; ++r) s_xs[(st * GPS + g) * ROWS + h + 4 * r] = s[r];
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+  const Q4Masks masks;
+  const uint32_t keepb = sym ? 0u : 0xFFFFFFFFu;  // symmetric: no biases, and 8 less
+  const float zero = sym ? -24.0f : -16.0f;
+  const uint32_t xat = (uint32_t)(h * ROWS + (r16 >> 2) + 4 * (r16 & (RB - 1))) * 16;
+  float acc[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) acc[r] = 0.0f;
+  int ct = t0 + first / units, cu = first % units, from = cu, piece = 0;
+  // lane: weight row r16 of the tile, rows h + 4 r
+  auto finish = [&](bool whole) {
+    const int v = ct * 16 + r16;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      if (!whole) s_part[((wv * 2 + piece) * RB + r) * WAVE + lane] = acc[r];
+      else if (v < a.w.V && h + 4 * r < a.B) q4_store(a, h + 4 * r, v, acc[r]);
+      acc[r] = 0.0f;
+    }
+    piece = 1;
+  };
+  auto compute = [&](Unit& u) {
+    if constexpr (!WHOLE) {  // the scales moved back for want of room move into place
+      const int back = max(0, cu * 4 * GPS + sofs + 2 * SW - groups);
+#pragma unroll
+      for (int d = SW / 2; d > 0; d /= 2)  // by d words
+#pragma unroll
+        for (int e = 0; e < SW; ++e)
+          u.s[e] = back & (2 * d) ? (e + d < SW ? u.s[e + d] : 0u) : u.s[e];
+      const bool whole_words = back >= 2 * SW;
+#pragma unroll
+      for (int e = 0; e < SW; ++e) {
+        const uint32_t half = (u.s[e] >> 16) | (e + 1 < SW ? u.s[e + 1] << 16 : 0u);
+        u.s[e] = whole_words ? 0u : back & 1 ? half : u.s[e];
+      }
+    }
+    uint32_t sw[2 * GPS], bw[2 * GPS];  // the unit's scales and biases, in every quarter
+#pragma unroll
+    for (int e = 0; e < SW; ++e) {
+      uint32_t s0 = u.s[e], b0 = u.s[e];
+      q4_swap16(s0, b0);
+      if constexpr (G == 32) {
+        uint32_t s1 = s0, b1 = b0;
+        q4_swap32(s0, s1);
+        q4_swap32(b0, b1);
+        sw[4 + e] = s1, bw[4 + e] = b1;
+      }
+      sw[e] = s0, bw[e] = b0;
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      uint32_t w[4];
+      q4_order<G>(u.w[p], w);
+#pragma unroll
+      for (int g = 0; g < GPS; ++g) {
+        const int i = p * GPS + g;
+        const float sc = __uint_as_float(i & 1 ? sw[i / 2] & 0xFFFF0000u : sw[i / 2] << 16);
+        const float bi = __uint_as_float((i & 1 ? bw[i / 2] & 0xFFFF0000u : bw[i / 2] << 16) & keepb);
+        const float off = __builtin_fmaf(zero, sc, bi);
+        qf32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < MPG; ++q) {
+          const int m = g * MPG + q;
+          const qu32x4 x = *(const qu32x4*)(s_x + ((cu * 4 + p) * 4 + m) * (4 * ROWS * 16) + xat);
+          t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x),
+                                                      q4_codes(w[m], masks), t, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const float xs = s_xs[((cu * 4 + p) * GPS + g) * ROWS + h + 4 * r];
+          acc[r] = __builtin_fmaf(sc, t[r], __builtin_fmaf(off, xs, acc[r]));
+        }
+      }
+    }
+    if (++cu == units) {
+      finish(from == 0);
+      cu = from = 0;
+      ++ct;
+    }
+  };
+  for (int i = first; i < last; i += D) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (i + d >= last) goto done;
+      compute(buf[d]);
+      load(buf[d]);
+    }
+  }
+done:
+  if (cu != from) finish(false);
+  __syncthreads();
+  // tiles that more than one wave has units of
+  for (int t = wv; t * units < run; t += QS_NW) {
+    const int b0 = t * units, b1 = b0 + units;  // its part of the run
+    int w0 = (int)((int64_t)b0 * QS_NW / run);
+    while (run * (w0 + 1) / QS_NW <= b0) ++w0;
+    if (run * (w0 + 1) / QS_NW >= b1 && run * w0 / QS_NW <= b0) continue;
+    float y[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) y[r] = 0.0f;
+    for (int w = w0; w < QS_NW && run * w / QS_NW < b1; ++w) {
+      if (run * (w + 1) / QS_NW == run * w / QS_NW) continue;
+      const int p = run * w / QS_NW / units == t ? 0 : 1;  // the wave's first tile, or its last
+#pragma unroll
+      for (int r = 0; r < RB; ++r) y[r] += s_part[((w * 2 + p) * RB + r) * WAVE + lane];
+    }
+    const int v = (t0 + t) * 16 + r16;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+      if (v < a.w.V && h + 4 * r < a.B) q4_store(a, h + 4 * r, v, y[r]);
+  }
+}
+
+// 64 lanes' 16 bytes each, straight to LDS from `lds` (the same in every lane) in lane order.
+// ONCE: the lines are not read again.
+template <bool ONCE>
+__device__ __forceinline__ void q4_load_lds(uint32_t lds, const void* p) {
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+                 ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p) : "memory");
+}
+
+template <int G, int RB, bool WHOLE>
+__global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int tiles) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, ROWS = 4 * RB;
+  constexpr int GPW = G == 32 ? 8 : 4 * GPS;  // groups a lane's scale load is wanted for
+  constexpr int UNIT = 5 * 1024;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t s_all[];
+  const int lane = threadIdx.x & (WAVE - 1), wv = wave_id(), h = lane >> 4, r16 = lane & 15;
+  const int nw = blockDim.x / WAVE;
+  const int units = (a.w.K + 511) / 512, groups = a.w.K / G, pieces = a.w.K / 32;
+  uint8_t* s_w = s_all + wv * 2 * UNIT;                        // this wave's two units
+  uint8_t* s_x = s_all + nw * 2 * UNIT;                        // [step][MFMA][quarter][row] 16 B
+  float* s_xs = (float*)(s_x + units * 4 * (16 * ROWS * 16));  // [group][row]
+  float* s_part = (float*)s_all;                               // at the end: [wave][2][RB][64]
+  const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_w;
+  // this workgroup's tiles, and this wave's units of their run
+  const int t0 = (int)((int64_t)blockIdx.x * tiles / gridDim.x);
+  const int run = ((int)((int64_t)(blockIdx.x + 1) * tiles / gridDim.x) - t0) * units;
+  const int first = run * wv / nw, last = run * (wv + 1) / nw;
+
+  const bool sym = a.w.biases == nullptr;
+  const uint16_t* side = (h & 1) && !sym ? a.w.biases : a.w.scales;
+  const int sofs = G == 32 ? 8 * (h >> 1) : 0;  // the upper quarters: a unit's second eight
+  int lt = t0 + first / units, lu = first % units;  // the next request
+  auto load = [&](int slot) {
+    const int v0 = lt * 16, most = a.w.V - 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // four rows, 256 bytes of each
+      const int r = 4 * j + h, c = 16 * lu + (r16 ^ r);
+      q4_load_lds<true>(ring + slot * UNIT + j * 1024,
+                  a.w.words + (int64_t)min(v0 + r, most) * a.w.words_stride +
+                      4 * (WHOLE ? c : min(c, pieces - 1)));
+    }
+    const int g0 = lu * 4 * GPS + sofs;
+    q4_load_lds<false>(ring + slot * UNIT + 4096, side + (int64_t)min(v0 + r16, most) * a.w.scales_stride +
+                                               min(g0, groups - 8));
+    if (++lu == units) lu = 0, ++lt;
+  };
+  if (first < last) load(0);
+  if (first + 1 < last) load(1);
+
+  // the hidden rows: lane = (quarter, place) of a step's four MFMAs
+  for (int st = wv; st < units * 4; st += nw) {
+    const int m = r16, b = (m >> 2) + 4 * (m & (RB - 1));  // (the other places repeat these)
+    const uint16_t* xr = a.x + (int64_t)min(b, a.B - 1) * a.x_stride;
+    qu32x4 x[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = *(const qu32x4*)(xr + min(st * 128 + q4_koff<G>(t, h), a.w.K - 8));
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const bool in = b < a.B && st * 128 + q4_koff<G>(t, h) < a.w.K;
+      x[t] = q4_interleave(x[t]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][e] = in ? x[t][e] : 0u;
+      if ((m & 3) < RB) *(qu32x4*)(s_x + ((st * 4 + t) * 4 + h) * ROWS * 16 + b * 16) = x[t];
+    }
+#pragma unroll
+    for (int g = 0; g < GPS; ++g) {
+      qf32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < MPG; ++q) s = q4_sum(x[g * MPG + q], s);
+      if (r16 == 0)
+#pragma unroll
+        for (int r = 0; r < RB; ++r) s_xs[(st * GPS + g) * ROWS + h + 4 * r] = s[r];
+    }
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+  const Q4Masks masks;
+  const uint32_t keepb = sym ? 0u : 0xFFFFFFFFu;  // symmetric: no biases, and 8 less
+  const float zero = sym ? -24.0f : -16.0f;
+  const uint32_t xat = (uint32_t)(h * ROWS + (r16 >> 2) + 4 * (r16 & (RB - 1))) * 16;
+  float acc[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) acc[r] = 0.0f;
+  float part[2][RB];  // pieces of the wave's first and last tile
+  int ct = t0 + first / units, cu = first % units, from = cu, piece = 0;
+  // lane: weight row r16 of the tile, rows h + 4 r
+  auto finish = [&](bool whole) {
+    const int v = ct * 16 + r16;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) {
+      if (!whole) part[piece][r] = acc[r];
+      else if (v < a.w.V && h + 4 * r < a.B) q4_store(a, h + 4 * r, v, acc[r]);
+      acc[r] = 0.0f;
+    }
+    piece = 1;
+  };
+  for (int i = first, slot = 0; i < last; ++i, slot ^= 1) {
+    if (i + 1 < last) asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    const uint8_t* u = s_w + slot * UNIT;
+    qu32x4 wd[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) wd[p] = *(const qu32x4*)(u + r16 * 256 + (((4 * p + h) ^ r16) << 4));
+    constexpr int SW = GPW / 2;  // words of scales from one lane's load
+    uint32_t sw[2 * GPS], bw[2 * GPS];
+#pragma unroll
+    for (int half = 0; half < 2 * GPS / SW; ++half) {
+      const uint32_t* sp = (const uint32_t*)(u + 4096 + (half * 32 + r16) * 16);
+      if constexpr (WHOLE && SW == 4) {
+        const qu32x4 s4 = *(const qu32x4*)sp, b4 = *(const qu32x4*)(sp + 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sw[4 * half + e] = s4[e], bw[4 * half + e] = b4[e];
+      } else {
+        // a load that would pass the row's end began earlier
+        const int g0 = cu * 4 * GPS + 8 * half, back = max(0, g0 + 8 - groups) / 2;
+#pragma unroll
+        for (int e = 0; e < SW; ++e) {
+          const bool in = g0 + 2 * e < groups;  // (an even number of groups)
+          const uint32_t sv = sp[min(back + e, 3)], bv = sp[64 + min(back + e, 3)];
+          sw[SW * half + e] = in ? sv : 0u;
+          bw[SW * half + e] = in ? bv : 0u;
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      uint32_t w[4];
+      q4_order<G>(wd[p], w);
+#pragma unroll
+      for (int g = 0; g < GPS; ++g) {
+        const int n = p * GPS + g;
+        const float sc = __uint_as_float(n & 1 ? sw[n / 2] & 0xFFFF0000u : sw[n / 2] << 16);
+        const float bi = __uint_as_float((n & 1 ? bw[n / 2] & 0xFFFF0000u : bw[n / 2] << 16) & keepb);
+        const float off = __builtin_fmaf(zero, sc, bi);
+        qf32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < MPG; ++q) {
+          const int m = g * MPG + q;
+          const qu32x4 x = *(const qu32x4*)(s_x + ((cu * 4 + p) * 4 + m) * (4 * ROWS * 16) + xat);
+          t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x),
+                                                      q4_codes(w[m], masks), t, 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < RB; ++r) {
+          const float xs = s_xs[((cu * 4 + p) * GPS + g) * ROWS + h + 4 * r];
+          acc[r] = __builtin_fmaf(sc, t[r], __builtin_fmaf(off, xs, acc[r]));
+        }
+      }
+    }
+    // every read of the slot has returned before it is filled again
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (i + 2 < last) load(slot);
+    if (++cu == units) {
+      finish(from == 0);
+      cu = from = 0;
+      ++ct;
+    }
+  }
+  if (cu != from) finish(false);
+  __syncthreads();  // the ring is free in every wave: it takes the pieces
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+#pragma unroll
+    for (int r = 0; r < RB; ++r) s_part[((wv * 2 + q) * RB + r) * WAVE + lane] = part[q][r];
+  __syncthreads();
+  // tiles that more than one wave has units of
+  for (int t = wv; t * units < run; t += nw) {
+    const int b0 = t * units, b1 = b0 + units;  // its part of the run
+    int w0 = (int)((int64_t)b0 * nw / run);
+    while (run * (w0 + 1) / nw <= b0) ++w0;
+    if (run * (w0 + 1) / nw >= b1 && run * w0 / nw <= b0) continue;
+    float y[RB];
+#pragma unroll
+    for (int r = 0; r < RB; ++r) y[r] = 0.0f;
+    for (int w = w0; w < nw && run * w / nw < b1; ++w) {
+      if (run * (w + 1) / nw == run * w / nw) continue;
+      const int q = run * w / nw / units == t ? 0 : 1;  // the wave's first tile, or its last
+#pragma unroll
+      for (int r = 0; r < RB; ++r) y[r] += s_part[((w * 2 + q) * RB + r) * WAVE + lane];
+    }
+    const int v = (t0 + t) * 16 + r16;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+      if (v < a.w.V && h + 4 * r < a.B) q4_store(a, h + 4 * r, v, y[r]);
   }
 }
 
@@ -249,6 +666,7 @@ __global__ __launch_bounds__(NW* WAVE) void k_q4_stage(const Q4Args a) {
   constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
   __shared__ __attribute__((aligned(1024))) uint8_t s_x[2][BLOCK];
   const int lane = threadIdx.x & (WAVE - 1), wv = wave_id(), h = lane >> 4, r16 = lane & 15;
+  const Q4Masks masks;
   const int v0 = (blockIdx.x * NW + wv) * RT * 16;
   const int steps = (a.w.K + 127) / 128, groups = a.w.K / G, pieces = a.w.K / 32;
   const uint32_t* wrow[RT];
@@ -288,7 +706,7 @@ __global__ __launch_bounds__(NW* WAVE) void k_q4_stage(const Q4Args a) {
           for (int q = 0; q < MPG; ++q) {
             const int m = g * MPG + q;
             const qu32x4 x = *(const qu32x4*)&s_x[0][(m * NT + nt) * 1024 + lane * 16];
-            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), q4_codes(w[m]), t, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), q4_codes(w[m], masks), t, 0, 0, 0);
           }
           const qf32x4 xs = *(const qf32x4*)&s_x[0][4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4];
 #pragma unroll
@@ -319,8 +737,43 @@ int64_t q4_workspace(int B, int K) {
   return ((K + 127) / 128) * (4 * nt + 1) * 1024;
 }
 
+// A launch with more than 64 KB of LDS, which a kernel has to be told of once.
+template <auto KERNEL>
+static bool q4_big_lds(dim3 grid, size_t lds, hipStream_t st, const Q4Args& a, int tiles,
+                       int waves = QS_NW) {
+  static const hipError_t told = hipFuncSetAttribute(
+      (const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)QS_LDS);
+  (void)told;
+  hipLaunchKernelGGL(KERNEL, grid, dim3(waves * WAVE), lds, st, a, tiles);
+  return true;
+}
+
+template <int G, int RB, int D>
+static bool q4_stream(const Q4Args& a, hipStream_t st) {
+  const int steps = (a.w.K + 511) / 512 * 4, tiles = (a.w.V + 15) / 16;
+  const size_t own = (size_t)steps * q4_step_bytes<G, RB>();
+  const bool even = (a.w.K / G) % 2 == 0 && a.w.scales_stride % 2 == 0 && ((uintptr_t)a.w.scales & 3) == 0 &&
+                    ((uintptr_t)a.w.biases & 3) == 0 && a.w.K >= 8 * G;
+  const int nw = own < QS_LDS ? (int)((QS_LDS - own) / 10240) : 0;
+  if (even && nw >= 6) {
+    const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
+    const int w = nw < QS_NW ? nw : QS_NW;
+    const size_t lds = own + (size_t)w * 10240;
+    return a.w.K % 512 == 0 ? q4_big_lds<k_q4_dma<G, RB, true>>(grid, lds, st, a, tiles, w)
+                            : q4_big_lds<k_q4_dma<G, RB, false>>(grid, lds, st, a, tiles, w);
+  }
+  const size_t lds = (size_t)steps * q4_step_bytes<G, RB>() + (size_t)QS_NW * 2 * RB * WAVE * 4;
+  if (lds > QS_LDS || a.w.K < 8 * G) return false;
+  const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
+  return a.w.K % 512 == 0 ? q4_big_lds<k_q4_stream<G, RB, D, true>>(grid, lds, st, a, tiles)
+                          : q4_big_lds<k_q4_stream<G, RB, D, false>>(grid, lds, st, a, tiles);
+}
+
 template <int G>
 static void q4_logits(const Q4Args& a, hipStream_t st) {
+  if (a.B <= 4 && q4_stream<G, 1, 2>(a, st)) return;
+  if (a.B <= 8 && q4_stream<G, 2, 2>(a, st)) return;
+  if (a.B <= 16 && q4_stream<G, 4, 2>(a, st)) return;
   const dim3 steps((unsigned)((a.w.K + 127) / 128)), grid((unsigned)((a.w.V + 127) / 128));
 #define STRIM_Q4(NT_)                                                            \
   do {                                                                           \
