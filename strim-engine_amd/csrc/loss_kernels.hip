@@ -222,31 +222,59 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
 
+  // Two stages in LDS and two halves (32 of a stage's 64) in registers: while a half is
+  // multiplied the next one is read from LDS, so that a stage's first half is read, and the
+  // barrier that says it has arrived passed, before the multiplies of the stage before it are
+  // over. The stage after it is requested into the place that this barrier frees.
+  lbf16x8 af[2][TM], bf[2][TN];
+  auto frags = [&](uint32_t at, int kk) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) bf[kk][j] = fb.get(at + TileA::BYTES, j, kk);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) af[kk][i] = fa.get(at, i, kk);
+  };
+  auto multiply = [&](int kk) {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[kk][i], bf[kk][j], acc[i][j], 0, 0, 0);
+  };
+  // one LDS read to every few multiplies
+  auto interleave = [&]() {
+    constexpr int READS = TM * (ATR ? 2 : 1) + TN * (BTR ? 2 : 1), MUL = TM * TN;
+    constexpr int EACH = MUL / READS > 0 ? MUL / READS : 1;
+#pragma unroll
+    for (int i = 0; i < READS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, MUL, 0);
+  };
   if (steps > 0) {
     ta.load(lds, 0, red);
     tb.load(lds + TileA::BYTES, 0, red);
-  }
-  for (int s = 0; s < steps; ++s) {
-    const uint32_t cur = lds + (uint32_t)((s & 1) * STAGE);
-    const uint32_t nxt = lds + (uint32_t)(((s & 1) ^ 1) * STAGE);
-    // this stage has arrived, and every wave has read the other one
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (s + 1 < steps) {
-      ta.load(nxt, s + 1, red);
-      tb.load(nxt + TileA::BYTES, s + 1, red);
+    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (steps > 1) {
+      ta.load(lds + STAGE, 1, red);
+      tb.load(lds + STAGE + TileA::BYTES, 1, red);
     }
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      lbf16x8 bf[TN], af[TM];
-#pragma unroll
-      for (int j = 0; j < TN; ++j) bf[j] = fb.get(cur + TileA::BYTES, j, kk);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) af[i] = fa.get(cur, i, kk);
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(af[i], bf[j], acc[i][j], 0, 0, 0);
+    frags(lds, 0);
+    for (int s = 0; s < steps; ++s) {
+      const uint32_t cur = lds + (uint32_t)((s & 1) * STAGE);
+      const uint32_t nxt = lds + (uint32_t)(((s & 1) ^ 1) * STAGE);
+      frags(cur, 1);
+      multiply(0);
+      interleave();
+      // the next stage has arrived, and every wave has read this one
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (s + 2 < steps) {
+        ta.load(cur, s + 2, red);
+        tb.load(cur + TileA::BYTES, s + 2, red);
+      }
+      frags(nxt, 0);  // (after the last stage: a stale one, unused)
+      multiply(1);
+      interleave();
     }
   }
 
