@@ -63,14 +63,24 @@ struct LossGemm {
   int32_t accumulate;      // LM_DHID: add to what out32 holds
 };
 
-__device__ __forceinline__ uint32_t loss_bf16(float f) {
-  const uint32_t u = __float_as_uint(f);
-  if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (u >> 16) | 0x0040u;
-  return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+typedef float lf32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 lbf16x2 __attribute__((ext_vector_type(2)));
+
+// Two floats rounded to nearest even, as one word (NaN stays NaN).
+__device__ __forceinline__ uint32_t loss_pack2(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(lf32x2{lo, hi}, lbf16x2));
 }
 __device__ __forceinline__ uint2 loss_pack4(const float* f) {
-  return make_uint2(loss_bf16(f[0]) | (loss_bf16(f[1]) << 16),
-                    loss_bf16(f[2]) | (loss_bf16(f[3]) << 16));
+  return make_uint2(loss_pack2(f[0], f[1]), loss_pack2(f[2], f[3]));
+}
+
+// Words of two neighbouring 16 x 16 tiles, four rows (two words) a lane each, exchanged so that
+// a lane has eight rows of one of them: even quarters of the wave the first tile's rows 8 (h / 2)
+// .. + 7, odd ones the second's.
+__device__ __forceinline__ uint4 loss_join8(uint2 a, uint2 b) {
+  const auto x = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
+  const auto y = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+  return make_uint4(x[0], y[0], x[1], y[1]);
 }
 
 __device__ __forceinline__ float loss_exp(float x) {
@@ -280,23 +290,39 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
 
   // lane l holds C[row 4 (l / 16) + r][column l % 16] of each 16 x 16 tile
   const int h = lane >> 4, c16 = lane & 15;
-  const int m0 = tm * BM + wm * TM * 16 + 4 * h;
+  const int mw = tm * BM + wm * TM * 16, m0 = mw + 4 * h;
   const int n0 = tn * BN + wn * TN * 16 + c16;
+  // bf16 results of column `row` (rows of `out` run along the M side): sixteen bytes a lane
+  const int mh = mw + 16 * (h & 1) + 8 * (h >> 1);
+  auto store = [&](uint16_t* out, int i, uint2 a, uint2 b, int valid) {
+    const uint4 q = loss_join8(a, b);
+    if (mh + 16 * i < valid) *(uint4*)(out + mh + 16 * i) = q;
+  };
+  static_assert(TM % 2 == 0, "tiles are stored by twos");
   if constexpr (MODE == LM_STATS) {
+    if (mw + TM * 16 > g.V) {  // past the vocabulary: nothing
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (m0 + 16 * i + r >= g.V)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j][r] = -INFINITY;
+    }
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + 16 * j;
       const int t = n < g.b.rows ? g.targets[n] : -1;
+      const int at = t < g.V ? t - m0 : -1;  // the target's place among this lane's rows
       float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i) {
+        if (at >= 16 * i && at < 16 * i + 4)
+          g.tlogit[n] = at == 16 * i ? acc[i][j][0] : at == 16 * i + 1 ? acc[i][j][1]
+                        : at == 16 * i + 2 ? acc[i][j][2] : acc[i][j][3];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int v = m0 + 16 * i + r;
-          if (v == t && v < g.V) g.tlogit[n] = acc[i][j][r];
-          if (v >= g.V) acc[i][j][r] = -INFINITY;
-          mx = fmaxf(mx, acc[i][j][r]);
-        }
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
+      }
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
       const float ref = mx == -INFINITY ? 0.0f : mx;  // a slice of -inf alone adds nothing
@@ -313,24 +339,31 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
   } else if constexpr (MODE == LM_PROB) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = n0 + 16 * j;
-      if (n >= g.b.rows) continue;
+      const int n = min(n0 + 16 * j, g.b.rows - 1);
       const int t = g.targets[n];
       const bool live = t != g.ignore_index && t >= 0 && t < g.V;
       const float gl = live ? g.grad_loss[n] : 0.0f;
       const float top = live && g.grad_lse ? gl + g.grad_lse[n] : gl;
       const float lse = g.lse[n];
+      const uint32_t keep = live ? 0xFFFFFFFFu : 0u;  // whatever a dead row holds (a NaN too)
+      const int at = t - g.v0 - m0;                    // the target's place among this lane's rows
+      uint2 w[TM];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         float p[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int v = g.v0 + m0 + 16 * i + r;
-          const float y = top * loss_exp(acc[i][j][r] - lse) - (v == t ? gl : 0.0f);
-          p[r] = live && v < g.V ? y : 0.0f;
-        }
-        *(uint2*)(g.out16 + (int64_t)n * g.out_stride + m0 + 16 * i) = loss_pack4(p);
+        for (int r = 0; r < 4; ++r) p[r] = top * loss_exp(acc[i][j][r] - lse);
+        if (at >= 16 * i && at < 16 * i + 4)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) p[r] -= at == 16 * i + r ? gl : 0.0f;
+        w[i] = loss_pack4(p);
+        w[i].x &= keep, w[i].y &= keep;
       }
+      // (columns past the vocabulary are inside the row, and read by nothing)
+      if (n0 + 16 * j < g.b.rows)
+#pragma unroll
+        for (int i = 0; i < TM; i += 2)
+          store(g.out16 + (int64_t)n * g.out_stride, i, w[i], w[i + 1], (int)g.out_stride);
     }
   } else if constexpr (MODE == LM_DHID) {
     float* out = g.out32 + (int64_t)split * g.b.rows * g.out_stride;
@@ -350,18 +383,19 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int v = n0 + 16 * j;
-      if (v >= g.b.rows) continue;
+      uint2 w[TM];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const int k = m0 + 16 * i;
-        if (k >= g.a.rows) continue;
         const float f[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        *(uint2*)(g.out16 + (int64_t)v * g.out_stride + k) = loss_pack4(f);
+        w[i] = loss_pack4(f);
       }
+      if (v < g.b.rows)
+#pragma unroll
+        for (int i = 0; i < TM; i += 2)
+          store(g.out16 + (int64_t)v * g.out_stride, i, w[i], w[i + 1], g.a.rows);
     }
   }
 }
-
 
 // Merges two (max, sum exp(x - max)) pairs; a max of -inf carries no sum.
 __device__ __forceinline__ void loss_merge(float& m, float& s, float m2, float s2) {
@@ -382,10 +416,23 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2* part, int slice
   const int tok = threadIdx.x % TOK, w = threadIdx.x / TOK;
   const int n = blockIdx.x * TOK + tok;
   float m = -INFINITY, s = 0.0f;
+  constexpr int U = 8;  // slices requested together
   if (n < N)
-    for (int q = w; q < slices; q += W) {
-      const float2 p = part[(int64_t)q * N + n];
-      loss_merge(m, s, p.x, p.y);
+    for (int q = w; q < slices; q += U * W) {
+      float2 p[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) p[u] = part[(int64_t)min(q + u * W, slices - 1) * N + n];
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (q + u * W >= slices) p[u] = make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, p[u].x);
+      }
+      const float ref = top == -INFINITY ? 0.0f : top;
+      s *= loss_exp(m - ref);
+#pragma unroll
+      for (int u = 0; u < U; ++u) s += p[u].y * loss_exp(p[u].x - ref);
+      m = top;
     }
   s_p[w][tok] = make_float2(m, s);
   for (int d = W / 2; d > 0; d >>= 1) {
