@@ -200,27 +200,33 @@ __device__ __forceinline__ void loss_tile(int tiles_m, int tiles_n, int splits, 
   tm = r / wide;
 }
 
-template <int MODE, int WM, int WN, int TM, int TN>
+// WM x WN waves of TM x TN tiles of 16 x 16; R stages in LDS.
+template <int MODE, int WM, int WN, int TM, int TN, int R>
 __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g) {
   constexpr bool ATR = MODE == LM_DHID || MODE == LM_DHEAD, BTR = MODE == LM_DHEAD;
   constexpr int NW = WM * WN, BM = WM * TM * 16, BN = WN * TN * 16;
   typedef LossTile<ATR, BM, NW> TileA;
   typedef LossTile<BTR, BN, NW> TileB;
-  constexpr int STAGE = TileA::BYTES + TileB::BYTES;
-  __shared__ __attribute__((aligned(1024))) uint8_t s_buf[2 * STAGE];
+  constexpr int STAGE = TileA::BYTES + TileB::BYTES, LOADS = TileA::NI + TileB::NI;
+  __shared__ __attribute__((aligned(1024))) uint8_t s_buf[R * STAGE];
   const uint32_t lds = (uint32_t)(uintptr_t)(lds_u8*)s_buf;
   const int lane = threadIdx.x & (WAVE - 1), wv = wave_id();
   const int wm = wv / WN, wn = wv % WN;
   int tm, tn, split;
   loss_tile(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
-  const int red0 = split * g.split_red;
-  const int red = max(0, min(g.split_red, g.red - red0));
+  const int red0 = split * g.split_red, red = max(0, min(g.split_red, g.red - red0));
   const int steps = (red + LG_BK - 1) / LG_BK;
-
   TileA ta;
   TileB tb;
   ta.init(g.a, tm * BM, red0, wv, lane);
   tb.init(g.b, tn * BN, red0, wv, lane);
+  auto request = [&](uint32_t at, int s) {
+    ta.load(at, s, red);
+    tb.load(at + TileA::BYTES, s, red);
+  };
+  // (past the reduction's end zeros are requested: the count of open requests is fixed)
+#pragma unroll
+  for (int s = 0; s < R; ++s) request(lds + s * STAGE, s);
   LossFrag<ATR, BM> fa;
   LossFrag<BTR, BN> fb;
   fa.init(wm * TM, lane);
@@ -232,10 +238,10 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = lf32x4{0.f, 0.f, 0.f, 0.f};
 
-  // Two stages in LDS and two halves (32 of a stage's 64) in registers: while a half is
+  // R stages in LDS and two halves (32 of a stage's 64) in registers: while a half is
   // multiplied the next one is read from LDS, so that a stage's first half is read, and the
   // barrier that says it has arrived passed, before the multiplies of the stage before it are
-  // over. The stage after it is requested into the place that this barrier frees.
+  // over. The stage R after one is requested into the place that this barrier frees.
   lbf16x8 af[2][TM], bf[2][TN];
   auto frags = [&](uint32_t at, int kk) {
 #pragma unroll
@@ -261,32 +267,23 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
     }
     __builtin_amdgcn_sched_group_barrier(0x008, MUL, 0);
   };
-  if (steps > 0) {
-    ta.load(lds, 0, red);
-    tb.load(lds + TileA::BYTES, 0, red);
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    if (steps > 1) {
-      ta.load(lds + STAGE, 1, red);
-      tb.load(lds + STAGE + TileA::BYTES, 1, red);
-    }
-    frags(lds, 0);
-    for (int s = 0; s < steps; ++s) {
-      const uint32_t cur = lds + (uint32_t)((s & 1) * STAGE);
-      const uint32_t nxt = lds + (uint32_t)(((s & 1) ^ 1) * STAGE);
-      frags(cur, 1);
-      multiply(0);
-      interleave();
-      // the next stage has arrived, and every wave has read this one
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (s + 2 < steps) {
-        ta.load(cur, s + 2, red);
-        tb.load(cur + TileA::BYTES, s + 2, red);
-      }
-      frags(nxt, 0);  // (after the last stage: a stale one, unused)
-      multiply(1);
-      interleave();
-    }
+  uint32_t cur = lds;
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((R - 1) * LOADS) : "memory");
+  frags(cur, 0);
+  for (int s = 0; s < steps; ++s) {
+    const uint32_t nxt = cur == lds + (R - 1) * STAGE ? lds : cur + STAGE;
+    frags(cur, 1);
+    multiply(0);
+    interleave();
+    // the next stage has arrived, and every wave has read this one
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R - 2) * LOADS) : "memory");
+    if (R > 2 || s + R < steps) request(cur, s + R);
+    frags(nxt, 0);  // (after the last stage: zeros, unused)
+    multiply(1);
+    interleave();
+    cur = nxt;
   }
+  if (R > 2) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (none left open)
 
   // lane l holds C[row 4 (l / 16) + r][column l % 16] of each 16 x 16 tile
   const int h = lane >> 4, c16 = lane & 15;
@@ -491,8 +488,44 @@ constexpr int64_t LOSS_P_BYTES = (int64_t)512 << 20;  // p of one vocabulary pie
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t up256(int64_t b) { return (b + 255) & ~(int64_t)255; }
 
+enum LossShape { LS_256x256, LS_256x128, LS_256x64, LS_128x128, LS_128x64 };
+static int shape_m(LossShape s) { return s == LS_128x128 || s == LS_128x64 ? 128 : 256; }
+static int shape_n(LossShape s) {
+  return s == LS_256x256 ? 256 : s == LS_256x64 || s == LS_128x64 ? 64 : 128;
+}
+// rows of the M side that one wave has (its vocabulary slice in LM_STATS)
+static int shape_slice(LossShape s) {
+  return s == LS_256x256 ? 128 : s == LS_128x64 || s == LS_256x64 ? 32 : 64;
+}
+static int64_t loss_slices(int V, LossShape s) {
+  return ceil_div(V, shape_m(s)) * (shape_m(s) / shape_slice(s));
+}
+// about how long a step (64 along the reduction) of a CU's round of tiles takes, us, and how
+// many tiles a round has
+static double shape_us(LossShape s) {
+  return s == LS_256x256 ? 1.7 : s == LS_256x128 ? 1.0 : s == LS_256x64 ? 0.7 : s == LS_128x128 ? 1.1 : 0.7;
+}
+static int64_t shape_round(LossShape s) { return shape_m(s) == 128 ? 2 * LG_CUS : LG_CUS; }
+
+// The tile for an M x N result, `splits` times over: the one whose rounds take least.
+static LossShape loss_shape(int64_t m, int64_t n, int64_t splits, bool head) {
+  LossShape best = LS_256x256;
+  double least = 1e30;
+  for (LossShape s : {LS_256x256, LS_256x128, LS_256x64, LS_128x128, LS_128x64}) {
+    if (head && s != LS_256x256 && s != LS_128x128) continue;
+    const int64_t tiles = ceil_div(m, shape_m(s)) * ceil_div(n, shape_n(s)) * splits;
+    // (a round of few 128-row tiles leaves each a CU of its own)
+    const double alone = tiles <= LG_CUS && shape_m(s) == 128 ? 0.6 : 1.0;
+    const double us = alone * shape_us(s) * (double)ceil_div(tiles, shape_round(s));
+    if (us < least * 0.999) least = us, best = s;
+  }
+  return best;
+}
+
 struct LossPlan {
-  int bn;          // tokens a tile: 64, 128 or 256
+  LossShape prob;  // tile of the logits' products
+  LossShape hid;   // of d_hidden's
+  LossShape head;  // of d_lm_head's
   int piece;       // vocabulary rows a piece (a multiple of 256)
   int splits;      // d_hidden: parts of a piece's vocabulary
   int64_t part, tlogit, p, acc, rows, bytes;  // offsets into the workspace
@@ -500,8 +533,7 @@ struct LossPlan {
 
 static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
   LossPlan q{};
-  q.bn = N <= 64 ? 64 : N <= 128 ? 128 : 256;
-  const int64_t tn = ceil_div(N, q.bn);
+  q.prob = loss_shape(V, N, 1, false);
   int64_t off = 0;
   auto take = [&](int64_t bytes) {
     const int64_t at = off;
@@ -515,7 +547,7 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
     return q;
   }
   // pieces of the vocabulary whose tiles fill the CUs best
-  const int64_t vt = ceil_div(V, 256);
+  const int64_t vt = ceil_div(V, 256), tn = ceil_div(N, 256);
   const int64_t most = LOSS_P_BYTES / (512 * (int64_t)N) > 1 ? LOSS_P_BYTES / (512 * (int64_t)N) : 1;
   int64_t best = -1, tiles = vt;
   for (int64_t np = ceil_div(vt, most), e = np + 4; np < e; ++np) {
@@ -524,15 +556,19 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
     if (best < 0 || rounds < best) best = rounds, tiles = t;
   }
   q.piece = (int)(tiles * 256);
+  q.prob = loss_shape(V < q.piece ? V : q.piece, N, 1, false);
+  q.head = loss_shape(K, V < q.piece ? V : q.piece, 1, true);
   // d_hidden's reduction is split until its tiles fill the CUs; each split costs a pass over
   // its float32 sums
-  const int64_t dt = ceil_div(K, 256) * tn, steps = ceil_div(q.piece, LG_BK);
-  q.splits = 1;
+  const int64_t steps = ceil_div(q.piece, LG_BK);
   double least = 1e30;
   for (int s = 1; s <= 64 && s <= steps; ++s) {
-    const double us = 0.9 * q.bn / 256 * (double)(ceil_div(dt * s, LG_CUS) * ceil_div(steps, s)) +
+    const LossShape shape = loss_shape(K, N, s, false);
+    const int64_t turns = ceil_div(K, shape_m(shape)) * ceil_div(N, shape_n(shape)) * s;
+    const double alone = turns <= LG_CUS && shape_m(shape) == 128 ? 0.6 : 1.0;
+    const double us = alone * shape_us(shape) * (double)(ceil_div(turns, shape_round(shape)) * ceil_div(steps, s)) +
                       8.0 * s * N * (double)K / 4e6;
-    if (us < least) least = us, q.splits = s;
+    if (us < least) least = us, q.splits = s, q.hid = shape;
   }
   q.p = take((int64_t)N * q.piece * 2);
   if (hid) q.acc = take((int64_t)q.splits * N * K * 4);
@@ -545,19 +581,22 @@ int64_t loss_workspace(int N, int K, int V, bool hid, bool head) {
   return loss_plan(N, K, V, hid, head).bytes;
 }
 
+template <int MODE, int WM, int WN, int TM, int TN, int R>
+static void loss_gemm_as(LossGemm g, int64_t m, int64_t n, hipStream_t st) {
+  g.tiles_m = (int)ceil_div(m, WM * TM * 16);
+  g.tiles_n = (int)ceil_div(n, WN * TN * 16);
+  const dim3 grid((unsigned)((int64_t)g.tiles_m * g.tiles_n * g.splits));
+  hipLaunchKernelGGL((k_loss_gemm<MODE, WM, WN, TM, TN, R>), grid, dim3(WM * WN * WAVE), 0, st, g);
+}
+
 template <int MODE>
-static void loss_gemm(const LossGemm& g0, int bn, int64_t m, int64_t n, hipStream_t st) {
-  LossGemm g = g0;
-  g.tiles_m = (int)ceil_div(m, 256);
-  g.tiles_n = (int)ceil_div(n, bn);
-  const dim3 grid((unsigned)(g.tiles_m * g.tiles_n * g.splits));
-  if (bn == 256)
-    hipLaunchKernelGGL((k_loss_gemm<MODE, 2, 4, 8, 4>), grid, dim3(512), 0, st, g);
+static void loss_gemm(const LossGemm& g, LossShape s, int64_t m, int64_t n, hipStream_t st) {
+  if (s == LS_256x256) loss_gemm_as<MODE, 2, 4, 8, 4, 2>(g, m, n, st);
+  else if (s == LS_128x128) loss_gemm_as<MODE, 2, 2, 4, 4, 2>(g, m, n, st);
   else if constexpr (MODE != LM_DHEAD) {
-    if (bn == 128)
-      hipLaunchKernelGGL((k_loss_gemm<MODE, 4, 2, 4, 4>), grid, dim3(512), 0, st, g);
-    else
-      hipLaunchKernelGGL((k_loss_gemm<MODE, 8, 1, 2, 4>), grid, dim3(512), 0, st, g);
+    if (s == LS_256x128) loss_gemm_as<MODE, 4, 2, 4, 4, 3>(g, m, n, st);
+    else if (s == LS_256x64) loss_gemm_as<MODE, 8, 1, 2, 4, 3>(g, m, n, st);
+    else loss_gemm_as<MODE, 4, 1, 2, 4, 3>(g, m, n, st);
   }
 }
 
@@ -577,8 +616,8 @@ hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void*
   g.targets = targets;
   g.part = (float2*)(w8 + q.part);
   g.tlogit = (float*)(w8 + q.tlogit);
-  loss_gemm<LM_STATS>(g, q.bn, V, N, st);
-  const int slices = (int)ceil_div(V, 256) * (q.bn == 256 ? 2 : q.bn == 128 ? 4 : 8);
+  loss_gemm<LM_STATS>(g, q.prob, V, N, st);
+  const int slices = (int)loss_slices(V, q.prob);
   if (N >= 1024)
     hipLaunchKernelGGL(k_loss_rows<16>, dim3((unsigned)ceil_div(N, 16)), dim3(256), 0, st, g.part,
                        slices, N, g.tlogit, targets, ignore_index, V, loss, lse, status);
@@ -600,7 +639,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
     z.splits = 1;
     z.out16 = (uint16_t*)d_head;
     z.out_stride = dws;
-    if (d_head) loss_gemm<LM_DHEAD>(z, 256, K, V, st);
+    if (d_head) loss_gemm<LM_DHEAD>(z, LS_256x256, K, V, st);
     return hipGetLastError();
   }
   const LossPlan q = loss_plan(N, K, V, d_hidden != nullptr, d_head != nullptr);
@@ -627,7 +666,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
     g.grad_lse = grad_lse;
     g.out16 = p;
     g.out_stride = q.piece;
-    loss_gemm<LM_PROB>(g, q.bn, vn, N, st);
+    loss_gemm<LM_PROB>(g, q.prob, vn, N, st);
     if (d_hidden) {
       LossGemm h{};
       h.a = LossOperand{wv, ws, K};
@@ -638,7 +677,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
       h.out32 = (float*)(w8 + q.acc);
       h.out_stride = K;
       h.accumulate = v0 > 0;
-      loss_gemm<LM_DHID>(h, q.bn, K, N, st);
+      loss_gemm<LM_DHID>(h, q.hid, K, N, st);
     }
     if (d_head) {
       LossGemm h{};
@@ -649,7 +688,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
       h.split_red = (int)(ceil_div(N, LG_BK) * LG_BK);
       h.out16 = (uint16_t*)d_head + (int64_t)v0 * dws;
       h.out_stride = dws;
-      loss_gemm<LM_DHEAD>(h, 256, K, vn, st);
+      loss_gemm<LM_DHEAD>(h, q.head, K, vn, st);
     }
   }
   if (d_hidden)
