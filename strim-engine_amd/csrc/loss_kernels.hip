@@ -57,6 +57,7 @@ struct LossGemm {
   float2* part;            // LM_STATS [slice][N]: max, sum exp(x - max) of a vocabulary slice
   float* tlogit;           // LM_STATS [N]: the target's logit
   const float *lse, *grad_loss, *grad_lse;
+  float* scale;            // what p was divided by: LM_PROB writes it, the gradients read it
   uint16_t* out16;         // LM_PROB p [N][out_stride]; LM_DHEAD [v][out_stride]
   int64_t out_stride;
   float* out32;            // LM_DHID [split][N][out_stride]
@@ -200,6 +201,26 @@ __device__ __forceinline__ void loss_tile(int tiles_m, int tiles_n, int splits, 
   tm = r / wide;
 }
 
+// The number that p is held divided by: the first nonzero gradient of a row that counts, among
+// the first 1,024 (ordinary sizes only; else 1). Where every row weighs the same, as in a mean,
+// p then holds exp(x - lse) - [v = t] itself, whose -1 is exact. With the weight in it every
+// target's -g would be rounded alike, an error that no sum averages out: N = 2,000 rows at
+// weights of 1/1,600 gave d_lm_head 1.5 times the relative error of a float32 evaluation rounded
+// once, and 1.2 times without.
+__device__ __forceinline__ float loss_scale(const LossGemm& g, int lane) {
+  for (int n0 = 0; n0 < min(g.b.rows, 1024); n0 += WAVE) {
+    const int n = min(n0 + lane, g.b.rows - 1), t = g.targets[n];
+    float c = 0.0f;
+    if (t != g.ignore_index && t >= 0 && t < g.V) {
+      c = g.grad_loss[n];
+      if (c == 0.0f && g.grad_lse) c = g.grad_lse[n];
+    }
+    const uint64_t have = __ballot(fabsf(c) > 1e-12f && fabsf(c) < 1e12f);
+    if (have) return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), __builtin_ctzll(have)));
+  }
+  return 1.0f;
+}
+
 // WM x WN waves of TM x TN tiles of 16 x 16; R stages in LDS.
 template <int MODE, int WM, int WN, int TM, int TN, int R>
 __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g) {
@@ -334,13 +355,15 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
         g.part[(int64_t)(tm * WM + wm) * g.b.rows + n] = make_float2(mx, sum);
     }
   } else if constexpr (MODE == LM_PROB) {
+    const float scale = loss_scale(g, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *g.scale = scale;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = min(n0 + 16 * j, g.b.rows - 1);
       const int t = g.targets[n];
       const bool live = t != g.ignore_index && t >= 0 && t < g.V;
-      const float gl = live ? g.grad_loss[n] : 0.0f;
-      const float top = live && g.grad_lse ? gl + g.grad_lse[n] : gl;
+      const float g0 = live ? g.grad_loss[n] : 0.0f;
+      const float gl = g0 / scale, top = (live && g.grad_lse ? g0 + g.grad_lse[n] : g0) / scale;
       const float lse = g.lse[n];
       const uint32_t keep = live ? 0xFFFFFFFFu : 0u;  // whatever a dead row holds (a NaN too)
       const int at = t - g.v0 - m0;                    // the target's place among this lane's rows
@@ -363,6 +386,7 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
           store(g.out16 + (int64_t)n * g.out_stride, i, w[i], w[i + 1], (int)g.out_stride);
     }
   } else if constexpr (MODE == LM_DHID) {
+    const float scale = *g.scale;
     float* out = g.out32 + (int64_t)split * g.b.rows * g.out_stride;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
@@ -373,17 +397,20 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
         const int k = m0 + 16 * i;
         if (k >= g.a.rows) continue;
         lf32x4* at = (lf32x4*)(out + (int64_t)n * g.out_stride + k);
-        *at = g.accumulate ? *at + acc[i][j] : acc[i][j];
+        const lf32x4 y = scale * acc[i][j];
+        *at = g.accumulate ? *at + y : y;
       }
     }
   } else {
+    const float scale = g.scale ? *g.scale : 1.0f;  // (none without rows)
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int v = n0 + 16 * j;
       uint2 w[TM];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const float f[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        const float f[4] = {scale * acc[i][j][0], scale * acc[i][j][1], scale * acc[i][j][2],
+                            scale * acc[i][j][3]};
         w[i] = loss_pack4(f);
       }
       if (v < g.b.rows)
@@ -528,7 +555,7 @@ struct LossPlan {
   LossShape head;  // of d_lm_head's
   int piece;       // vocabulary rows a piece (a multiple of 256)
   int splits;      // d_hidden: parts of a piece's vocabulary
-  int64_t part, tlogit, p, acc, rows, bytes;  // offsets into the workspace
+  int64_t part, tlogit, scale, p, acc, rows, bytes;  // offsets into the workspace
 };
 
 static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
@@ -570,6 +597,7 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
                       8.0 * s * N * (double)K / 4e6;
     if (us < least) least = us, q.splits = s, q.hid = shape;
   }
+  q.scale = take(4);
   q.p = take((int64_t)N * q.piece * 2);
   if (hid) q.acc = take((int64_t)q.splits * N * K * 4);
   if (head) q.rows = take((int64_t)N * K * 2);
@@ -664,6 +692,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
     g.lse = lse;
     g.grad_loss = grad_loss;
     g.grad_lse = grad_lse;
+    g.scale = (float*)(w8 + q.scale);
     g.out16 = p;
     g.out_stride = q.piece;
     loss_gemm<LM_PROB>(g, q.prob, vn, N, st);
@@ -674,6 +703,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
       h.red = vn;
       h.splits = q.splits;
       h.split_red = (int)(ceil_div(ceil_div(vn, LG_BK), q.splits) * LG_BK);
+      h.scale = g.scale;
       h.out32 = (float*)(w8 + q.acc);
       h.out_stride = K;
       h.accumulate = v0 > 0;
@@ -686,6 +716,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
       h.red = N;
       h.splits = 1;
       h.split_red = (int)(ceil_div(N, LG_BK) * LG_BK);
+      h.scale = g.scale;
       h.out16 = (uint16_t*)d_head + (int64_t)v0 * dws;
       h.out_stride = dws;
       loss_gemm<LM_DHEAD>(h, q.head, K, vn, st);
