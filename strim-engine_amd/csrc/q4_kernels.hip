@@ -660,65 +660,153 @@ __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int t
   }
 }
 
-// NT batch tiles; NW waves a workgroup, each RT 16-row weight tiles over the whole of K.
-template <int G, int NT, int RT, int NW>
-__global__ __launch_bounds__(NW* WAVE) void k_q4_stage(const Q4Args a) {
-  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
-  __shared__ __attribute__((aligned(1024))) uint8_t s_x[2][BLOCK];
+// More rows (or few rows and a K too long for k_q4_stream): the hidden rows come through LDS in
+// chunks of four steps, two chunks at a time (straight from k_q4_blocks' image of them), and a
+// wave goes through its MT row tiles chunk by chunk, their sums in registers. Two units of
+// weights are in flight; the code of a chunk has no branches between its requests (see
+// k_q4_dma), so chunks go by twos where MT is odd. Any alignment, any number of groups.
+constexpr int QC_NW = 8;
+
+template <int G, int NT, int MT>
+__global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024, CHUNK = 4 * BLOCK;
+  constexpr int SW = G == 128 ? 2 : 4;  // words of scales a lane loads
+  extern __shared__ __attribute__((aligned(1024))) uint8_t s_all[];
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_all;
   const int lane = threadIdx.x & (WAVE - 1), wv = wave_id(), h = lane >> 4, r16 = lane & 15;
+  const int nw = blockDim.x / WAVE;
+  const int units = (a.w.K + 511) / 512, groups = a.w.K / G, pieces = a.w.K / 32;
+  const int v0 = (blockIdx.x * nw + wv) * MT * 16;
+  const bool sym = a.w.biases == nullptr;
+  const uint16_t* side = (h & 1) && !sym ? a.w.biases : a.w.scales;
+  const int sofs = G == 32 ? 8 * (h >> 1) : 0;  // the upper quarters: a unit's second eight
+
+  struct Unit {
+    qu32x4 w[4];
+    uint32_t s[SW];
+  } buf[2];
+  // scales are loaded in whole vectors that end inside the row
+  auto back_of = [&](int c) { return max(0, c * 4 * GPS + sofs + 2 * SW - groups); };
+  auto load = [&](Unit& u, int c, int mt) {
+    c = min(c, units - 1);
+    const int v = min(v0 + 16 * mt + r16, a.w.V - 1);
+    const uint32_t* wp = a.w.words + (int64_t)v * a.w.words_stride;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) u.w[p] = *(const qu32x4*)(wp + 4 * min(16 * c + 4 * p + h, pieces - 1));
+    const uint16_t* sp = side + (int64_t)v * a.w.scales_stride + c * 4 * GPS + sofs - back_of(c);
+    if constexpr (SW == 2) {
+      const qu32x2u q = *(const qu32x2u*)sp;
+      u.s[0] = q[0], u.s[1] = q[1];
+    } else {
+      const qu32x4u q = *(const qu32x4u*)sp;
+      u.s[0] = q[0], u.s[1] = q[1], u.s[2] = q[2], u.s[3] = q[3];
+    }
+  };
+  // the hidden rows' chunk c into half c & 1: piece i of nw waves' CHUNK / 1024
+  const int share = (CHUNK / 1024 + nw - 1) / nw;
+  auto bring = [&](int c) {
+    c = min(c, units - 1);
+    const uint8_t* from = a.blocks + (int64_t)c * CHUNK + lane * 16;
+    for (int i = 0; i < share; ++i) {
+      const int e = min(wv * share + i, CHUNK / 1024 - 1) * 1024;
+      q4_load_lds<false>(lds + (c & 1) * CHUNK + e, from + e);
+    }
+  };
+
   const Q4Masks masks;
-  const int v0 = (blockIdx.x * NW + wv) * RT * 16;
-  const int steps = (a.w.K + 127) / 128, groups = a.w.K / G, pieces = a.w.K / 32;
-  const uint32_t* wrow[RT];
-  const uint16_t *srow[RT], *brow[RT];
+  const uint32_t keepb = sym ? 0u : 0xFFFFFFFFu;  // symmetric: no biases, and 8 less
+  const float zero = sym ? -24.0f : -16.0f;
+  qf32x4 acc[MT][NT];
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
-    const int v = min(v0 + 16 * i + r16, a.w.V - 1);
-    wrow[i] = a.w.words + (int64_t)v * a.w.words_stride;
-    srow[i] = a.w.scales + (int64_t)v * a.w.scales_stride;
-    brow[i] = a.w.biases ? a.w.biases + (int64_t)v * a.w.scales_stride : nullptr;
-  }
-  qf32x4 acc[RT][NT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
+  for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[i][nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < steps; ++s) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < BLOCK / 16; e += NW * WAVE)
-      *(qu32x4*)&s_x[0][e * 16] = *(const qu32x4*)(a.blocks + (int64_t)s * BLOCK + e * 16);
-    __syncthreads();
+
+  auto compute = [&](Unit& u, int c, int mt) {
+    // the scales moved back for want of room move into place
+    const int back = back_of(c);
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
+    for (int d = SW / 2; d > 0; d /= 2)  // by d words
+#pragma unroll
+      for (int e = 0; e < SW; ++e) u.s[e] = back & (2 * d) ? (e + d < SW ? u.s[e + d] : 0u) : u.s[e];
+#pragma unroll
+    for (int e = 0; e < SW; ++e) {
+      const uint32_t half = (u.s[e] >> 16) | (e + 1 < SW ? u.s[e + 1] << 16 : 0u);
+      u.s[e] = back >= 2 * SW ? 0u : back & 1 ? half : u.s[e];
+    }
+    uint32_t sw[2 * GPS], bw[2 * GPS];  // the unit's scales and biases, in every quarter
+#pragma unroll
+    for (int e = 0; e < SW; ++e) {
+      uint32_t s0 = u.s[e], b0 = u.s[e];
+      q4_swap16(s0, b0);
+      if constexpr (G == 32) {
+        uint32_t s1 = s0, b1 = b0;
+        q4_swap32(s0, s1);
+        q4_swap32(b0, b1);
+        sw[4 + e] = s1, bw[4 + e] = b1;
+      }
+      sw[e] = s0, bw[e] = b0;
+    }
+    const uint8_t* xc = s_all + (c & 1) * CHUNK;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
       uint32_t w[4];
-      q4_order<G>(*(const qu32x4*)(wrow[i] + 4 * min(4 * s + h, pieces - 1)), w);
+      q4_order<G>(u.w[p], w);
 #pragma unroll
       for (int g = 0; g < GPS; ++g) {
-        const int gi = s * GPS + g;
-        if (gi >= groups) break;
-        const float sc = __uint_as_float((uint32_t)srow[i][gi] << 16);
-        const float bi = brow[i] ? __uint_as_float((uint32_t)brow[i][gi] << 16) : -8.0f * sc;
-        const float off = bi - 16.0f * sc;
+        const int i = p * GPS + g;
+        const float sc = __uint_as_float(i & 1 ? sw[i / 2] & 0xFFFF0000u : sw[i / 2] << 16);
+        const float bi = __uint_as_float((i & 1 ? bw[i / 2] & 0xFFFF0000u : bw[i / 2] << 16) & keepb);
+        const float off = __builtin_fmaf(zero, sc, bi);
+        qf32x4 t[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) t[nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < MPG; ++q) {
+          const int m = g * MPG + q;
+          const qbf16x8 codes = q4_codes(w[m], masks);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const qu32x4 x = *(const qu32x4*)(xc + p * BLOCK + (m * NT + nt) * 1024 + lane * 16);
+            t[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), codes, t[nt], 0, 0, 0);
+          }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          qf32x4 t = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int q = 0; q < MPG; ++q) {
-            const int m = g * MPG + q;
-            const qu32x4 x = *(const qu32x4*)&s_x[0][(m * NT + nt) * 1024 + lane * 16];
-            t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), q4_codes(w[m], masks), t, 0, 0, 0);
-          }
-          const qf32x4 xs = *(const qf32x4*)&s_x[0][4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4];
+          const qf32x4 xs = *(const qf32x4*)(xc + p * BLOCK + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            acc[i][nt][r] = __builtin_fmaf(sc, t[r], __builtin_fmaf(off, xs[r], acc[i][nt][r]));
+            acc[mt][nt][r] = __builtin_fmaf(sc, t[nt][r], __builtin_fmaf(off, xs[r], acc[mt][nt][r]));
         }
       }
     }
+  };
+  auto chunk = [&](int c, int first) {  // first: the buffer of its first tile
+    // every wave's part of the chunk has arrived (a unit's request is four loads or more, and one
+    // or more units were requested since), and none reads the other half any more
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(MT > 1 ? 8 : 4) : "memory");
+    if (c + 1 < units) bring(c + 1);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      Unit& u = buf[(first + mt) & 1];
+      __builtin_amdgcn_sched_barrier(0);
+      compute(u, c, mt);
+      __builtin_amdgcn_sched_barrier(0);
+      load(u, c + (mt + 2) / MT, (mt + 2) % MT);
+    }
+  };
+  bring(0);
+  load(buf[0], 0, 0);
+  load(buf[1], 1 / MT, 1 % MT);
+  for (int c = 0;; c += 2) {
+    chunk(c, 0);
+    if (c + 1 >= units) break;
+    chunk(c + 1, MT & 1);
+    if (c + 2 >= units) break;
   }
   // lane: weight row r16, places 4 h + r of each batch tile
 #pragma unroll
-  for (int i = 0; i < RT; ++i) {
+  for (int i = 0; i < MT; ++i) {
     const int v = v0 + 16 * i + r16;
     if (v >= a.w.V) continue;
 #pragma unroll
@@ -731,20 +819,71 @@ __global__ __launch_bounds__(NW* WAVE) void k_q4_stage(const Q4Args a) {
   }
 }
 
+// K of fewer than eight groups: one wave a row tile, straightforwardly.
+template <int G, int NT>
+__global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
+  const int lane = threadIdx.x, h = lane >> 4, r16 = lane & 15;
+  const int steps = (a.w.K + 127) / 128, groups = a.w.K / G, pieces = a.w.K / 32;
+  const int row = blockIdx.x * 16 + r16, v = min(row, a.w.V - 1);
+  const uint32_t* wp = a.w.words + (int64_t)v * a.w.words_stride;
+  const uint16_t* sp = a.w.scales + (int64_t)v * a.w.scales_stride;
+  const uint16_t* bp = a.w.biases ? a.w.biases + (int64_t)v * a.w.scales_stride : nullptr;
+  const Q4Masks masks;
+  qf32x4 acc[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) acc[nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < steps; ++s) {
+    const uint8_t* xc = a.blocks + (int64_t)s * BLOCK;
+    uint32_t w[4];
+    q4_order<G>(*(const qu32x4*)(wp + 4 * min(4 * s + h, pieces - 1)), w);
+#pragma unroll
+    for (int g = 0; g < GPS; ++g) {
+      const int gi = s * GPS + g;
+      if (gi >= groups) break;
+      const float sc = __uint_as_float((uint32_t)sp[gi] << 16);
+      const float bi = bp ? __uint_as_float((uint32_t)bp[gi] << 16) : -8.0f * sc;
+      const float off = bi - 16.0f * sc;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        qf32x4 t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < MPG; ++q) {
+          const int m = g * MPG + q;
+          const qu32x4 x = *(const qu32x4*)(xc + (m * NT + nt) * 1024 + lane * 16);
+          t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), q4_codes(w[m], masks), t, 0, 0, 0);
+        }
+        const qf32x4 xs = *(const qf32x4*)(xc + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[nt][r] = __builtin_fmaf(sc, t[r], __builtin_fmaf(off, xs[r], acc[nt][r]));
+      }
+    }
+  }
+  if (row >= a.w.V) return;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int b = 16 * nt + q4_row(4 * h + r);
+      if (b < a.B) q4_store(a, b, row, acc[nt][r]);
+    }
+}
+
 // ---- host ---------------------------------------------------------------------------------
+static int q4_tiles_n(int B) { return B <= 16 ? 1 : B <= 32 ? 2 : 4; }
+
 int64_t q4_workspace(int B, int K) {
-  const int64_t nt = ((B < 64 ? B : 64) + 15) / 16;
-  return ((K + 127) / 128) * (4 * nt + 1) * 1024;
+  return ((int64_t)K + 511) / 512 * 4 * (4 * q4_tiles_n(B) + 1) * 1024;
 }
 
 // A launch with more than 64 KB of LDS, which a kernel has to be told of once.
-template <auto KERNEL>
-static bool q4_big_lds(dim3 grid, size_t lds, hipStream_t st, const Q4Args& a, int tiles,
-                       int waves = QS_NW) {
+template <auto KERNEL, class... More>
+static bool q4_big_lds(dim3 grid, size_t lds, hipStream_t st, const Q4Args& a, int waves, More... more) {
   static const hipError_t told = hipFuncSetAttribute(
       (const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)QS_LDS);
   (void)told;
-  hipLaunchKernelGGL(KERNEL, grid, dim3(waves * WAVE), lds, st, a, tiles);
+  hipLaunchKernelGGL(KERNEL, grid, dim3(waves * WAVE), lds, st, a, more...);
   return true;
 }
 
@@ -759,32 +898,57 @@ static bool q4_stream(const Q4Args& a, hipStream_t st) {
     const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
     const int w = nw < QS_NW ? nw : QS_NW;
     const size_t lds = own + (size_t)w * 10240;
-    return a.w.K % 512 == 0 ? q4_big_lds<k_q4_dma<G, RB, true>>(grid, lds, st, a, tiles, w)
-                            : q4_big_lds<k_q4_dma<G, RB, false>>(grid, lds, st, a, tiles, w);
+    return a.w.K % 512 == 0 ? q4_big_lds<k_q4_dma<G, RB, true>>(grid, lds, st, a, w, tiles)
+                            : q4_big_lds<k_q4_dma<G, RB, false>>(grid, lds, st, a, w, tiles);
   }
   const size_t lds = (size_t)steps * q4_step_bytes<G, RB>() + (size_t)QS_NW * 2 * RB * WAVE * 4;
   if (lds > QS_LDS || a.w.K < 8 * G) return false;
   const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
-  return a.w.K % 512 == 0 ? q4_big_lds<k_q4_stream<G, RB, D, true>>(grid, lds, st, a, tiles)
-                          : q4_big_lds<k_q4_stream<G, RB, D, false>>(grid, lds, st, a, tiles);
+  return a.w.K % 512 == 0 ? q4_big_lds<k_q4_stream<G, RB, D, true>>(grid, lds, st, a, QS_NW, tiles)
+                          : q4_big_lds<k_q4_stream<G, RB, D, false>>(grid, lds, st, a, QS_NW, tiles);
+}
+
+template <int G, int NT, int MT>
+static void q4_chunk(const Q4Args& a, int nw, hipStream_t st) {
+  const int tiles = (a.w.V + 15) / 16, each = nw * MT;
+  q4_big_lds<k_q4_chunk<G, NT, MT>>(dim3((unsigned)((tiles + each - 1) / each)),
+                                    (size_t)2 * 4 * (4 * NT + 1) * 1024, st, a, nw);
+}
+
+// (narrow groups by 64 rows: more than the registers hold)
+template <int G, int NT>
+constexpr bool Q4_FIVE = !(G == 32 && NT == 4);
+
+template <int G, int NT>
+static void q4_blocks(const Q4Args& a, hipStream_t st) {
+  const int tiles = (a.w.V + 15) / 16;
+  hipLaunchKernelGGL((k_q4_blocks<G, NT>), dim3((unsigned)((a.w.K + 511) / 512 * 4)), dim3(WAVE), 0, st, a);
+  if (a.w.K < 8 * G) {
+    hipLaunchKernelGGL((k_q4_short<G, NT>), dim3((unsigned)tiles), dim3(WAVE), 0, st, a);
+    return;
+  }
+  // tiles a wave: what takes the fewest tile times over all rounds; few tiles: smaller workgroups
+  const int nw = tiles >= 4 * 256 ? QC_NW : tiles >= 2 * 256 ? 4 : 2;
+  int best = 1, least = 1 << 30;
+  for (int mt : {1, 2, 3, 5}) {
+    if (mt == 5 && !Q4_FIVE<G, NT>) continue;
+    const int round = 256 * nw * mt, cost = (tiles + round - 1) / round * mt;
+    if (cost < least) least = cost, best = mt;
+  }
+  if (best == 1) q4_chunk<G, NT, 1>(a, nw, st);
+  else if (best == 2) q4_chunk<G, NT, 2>(a, nw, st);
+  else if (best == 3) q4_chunk<G, NT, 3>(a, nw, st);
+  else if constexpr (Q4_FIVE<G, NT>) q4_chunk<G, NT, 5>(a, nw, st);
 }
 
 template <int G>
 static void q4_logits(const Q4Args& a, hipStream_t st) {
   if (a.B <= 4 && q4_stream<G, 1, 2>(a, st)) return;
   if (a.B <= 8 && q4_stream<G, 2, 2>(a, st)) return;
-  if (a.B <= 16 && q4_stream<G, 4, 2>(a, st)) return;
-  const dim3 steps((unsigned)((a.w.K + 127) / 128)), grid((unsigned)((a.w.V + 127) / 128));
-#define STRIM_Q4(NT_)                                                            \
-  do {                                                                           \
-    hipLaunchKernelGGL((k_q4_blocks<G, NT_>), steps, dim3(WAVE), 0, st, a);      \
-    hipLaunchKernelGGL((k_q4_stage<G, NT_, 2, 4>), grid, dim3(4 * WAVE), 0, st, a); \
-  } while (0)
-  if (a.B <= 16) STRIM_Q4(1);
-  else if (a.B <= 32) STRIM_Q4(2);
-  else if (a.B <= 48) STRIM_Q4(3);
-  else STRIM_Q4(4);
-#undef STRIM_Q4
+  const int nt = q4_tiles_n(a.B);
+  if (nt == 1) q4_blocks<G, 1>(a, st);
+  else if (nt == 2) q4_blocks<G, 2>(a, st);
+  else q4_blocks<G, 4>(a, st);
 }
 
 hipError_t launch_q4_logits(const void* x, int64_t x_stride, int B, int K, const uint32_t* words,
