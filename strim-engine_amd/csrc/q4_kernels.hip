@@ -662,10 +662,15 @@ __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int t
 
 // More rows (or few rows and a K too long for k_q4_stream): the hidden rows come through LDS in
 // chunks of four steps, two chunks at a time (straight from k_q4_blocks' image of them), and a
-// wave goes through its MT row tiles chunk by chunk, their sums in registers. Two units of
-// weights are in flight; the code of a chunk has no branches between its requests (see
-// k_q4_dma), so chunks go by twos where MT is odd. Any alignment, any number of groups.
+// wave goes through its MT row tiles chunk by chunk, two at a time (a fragment read from LDS
+// serves both), their sums in registers. The code of a chunk has no branches between its
+// requests, so that each wait is for the oldest alone. Any alignment, any number of groups.
 constexpr int QC_NW = 8;
+
+template <int I>
+struct QInt {
+  static constexpr int value = I;
+};
 
 template <int G, int NT, int MT>
 __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
@@ -681,18 +686,23 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
   const uint16_t* side = (h & 1) && !sym ? a.w.biases : a.w.scales;
   const int sofs = G == 32 ? 8 * (h >> 1) : 0;  // the upper quarters: a unit's second eight
 
+  // Two units of weights, the tiles 2 i and 2 i + 1 of a chunk (and the last alone where MT is
+  // odd); each part of one is requested anew, for the tile that has the place next, as soon as
+  // it has been taken up.
   struct Unit {
     qu32x4 w[4];
     uint32_t s[SW];
   } buf[2];
   // scales are loaded in whole vectors that end inside the row
   auto back_of = [&](int c) { return max(0, c * 4 * GPS + sofs + 2 * SW - groups); };
-  auto load = [&](Unit& u, int c, int mt) {
+  auto load_words = [&](Unit& u, int c, int mt, int p) {
+    const int v = min(v0 + 16 * mt + r16, a.w.V - 1);
+    u.w[p] = *(const qu32x4*)(a.w.words + (int64_t)v * a.w.words_stride +
+                              4 * min(16 * min(c, units - 1) + 4 * p + h, pieces - 1));
+  };
+  auto load_scales = [&](Unit& u, int c, int mt) {
     c = min(c, units - 1);
     const int v = min(v0 + 16 * mt + r16, a.w.V - 1);
-    const uint32_t* wp = a.w.words + (int64_t)v * a.w.words_stride;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) u.w[p] = *(const qu32x4*)(wp + 4 * min(16 * c + 4 * p + h, pieces - 1));
     const uint16_t* sp = side + (int64_t)v * a.w.scales_stride + c * 4 * GPS + sofs - back_of(c);
     if constexpr (SW == 2) {
       const qu32x2u q = *(const qu32x2u*)sp;
@@ -722,87 +732,99 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) acc[i][nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
 
-  auto compute = [&](Unit& u, int c, int mt) {
-    // the scales moved back for want of room move into place
+  // tiles mt .. mt + CNT - 1 of chunk c; the places' next tiles are those of tile mt + 2, + 3,
+  // or of the next chunk
+  auto compute = [&](int c, auto mt_, auto cnt_) {
+    constexpr int M0 = decltype(mt_)::value, CNT = decltype(cnt_)::value;
+    uint32_t sw[CNT][2 * GPS], bw[CNT][2 * GPS];  // the units' scales and biases, in every quarter
     const int back = back_of(c);
 #pragma unroll
-    for (int d = SW / 2; d > 0; d /= 2)  // by d words
+    for (int j = 0; j < CNT; ++j) {
+      Unit& u = buf[j];
+      // the scales moved back for want of room move into place
 #pragma unroll
-      for (int e = 0; e < SW; ++e) u.s[e] = back & (2 * d) ? (e + d < SW ? u.s[e + d] : 0u) : u.s[e];
+      for (int d = SW / 2; d > 0; d /= 2)  // by d words
 #pragma unroll
-    for (int e = 0; e < SW; ++e) {
-      const uint32_t half = (u.s[e] >> 16) | (e + 1 < SW ? u.s[e + 1] << 16 : 0u);
-      u.s[e] = back >= 2 * SW ? 0u : back & 1 ? half : u.s[e];
-    }
-    uint32_t sw[2 * GPS], bw[2 * GPS];  // the unit's scales and biases, in every quarter
+        for (int e = 0; e < SW; ++e) u.s[e] = back & (2 * d) ? (e + d < SW ? u.s[e + d] : 0u) : u.s[e];
 #pragma unroll
-    for (int e = 0; e < SW; ++e) {
-      uint32_t s0 = u.s[e], b0 = u.s[e];
-      q4_swap16(s0, b0);
-      if constexpr (G == 32) {
-        uint32_t s1 = s0, b1 = b0;
-        q4_swap32(s0, s1);
-        q4_swap32(b0, b1);
-        sw[4 + e] = s1, bw[4 + e] = b1;
+      for (int e = 0; e < SW; ++e) {
+        const uint32_t half = (u.s[e] >> 16) | (e + 1 < SW ? u.s[e + 1] << 16 : 0u);
+        u.s[e] = back >= 2 * SW ? 0u : back & 1 ? half : u.s[e];
       }
-      sw[e] = s0, bw[e] = b0;
+#pragma unroll
+      for (int e = 0; e < SW; ++e) {
+        uint32_t s0 = u.s[e], b0 = u.s[e];
+        q4_swap16(s0, b0);
+        if constexpr (G == 32) {
+          uint32_t s1 = s0, b1 = b0;
+          q4_swap32(s0, s1);
+          q4_swap32(b0, b1);
+          sw[j][4 + e] = s1, bw[j][4 + e] = b1;
+        }
+        sw[j][e] = s0, bw[j][e] = b0;
+      }
+      load_scales(u, M0 + 2 + j < MT ? c : c + 1, M0 + 2 + j < MT ? M0 + 2 + j : j);
     }
     const uint8_t* xc = s_all + (c & 1) * CHUNK;
+    uint32_t w[CNT][4];
+    qf32x4 t[CNT][NT];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      uint32_t w[4];
-      q4_order<G>(u.w[p], w);
+    for (int m = 0; m < 16; ++m) {  // the chunk's MFMA words
+      const int p = m >> 2, g = (m & 3) / MPG, i = p * GPS + g;
+      if (m % 4 == 0) {
 #pragma unroll
-      for (int g = 0; g < GPS; ++g) {
-        const int i = p * GPS + g;
-        const float sc = __uint_as_float(i & 1 ? sw[i / 2] & 0xFFFF0000u : sw[i / 2] << 16);
-        const float bi = __uint_as_float((i & 1 ? bw[i / 2] & 0xFFFF0000u : bw[i / 2] << 16) & keepb);
-        const float off = __builtin_fmaf(zero, sc, bi);
-        qf32x4 t[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) t[nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < MPG; ++q) {
-          const int m = g * MPG + q;
-          const qbf16x8 codes = q4_codes(w[m], masks);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const qu32x4 x = *(const qu32x4*)(xc + p * BLOCK + (m * NT + nt) * 1024 + lane * 16);
-            t[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), codes, t[nt], 0, 0, 0);
-          }
+        for (int j = 0; j < CNT; ++j) {
+          q4_order<G>(buf[j].w[p], w[j]);
+          load_words(buf[j], M0 + 2 + j < MT ? c : c + 1, M0 + 2 + j < MT ? M0 + 2 + j : j, p);
         }
+      }
+      qbf16x8 codes[CNT];
+#pragma unroll
+      for (int j = 0; j < CNT; ++j) codes[j] = q4_codes(w[j][m & 3], masks);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const qu32x4 x = *(const qu32x4*)(xc + p * BLOCK + ((m & 3) * NT + nt) * 1024 + lane * 16);
+#pragma unroll
+        for (int j = 0; j < CNT; ++j) {
+          if (m % MPG == 0) t[j][nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
+          t[j][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), codes[j],
+                                                            t[j][nt], 0, 0, 0);
+        }
+      }
+      if (m % MPG == MPG - 1) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const qf32x4 xs = *(const qf32x4*)(xc + p * BLOCK + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            acc[mt][nt][r] = __builtin_fmaf(sc, t[nt][r], __builtin_fmaf(off, xs[r], acc[mt][nt][r]));
+          for (int j = 0; j < CNT; ++j) {
+            const float sc = __uint_as_float(i & 1 ? sw[j][i / 2] & 0xFFFF0000u : sw[j][i / 2] << 16);
+            const float bi = __uint_as_float((i & 1 ? bw[j][i / 2] & 0xFFFF0000u : bw[j][i / 2] << 16) & keepb);
+            const float off = __builtin_fmaf(zero, sc, bi);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              acc[M0 + j][nt][r] = __builtin_fmaf(sc, t[j][nt][r], __builtin_fmaf(off, xs[r], acc[M0 + j][nt][r]));
+          }
         }
       }
     }
+    // (64 rows: two pairs of tiles at once are more than the registers hold)
+    if constexpr (NT == 4) __builtin_amdgcn_sched_barrier(0);
   };
-  auto chunk = [&](int c, int first) {  // first: the buffer of its first tile
+  bring(0);
+#pragma unroll
+  for (int j = 0; j < (MT > 1 ? 2 : 1); ++j) {
+    load_scales(buf[j], 0, j);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) load_words(buf[j], 0, j, p);
+  }
+  for (int c = 0; c < units; ++c) {
     // every wave's part of the chunk has arrived (a unit's request is four loads or more, and one
     // or more units were requested since), and none reads the other half any more
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(MT > 1 ? 8 : 4) : "memory");
     if (c + 1 < units) bring(c + 1);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      Unit& u = buf[(first + mt) & 1];
-      __builtin_amdgcn_sched_barrier(0);
-      compute(u, c, mt);
-      __builtin_amdgcn_sched_barrier(0);
-      load(u, c + (mt + 2) / MT, (mt + 2) % MT);
-    }
-  };
-  bring(0);
-  load(buf[0], 0, 0);
-  load(buf[1], 1 / MT, 1 % MT);
-  for (int c = 0;; c += 2) {
-    chunk(c, 0);
-    if (c + 1 >= units) break;
-    chunk(c + 1, MT & 1);
-    if (c + 2 >= units) break;
+    if constexpr (MT > 1) compute(c, QInt<0>{}, QInt<2>{});
+    if constexpr (MT > 3) compute(c, QInt<2>{}, QInt<2>{});
+    if constexpr (MT % 2) compute(c, QInt<MT - 1>{}, QInt<1>{});
   }
   // lane: weight row r16, places 4 h + r of each batch tile
 #pragma unroll
