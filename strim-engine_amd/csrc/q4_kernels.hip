@@ -807,8 +807,8 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
         }
       }
     }
-    // (64 rows: two pairs of tiles at once are more than the registers hold)
-    if constexpr (NT == 4) __builtin_amdgcn_sched_barrier(0);
+    // (more than 16 rows: two pairs of tiles at once are more than the registers hold)
+    if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
   };
   bring(0);
 #pragma unroll

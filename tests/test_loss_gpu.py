@@ -15,6 +15,7 @@ import pytest
 import torch
 
 from strim_amd import _native as N
+from strim_amd import loss as L
 from strim_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -220,6 +221,58 @@ def test_differences():
         lin = (dh.double() * d).sum(1)
         tol = 16e-5 + 0.1 ** 3 / 6 * 16 + 2.0 ** -8 * (dh.double() * d).abs().sum(1)
         assert bool(((diff - lin).abs() <= tol).all()), float(((diff - lin).abs() - tol).max())
+
+
+def test_autograd():
+    """The differentiable form: shapes, target types, reductions, gradients through both
+    outputs, a broadcast upstream gradient, a frozen projection, int64 ids past 32 bits."""
+    h, w, t, _ = inputs(60, 72, 500, seed=31, ignored=0.3)
+    h3, t3 = h.reshape(3, 20, 72).clone().requires_grad_(), t.reshape(3, 20).long()
+    t3[0, 0], t3[0, 1], t3[2, 19] = 500, 2 ** 40, -2 ** 40
+    ids = torch.where((t3 >= 0) & (t3 < 500), t3, -100).reshape(-1).int()
+    count = int((ids >= 0).sum())
+    w1 = w.clone().requires_grad_()
+    value = L.head_cross_entropy(h3, w1, t3)
+    value.backward()
+    value = value.detach()
+    g = torch.full((60,), 1.0 / count, device="cuda")
+    E = Exact(h, w, ids, g)
+    assert abs(float(value) - float(E.loss.sum()) / count) < float(E.tol.max()) + 1e-6 * float(value)
+    within(h3.grad.reshape(60, 72), E.dh, E.tol_h, "d_hidden")
+    within(w1.grad, E.dw, E.tol_w, "d_lm_head")
+    # the sum, with a frozen projection; the log-sum-exp's gradient beside it
+    h4 = h.clone().requires_grad_()
+    value, lse, status = L.head_loss(h4, w, ids)
+    assert not status.requires_grad
+    (value.sum() + (lse * 0.25).sum()).backward()
+    E = Exact(h, w, ids, torch.ones(60, device="cuda"), torch.full((60,), 0.25, device="cuda"))
+    within(h4.grad, E.dh, E.tol_h, "d_hidden")
+    # the log-sum-exp alone
+    w2 = w.clone().requires_grad_()
+    L.head_loss(h, w2, ids)[1].sum().backward()
+    E = Exact(h, w, ids, torch.zeros(60, device="cuda"), torch.ones(60, device="cuda"))
+    within(w2.grad, E.dw, E.tol_w, "d_lm_head")
+    lp = L.token_logprobs(h, w, ids.clamp_min(0))
+    E = Exact(h, w, ids.clamp_min(0))
+    within(-lp, E.loss, E.tol, "log-probabilities")
+    assert float(L.head_cross_entropy(h, w, torch.full_like(ids, -100))) == 0.0
+    with pytest.raises(ValueError):
+        L.head_cross_entropy(h, w, t3)
+    with pytest.raises(TypeError):
+        L.head_cross_entropy(h, w, ids.float())
+    with pytest.raises(ValueError):
+        L.head_cross_entropy(h, w, ids, reduction="max")
+
+
+def test_weights_of_many_sizes():
+    """Rows whose weights span many powers of two, the first of them ignored or weightless."""
+    h, w, t, gl = inputs(150, 64, 400, seed=41, ignored=0.0)
+    t[:70] = -100
+    gl *= torch.exp2(torch.arange(150, device="cuda") % 40 - 20.0)
+    gl[70:75] = 0.0
+    check(h, w, t, gl, label="weights")
+    gz = gl.flip(0).contiguous()
+    check(h, w, t, torch.zeros_like(gl), gz, label="weights of lse")
 
 
 def test_repeatable_and_in_a_graph():

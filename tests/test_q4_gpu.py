@@ -121,7 +121,9 @@ LOGITS = [(1, 32, 1, 32), (1, 64, 15, 64), (1, 128, 17, 128), (2, 96, 33, 32), (
           (32, 8192, 300, 64), (33, 1056, 130, 32), (48, 5120, 700, 64), (49, 320, 64, 64),
           (63, 2560, 200, 128), (64, 5120, 999, 32), (65, 256, 40, 64), (130, 512, 70, 32),
           (1, 5120, 5000, 64), (1, 20480, 140, 64), (6, 12800, 64, 128), (1, 9216, 2100, 32),
-          (20, 20480, 50, 32)]
+          (20, 20480, 50, 32), (3, 1152, 500, 64), (7, 1152, 333, 32), (2, 1280, 77, 128),
+          (6, 2560, 4000, 64), (12, 1280, 9000, 64), (24, 1088, 33_000, 64), (64, 1024, 33_000, 128),
+          (50, 512, 70_003, 32), (10, 576, 90_000, 64), (64, 640, 160_001, 64)]
 
 
 @pytest.mark.parametrize("symmetric", [False, True])
