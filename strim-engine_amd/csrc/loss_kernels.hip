@@ -210,16 +210,19 @@ __device__ __forceinline__ void loss_tile(int tiles_m, int tiles_n, int splits, 
 __device__ __forceinline__ float loss_scale(const LossGemm& g, int lane) {
   for (int n0 = 0; n0 < min(g.b.rows, 1024); n0 += WAVE) {
     const int n = min(n0 + lane, g.b.rows - 1), t = g.targets[n];
-    float c = 0.0f;
-    if (t != g.ignore_index && t >= 0 && t < g.V) {
-      c = g.grad_loss[n];
-      if (c == 0.0f && g.grad_lse) c = g.grad_lse[n];
-    }
+    const float gl = g.grad_loss[n], gz = g.grad_lse ? g.grad_lse[n] : 0.0f;
+    const float c = t == g.ignore_index || t < 0 || t >= g.V ? 0.0f : gl != 0.0f ? gl : gz;
     const uint64_t have = __ballot(fabsf(c) > 1e-12f && fabsf(c) < 1e12f);
     if (have) return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c), __builtin_ctzll(have)));
   }
   return 1.0f;
 }
+
+// What LM_PROB needs of a token.
+struct LossRow {
+  float lse, top, gl;  // p = top exp(x - lse) - gl [v = target]
+  int32_t target;      // INT_MIN: the row counts for nothing
+};
 
 // WM x WN waves of TM x TN tiles of 16 x 16; R stages in LDS.
 template <int MODE, int WM, int WN, int TM, int TN, int R>
@@ -248,6 +251,19 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
   // (past the reduction's end zeros are requested: the count of open requests is fixed)
 #pragma unroll
   for (int s = 0; s < R; ++s) request(lds + s * STAGE, s);
+  // (here their loads wait with the first stages, after the product they would wait alone: 8 us of
+  // every tile)
+  __shared__ LossRow s_row[MODE == LM_PROB ? BN : 1];
+  if constexpr (MODE == LM_PROB) {
+    const float scale = loss_scale(g, lane);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *g.scale = scale;
+    for (int c = threadIdx.x; c < BN; c += NW * WAVE) {
+      const int n = min(tn * BN + c, g.b.rows - 1), t = g.targets[n];
+      const float gl = g.grad_loss[n], gz = g.grad_lse ? g.grad_lse[n] : 0.0f, lse = g.lse[n];
+      const bool live = t != g.ignore_index && t >= 0 && t < g.V;
+      s_row[c] = live ? LossRow{lse, (gl + gz) / scale, gl / scale, t} : LossRow{0.0f, 0.0f, 0.0f, INT_MIN};
+    }
+  }
   LossFrag<ATR, BM> fa;
   LossFrag<BTR, BN> fb;
   fa.init(wm * TM, lane);
@@ -289,7 +305,7 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
     __builtin_amdgcn_sched_group_barrier(0x008, MUL, 0);
   };
   uint32_t cur = lds;
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((R - 1) * LOADS) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((R - 1) * LOADS) : "memory");
   frags(cur, 0);
   for (int s = 0; s < steps; ++s) {
     const uint32_t nxt = cur == lds + (R - 1) * STAGE ? lds : cur + STAGE;
@@ -355,18 +371,13 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
         g.part[(int64_t)(tm * WM + wm) * g.b.rows + n] = make_float2(mx, sum);
     }
   } else if constexpr (MODE == LM_PROB) {
-    const float scale = loss_scale(g, lane);
-    if (blockIdx.x == 0 && threadIdx.x == 0) *g.scale = scale;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int n = min(n0 + 16 * j, g.b.rows - 1);
-      const int t = g.targets[n];
-      const bool live = t != g.ignore_index && t >= 0 && t < g.V;
-      const float g0 = live ? g.grad_loss[n] : 0.0f;
-      const float gl = g0 / scale, top = (live && g.grad_lse ? g0 + g.grad_lse[n] : g0) / scale;
-      const float lse = g.lse[n];
-      const uint32_t keep = live ? 0xFFFFFFFFu : 0u;  // whatever a dead row holds (a NaN too)
-      const int at = t - g.v0 - m0;                    // the target's place among this lane's rows
+      const int n = n0 + 16 * j;
+      const LossRow row = s_row[n - tn * BN];
+      const float lse = row.lse, top = row.top, gl = row.gl;
+      const uint32_t keep = row.target != INT_MIN ? 0xFFFFFFFFu : 0u;  // whatever a dead row holds
+      const int at = row.target != INT_MIN ? row.target - g.v0 - m0 : -1;  // the target among this lane's rows
       uint2 w[TM];
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
@@ -380,7 +391,7 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
         w[i].x &= keep, w[i].y &= keep;
       }
       // (columns past the vocabulary are inside the row, and read by nothing)
-      if (n0 + 16 * j < g.b.rows)
+      if (n < g.b.rows)
 #pragma unroll
         for (int i = 0; i < TM; i += 2)
           store(g.out16 + (int64_t)n * g.out_stride, i, w[i], w[i + 1], (int)g.out_stride);
