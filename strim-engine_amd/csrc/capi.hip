@@ -842,13 +842,15 @@ int strim_head_logits_packed(void* stream, const void* hidden, int64_t hidden_st
                          const void* biases, int64_t scales_stride, int32_t group, int32_t V,
                          void* workspace, int64_t workspace_bytes, void* out_logits, int32_t dtype,
                          int64_t out_stride) {
-  if (!hidden || !words || !scales || !out_logits || !workspace || B < 1 || V <= 0 || V > STRIM_PACKED_MAX_VOCAB ||
+  if (!hidden || !words || !scales || !out_logits || B < 1 || V <= 0 || V > STRIM_PACKED_MAX_VOCAB ||
       !group_ok(K, group) || !dtype_ok(dtype) || hidden_stride < K || hidden_stride % 8 != 0 ||
       !al16(hidden) || words_stride < K / 8 || words_stride % 4 != 0 || !al16(words) ||
       scales_stride < K / group || out_stride < V || !(eps >= 0.0f) || !al16(workspace))
     return STRIM_EINVAL;
   if (norm_weight && (!xn || !al16(xn) || !al16(norm_weight))) return STRIM_EINVAL;
-  if (workspace_bytes < q4_workspace(B, K)) return STRIM_ECAPACITY;
+  const int64_t need = q4_workspace(B, K);
+  if (need > 0 && !workspace) return STRIM_EINVAL;
+  if (workspace_bytes < need) return STRIM_ECAPACITY;
   if (norm_weight) {
     launch_head_norm(hidden, hidden_stride, B, K, norm_weight, eps, xn, (hipStream_t)stream);
     hidden = xn;

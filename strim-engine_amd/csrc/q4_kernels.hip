@@ -895,7 +895,12 @@ __global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
 // ---- host ---------------------------------------------------------------------------------
 static int q4_tiles_n(int B) { return B <= 16 ? 1 : B <= 32 ? 2 : 4; }
 
+// None where k_q4_stream (or k_q4_dma) takes the rows whatever the groups: they fit its LDS.
 int64_t q4_workspace(int B, int K) {
+  const int64_t steps = ((int64_t)K + 511) / 512 * 4;
+  const bool one = B <= 4 && steps * q4_step_bytes<32, 1>() + QS_NW * 2 * 1 * WAVE * 4 <= (int64_t)QS_LDS;
+  const bool two = B <= 8 && steps * q4_step_bytes<32, 2>() + QS_NW * 2 * 2 * WAVE * 4 <= (int64_t)QS_LDS;
+  if (K >= 8 * 128 && (one || two)) return 0;
   return ((int64_t)K + 511) / 512 * 4 * (4 * q4_tiles_n(B) + 1) * 1024;
 }
 

@@ -6,6 +6,7 @@ computation runs in libstrim_sampler.so. Inputs must already live on the GPU.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import numpy as np
 import torch
@@ -13,8 +14,8 @@ import torch
 from . import _native as N
 
 
-def _ptr(t) -> ctypes.c_void_p | None:
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+def _ptr(t) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _stream(stream=None) -> ctypes.c_void_p:
@@ -317,52 +318,73 @@ def head_greedy(ctx: "Context", hidden: torch.Tensor, lm_head: torch.Tensor,
     return ids, status
 
 
+# What a small call costs is mostly this file's own time, so the checks of the loss and of the
+# 4-bit projections ask each tensor for as little as they can.
 def _check_bf16_rows(name: str, t: torch.Tensor) -> None:
     """A bf16 operand of the loss: [R, K] with contiguous rows, 16-byte aligned."""
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
     if not t.is_cuda:
         raise ValueError("every tensor argument must be on the GPU")
-    if t.dim() != 2 or (t.shape[0] > 0 and t.stride(1) != 1):
+    if t.dim() != 2 or (not t.is_contiguous() and t.stride(1) != 1):
         raise ValueError(f"{name} must be [rows, K] with contiguous rows")
 
 
-def _same_device(*ts):
-    if len({t.device for t in ts if t is not None}) > 1:
-        raise ValueError("every tensor argument must be on the same GPU")
+def _check_with(device: torch.device, *ts) -> None:
+    """Contiguous tensors (or None) on `device`."""
+    for t in ts:
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError("every tensor argument must be on the same GPU")
+        if not t.is_contiguous():
+            raise ValueError("tensor arguments must be contiguous")
 
 
 def _loss_args(hidden, lm_head, targets):
     _check_bf16_rows("hidden", hidden)
     _check_bf16_rows("lm_head", lm_head)
-    _check_cuda(targets)
-    _same_device(hidden, lm_head, targets)
-    N_, K = hidden.shape
-    V = lm_head.shape[0]
-    if lm_head.shape[1] != K:
-        raise ValueError(f"lm_head is [{V}, {lm_head.shape[1]}], hidden K={K}")
-    if targets.dtype != torch.int32 or tuple(targets.shape) != (N_,):
-        raise ValueError(f"targets must be int32 [{N_}]")
-    return N_, K, V
+    _check_with(hidden.device, targets)
+    R, K = hidden.shape
+    V, KW = lm_head.shape
+    if lm_head.device != hidden.device:
+        raise ValueError("every tensor argument must be on the same GPU")
+    if KW != K:
+        raise ValueError(f"lm_head is [{V}, {KW}], hidden K={K}")
+    if targets.dtype != torch.int32 or targets.shape != (R,):
+        raise ValueError(f"targets must be int32 [{R}]")
+    return R, K, V
 
 
-def _workspace(workspace, need: int, device) -> torch.Tensor:
-    if need < 0:
-        raise N.StrimError(need, "workspace size")
+def _workspace(workspace, need: int, device) -> torch.Tensor | None:
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    _check_cuda(workspace)
+        return torch.empty(need, dtype=torch.uint8, device=device) if need > 0 else None
+    _check_with(device, workspace)
     if workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace must hold {need} bytes")
     return workspace
 
 
+def _bytes(t) -> int:
+    return 0 if t is None else t.numel() * t.element_size()
+
+
+@lru_cache(maxsize=256)
 def head_loss_workspace(rows: int, K: int, V: int, want_hidden: bool = False,
                         want_lm_head: bool = False) -> int:
     """Bytes of workspace that head_loss (no gradient wanted) or head_loss_grad takes."""
     need = N.lib().strim_head_loss_workspace(rows, K, V, int(want_hidden), int(want_lm_head))
     if need < 0:
         raise N.StrimError(need, "strim_head_loss_workspace")
+    return need
+
+
+@lru_cache(maxsize=256)
+def head_logits_q4_workspace(B: int, K: int) -> int:
+    """Bytes of workspace that head_logits_q4 takes (0 for a few rows)."""
+    need = N.lib().strim_head_logits_packed_workspace(B, K)
+    if need < 0:
+        raise N.StrimError(need, "strim_head_logits_packed_workspace")
     return need
 
 
@@ -375,13 +397,14 @@ def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor
     0. strim_amd.loss has the differentiable form."""
     R, K, V = _loss_args(hidden, lm_head, targets)
     dev = hidden.device
-    loss, lse = torch.empty(2, R, dtype=torch.float32, device=dev).unbind(0)
+    loss = torch.empty(R, dtype=torch.float32, device=dev)
+    lse = torch.empty(R, dtype=torch.float32, device=dev)
     status = torch.empty(R, dtype=torch.int32, device=dev)
-    ws = _workspace(workspace, N.lib().strim_head_loss_workspace(R, K, V, 0, 0), dev)
+    ws = _workspace(workspace, head_loss_workspace(R, K, V), dev)
     N.check(N.lib().strim_head_loss(_stream(stream), _ptr(hidden), _row_stride(hidden), R, K,
                                     _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
-                                    ignore_index, _ptr(ws), ws.numel() * ws.element_size(),
-                                    _ptr(loss), _ptr(lse), _ptr(status)), "strim_head_loss")
+                                    ignore_index, _ptr(ws), _bytes(ws), _ptr(loss), _ptr(lse),
+                                    _ptr(status)), "strim_head_loss")
     return loss, lse, status
 
 
@@ -394,23 +417,21 @@ def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.T
     from lse as head_loss gave it and the float32 [N] gradients of its loss and (optional)
     its lse."""
     R, K, V = _loss_args(hidden, lm_head, targets)
-    _check_cuda(lse, grad_loss, grad_lse)
-    _same_device(hidden, lse, grad_loss, grad_lse)
-    for t in (lse, grad_loss, grad_lse):
-        if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (R,)):
-            raise ValueError(f"lse and the gradients must be float32 [{R}]")
     dev = hidden.device
-    dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
-    dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
+    _check_with(dev, lse, grad_loss, grad_lse)
+    for t in (lse, grad_loss, grad_lse):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (R,)):
+            raise ValueError(f"lse and the gradients must be float32 [{R}]")
     if not (want_hidden or want_lm_head):
         return None, None
-    ws = _workspace(workspace, N.lib().strim_head_loss_workspace(R, K, V, int(want_hidden),
-                                                                 int(want_lm_head)), dev)
+    dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
+    dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
+    ws = _workspace(workspace, head_loss_workspace(R, K, V, want_hidden, want_lm_head), dev)
     N.check(N.lib().strim_head_loss_grad(_stream(stream), _ptr(hidden), _row_stride(hidden), R, K,
                                          _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
                                          ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(grad_lse),
-                                         _ptr(ws), ws.numel() * ws.element_size(), _ptr(dh), K,
-                                         _ptr(dw), K), "strim_head_loss_grad")
+                                         _ptr(ws), _bytes(ws), _ptr(dh), K, _ptr(dw), K),
+            "strim_head_loss_grad")
     return dh, dw
 
 
@@ -424,16 +445,17 @@ class Q4Weight:
                  biases: torch.Tensor | None = None, group: int = 64):
         if words.dtype != torch.int32 or words.dim() != 2:
             raise ValueError("words must be int32 [V, K / 8]")
-        V, K = words.shape[0], 8 * words.shape[1]
-        if group not in (32, 64, 128) or K % group:
-            raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
+        if not words.is_cuda:
+            raise ValueError("every tensor argument must be on the GPU")
+        V, W = words.shape
+        if group not in (32, 64, 128) or 8 * W % group:
+            raise ValueError(f"group must be 32, 64 or 128 and divide K={8 * W}, got {group}")
         for t in (scales, biases):
-            if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (V, K // group)):
-                raise ValueError(f"scales and biases must be bfloat16 [{V}, {K // group}]")
-        _check_cuda(words, scales, biases)
-        _same_device(words, scales, biases)
+            if t is not None and (t.dtype != torch.bfloat16 or t.shape != (V, 8 * W // group)):
+                raise ValueError(f"scales and biases must be bfloat16 [{V}, {8 * W // group}]")
+        _check_with(words.device, words, scales, biases)
         self.words, self.scales, self.biases, self.group = words, scales, biases, group
-        self.V, self.K = V, K
+        self.V, self.K = V, 8 * W
 
 
 def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
@@ -474,26 +496,29 @@ def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor 
     if hidden.dim() == 1:
         hidden = hidden.unsqueeze(0)
     _check_bf16_rows("hidden", hidden)
-    _check_cuda(norm_weight, out, xn)
-    _same_device(hidden, q.words, norm_weight, out, xn)
+    dev = q.words.device
+    _check_with(dev, norm_weight, out, xn)
     B, K = hidden.shape
+    if hidden.device != dev:
+        raise ValueError("every tensor argument must be on the same GPU")
     if K != q.K:
         raise ValueError(f"the projection has K={q.K}, hidden K={K}")
     if norm_weight is not None:
-        if norm_weight.dtype != torch.bfloat16 or tuple(norm_weight.shape) != (K,):
+        if norm_weight.dtype != torch.bfloat16 or norm_weight.shape != (K,):
             raise ValueError(f"norm_weight must be bfloat16 [{K}]")
         if xn is None:
-            xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
+            xn = torch.empty(B, K, dtype=torch.bfloat16, device=dev)
+        elif xn.dtype != torch.bfloat16 or xn.shape != (B, K):
+            raise ValueError(f"xn must be bfloat16 [{B}, {K}]")
     if out is None:
-        out = torch.empty(B, q.V, dtype=out_dtype, device=hidden.device)
-    elif tuple(out.shape) != (B, q.V):
+        out = torch.empty(B, q.V, dtype=out_dtype, device=dev)
+    elif out.shape != (B, q.V):
         raise ValueError(f"out must be [{B}, {q.V}]")
-    ws = _workspace(workspace, N.lib().strim_head_logits_packed_workspace(B, K), hidden.device)
+    ws = _workspace(workspace, head_logits_q4_workspace(B, K), dev)
     N.check(N.lib().strim_head_logits_packed(
-        _stream(stream), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), float(eps),
+        _stream(stream), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
         _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
-        q.V, _ptr(ws), ws.numel() * ws.element_size(), _ptr(out), _dtype_code(out), q.V),
-        "strim_head_logits_packed")
+        q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
     return out
 
 
