@@ -330,6 +330,12 @@ def _check_bf16_rows(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} must be [rows, K] with contiguous rows")
 
 
+def _stream_of(stream, device: torch.device) -> int:
+    """The given stream's handle, or `device`'s current one (without the Stream object that
+    torch.cuda.current_stream makes, 2.6 us)."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _check_with(device: torch.device, *ts) -> None:
     """Contiguous tensors (or None) on `device`."""
     for t in ts:
@@ -401,7 +407,7 @@ def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor
     lse = torch.empty(R, dtype=torch.float32, device=dev)
     status = torch.empty(R, dtype=torch.int32, device=dev)
     ws = _workspace(workspace, head_loss_workspace(R, K, V), dev)
-    N.check(N.lib().strim_head_loss(_stream(stream), _ptr(hidden), _row_stride(hidden), R, K,
+    N.check(N.lib().strim_head_loss(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), R, K,
                                     _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
                                     ignore_index, _ptr(ws), _bytes(ws), _ptr(loss), _ptr(lse),
                                     _ptr(status)), "strim_head_loss")
@@ -427,7 +433,7 @@ def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.T
     dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
     dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
     ws = _workspace(workspace, head_loss_workspace(R, K, V, want_hidden, want_lm_head), dev)
-    N.check(N.lib().strim_head_loss_grad(_stream(stream), _ptr(hidden), _row_stride(hidden), R, K,
+    N.check(N.lib().strim_head_loss_grad(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), R, K,
                                          _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
                                          ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(grad_lse),
                                          _ptr(ws), _bytes(ws), _ptr(dh), K, _ptr(dw), K),
@@ -471,7 +477,7 @@ def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
     words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
     scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
     biases = None if symmetric else torch.empty_like(scales)
-    N.check(N.lib().strim_pack_weights(_stream(stream), _ptr(weight), code, _row_stride(weight), V,
+    N.check(N.lib().strim_pack_weights(_stream_of(stream, dev), _ptr(weight), code, _row_stride(weight), V,
                                        K, group, _ptr(words), _ptr(scales), _ptr(biases)),
             "strim_pack_weights")
     return Q4Weight(words, scales, biases, group)
@@ -480,7 +486,7 @@ def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
 def q4_unpack(q: Q4Weight, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """The values [V, K] that a packed projection stands for, as bf16 or float32."""
     out = torch.empty(q.V, q.K, dtype=dtype, device=q.words.device)
-    N.check(N.lib().strim_unpack_weights(_stream(stream), _ptr(q.words), q.K // 8, _ptr(q.scales),
+    N.check(N.lib().strim_unpack_weights(_stream_of(stream, out.device), _ptr(q.words), q.K // 8, _ptr(q.scales),
                                          _ptr(q.biases), q.K // q.group, q.V, q.K, q.group,
                                          _ptr(out), _dtype_code(out), q.K),
             "strim_unpack_weights")
@@ -516,7 +522,7 @@ def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor 
         raise ValueError(f"out must be [{B}, {q.V}]")
     ws = _workspace(workspace, head_logits_q4_workspace(B, K), dev)
     N.check(N.lib().strim_head_logits_packed(
-        _stream(stream), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
+        _stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
         _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
         q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
     return out
