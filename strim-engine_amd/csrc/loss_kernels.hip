@@ -569,6 +569,10 @@ struct LossPlan {
   int64_t part, tlogit, scale, p, acc, rows, bytes;  // offsets into the workspace
 };
 
+// p's rows end a line apart from a whole piece: rows a multiple of 8 KB apart, as pieces that
+// make whole rounds have them, meet in few memory channels.
+static int64_t loss_p_stride(int piece) { return piece + 64; }
+
 static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
   LossPlan q{};
   q.prob = loss_shape(V, N, 1, false);
@@ -584,15 +588,27 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
     q.bytes = off;
     return q;
   }
-  // pieces of the vocabulary whose tiles fill the CUs best
-  const int64_t vt = ceil_div(V, 256), tn = ceil_div(N, 256);
+  // The piece whose rounds of 256 x 256 tiles take least over all pieces: equal ones, or ones
+  // that end with whole rounds. (N = 4,096, V = 151,936, K = 5,120: 256 + 256 + 82 tiles of the
+  // vocabulary take 38 rounds of logits' products, three pieces of 198 take 39.)
+  const int64_t vt = ceil_div(V, 256), tn = ceil_div(N, 256), kt = ceil_div(K, 256);
   const int64_t most = LOSS_P_BYTES / (512 * (int64_t)N) > 1 ? LOSS_P_BYTES / (512 * (int64_t)N) : 1;
   int64_t best = -1, tiles = vt;
-  for (int64_t np = ceil_div(vt, most), e = np + 4; np < e; ++np) {
-    const int64_t t = ceil_div(vt, np), last = vt - t * (ceil_div(vt, t) - 1);
-    const int64_t rounds = (ceil_div(vt, t) - 1) * ceil_div(t * tn, LG_CUS) + ceil_div(last * tn, LG_CUS);
-    if (best < 0 || rounds < best) best = rounds, tiles = t;
-  }
+  auto offer = [&](int64_t t) {
+    if (t < 1 || t > most) return;
+    const int64_t full = ceil_div(vt, t) - 1, last = vt - t * full;
+    auto rounds = [&](int64_t side) {
+      return full * ceil_div(t * side, LG_CUS) + ceil_div(last * side, LG_CUS);
+    };
+    const int64_t cost = rounds(tn) * K + (head ? rounds(kt) * N : 0);
+    if (best < 0 || cost < best) best = cost, tiles = t;
+  };
+  const int64_t np = ceil_div(vt, most);
+  for (int64_t p = np; p < np + 3; ++p) offer(ceil_div(vt, p));
+  int64_t whole = LG_CUS;  // tiles of the vocabulary that make whole rounds
+  while (whole > 1 && whole / 2 * tn % LG_CUS == 0) whole /= 2;
+  if (np > 1)
+    for (int64_t t = most / whole * whole, e = t - 4 * whole; t > e; t -= whole) offer(t);
   q.piece = (int)(tiles * 256);
   q.prob = loss_shape(V < q.piece ? V : q.piece, N, 1, false);
   q.head = loss_shape(K, V < q.piece ? V : q.piece, 1, true);
@@ -609,7 +625,7 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
     if (us < least) least = us, q.splits = s, q.hid = shape;
   }
   q.scale = take(4);
-  q.p = take((int64_t)N * q.piece * 2);
+  q.p = take((int64_t)N * loss_p_stride(q.piece) * 2);
   if (hid) q.acc = take((int64_t)q.splits * N * K * 4);
   if (head) q.rows = take((int64_t)N * K * 2);
   q.bytes = off;
@@ -705,12 +721,12 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
     g.grad_lse = grad_lse;
     g.scale = (float*)(w8 + q.scale);
     g.out16 = p;
-    g.out_stride = q.piece;
+    g.out_stride = loss_p_stride(q.piece);
     loss_gemm<LM_PROB>(g, q.prob, vn, N, st);
     if (d_hidden) {
       LossGemm h{};
       h.a = LossOperand{wv, ws, K};
-      h.b = LossOperand{p, q.piece, N};
+      h.b = LossOperand{p, loss_p_stride(q.piece), N};
       h.red = vn;
       h.splits = q.splits;
       h.split_red = (int)(ceil_div(ceil_div(vn, LG_BK), q.splits) * LG_BK);
@@ -723,7 +739,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
     if (d_head) {
       LossGemm h{};
       h.a = LossOperand{rows, K, K};
-      h.b = LossOperand{p, q.piece, vn};
+      h.b = LossOperand{p, loss_p_stride(q.piece), vn};
       h.red = N;
       h.splits = 1;
       h.split_red = (int)(ceil_div(N, LG_BK) * LG_BK);
