@@ -42,15 +42,43 @@ struct Q4Pack {
   uint16_t *scales, *biases;
 };
 
+// Largest (or least) of the lanes of a group of 4, 8 or 16, in every lane: neighbours, pairs,
+// then the mirrored half rows and rows.
+template <int LANES, bool MAX>
+__device__ __forceinline__ float q4_extreme(float v) {
+  auto with = [&](int other) {
+    const float o = __int_as_float(other);
+    v = MAX ? fmaxf(v, o) : fminf(v, o);
+  };
+  with(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0xB1, 0xF, 0xF, false));  // 1 0 3 2
+  with(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x4E, 0xF, 0xF, false));  // 2 3 0 1
+  if constexpr (LANES > 4) with(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, false));
+  if constexpr (LANES > 8) with(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, false));
+  return v;
+}
+
+// The items (row, eight elements) that a thread takes: every `stride` of the whole.
+struct Q4Walk {
+  int64_t v, dv;
+  int c, dc, per_row;
+  __device__ __forceinline__ Q4Walk(int K) : per_row(K / 8) {
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, stride = (int64_t)gridDim.x * 256;
+    v = first / per_row, c = (int)(first - v * per_row);
+    dv = stride / per_row, dc = (int)(stride - dv * per_row);
+  }
+  __device__ __forceinline__ void next() {
+    v += dv, c += dc;
+    if (c >= per_row) c -= per_row, ++v;
+  }
+};
+
 template <int G, bool F32, bool SYM>
 __global__ __launch_bounds__(256) void k_q4_pack(const Q4Pack a) {
-  const int per_row = a.K / 8;
-  const int64_t total = (int64_t)a.V * per_row;
-  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  // whole groups: total and the stride are multiples of G / 8, which divides a wave
-  for (int64_t i = first; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t v = i / per_row;
-    const int c = (int)(i - v * per_row);
+  // (a group's lanes run together: K / 8 and the stride are multiples of G / 8, which divides a row
+  // of 16 lanes)
+  for (Q4Walk at(a.K); at.v < a.V; at.next()) {
+    const int64_t v = at.v;
+    const int c = at.c;
     float x[8];
     if constexpr (F32) {
       const float4* p = (const float4*)((const float*)a.w + v * a.w_stride + 8 * c);
@@ -73,23 +101,39 @@ __global__ __launch_bounds__(256) void k_q4_pack(const Q4Pack a) {
       lo = fminf(lo, x[e]);
       bad += 0.0f * x[e];  // NaN where an element is not finite
     }
-#pragma unroll
-    for (int d = 1; d < G / 8; d <<= 1) {
-      hi = fmaxf(hi, __shfl_xor(hi, d));
-      if constexpr (!SYM) lo = fminf(lo, __shfl_xor(lo, d));
-      bad += __shfl_xor(bad, d);
-    }
-    const uint32_t s16 = q4_bf16((SYM ? hi * (1.0f / 7.0f) : (hi - lo) * (1.0f / 15.0f)) + bad);
-    const uint32_t b16 = SYM ? 0u : q4_bf16(lo + bad);
+    // (as an infinity, which the maximum carries on)
+    if (!(bad == 0.0f)) hi = INFINITY;
+    hi = q4_extreme<G / 8, true>(hi);
+    if constexpr (!SYM) lo = q4_extreme<G / 8, false>(lo);
+    const float nan = hi < INFINITY ? 0.0f : __uint_as_float(0x7FC00000u);
+    const uint32_t s16 = q4_bf16((SYM ? hi * (1.0f / 7.0f) : (hi - lo) * (1.0f / 15.0f)) + nan);
+    const uint32_t b16 = SYM ? 0u : q4_bf16(lo + nan);
     const float s = __uint_as_float(s16 << 16), b = __uint_as_float(b16 << 16);
+    // The correctly rounded quotient from the correctly rounded reciprocal, with one correction
+    // (Markstein's theorem; scales near the ends of the range divide instead), and its rounding to
+    // an integer by a sum whose unit is one.
+    constexpr float ONE = 12582912.0f;  // 1.5 2^23
+    constexpr float LO = SYM ? -8.0f : 0.0f, HI = SYM ? 7.0f : 15.0f;
+    float q[8];
+    const bool plain = s == 0.0f || (s > 0x1p-60f && s < 0x1p60f);
+    if (__ballot(!plain) == 0) {
+      const float r = s > 0.0f ? 1.0f / s : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = SYM ? x[e] : x[e] - b, t = d * r;
+        q[e] = __builtin_fmaf(__builtin_fmaf(-t, s, d), r, t);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = s > 0.0f ? (SYM ? x[e] : x[e] - b) / s : 0.0f;
+    }
     uint32_t word = 0u;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float q = s > 0.0f ? rintf((SYM ? x[e] : x[e] - b) / s) : 0.0f;
-      if constexpr (SYM) q += 8.0f;
-      word |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * e);
+      const float n = fminf(fmaxf(q[e], LO), HI) + (ONE + (SYM ? 8.0f : 0.0f));
+      word |= (__float_as_uint(n) & 15u) << (4 * e);
     }
-    a.words[i] = word;
+    a.words[v * at.per_row + c] = word;
     if (c % (G / 8) == 0) {
       const int64_t g = v * (a.K / G) + c / (G / 8);
       a.scales[g] = (uint16_t)s16;
@@ -109,11 +153,9 @@ struct Q4Weights {
 
 template <int G, bool F32>
 __global__ __launch_bounds__(256) void k_q4_unpack(const Q4Weights a, void* out, int64_t out_stride) {
-  const int per_row = a.K / 8;
-  const int64_t total = (int64_t)a.V * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t v = i / per_row;
-    const int c = (int)(i - v * per_row);
+  for (Q4Walk at(a.K); at.v < a.V; at.next()) {
+    const int64_t v = at.v;
+    const int c = at.c;
     const uint32_t word = a.words[v * a.words_stride + c];
     const int64_t g = v * a.scales_stride + c / (G / 8);
     const float s = __uint_as_float((uint32_t)a.scales[g] << 16);

@@ -268,3 +268,24 @@ def test_refusals():
     assert call(ws=None) == N.EINVAL
     assert call(wb=need - 1) == N.ECAPACITY
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_pack_scales_near_the_ends_of_the_range(symmetric):
+    """Groups whose scale is subnormal, huge, or exactly between two codes everywhere: the codes
+    are those of the correctly rounded quotient."""
+    K, G = 256, 64
+    w = torch.randn(40, K, device="cuda", generator=gen(6))
+    w *= torch.exp2(torch.linspace(-140, 120, 40, device="cuda"))[:, None]
+    w[3] = (torch.arange(K, device="cuda") % 31) * 0.5  # halves of a step
+    w[3, ::G] = 0.0
+    w[3, 1::G] = 15.0
+    w[3, 2::G] = -7.0 if symmetric else 0.0
+    q = ops.q4_pack(w, G, symmetric)
+    d = w.reshape(40, -1, G)
+    s = q.scales.float()[..., None]
+    if symmetric:
+        ref = torch.where(s > 0, d / s, 0.0).round() + 8
+    else:
+        ref = torch.where(s > 0, (d - q.biases.float()[..., None]) / s, 0.0).round()
+    assert torch.equal(codes(q), ref.clamp(0, 15).double())
