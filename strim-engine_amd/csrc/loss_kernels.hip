@@ -334,12 +334,13 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
   };
   static_assert(TM % 2 == 0, "tiles are stored by twos");
   if constexpr (MODE == LM_STATS) {
-    if (mw + TM * 16 > g.V) {  // past the vocabulary: nothing
+    const int left = g.V - g.v0;
+    if (mw + TM * 16 > left) {  // past the vocabulary: nothing
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (m0 + 16 * i + r >= g.V)
+          if (m0 + 16 * i + r >= left)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j][r] = -INFINITY;
     }
@@ -347,7 +348,7 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + 16 * j;
       const int t = n < g.b.rows ? g.targets[n] : -1;
-      const int at = t < g.V ? t - m0 : -1;  // the target's place among this lane's rows
+      const int at = t >= 0 && t < g.V ? t - g.v0 - m0 : -1;  // the target's place among this lane's rows
       float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
@@ -535,9 +536,6 @@ static int shape_n(LossShape s) {
 static int shape_slice(LossShape s) {
   return s == LS_256x256 ? 128 : s == LS_128x64 || s == LS_256x64 ? 32 : 64;
 }
-static int64_t loss_slices(int V, LossShape s) {
-  return ceil_div(V, shape_m(s)) * (shape_m(s) / shape_slice(s));
-}
 // about how long a step (64 along the reduction) of a CU's round of tiles takes, us, and how
 // many tiles a round has
 static double shape_us(LossShape s) {
@@ -545,19 +543,40 @@ static double shape_us(LossShape s) {
 }
 static int64_t shape_round(LossShape s) { return shape_m(s) == 128 ? 2 * LG_CUS : LG_CUS; }
 
-// The tile for an M x N result, `splits` times over: the one whose rounds take least.
+// us a step that an M x N result, `splits` times over, takes in tiles of one shape
+static double shape_cost(LossShape s, int64_t m, int64_t n, int64_t splits) {
+  const int64_t tiles = ceil_div(m, shape_m(s)) * ceil_div(n, shape_n(s)) * splits;
+  // (a round of few 128-row tiles leaves each a CU of its own)
+  const double alone = tiles <= LG_CUS && shape_m(s) == 128 ? 0.6 : 1.0;
+  return alone * shape_us(s) * (double)ceil_div(tiles, shape_round(s));
+}
+
+// The shape whose rounds take least.
 static LossShape loss_shape(int64_t m, int64_t n, int64_t splits, bool head) {
   LossShape best = LS_256x256;
   double least = 1e30;
   for (LossShape s : {LS_256x256, LS_256x128, LS_256x64, LS_128x128, LS_128x64}) {
     if (head && s != LS_256x256 && s != LS_128x128) continue;
-    const int64_t tiles = ceil_div(m, shape_m(s)) * ceil_div(n, shape_n(s)) * splits;
-    // (a round of few 128-row tiles leaves each a CU of its own)
-    const double alone = tiles <= LG_CUS && shape_m(s) == 128 ? 0.6 : 1.0;
-    const double us = alone * shape_us(s) * (double)ceil_div(tiles, shape_round(s));
+    const double us = shape_cost(s, m, n, splits);
     if (us < least * 0.999) least = us, best = s;
   }
   return best;
+}
+
+// Of `v` vocabulary rows by `other` in large tiles, those (a multiple of 256) of whole rounds,
+// where the rest takes half a round of large ones or less in smaller tiles (`rest`) and a launch of
+// its own; else all. (N = 1,003, V = 100,003, K = 2,056, 28 tiles past six rounds: the loss 478 ->
+// 442 us; with two thirds of a round, N = 700, V = 50,000, K = 2,048: the gradients 486 -> 497.)
+static int64_t loss_main(LossShape shape, int64_t v, int64_t other, int64_t steps, bool head,
+                         LossShape& rest) {
+  if (shape != LS_256x256) return v;
+  const int64_t row = ceil_div(other, 256), rounds = ceil_div(v, 256) * row / LG_CUS;
+  const int64_t main = rounds * LG_CUS / row * 256;
+  if (main == 0 || main >= v) return v;
+  rest = head ? loss_shape(other, v - main, 1, true) : loss_shape(v - main, other, 1, false);
+  const double all = shape_cost(shape, v, other, 1), large = shape_cost(shape, main, other, 1);
+  const double small = head ? shape_cost(rest, other, v - main, 1) : shape_cost(rest, v - main, other, 1);
+  return small <= 0.5 * shape_us(LS_256x256) && (all - large - small) * steps > 20.0 ? main : v;
 }
 
 struct LossPlan {
@@ -568,6 +587,14 @@ struct LossPlan {
   int splits;      // d_hidden: parts of a piece's vocabulary
   int64_t part, tlogit, scale, p, acc, rows, bytes;  // offsets into the workspace
 };
+
+// slices that LM_STATS writes
+static int64_t loss_slices(int64_t V, int64_t N, int64_t K, LossShape s) {
+  auto slices = [](int64_t v, LossShape t) { return ceil_div(v, shape_m(t)) * (shape_m(t) / shape_slice(t)); };
+  LossShape rest = s;
+  const int64_t main = loss_main(s, V, N, ceil_div(K, LG_BK), false, rest);
+  return slices(main, s) + (main < V ? slices(V - main, rest) : 0);
+}
 
 // p's rows end a line apart from a whole piece: rows a multiple of 8 KB apart, as pieces that
 // make whole rounds have them, meet in few memory channels.
@@ -655,6 +682,29 @@ static void loss_gemm(const LossGemm& g, LossShape s, int64_t m, int64_t n, hipS
   }
 }
 
+// The products along the vocabulary (M side; LM_DHEAD: N side): large tiles, then the rest of them.
+template <int MODE>
+static void loss_gemm_vocab(const LossGemm& g, LossShape s, int64_t v, int64_t other, hipStream_t st) {
+  constexpr bool HEAD = MODE == LM_DHEAD;
+  LossShape rest = s;
+  const int64_t main = loss_main(s, v, other, ceil_div(g.red, LG_BK), HEAD, rest);
+  loss_gemm<MODE>(g, s, HEAD ? other : main, HEAD ? main : other, st);
+  if (main == v) return;
+  LossGemm t = g;
+  t.v0 += (int)main;
+  if constexpr (HEAD) {
+    t.b.p += main;
+    t.b.rows -= (int)main;
+    t.out16 += main * g.out_stride;
+  } else {
+    t.a.p += main * g.a.stride;
+    t.a.rows -= (int)main;
+    if constexpr (MODE == LM_STATS) t.part += main / shape_slice(s) * g.b.rows;
+    else t.out16 += main;
+  }
+  loss_gemm<MODE>(t, rest, HEAD ? other : v - main, HEAD ? v - main : other, st);
+}
+
 hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws, int V,
                        const int32_t* targets, int ignore_index, void* workspace, float* loss,
                        float* lse, int32_t* status, hipStream_t st) {
@@ -671,8 +721,8 @@ hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void*
   g.targets = targets;
   g.part = (float2*)(w8 + q.part);
   g.tlogit = (float*)(w8 + q.tlogit);
-  loss_gemm<LM_STATS>(g, q.prob, V, N, st);
-  const int slices = (int)loss_slices(V, q.prob);
+  loss_gemm_vocab<LM_STATS>(g, q.prob, V, N, st);
+  const int slices = (int)loss_slices(V, N, K, q.prob);
   if (N >= 1024)
     hipLaunchKernelGGL(k_loss_rows<16>, dim3((unsigned)ceil_div(N, 16)), dim3(256), 0, st, g.part,
                        slices, N, g.tlogit, targets, ignore_index, V, loss, lse, status);
@@ -722,7 +772,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
     g.scale = (float*)(w8 + q.scale);
     g.out16 = p;
     g.out_stride = loss_p_stride(q.piece);
-    loss_gemm<LM_PROB>(g, q.prob, vn, N, st);
+    loss_gemm_vocab<LM_PROB>(g, q.prob, vn, N, st);
     if (d_hidden) {
       LossGemm h{};
       h.a = LossOperand{wv, ws, K};
@@ -746,7 +796,7 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
       h.scale = g.scale;
       h.out16 = (uint16_t*)d_head + (int64_t)v0 * dws;
       h.out_stride = dws;
-      loss_gemm<LM_DHEAD>(h, q.head, K, vn, st);
+      loss_gemm_vocab<LM_DHEAD>(h, q.head, vn, K, st);
     }
   }
   if (d_hidden)

@@ -139,6 +139,17 @@ def test_pieces_of_the_vocabulary():
     within(dw, dwr, tol_w + 2.0 ** -8 * dwr.abs(), "d_lm_head")
 
 
+@pytest.mark.parametrize("R,K,V", [(1000, 1536, 66_003), (1003, 2048, 33_100), (2050, 1024, 33_281)])
+def test_rest_in_smaller_tiles(R, K, V):
+    """More tiles than whole rounds over the chip, so that the last of the vocabulary is computed
+    apart in smaller ones: targets on both sides of every seam."""
+    print(f"[loss] rest N={R} K={K} V={V}", flush=True)
+    h, w, t, gl = inputs(R, K, V, seed=V, ignored=0.1)
+    edge = V - 1 - 64 * torch.arange(200, device="cuda")
+    t[:200] = edge.to(torch.int32)
+    check(h, w, t, gl, label=f"N={R} K={K} V={V}")
+
+
 def test_padding_counts_for_nothing():
     """Rows without a target, and with one outside the vocabulary: no loss, no gradient,
     whatever their states and their gradients hold."""
