@@ -610,7 +610,7 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
     return at;
   };
   if (!hid && !head) {
-    q.part = take(ceil_div(V, 256) * 8 * N * (int64_t)sizeof(float2));
+    q.part = take(loss_slices(V, N, K, q.prob) * N * (int64_t)sizeof(float2));
     q.tlogit = take(4 * (int64_t)N);
     q.bytes = off;
     return q;

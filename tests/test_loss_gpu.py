@@ -364,3 +364,40 @@ def test_refusals():
     assert call(wb=16) == N.ECAPACITY
     assert lib.strim_head_loss_workspace(4, 60, 100, 0, 0) == N.EINVAL
     torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits():
+    """A projection, and its gradient, of more than 2^31 elements: rows at both ends."""
+    V, K, R = 210_000, 10_240, 3
+    print("[loss] 2^31 elements", flush=True)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(51)
+    w = torch.randn(V, K, device="cuda", generator=g, dtype=torch.bfloat16).mul_(0.01)
+    t = torch.tensor([V - 1, 0, V - 131], dtype=torch.int32, device="cuda")
+    h = (torch.randn(R, K, device="cuda", generator=g) + 30 * w[t.long()].float()).to(torch.bfloat16)
+    x = torch.cat([h.double() @ w[a:a + 30_000].double().T for a in range(0, V, 30_000)], 1)
+    lse = torch.logsumexp(x, 1)
+    ref = lse - x.gather(1, t.long()[:, None])[:, 0]
+    S = max(float((h[i].double().abs() * w[t[i].long()].double().abs()).sum()) for i in range(R)) * 2
+    e = 2e-6 * S + 4e-6 + 2.0 ** -22 * float(lse.abs().max())
+    loss, got, _ = ops.head_loss(h, w, t)
+    assert float((loss.double() - ref).abs().max()) <= e
+    one = torch.ones(R, device="cuda")
+    _, dw = ops.head_loss_grad(h, w, t, got, one, want_hidden=False)
+    p = torch.exp(x - lse[:, None])
+    p.scatter_add_(1, t.long()[:, None], -one.double()[:, None])
+    for rows in (slice(0, 40), slice(V - 140, V)):
+        want = p[:, rows].T @ h.double()
+        bound = (p[:, rows].abs().T @ h.double().abs()) * (2.0 ** -7 + 4 * e) + 1e-30
+        # (not the targets' rows, where p is the small difference of two rounded terms)
+        other = torch.ones(V, dtype=torch.bool, device="cuda")
+        other[t.long()] = False
+        other = other[rows]
+        within(dw[rows][other], want[other], bound[other], "d_lm_head")
+
+
+def test_many_rows():
+    """More rows than a workgroup's worth of everything, at the smallest sizes."""
+    R, K, V = 70_001, 16, 300
+    h, w, t, gl = inputs(R, K, V, seed=61)
+    check(h, w, t, gl, label="many rows")

@@ -289,3 +289,21 @@ def test_pack_scales_near_the_ends_of_the_range(symmetric):
     else:
         ref = torch.where(s > 0, (d - q.biases.float()[..., None]) / s, 0.0).round()
     assert torch.equal(codes(q), ref.clamp(0, 15).double())
+
+
+def test_offsets_past_32_bits():
+    """Words of more than 2^31 bytes: the last rows' logits, read back values and packing."""
+    V, K, G = 430_000, 10_240, 128
+    print("[q4] 2^31 bytes", flush=True)
+    q = weight(V, K, G, False, seed=77)
+    tail = ops.Q4Weight(q.words[-300:].contiguous(), q.scales[-300:].contiguous(),
+                        q.biases[-300:].contiguous(), G)
+    for B in (2, 20):
+        x = torch.randn(B, K, device="cuda", generator=gen(B)).to(torch.bfloat16)
+        got = ops.head_logits_q4(x, q)
+        check_logits(x, tail, got[:, -300:], f"B={B}")
+    v = ops.q4_unpack(q)
+    assert torch.equal(v[-300:], ops.q4_unpack(tail))
+    p = ops.q4_pack(v, G)
+    t = ops.q4_pack(v[-300:].contiguous(), G)
+    assert torch.equal(p.words[-300:], t.words) and torch.equal(p.scales[-300:], t.scales)
