@@ -28,7 +28,8 @@ __device__ __forceinline__ uint32_t q4_bf16(float f) {
 }
 
 // ---- packing ------------------------------------------------------------------------------
-// Eight elements a thread, G / 8 neighbouring lanes a group.
+// Eight elements a thread, G / 8 neighbouring lanes a group; bound by HBM (V = 32,768, K = 5,120,
+// bf16, groups of 64: 103 us, 4.2 TB/s; reading back 83 us, 5.2 TB/s).
 //   biased:    s = bf16((max - min) / 15), b = bf16(min), q = clamp(rint((w - b) / s), 0, 15)
 //   symmetric: s = bf16(max|w| / 7),                      q = clamp(rint(w / s) + 8, 0, 15)
 // s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). The divisions by 15 and 7
@@ -298,14 +299,15 @@ __global__ __launch_bounds__(WAVE) void k_q4_blocks(const Q4Args a) {
 // waves read their weights without meeting. A unit is four steps of a row tile; the workgroup's
 // row tiles are one run of units, cut evenly between the waves, so a wave has whole tiles and at
 // most a piece at either end. The pieces are added through LDS at the end, in the order of the
-// waves. RB: result registers a lane that hold rows (1, 2 or 4 for up to 4, 8, 16 rows). D:
-// units in flight. WHOLE: K a multiple of a unit's 512; otherwise K of 8 groups or more.
+// waves. RB: result registers a lane that hold rows (1 or 2 for up to 4 or 8 rows). D: units in
+// flight. WHOLE: K a multiple of a unit's 512; otherwise K of 8 groups or more. This form, with the
+// weights through registers, is for scales that k_q4_dma cannot take (one row at V = 151,936,
+// K = 5,120, groups of 64: 105 us, k_q4_dma 90).
 //
 // What bounds it is the address unit: lanes of one 16-byte load that are neighbours are in
 // different rows, so each lane's piece is looked up by itself, 16 bytes a cycle. A unit's scales
 // and biases therefore come by one such load (even quarters the scales, odd ones the biases,
-// exchanged between the quarters afterwards) and not by one a step: with those this kernel took
-// 178 us for one row at V = 151,936, K = 5,120, groups of 64.
+// exchanged between the quarters afterwards) and not by one a step: with those it took 178 us.
 constexpr int QS_NW = 16;
 constexpr size_t QS_LDS = 160 * 1024;
 
@@ -524,6 +526,14 @@ __device__ __forceinline__ void q4_load_lds(uint32_t lds, const void* p) {
                  ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(p) : "memory");
 }
 
+// k_q4_stream with the weights straight to LDS, each wave's two units in a ring of its own (as many
+// waves as the hidden rows leave room for, six or more): an instruction's lanes take four rows of 256
+// bytes, sixteen neighbours to a row, so the address unit no longer bounds it but HBM does (one row
+// at V = 151,936, K = 5,120, groups of 64, 438 MB: 90 us, 5.7 of them the launch's start and end, the
+// rest at 5.2 TB/s). A row's pieces lie in its place xor its number, where the waves' reads meet all
+// banks evenly. The weights are marked as not read again: the scales' lines, read a piece at a time
+// by unit after unit, stay in L2 (99 us and 493 MB from HBM without). An even number of groups, scales
+// and biases 4-byte aligned, K of 8 groups or more.
 template <int G, int RB, bool WHOLE>
 __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int tiles) {
   constexpr int GPS = 128 / G, MPG = 4 / GPS, ROWS = 4 * RB;
@@ -706,7 +716,10 @@ __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int t
 // chunks of four steps, two chunks at a time (straight from k_q4_blocks' image of them), and a
 // wave goes through its MT row tiles chunk by chunk, two at a time (a fragment read from LDS
 // serves both), their sums in registers. The code of a chunk has no branches between its
-// requests, so that each wait is for the oldest alone. Any alignment, any number of groups.
+// requests, so that each wait is for the oldest alone. Any alignment, any number of groups. At
+// V = 151,936, K = 5,120, groups of 64: 16 rows 116 us, 32 rows 146, 64 rows 219 (128: 200); the
+// arithmetic alone takes 57 of the 116 and 177 of the 219, its vector instructions and MFMA hardly
+// side by side with two waves a SIMD.
 constexpr int QC_NW = 8;
 
 template <int I>
@@ -960,10 +973,13 @@ template <int G, int RB, int D>
 static bool q4_stream(const Q4Args& a, hipStream_t st) {
   const int steps = (a.w.K + 511) / 512 * 4, tiles = (a.w.V + 15) / 16;
   const size_t own = (size_t)steps * q4_step_bytes<G, RB>();
+  // Through LDS with seven waves or more, where each lane's scale load may be two groups by two:
+  // at V = 65,536, groups of 64, 8 rows, K = 5,120 (seven waves) 48.1 us, through registers 50.8;
+  // K = 6,656 (five) 67.1 against 60.2, K = 8,192 (two) 139 against 76.
   const bool even = (a.w.K / G) % 2 == 0 && a.w.scales_stride % 2 == 0 && ((uintptr_t)a.w.scales & 3) == 0 &&
                     ((uintptr_t)a.w.biases & 3) == 0 && a.w.K >= 8 * G;
   const int nw = own < QS_LDS ? (int)((QS_LDS - own) / 10240) : 0;
-  if (even && nw >= 6) {
+  if (even && nw >= 7) {
     const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
     const int w = nw < QS_NW ? nw : QS_NW;
     const size_t lds = own + (size_t)w * 10240;
@@ -997,6 +1013,7 @@ static void q4_blocks(const Q4Args& a, hipStream_t st) {
     return;
   }
   // tiles a wave: what takes the fewest tile times over all rounds; few tiles: smaller workgroups
+  // (K = 5,120, 16 rows, V = 4,096: 19.6 us, by eight waves 23.2; V = 16,000: 26.2 against 28.8)
   const int nw = tiles >= 4 * 256 ? QC_NW : tiles >= 2 * 256 ? 4 : 2;
   int best = 1, least = 1 << 30;
   for (int mt : {1, 2, 3, 5}) {
@@ -1010,6 +1027,8 @@ static void q4_blocks(const Q4Args& a, hipStream_t st) {
   else if constexpr (Q4_FIVE<G, NT>) q4_chunk<G, NT, 5>(a, nw, st);
 }
 
+// Up to 8 rows from LDS (V = 151,936, K = 5,120, groups of 64, 8 rows: 99 us, by k_q4_chunk 116; V =
+// 8,192: 12.7 against 21.4), up to 4 of them with half the places (4 rows: 92.8 us, as up to 8: 95.6).
 template <int G>
 static void q4_logits(const Q4Args& a, hipStream_t st) {
   if (a.B <= 4 && q4_stream<G, 1, 2>(a, st)) return;
