@@ -247,10 +247,11 @@ struct Q4Args {
   const uint16_t* x;   // hidden [B][x_stride]
   int64_t x_stride;
   int32_t B;
-  uint8_t* blocks;     // k_q4_stage: the hidden rows' fragments and group sums, by steps
+  uint8_t* blocks;     // k_q4_blocks: the hidden rows' fragments and group sums, by steps
   void* out;
   int64_t out_stride;
   int32_t out_f32;
+  float* part;         // k_q4_chunk split along K: sums [split][B][V]
 };
 
 // Row of the batch at place m of an MFMA's 16: rows 0 .. 3 at places 0, 4, 8, 12, so that
@@ -270,28 +271,26 @@ __device__ __forceinline__ qf32x4 q4_sum(qu32x4 x, qf32x4 acc) {
 }
 
 // The hidden rows by steps: per step 4 NT fragments of 1 KB (MFMA t of batch tile nt at t NT +
-// nt, 16 bytes a lane), then the sums X [group][NT][16 places], padded to 1 KB.
+// nt, 16 bytes a lane), then the sums X [group][NT][16 places], padded to 1 KB. A wave a step and
+// batch tile.
 template <int G, int NT>
 __global__ __launch_bounds__(WAVE) void k_q4_blocks(const Q4Args a) {
   constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
-  const int lane = threadIdx.x, h = lane >> 4, m = lane & 15, step = blockIdx.x;
+  const int lane = threadIdx.x, h = lane >> 4, m = lane & 15, step = blockIdx.x, nt = blockIdx.y;
   uint8_t* blk = a.blocks + (int64_t)step * BLOCK;
+  const int b = 16 * nt + q4_row(m);
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int b = 16 * nt + q4_row(m);
+  for (int g = 0; g < GPS; ++g) {
+    qf32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < GPS; ++g) {
-      qf32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int q = 0; q < MPG; ++q) {
-        const int t = g * MPG + q, k = step * 128 + q4_koff<G>(t, h);
-        qu32x4 x = {0u, 0u, 0u, 0u};
-        if (b < a.B && k < a.w.K) x = q4_interleave(*(const qu32x4*)(a.x + (int64_t)b * a.x_stride + k));
-        *(qu32x4*)(blk + (t * NT + nt) * 1024 + lane * 16) = x;
-        s = q4_sum(x, s);
-      }
-      if (m == 0) *(qf32x4*)(blk + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4) = s;
+    for (int q = 0; q < MPG; ++q) {
+      const int t = g * MPG + q, k = step * 128 + q4_koff<G>(t, h);
+      qu32x4 x = {0u, 0u, 0u, 0u};
+      if (b < a.B && k < a.w.K) x = q4_interleave(*(const qu32x4*)(a.x + (int64_t)b * a.x_stride + k));
+      *(qu32x4*)(blk + (t * NT + nt) * 1024 + lane * 16) = x;
+      s = q4_sum(x, s);
     }
+    if (m == 0) *(qf32x4*)(blk + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4) = s;
   }
 }
 
@@ -716,7 +715,8 @@ __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int t
 // chunks of four steps, two chunks at a time (straight from k_q4_blocks' image of them), and a
 // wave goes through its MT row tiles chunk by chunk, two at a time (a fragment read from LDS
 // serves both), their sums in registers. The code of a chunk has no branches between its
-// requests, so that each wait is for the oldest alone. Any alignment, any number of groups. At
+// requests, so that each wait is for the oldest alone. Any alignment, any number of groups. PARTS:
+// gridDim.y parts of K, their sums to `part`. At
 // V = 151,936, K = 5,120, groups of 64: 16 rows 116 us, 32 rows 146, 64 rows 219 (128: 200); the
 // arithmetic alone takes 57 of the 116 and 177 of the 219, its vector instructions and MFMA hardly
 // side by side with two waves a SIMD.
@@ -727,7 +727,7 @@ struct QInt {
   static constexpr int value = I;
 };
 
-template <int G, int NT, int MT>
+template <int G, int NT, int MT, bool PARTS>
 __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
   constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024, CHUNK = 4 * BLOCK;
   constexpr int SW = G == 128 ? 2 : 4;  // words of scales a lane loads
@@ -737,6 +737,11 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
   const int nw = blockDim.x / WAVE;
   const int units = (a.w.K + 511) / 512, groups = a.w.K / G, pieces = a.w.K / 32;
   const int v0 = (blockIdx.x * nw + wv) * MT * 16;
+  int first = 0, last = units;  // this workgroup's chunks of K
+  if constexpr (PARTS) {
+    first = (int)((int64_t)units * blockIdx.y / gridDim.y);
+    last = (int)((int64_t)units * (blockIdx.y + 1) / gridDim.y);
+  }
   const bool sym = a.w.biases == nullptr;
   const uint16_t* side = (h & 1) && !sym ? a.w.biases : a.w.scales;
   const int sofs = G == 32 ? 8 * (h >> 1) : 0;  // the upper quarters: a unit's second eight
@@ -865,18 +870,18 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
     // (more than 16 rows: two pairs of tiles at once are more than the registers hold)
     if constexpr (NT > 1) __builtin_amdgcn_sched_barrier(0);
   };
-  bring(0);
+  bring(first);
 #pragma unroll
   for (int j = 0; j < (MT > 1 ? 2 : 1); ++j) {
-    load_scales(buf[j], 0, j);
+    load_scales(buf[j], first, j);
 #pragma unroll
-    for (int p = 0; p < 4; ++p) load_words(buf[j], 0, j, p);
+    for (int p = 0; p < 4; ++p) load_words(buf[j], first, j, p);
   }
-  for (int c = 0; c < units; ++c) {
+  for (int c = first; c < last; ++c) {
     // every wave's part of the chunk has arrived (a unit's request is four loads or more, and one
     // or more units were requested since), and none reads the other half any more
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(MT > 1 ? 8 : 4) : "memory");
-    if (c + 1 < units) bring(c + 1);
+    if (c + 1 < last) bring(c + 1);
     if constexpr (MT > 1) compute(c, QInt<0>{}, QInt<2>{});
     if constexpr (MT > 3) compute(c, QInt<2>{}, QInt<2>{});
     if constexpr (MT % 2) compute(c, QInt<MT - 1>{}, QInt<1>{});
@@ -891,9 +896,21 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int b = 16 * nt + q4_row(4 * h + r);
-        if (b < a.B) q4_store(a, b, v, acc[i][nt][r]);
+        if (b >= a.B) continue;
+        if (!PARTS) q4_store(a, b, v, acc[i][nt][r]);
+        else a.part[((int64_t)blockIdx.y * a.B + b) * a.w.V + v] = acc[i][nt][r];
       }
   }
+}
+
+// The results of a product split along K: its parts' sums, in their order.
+__global__ __launch_bounds__(256) void k_q4_join(const Q4Args a, int splits) {
+  const int v = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+  if (v >= a.w.V) return;
+  float y = 0.0f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) y += a.part[((int64_t)s * a.B + b) * a.w.V + v];
+  q4_store(a, b, v, y);
 }
 
 // K of fewer than eight groups: one wave a row tile, straightforwardly.
@@ -950,13 +967,21 @@ __global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
 // ---- host ---------------------------------------------------------------------------------
 static int q4_tiles_n(int B) { return B <= 16 ? 1 : B <= 32 ? 2 : 4; }
 
+static int64_t q4_blocks_bytes(int B, int K) {
+  return ((int64_t)K + 511) / 512 * 4 * (4 * q4_tiles_n(B) + 1) * 1024;
+}
+
+// k_q4_chunk's row tiles, over all its parts of K, are this many at most: eight waves a CU.
+constexpr int QC_SPLIT = 2048;
+
 // None where k_q4_stream (or k_q4_dma) takes the rows whatever the groups: they fit its LDS.
 int64_t q4_workspace(int B, int K) {
   const int64_t steps = ((int64_t)K + 511) / 512 * 4;
   const bool one = B <= 4 && steps * q4_step_bytes<32, 1>() + QS_NW * 2 * 1 * WAVE * 4 <= (int64_t)QS_LDS;
   const bool two = B <= 8 && steps * q4_step_bytes<32, 2>() + QS_NW * 2 * 2 * WAVE * 4 <= (int64_t)QS_LDS;
   if (K >= 8 * 128 && (one || two)) return 0;
-  return ((int64_t)K + 511) / 512 * 4 * (4 * q4_tiles_n(B) + 1) * 1024;
+  const int rows = B < 64 ? B : 64;
+  return q4_blocks_bytes(B, K) + (int64_t)QC_SPLIT * 16 * rows * 4;
 }
 
 // A launch with more than 64 KB of LDS, which a kernel has to be told of once.
@@ -993,10 +1018,10 @@ static bool q4_stream(const Q4Args& a, hipStream_t st) {
                           : q4_big_lds<k_q4_stream<G, RB, D, false>>(grid, lds, st, a, QS_NW, tiles);
 }
 
-template <int G, int NT, int MT>
-static void q4_chunk(const Q4Args& a, int nw, hipStream_t st) {
+template <int G, int NT, int MT, bool PARTS = false>
+static void q4_chunk(const Q4Args& a, int nw, int splits, hipStream_t st) {
   const int tiles = (a.w.V + 15) / 16, each = nw * MT;
-  q4_big_lds<k_q4_chunk<G, NT, MT>>(dim3((unsigned)((tiles + each - 1) / each)),
+  q4_big_lds<k_q4_chunk<G, NT, MT, PARTS>>(dim3((unsigned)((tiles + each - 1) / each), (unsigned)splits),
                                     (size_t)2 * 4 * (4 * NT + 1) * 1024, st, a, nw);
 }
 
@@ -1007,24 +1032,43 @@ constexpr bool Q4_FIVE = !(G == 32 && NT == 4);
 template <int G, int NT>
 static void q4_blocks(const Q4Args& a, hipStream_t st) {
   const int tiles = (a.w.V + 15) / 16;
-  hipLaunchKernelGGL((k_q4_blocks<G, NT>), dim3((unsigned)((a.w.K + 511) / 512 * 4)), dim3(WAVE), 0, st, a);
+  hipLaunchKernelGGL((k_q4_blocks<G, NT>), dim3((unsigned)((a.w.K + 511) / 512 * 4), NT), dim3(WAVE), 0, st, a);
   if (a.w.K < 8 * G) {
     hipLaunchKernelGGL((k_q4_short<G, NT>), dim3((unsigned)tiles), dim3(WAVE), 0, st, a);
     return;
   }
-  // tiles a wave: what takes the fewest tile times over all rounds; few tiles: smaller workgroups
-  // (K = 5,120, 16 rows, V = 4,096: 19.6 us, by eight waves 23.2; V = 16,000: 26.2 against 28.8)
-  const int nw = tiles >= 4 * 256 ? QC_NW : tiles >= 2 * 256 ? 4 : 2;
+  // Less than a round of row tiles: K is split over workgroups and the parts' sums joined, where
+  // that saves more chunks (about `alone` us each, `full` with eight waves) than the join costs;
+  // then the fewest waves a workgroup that fill the CUs. (K = 5,120, groups of 64, split and not:
+  // 16 rows, V = 4,096 13.3 and 20.3 us, V = 16,000 22.9 and 26.2; 64 rows, V = 4,096 20.9 and
+  // 39.5, V = 16,000 33.7 and 39.6; 16 rows, K = 1,024, V = 8,192 13.6 and 12.3. Without a split,
+  // 16 rows, V = 4,096, eight waves: 24.0.)
+  if (tiles < QC_SPLIT) {
+    const int units = (a.w.K + 511) / 512;
+    const double alone = NT == 1 ? 1.7 : NT == 2 ? 2.2 : 3.5, full = NT == 1 ? 2.5 : NT == 2 ? 3.2 : 5.0;
+    int splits = QC_SPLIT / tiles < units ? QC_SPLIT / tiles : units;
+    if ((units + splits - 1) / splits * full + 3.0 > units * alone) splits = 1;
+    int nw = QC_NW;
+    while (nw > 2 && (tiles + nw / 2 - 1) / (nw / 2) * splits <= 256) nw /= 2;
+    if (splits == 1) {
+      q4_chunk<G, NT, 1>(a, nw, 1, st);
+      return;
+    }
+    q4_chunk<G, NT, 1, true>(a, nw, splits, st);
+    hipLaunchKernelGGL(k_q4_join, dim3((unsigned)((a.w.V + 255) / 256), (unsigned)a.B), dim3(256), 0, st, a, splits);
+    return;
+  }
+  // tiles a wave: what takes the fewest tile times over all rounds
   int best = 1, least = 1 << 30;
   for (int mt : {1, 2, 3, 5}) {
     if (mt == 5 && !Q4_FIVE<G, NT>) continue;
-    const int round = 256 * nw * mt, cost = (tiles + round - 1) / round * mt;
+    const int round = 256 * QC_NW * mt, cost = (tiles + round - 1) / round * mt;
     if (cost < least) least = cost, best = mt;
   }
-  if (best == 1) q4_chunk<G, NT, 1>(a, nw, st);
-  else if (best == 2) q4_chunk<G, NT, 2>(a, nw, st);
-  else if (best == 3) q4_chunk<G, NT, 3>(a, nw, st);
-  else if constexpr (Q4_FIVE<G, NT>) q4_chunk<G, NT, 5>(a, nw, st);
+  if (best == 1) q4_chunk<G, NT, 1>(a, QC_NW, 1, st);
+  else if (best == 2) q4_chunk<G, NT, 2>(a, QC_NW, 1, st);
+  else if (best == 3) q4_chunk<G, NT, 3>(a, QC_NW, 1, st);
+  else if constexpr (Q4_FIVE<G, NT>) q4_chunk<G, NT, 5>(a, QC_NW, 1, st);
 }
 
 // Up to 8 rows from LDS (V = 151,936, K = 5,120, groups of 64, 8 rows: 99 us, by k_q4_chunk 116; V =
@@ -1050,6 +1094,7 @@ hipError_t launch_q4_logits(const void* x, int64_t x_stride, int B, int K, const
     a.x_stride = x_stride;
     a.B = B - b < 64 ? B - b : 64;
     a.blocks = (uint8_t*)workspace;
+    a.part = (float*)(a.blocks + q4_blocks_bytes(B < 64 ? B : 64, K));
     a.out = (uint8_t*)out + (int64_t)b * out_stride * (out_f32 ? 4 : 2);
     a.out_stride = out_stride;
     a.out_f32 = out_f32;

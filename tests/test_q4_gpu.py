@@ -307,3 +307,18 @@ def test_offsets_past_32_bits():
     p = ops.q4_pack(v, G)
     t = ops.q4_pack(v[-300:].contiguous(), G)
     assert torch.equal(p.words[-300:], t.words) and torch.equal(p.scales[-300:], t.scales)
+
+
+@pytest.mark.parametrize("B,K,V,G,sym", [
+    (9, 2080, 1, 32, False), (16, 5152, 300, 32, True), (16, 5120, 4099, 64, False),
+    (33, 2112, 16_001, 64, True), (64, 8192, 4111, 128, False), (70, 5120, 2049, 64, False),
+    (130, 2048, 70, 128, True)])
+def test_few_weight_rows(B, K, V, G, sym):
+    """Less than a round of row tiles: K in parts, their sums joined."""
+    print(f"[q4] parts of K: B={B} V={V} K={K} G={G}", flush=True)
+    q = weight(V, K, G, sym, seed=B + K)
+    x = torch.randn(B, K, device="cuda", generator=gen(V)).to(torch.bfloat16)
+    check_logits(x, q, ops.head_logits_q4(x, q), "bf16")
+    y = ops.head_logits_q4(x, q, out_dtype=torch.float32)
+    check_logits(x, q, y, "f32")
+    assert torch.equal(y, ops.head_logits_q4(x, q, out_dtype=torch.float32))
