@@ -716,10 +716,9 @@ __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int t
 // wave goes through its MT row tiles chunk by chunk, two at a time (a fragment read from LDS
 // serves both), their sums in registers. The code of a chunk has no branches between its
 // requests, so that each wait is for the oldest alone. Any alignment, any number of groups. PARTS:
-// gridDim.y parts of K, their sums to `part`. At
-// V = 151,936, K = 5,120, groups of 64: 16 rows 116 us, 32 rows 146, 64 rows 219 (128: 200); the
-// arithmetic alone takes 57 of the 116 and 177 of the 219, its vector instructions and MFMA hardly
-// side by side with two waves a SIMD.
+// gridDim.y parts of K, their sums to `part`. (V = 151,936, K = 5,120, groups of 64: 16 rows 116 us,
+// 32 rows 133, 64 rows 175, groups of 128: 143. Few rows are bound by the weights' loads, as
+// k_q4_stream's, 64 by vector instructions and MFMA of two waves a SIMD.)
 constexpr int QC_NW = 8;
 
 template <int I>
@@ -1025,10 +1024,6 @@ static void q4_chunk(const Q4Args& a, int nw, int splits, hipStream_t st) {
                                     (size_t)2 * 4 * (4 * NT + 1) * 1024, st, a, nw);
 }
 
-// (narrow groups by 64 rows: more than the registers hold)
-template <int G, int NT>
-constexpr bool Q4_FIVE = !(G == 32 && NT == 4);
-
 template <int G, int NT>
 static void q4_blocks(const Q4Args& a, hipStream_t st) {
   const int tiles = (a.w.V + 15) / 16;
@@ -1058,17 +1053,30 @@ static void q4_blocks(const Q4Args& a, hipStream_t st) {
     hipLaunchKernelGGL(k_q4_join, dim3((unsigned)((a.w.V + 255) / 256), (unsigned)a.B), dim3(256), 0, st, a, splits);
     return;
   }
-  // tiles a wave: what takes the fewest tile times over all rounds
-  int best = 1, least = 1 << 30;
-  for (int mt : {1, 2, 3, 5}) {
-    if (mt == 5 && !Q4_FIVE<G, NT>) continue;
-    const int round = 256 * QC_NW * mt, cost = (tiles + round - 1) / round * mt;
-    if (cost < least) least = cost, best = mt;
+  // Tiles a wave, by the time of its rounds over the CUs (in tiles, as measured; the last round by
+  // how full it is). Two tiles read the hidden rows' fragments from LDS once, and more tiles wait
+  // fewer times, but a round of five tiles that is half empty takes as long as one of four. (K =
+  // 5,120, groups of 64, V = 151,936, one and five tiles: 64 rows 207 and 175 us, 32 rows 144 and
+  // 133; V = 65,536, one, two and five: 64 rows 88, 81 and 139. 16 rows, with four workgroups a CU:
+  // V = 151,936 115 us by one tile, 128 by five.)
+  int best = 1;
+  if constexpr (NT > 1) {
+    const double round[6] = {0.0, 1.35, 2.28, 3.2, 4.0, 5.0}, all = (double)tiles / (256 * QC_NW);
+    double least = NT == 2 ? 0.3 + 1.11 * all : 1e30;  // (32 rows, one tile: two workgroups a CU)
+    for (int mt = NT == 2 ? 3 : 1; mt <= 5; ++mt) {
+      const double n = all / mt, whole = (double)(int64_t)n;
+      const double cost = round[mt] * (n == whole ? n : whole + 0.75 + 0.25 * (n - whole));
+      if (cost < least) least = cost, best = mt;
+    }
   }
   if (best == 1) q4_chunk<G, NT, 1>(a, QC_NW, 1, st);
-  else if (best == 2) q4_chunk<G, NT, 2>(a, QC_NW, 1, st);
-  else if (best == 3) q4_chunk<G, NT, 3>(a, QC_NW, 1, st);
-  else if constexpr (Q4_FIVE<G, NT>) q4_chunk<G, NT, 5>(a, QC_NW, 1, st);
+  if constexpr (NT > 2)
+    if (best == 2) q4_chunk<G, NT, 2>(a, QC_NW, 1, st);
+  if constexpr (NT > 1) {
+    if (best == 3) q4_chunk<G, NT, 3>(a, QC_NW, 1, st);
+    if (best == 4) q4_chunk<G, NT, 4>(a, QC_NW, 1, st);
+    if (best == 5) q4_chunk<G, NT, 5>(a, QC_NW, 1, st);
+  }
 }
 
 // Up to 8 rows from LDS (V = 151,936, K = 5,120, groups of 64, 8 rows: 99 us, by k_q4_chunk 116; V =

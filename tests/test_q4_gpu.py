@@ -322,3 +322,15 @@ def test_few_weight_rows(B, K, V, G, sym):
     y = ops.head_logits_q4(x, q, out_dtype=torch.float32)
     check_logits(x, q, y, "f32")
     assert torch.equal(y, ops.head_logits_q4(x, q, out_dtype=torch.float32))
+
+
+@pytest.mark.parametrize("B,K,V,G", [
+    (33, 1024, 34_001, 64), (40, 544, 60_001, 32), (64, 640, 98_003, 64), (64, 1024, 130_007, 128),
+    (50, 1056, 160_001, 32), (64, 1152, 163_839, 128), (17, 640, 98_003, 64), (32, 544, 131_001, 32),
+    (32, 1152, 163_841, 128)])
+def test_several_tiles_a_wave(B, K, V, G):
+    """Rounds of two to five row tiles a wave, full and not."""
+    print(f"[q4] rounds: B={B} V={V} K={K} G={G}", flush=True)
+    q = weight(V, K, G, False, seed=B + K)
+    x = torch.randn(B, K, device="cuda", generator=gen(V)).to(torch.bfloat16)
+    check_logits(x, q, ops.head_logits_q4(x, q, out_dtype=torch.float32), "f32")
