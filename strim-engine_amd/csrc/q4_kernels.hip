@@ -270,28 +270,57 @@ __device__ __forceinline__ qf32x4 q4_sum(qu32x4 x, qf32x4 acc) {
                                                  __builtin_bit_cast(qbf16x8, one), acc, 0, 0, 0);
 }
 
-// The hidden rows by steps: per step 4 NT fragments of 1 KB (MFMA t of batch tile nt at t NT +
-// nt, 16 bytes a lane), then the sums X [group][NT][16 places], padded to 1 KB. A wave a step and
-// batch tile.
+// The hidden rows by chunks of 512: per chunk 16 NT fragments of 1 KB (MFMA t of step s, batch tile
+// nt, at (4 s + t) NT + nt, 16 bytes a lane), then the group sums as fragments too, of q4_chunk_sums
+// MFMAs by the words of scales and biases that k_q4_chunk's lanes load for a chunk: even quarters
+// scales, odd ones biases, eight groups (four and the same four again with groups of 128; with
+// groups of 32 the upper quarters the second eight). Y = -16 X by scales, X by biases (symmetric:
+// -24 X and 0) is in three bf16 parts that add up to its 24 bits: every product is exact. A workgroup
+// a chunk and batch tile, a wave a step.
+template <int G>
+constexpr int q4_chunk_sums() {
+  return 128 / G == 4 ? 3 : 128 / G;
+}
+
 template <int G, int NT>
-__global__ __launch_bounds__(WAVE) void k_q4_blocks(const Q4Args a) {
-  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
-  const int lane = threadIdx.x, h = lane >> 4, m = lane & 15, step = blockIdx.x, nt = blockIdx.y;
-  uint8_t* blk = a.blocks + (int64_t)step * BLOCK;
-  const int b = 16 * nt + q4_row(m);
+__global__ __launch_bounds__(4 * WAVE) void k_q4_blocks(const Q4Args a) {
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, NS = q4_chunk_sums<G>();
+  __shared__ float s_sum[4 * GPS][16];
+  const int lane = threadIdx.x & (WAVE - 1), step = wave_id(), h = lane >> 4, m = lane & 15;
+  const int nt = blockIdx.y, b = 16 * nt + q4_row(m);
+  uint8_t* blk = a.blocks + (int64_t)blockIdx.x * (16 + NS) * NT * 1024 + lane * 16;
 #pragma unroll
   for (int g = 0; g < GPS; ++g) {
     qf32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int q = 0; q < MPG; ++q) {
-      const int t = g * MPG + q, k = step * 128 + q4_koff<G>(t, h);
+      const int t = g * MPG + q, k = (blockIdx.x * 4 + step) * 128 + q4_koff<G>(t, h);
       qu32x4 x = {0u, 0u, 0u, 0u};
       if (b < a.B && k < a.w.K) x = q4_interleave(*(const qu32x4*)(a.x + (int64_t)b * a.x_stride + k));
-      *(qu32x4*)(blk + (t * NT + nt) * 1024 + lane * 16) = x;
+      *(qu32x4*)(blk + ((4 * step + t) * NT + nt) * 1024) = x;
       s = q4_sum(x, s);
     }
-    if (m == 0) *(qf32x4*)(blk + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4) = s;
+    if (m == 0) *(qf32x4*)&s_sum[step * GPS + g][4 * h] = s;
   }
+  __syncthreads();
+  if (step >= NS) return;
+  const bool sym = a.w.biases == nullptr;
+  const float by = h & 1 ? (sym ? 0.0f : 1.0f) : sym ? -24.0f : -16.0f;
+  qu32x4 y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int g = G == 32 ? 8 * (h >> 1) + e : G == 64 ? e : e & 3;
+    // which part: 3 none
+    const int part = G == 32 ? step : G == 64 ? (step == 0 ? h >> 1 : h < 2 ? 2 : 3)
+                                              : e < 4 ? (h < 2 ? 0 : 2) : h < 2 ? 1 : 3;
+    float f = by * s_sum[g][m];
+    uint32_t bits = q4_bf16(f);
+    for (int d = 0; d < 2; ++d)
+      if (d < part) f -= __uint_as_float(bits << 16), bits = q4_bf16(f);
+    if (part == 3) bits = 0u;
+    y[e / 2] = e & 1 ? y[e / 2] | bits << 16 : bits;
+  }
+  *(qu32x4*)(blk + ((16 + step) * NT + nt) * 1024) = y;
 }
 
 // Few rows: every workgroup keeps the hidden rows' fragments and sums X in LDS, whole, and its
@@ -716,9 +745,11 @@ __global__ __launch_bounds__(QS_NW* WAVE, 4) void k_q4_dma(const Q4Args a, int t
 // wave goes through its MT row tiles chunk by chunk, two at a time (a fragment read from LDS
 // serves both), their sums in registers. The code of a chunk has no branches between its
 // requests, so that each wait is for the oldest alone. Any alignment, any number of groups. PARTS:
-// gridDim.y parts of K, their sums to `part`. (V = 151,936, K = 5,120, groups of 64: 16 rows 116 us,
-// 32 rows 133, 64 rows 175, groups of 128: 143. Few rows are bound by the weights' loads, as
-// k_q4_stream's, 64 by vector instructions and MFMA of two waves a SIMD.)
+// gridDim.y parts of K, their sums to `part`. The sums (b - 16 s) X are MFMAs of the words of scales
+// and biases as loaded (by multiply-adds, 64 rows with groups of 32: 220 us instead of 187).
+// (V = 151,936, K = 5,120, groups of 64: 16 rows 116 us, 32 rows 129, 64 rows 158, groups of 128:
+// 139. Few rows are bound by the weights' loads, as k_q4_stream's, 64 by vector instructions and
+// MFMA of two waves a SIMD.)
 constexpr int QC_NW = 8;
 
 template <int I>
@@ -728,7 +759,8 @@ struct QInt {
 
 template <int G, int NT, int MT, bool PARTS>
 __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
-  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024, CHUNK = 4 * BLOCK;
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, NS = q4_chunk_sums<G>();
+  constexpr int CHUNK = (16 + NS) * NT * 1024;
   constexpr int SW = G == 128 ? 2 : 4;  // words of scales a lane loads
   extern __shared__ __attribute__((aligned(1024))) uint8_t s_all[];
   const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)s_all;
@@ -783,8 +815,6 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
   };
 
   const Q4Masks masks;
-  const uint32_t keepb = sym ? 0u : 0xFFFFFFFFu;  // symmetric: no biases, and 8 less
-  const float zero = sym ? -24.0f : -16.0f;
   qf32x4 acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -795,8 +825,9 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
   // or of the next chunk
   auto compute = [&](int c, auto mt_, auto cnt_) {
     constexpr int M0 = decltype(mt_)::value, CNT = decltype(cnt_)::value;
-    uint32_t sw[CNT][2 * GPS], bw[CNT][2 * GPS];  // the units' scales and biases, in every quarter
+    uint32_t sw[CNT][2 * GPS];  // the units' scales, in every quarter
     const int back = back_of(c);
+    const uint8_t* xc = s_all + (c & 1) * CHUNK + lane * 16;
 #pragma unroll
     for (int j = 0; j < CNT; ++j) {
       Unit& u = buf[j];
@@ -810,60 +841,64 @@ __global__ __launch_bounds__(QC_NW* WAVE, 2) void k_q4_chunk(const Q4Args a) {
         const uint32_t half = (u.s[e] >> 16) | (e + 1 < SW ? u.s[e + 1] << 16 : 0u);
         u.s[e] = back >= 2 * SW ? 0u : back & 1 ? half : u.s[e];
       }
+      // sum of (b - 16 s) X over the chunk's groups
+      const qu32x4 sb = {u.s[0], u.s[1], SW == 2 ? u.s[0] : u.s[SW - 2], SW == 2 ? u.s[1] : u.s[SW - 1]};
+#pragma unroll
+      for (int q = 0; q < NS; ++q)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const qu32x4 y = *(const qu32x4*)(xc + ((16 + q) * NT + nt) * 1024);
+          acc[M0 + j][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              __builtin_bit_cast(qbf16x8, y), __builtin_bit_cast(qbf16x8, sb), acc[M0 + j][nt], 0, 0, 0);
+        }
 #pragma unroll
       for (int e = 0; e < SW; ++e) {
-        uint32_t s0 = u.s[e], b0 = u.s[e];
-        q4_swap16(s0, b0);
+        uint32_t s0 = u.s[e], other = u.s[e];
+        q4_swap16(s0, other);
         if constexpr (G == 32) {
-          uint32_t s1 = s0, b1 = b0;
+          uint32_t s1 = s0;
           q4_swap32(s0, s1);
-          q4_swap32(b0, b1);
-          sw[j][4 + e] = s1, bw[j][4 + e] = b1;
+          sw[j][4 + e] = s1;
         }
-        sw[j][e] = s0, bw[j][e] = b0;
+        sw[j][e] = s0;
       }
       load_scales(u, M0 + 2 + j < MT ? c : c + 1, M0 + 2 + j < MT ? M0 + 2 + j : j);
     }
-    const uint8_t* xc = s_all + (c & 1) * CHUNK;
     uint32_t w[CNT][4];
-    qf32x4 t[CNT][NT];
 #pragma unroll
-    for (int m = 0; m < 16; ++m) {  // the chunk's MFMA words
-      const int p = m >> 2, g = (m & 3) / MPG, i = p * GPS + g;
-      if (m % 4 == 0) {
+    for (int i = 0; i < 4 * GPS; ++i) {  // the chunk's groups
+      const int p = i / GPS, g = i % GPS;
+      if (g == 0) {
 #pragma unroll
         for (int j = 0; j < CNT; ++j) {
           q4_order<G>(buf[j].w[p], w[j]);
           load_words(buf[j], M0 + 2 + j < MT ? c : c + 1, M0 + 2 + j < MT ? M0 + 2 + j : j, p);
         }
       }
-      qbf16x8 codes[CNT];
+      qbf16x8 codes[CNT][MPG];
+      float sc[CNT];
 #pragma unroll
-      for (int j = 0; j < CNT; ++j) codes[j] = q4_codes(w[j][m & 3], masks);
+      for (int j = 0; j < CNT; ++j) {
+#pragma unroll
+        for (int q = 0; q < MPG; ++q) codes[j][q] = q4_codes(w[j][g * MPG + q], masks);
+        sc[j] = __uint_as_float(i & 1 ? sw[j][i / 2] & 0xFFFF0000u : sw[j][i / 2] << 16);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const qu32x4 x = *(const qu32x4*)(xc + p * BLOCK + ((m & 3) * NT + nt) * 1024 + lane * 16);
+        qf32x4 t[CNT];
 #pragma unroll
-        for (int j = 0; j < CNT; ++j) {
-          if (m % MPG == 0) t[j][nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
-          t[j][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), codes[j],
-                                                            t[j][nt], 0, 0, 0);
-        }
-      }
-      if (m % MPG == MPG - 1) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const qf32x4 xs = *(const qf32x4*)(xc + p * BLOCK + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4);
+        for (int q = 0; q < MPG; ++q) {
+          const qu32x4 x = *(const qu32x4*)(xc + ((4 * p + g * MPG + q) * NT + nt) * 1024);
 #pragma unroll
           for (int j = 0; j < CNT; ++j) {
-            const float sc = __uint_as_float(i & 1 ? sw[j][i / 2] & 0xFFFF0000u : sw[j][i / 2] << 16);
-            const float bi = __uint_as_float((i & 1 ? bw[j][i / 2] & 0xFFFF0000u : bw[j][i / 2] << 16) & keepb);
-            const float off = __builtin_fmaf(zero, sc, bi);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[M0 + j][nt][r] = __builtin_fmaf(sc, t[j][nt][r], __builtin_fmaf(off, xs[r], acc[M0 + j][nt][r]));
+            if (q == 0) t[j] = qf32x4{0.f, 0.f, 0.f, 0.f};
+            t[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), codes[j][q], t[j], 0, 0, 0);
           }
         }
+#pragma unroll
+        for (int j = 0; j < CNT; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[M0 + j][nt][r] = __builtin_fmaf(sc[j], t[j][r], acc[M0 + j][nt][r]);
       }
     }
     // (more than 16 rows: two pairs of tiles at once are more than the registers hold)
@@ -915,7 +950,7 @@ __global__ __launch_bounds__(256) void k_q4_join(const Q4Args a, int splits) {
 // K of fewer than eight groups: one wave a row tile, straightforwardly.
 template <int G, int NT>
 __global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
-  constexpr int GPS = 128 / G, MPG = 4 / GPS, BLOCK = (4 * NT + 1) * 1024;
+  constexpr int GPS = 128 / G, MPG = 4 / GPS, CHUNK = (16 + q4_chunk_sums<G>()) * NT * 1024;
   const int lane = threadIdx.x, h = lane >> 4, r16 = lane & 15;
   const int steps = (a.w.K + 127) / 128, groups = a.w.K / G, pieces = a.w.K / 32;
   const int row = blockIdx.x * 16 + r16, v = min(row, a.w.V - 1);
@@ -927,7 +962,7 @@ __global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) acc[nt] = qf32x4{0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < steps; ++s) {
-    const uint8_t* xc = a.blocks + (int64_t)s * BLOCK;
+    const uint8_t* xc = a.blocks + (int64_t)(s >> 2) * CHUNK + (s & 3) * 4 * NT * 1024 + lane * 16;
     uint32_t w[4];
     q4_order<G>(*(const qu32x4*)(wp + 4 * min(4 * s + h, pieces - 1)), w);
 #pragma unroll
@@ -939,14 +974,14 @@ __global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
       const float off = bi - 16.0f * sc;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        qf32x4 t = {0.f, 0.f, 0.f, 0.f};
+        qf32x4 t = {0.f, 0.f, 0.f, 0.f}, xs = t;
 #pragma unroll
         for (int q = 0; q < MPG; ++q) {
           const int m = g * MPG + q;
-          const qu32x4 x = *(const qu32x4*)(xc + (m * NT + nt) * 1024 + lane * 16);
+          const qu32x4 x = *(const qu32x4*)(xc + (m * NT + nt) * 1024);
+          xs = q4_sum(x, xs);
           t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(qbf16x8, x), q4_codes(w[m], masks), t, 0, 0, 0);
         }
-        const qf32x4 xs = *(const qf32x4*)(xc + 4 * NT * 1024 + ((g * NT + nt) * 16 + 4 * h) * 4);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           acc[nt][r] = __builtin_fmaf(sc, t[r], __builtin_fmaf(off, xs[r], acc[nt][r]));
@@ -967,7 +1002,7 @@ __global__ __launch_bounds__(WAVE) void k_q4_short(const Q4Args a) {
 static int q4_tiles_n(int B) { return B <= 16 ? 1 : B <= 32 ? 2 : 4; }
 
 static int64_t q4_blocks_bytes(int B, int K) {
-  return ((int64_t)K + 511) / 512 * 4 * (4 * q4_tiles_n(B) + 1) * 1024;
+  return ((int64_t)K + 511) / 512 * (16 + 3) * q4_tiles_n(B) * 1024;
 }
 
 // k_q4_chunk's row tiles, over all its parts of K, are this many at most: eight waves a CU.
@@ -1021,13 +1056,13 @@ template <int G, int NT, int MT, bool PARTS = false>
 static void q4_chunk(const Q4Args& a, int nw, int splits, hipStream_t st) {
   const int tiles = (a.w.V + 15) / 16, each = nw * MT;
   q4_big_lds<k_q4_chunk<G, NT, MT, PARTS>>(dim3((unsigned)((tiles + each - 1) / each), (unsigned)splits),
-                                    (size_t)2 * 4 * (4 * NT + 1) * 1024, st, a, nw);
+                                    (size_t)2 * (16 + q4_chunk_sums<G>()) * NT * 1024, st, a, nw);
 }
 
 template <int G, int NT>
 static void q4_blocks(const Q4Args& a, hipStream_t st) {
   const int tiles = (a.w.V + 15) / 16;
-  hipLaunchKernelGGL((k_q4_blocks<G, NT>), dim3((unsigned)((a.w.K + 511) / 512 * 4), NT), dim3(WAVE), 0, st, a);
+  hipLaunchKernelGGL((k_q4_blocks<G, NT>), dim3((unsigned)((a.w.K + 511) / 512), NT), dim3(4 * WAVE), 0, st, a);
   if (a.w.K < 8 * G) {
     hipLaunchKernelGGL((k_q4_short<G, NT>), dim3((unsigned)tiles), dim3(WAVE), 0, st, a);
     return;
