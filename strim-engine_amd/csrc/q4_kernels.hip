@@ -29,7 +29,9 @@ __device__ __forceinline__ uint32_t q4_bf16(float f) {
 
 // ---- packing ------------------------------------------------------------------------------
 // Eight elements a thread, G / 8 neighbouring lanes a group; bound by HBM (V = 32,768, K = 5,120,
-// bf16, groups of 64: 103 us, 4.2 TB/s; reading back 83 us, 5.2 TB/s).
+// groups of 64: bf16 95 us, 4.5 TB/s, float32 153, 5.0 TB/s). The words do not go past the caches:
+// what reads them next finds them there (packed and read back, 8,193 x 2,048 in float32: 28 us, else
+// 33).
 //   biased:    s = bf16((max - min) / 15), b = bf16(min), q = clamp(rint((w - b) / s), 0, 15)
 //   symmetric: s = bf16(max|w| / 7),                      q = clamp(rint(w / s) + 8, 0, 15)
 // s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). The divisions by 15 and 7
@@ -88,8 +90,7 @@ __global__ __launch_bounds__(256) void k_q4_pack(const Q4Pack a) {
       x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
       x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
     } else {
-      const uint4 q = *(const uint4*)((const uint16_t*)a.w + v * a.w_stride + 8 * c);
-      const uint32_t d[4] = {q.x, q.y, q.z, q.w};
+      const qu32x4 d = *(const qu32x4*)((const uint16_t*)a.w + v * a.w_stride + 8 * c);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         x[2 * e] = __uint_as_float(d[e] << 16);
@@ -154,7 +155,8 @@ struct Q4Weights {
 };
 
 // Sixteen bytes a thread, so that a store's lines are whole (float32, eight elements a thread: 3.6
-// TB/s, four: 4.1).
+// TB/s, four: 4.1), and past the caches (V = 32,768, K = 5,120, groups of 64: bf16 90 -> 67 us, 6.4
+// TB/s; float32 185 -> 146, with a quarter of the workgroups 123, 6.2 TB/s, bf16 67 -> 76).
 template <int G, bool F32>
 __global__ __launch_bounds__(256) void k_q4_unpack(const Q4Weights a, void* out, int64_t out_stride) {
   constexpr int E = F32 ? 4 : 8;
@@ -170,12 +172,13 @@ __global__ __launch_bounds__(256) void k_q4_unpack(const Q4Weights a, void* out,
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = ((float)((word >> (4 * e)) & 15u) - z) * s + b;
     if constexpr (F32) {
-      *(float4*)((float*)out + v * out_stride + 4 * c) = make_float4(x[0], x[1], x[2], x[3]);
+      __builtin_nontemporal_store(qf32x4{x[0], x[1], x[2], x[3]},
+                                  (qf32x4*)((float*)out + v * out_stride + 4 * c));
     } else {
-      uint32_t d[4];
+      qu32x4 d;
 #pragma unroll
       for (int e = 0; e < 4; ++e) d[e] = q4_bf16(x[2 * e]) | (q4_bf16(x[2 * e + 1]) << 16);
-      *(uint4*)((uint16_t*)out + v * out_stride + 8 * c) = make_uint4(d[0], d[1], d[2], d[3]);
+      __builtin_nontemporal_store(d, (qu32x4*)((uint16_t*)out + v * out_stride + 8 * c));
     }
   }
 }
@@ -1176,7 +1179,8 @@ hipError_t launch_q4_unpack(const uint32_t* words, int64_t words_stride, const u
                             void* out, bool out_f32, int64_t out_stride, hipStream_t st) {
   const Q4Weights a{words, words_stride, scales, biases, scales_stride, V, K};
   const int64_t blocks = ((int64_t)V * (K / (out_f32 ? 4 : 8)) + 255) / 256;
-  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
+  const int64_t most = out_f32 ? 2048 : 8192;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most));
 #define STRIM_UNPACK(G_)                                                                          \
   do {                                                                                            \
     if (out_f32) hipLaunchKernelGGL((k_q4_unpack<G_, true>), grid, dim3(256), 0, st, a, out, out_stride); \
