@@ -1096,9 +1096,9 @@ static void q4_blocks(const Q4Args& a, hipStream_t st) {
   // Tiles a wave, by the time of its rounds over the CUs (in tiles, as measured; the last round by
   // how full it is). Two tiles read the hidden rows' fragments from LDS once, and more tiles wait
   // fewer times, but a round of five tiles that is half empty takes as long as one of four. (K =
-  // 5,120, groups of 64, V = 151,936, one and five tiles: 64 rows 207 and 175 us, 32 rows 144 and
-  // 133; V = 65,536, one, two and five: 64 rows 88, 81 and 139. 16 rows, with four workgroups a CU:
-  // V = 151,936 115 us by one tile, 128 by five.)
+  // 5,120, groups of 64, V = 151,936, one, three and five tiles: 64 rows 220, 192 and 172 us, 32 rows
+  // 146, 147 and 131; V = 65,536, 64 rows, one, two and five: 90, 77 and 125; 32 rows, one and five:
+  // 65 and 105. 16 rows, with four workgroups a CU: V = 151,936 115 us by one tile, 128 by five.)
   int best = 1;
   if constexpr (NT > 1) {
     const double round[6] = {0.0, 1.35, 2.28, 3.2, 4.0, 5.0}, all = (double)tiles / (256 * QC_NW);
