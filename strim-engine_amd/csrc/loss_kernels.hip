@@ -507,13 +507,15 @@ __global__ __launch_bounds__(256) void k_loss_rows_in(const uint16_t* x, int64_t
   }
 }
 
-// d_hidden from the splits' sums, added in order and rounded once.
+// d_hidden from the splits' sums, added in order and rounded once; eight are requested together (one
+// row, K = 1,024: 6.0 us, one after the other 18.0, sixteen 7.6).
 __global__ __launch_bounds__(256) void k_loss_join(const float* acc, int splits, int N, int K,
                                                    uint16_t* out, int64_t out_stride) {
   const int64_t total = (int64_t)N * K;
   const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
   if (i >= total) return;
   lf32x4 s = *(const lf32x4*)(acc + i);
+#pragma unroll 8
   for (int q = 1; q < splits; ++q) s += *(const lf32x4*)(acc + q * total + i);
   const float f[4] = {s[0], s[1], s[2], s[3]};
   const int64_t n = i / K;
