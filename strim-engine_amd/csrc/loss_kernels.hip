@@ -333,9 +333,11 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
     if (mh + 16 * i < valid) *(uint4*)(out + mh + 16 * i) = q;
   };
   static_assert(TM % 2 == 0, "tiles are stored by twos");
-  if constexpr (MODE == LM_STATS) {
+  if constexpr (MODE == LM_STATS || MODE == LM_PROB) {
+    // Past the vocabulary: nothing. (p's last columns too: d_hidden's product reads whole 16-byte
+    // pieces, and exp(0 - lse) would be infinite there for a row whose lse is below -88.7.)
     const int left = g.V - g.v0;
-    if (mw + TM * 16 > left) {  // past the vocabulary: nothing
+    if (mw + TM * 16 > left) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -344,6 +346,8 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j][r] = -INFINITY;
     }
+  }
+  if constexpr (MODE == LM_STATS) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = n0 + 16 * j;
@@ -391,7 +395,7 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
         w[i] = loss_pack4(p);
         w[i].x &= keep, w[i].y &= keep;
       }
-      // (columns past the vocabulary are inside the row, and read by nothing)
+      // (columns past the vocabulary are inside the row, and zero)
       if (n < g.b.rows)
 #pragma unroll
         for (int i = 0; i < TM; i += 2)

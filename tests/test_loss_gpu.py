@@ -401,3 +401,40 @@ def test_many_rows():
     R, K, V = 70_001, 16, 300
     h, w, t, gl = inputs(R, K, V, seed=61)
     check(h, w, t, gl, label="many rows")
+
+
+LOW = [(1, 64, 5), (3, 72, 601), (17, 64, 1023), (40, 136, 4099), (257, 64, 1501), (129, 256, 50_257),
+       (1000, 1536, 66_003), (1003, 2048, 33_100), (2050, 1024, 33_281)]
+
+
+def low_inputs(R, K, V, seed):
+    """Every row's logits around one number, from -30,000 to 64, most of them below -88.7 (where
+    exp(-lse) is past float32), and a vocabulary that ends inside a 16-byte piece."""
+    h, w, t, gl = inputs(R, K, V, seed=seed, ignored=0.1)
+    w[:, 0] = -1.0
+    h[:, 0] = torch.tensor([96.0, 88.0, 128.0, 90.0, -64.0, 1024.0, 100.0, 30_000.0, 0.0],
+                           device="cuda").repeat(-(-R // 9))[:R].to(torch.bfloat16)
+    return h, w, t, gl
+
+
+@pytest.mark.parametrize("R,K,V", LOW)
+def test_logits_far_below_zero(R, K, V):
+    """Nothing bounds a row's logits from below: no weight of a token past the vocabulary, whose
+    logit would be 0, reaches the gradients. Single tiles, whole rounds, and what is left of them
+    in smaller tiles."""
+    print(f"[loss] far below zero N={R} K={K} V={V}", flush=True)
+    assert V % 8
+    check(*low_inputs(R, K, V, seed=V), label=f"N={R} K={K} V={V}")
+
+
+def test_logits_far_below_zero_in_pieces():
+    """The same where the last of several pieces of the vocabulary is the short one."""
+    R, K, V = 2050, 64, 200_003
+    assert ops.head_loss_workspace(R, K, V, True, False) < 2 * R * V + 4 * R * K
+    h, w, t, gl = low_inputs(R, K, V, seed=12)
+    _, lse, _ = ops.head_loss(h, w, t)
+    dh, _ = ops.head_loss_grad(h, w, t, lse, gl, want_lm_head=False)
+    for a in range(0, R, 410):
+        s = slice(a, a + 410)
+        E = Exact(h[s], w, t[s], gl[s])
+        within(dh[s], E.dh, E.tol_h, "d_hidden")
