@@ -1,10 +1,13 @@
 """Device-tensor front end of the C ABI.
 
 Torch is used only to hold device memory and the current HIP stream; every
-computation runs in libstrim_sampler.so. Inputs must already live on the GPU.
+computation runs in libstrim_sampler.so. Inputs must already live on the GPU. A call with a
+`stream` is queued there: the caller makes that stream wait for the inputs, and whoever
+uses the results wait for that stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from functools import lru_cache
 
@@ -21,6 +24,33 @@ def _ptr(t) -> int | None:
 def _stream(stream=None) -> ctypes.c_void_p:
     s = stream if stream is not None else torch.cuda.current_stream()
     return ctypes.c_void_p(s.cuda_stream)
+
+
+_AS_IS = contextlib.nullcontext()
+
+
+@contextlib.contextmanager
+def _given(stream, tensors, results: list):
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, tensors[0].device)
+    caller = torch.cuda.current_stream(stream.device)
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        yield
+    for t in results:
+        if t is not None:
+            t.record_stream(caller)
+
+
+def _on(stream, tensors, results: list):
+    """The context in which a call allocates and launches. With a given stream that stream is
+    current: temporary memory is taken from it and goes back to it, in the order of its work (taken
+    from the caller's stream it would be handed out again while the kernels still use it).
+    `tensors`, the caller's own, are not handed out again before the stream is done with them, nor
+    `results` before the caller's stream is."""
+    return _AS_IS if stream is None else _given(stream, tensors, results)
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -272,14 +302,17 @@ def head_logits(hidden: torch.Tensor, lm_head: torch.Tensor,
     V = lm_head.shape[0]
     if lm_head.shape[1] != K:
         raise ValueError(f"lm_head is [{lm_head.shape[0]}, {lm_head.shape[1]}], hidden K={K}")
-    if out is None:
-        out = torch.empty(B, V, dtype=torch.bfloat16, device=hidden.device)
-    if norm_weight is not None and xn is None:
-        xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
-    N.check(N.lib().strim_head_logits(_stream(stream), _ptr(hidden), _row_stride(hidden), B, K,
-                                      _ptr(norm_weight), float(eps), _ptr(xn), _ptr(lm_head),
-                                      _row_stride(lm_head), V, _ptr(out), _row_stride(out)),
-            "strim_head_logits")
+    res = []
+    with _on(stream, (hidden, lm_head, norm_weight, out, xn), res):
+        if out is None:
+            out = torch.empty(B, V, dtype=torch.bfloat16, device=hidden.device)
+            res.append(out)
+        if norm_weight is not None and xn is None:
+            xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
+        N.check(N.lib().strim_head_logits(_stream(stream), _ptr(hidden), _row_stride(hidden), B, K,
+                                          _ptr(norm_weight), float(eps), _ptr(xn), _ptr(lm_head),
+                                          _row_stride(lm_head), V, _ptr(out), _row_stride(out)),
+                "strim_head_logits")
     return out
 
 
@@ -302,19 +335,22 @@ def head_greedy(ctx: "Context", hidden: torch.Tensor, lm_head: torch.Tensor,
     V = lm_head.shape[0]
     if lm_head.shape[1] != K:
         raise ValueError(f"lm_head is [{lm_head.shape[0]}, {lm_head.shape[1]}], hidden K={K}")
-    if norm_weight is not None and xn is None:
-        xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
-    if ids is None:
-        ids = torch.empty(B, dtype=torch.int32, device=hidden.device)
-    if status is None:
-        status = torch.empty(B, dtype=torch.int32, device=hidden.device)
-    N.check(N.lib().strim_head_greedy(ctx.handle, _stream(stream), _ptr(hidden),
-                                      _row_stride(hidden), B, K, _ptr(norm_weight), float(eps),
-                                      _ptr(xn), _ptr(lm_head), _row_stride(lm_head), V,
-                                      _ptr(out_logits),
-                                      _row_stride(out_logits) if out_logits is not None else 0,
-                                      _ptr(ids), _ptr(status)),
-            "strim_head_greedy")
+    res = []
+    with _on(stream, (hidden, lm_head, norm_weight, out_logits, xn, ids, status), res):
+        if norm_weight is not None and xn is None:
+            xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
+        if ids is None:
+            ids = torch.empty(B, dtype=torch.int32, device=hidden.device)
+        if status is None:
+            status = torch.empty(B, dtype=torch.int32, device=hidden.device)
+        res += [ids, status]
+        N.check(N.lib().strim_head_greedy(ctx.handle, _stream(stream), _ptr(hidden),
+                                          _row_stride(hidden), B, K, _ptr(norm_weight), float(eps),
+                                          _ptr(xn), _ptr(lm_head), _row_stride(lm_head), V,
+                                          _ptr(out_logits),
+                                          _row_stride(out_logits) if out_logits is not None else 0,
+                                          _ptr(ids), _ptr(status)),
+                "strim_head_greedy")
     return ids, status
 
 
@@ -403,14 +439,17 @@ def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor
     0. strim_amd.loss has the differentiable form."""
     R, K, V = _loss_args(hidden, lm_head, targets)
     dev = hidden.device
-    loss = torch.empty(R, dtype=torch.float32, device=dev)
-    lse = torch.empty(R, dtype=torch.float32, device=dev)
-    status = torch.empty(R, dtype=torch.int32, device=dev)
-    ws = _workspace(workspace, head_loss_workspace(R, K, V), dev)
-    N.check(N.lib().strim_head_loss(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), R, K,
-                                    _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
-                                    ignore_index, _ptr(ws), _bytes(ws), _ptr(loss), _ptr(lse),
-                                    _ptr(status)), "strim_head_loss")
+    res = []
+    with _on(stream, (hidden, lm_head, targets, workspace), res):
+        loss = torch.empty(R, dtype=torch.float32, device=dev)
+        lse = torch.empty(R, dtype=torch.float32, device=dev)
+        status = torch.empty(R, dtype=torch.int32, device=dev)
+        res += [loss, lse, status]
+        ws = _workspace(workspace, head_loss_workspace(R, K, V), dev)
+        N.check(N.lib().strim_head_loss(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), R,
+                                        K, _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
+                                        ignore_index, _ptr(ws), _bytes(ws), _ptr(loss), _ptr(lse),
+                                        _ptr(status)), "strim_head_loss")
     return loss, lse, status
 
 
@@ -430,14 +469,18 @@ def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.T
             raise ValueError(f"lse and the gradients must be float32 [{R}]")
     if not (want_hidden or want_lm_head):
         return None, None
-    dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
-    dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
-    ws = _workspace(workspace, head_loss_workspace(R, K, V, want_hidden, want_lm_head), dev)
-    N.check(N.lib().strim_head_loss_grad(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), R, K,
-                                         _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
-                                         ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(grad_lse),
-                                         _ptr(ws), _bytes(ws), _ptr(dh), K, _ptr(dw), K),
-            "strim_head_loss_grad")
+    res = []
+    with _on(stream, (hidden, lm_head, targets, lse, grad_loss, grad_lse, workspace), res):
+        dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
+        dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
+        res += [dh, dw]
+        ws = _workspace(workspace, head_loss_workspace(R, K, V, want_hidden, want_lm_head), dev)
+        N.check(N.lib().strim_head_loss_grad(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden),
+                                             R, K, _ptr(lm_head), _row_stride(lm_head), V,
+                                             _ptr(targets), ignore_index, _ptr(lse), _ptr(grad_loss),
+                                             _ptr(grad_lse), _ptr(ws), _bytes(ws), _ptr(dh), K,
+                                             _ptr(dw), K),
+                "strim_head_loss_grad")
     return dh, dw
 
 
@@ -474,22 +517,28 @@ def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
     if group not in (32, 64, 128) or K % group:
         raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
     dev = weight.device
-    words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
-    scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
-    biases = None if symmetric else torch.empty_like(scales)
-    N.check(N.lib().strim_pack_weights(_stream_of(stream, dev), _ptr(weight), code, _row_stride(weight), V,
-                                       K, group, _ptr(words), _ptr(scales), _ptr(biases)),
-            "strim_pack_weights")
+    res = []
+    with _on(stream, (weight,), res):
+        words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
+        scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
+        biases = None if symmetric else torch.empty_like(scales)
+        res += [words, scales, biases]
+        N.check(N.lib().strim_pack_weights(_stream_of(stream, dev), _ptr(weight), code,
+                                           _row_stride(weight), V, K, group, _ptr(words), _ptr(scales),
+                                           _ptr(biases)), "strim_pack_weights")
     return Q4Weight(words, scales, biases, group)
 
 
 def q4_unpack(q: Q4Weight, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """The values [V, K] that a packed projection stands for, as bf16 or float32."""
-    out = torch.empty(q.V, q.K, dtype=dtype, device=q.words.device)
-    N.check(N.lib().strim_unpack_weights(_stream_of(stream, out.device), _ptr(q.words), q.K // 8, _ptr(q.scales),
-                                         _ptr(q.biases), q.K // q.group, q.V, q.K, q.group,
-                                         _ptr(out), _dtype_code(out), q.K),
-            "strim_unpack_weights")
+    dev, res = q.words.device, []
+    with _on(stream, (q.words, q.scales, q.biases), res):
+        out = torch.empty(q.V, q.K, dtype=dtype, device=dev)
+        res.append(out)
+        N.check(N.lib().strim_unpack_weights(_stream_of(stream, dev), _ptr(q.words), q.K // 8,
+                                             _ptr(q.scales), _ptr(q.biases), q.K // q.group, q.V, q.K,
+                                             q.group, _ptr(out), _dtype_code(out), q.K),
+                "strim_unpack_weights")
     return out
 
 
@@ -512,19 +561,22 @@ def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor 
     if norm_weight is not None:
         if norm_weight.dtype != torch.bfloat16 or norm_weight.shape != (K,):
             raise ValueError(f"norm_weight must be bfloat16 [{K}]")
-        if xn is None:
-            xn = torch.empty(B, K, dtype=torch.bfloat16, device=dev)
-        elif xn.dtype != torch.bfloat16 or xn.shape != (B, K):
+        if xn is not None and (xn.dtype != torch.bfloat16 or xn.shape != (B, K)):
             raise ValueError(f"xn must be bfloat16 [{B}, {K}]")
-    if out is None:
-        out = torch.empty(B, q.V, dtype=out_dtype, device=dev)
-    elif out.shape != (B, q.V):
+    if out is not None and out.shape != (B, q.V):
         raise ValueError(f"out must be [{B}, {q.V}]")
-    ws = _workspace(workspace, head_logits_q4_workspace(B, K), dev)
-    N.check(N.lib().strim_head_logits_packed(
-        _stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
-        _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
-        q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
+    res = []
+    with _on(stream, (hidden, q.words, q.scales, q.biases, norm_weight, out, xn, workspace), res):
+        if norm_weight is not None and xn is None:
+            xn = torch.empty(B, K, dtype=torch.bfloat16, device=dev)
+        if out is None:
+            out = torch.empty(B, q.V, dtype=out_dtype, device=dev)
+            res.append(out)
+        ws = _workspace(workspace, head_logits_q4_workspace(B, K), dev)
+        N.check(N.lib().strim_head_logits_packed(
+            _stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
+            _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
+            q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
     return out
 
 
