@@ -9,6 +9,7 @@ and the draft head's over the truncated vocabulary (Sources/StrimCore/MTP.swift:
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -36,6 +37,7 @@ class _HeadLoss(torch.autograd.Function):
         return loss, lse, status
 
     @staticmethod
+    @once_differentiable  # (the gradients' own derivatives are not built: asking for them raises)
     def backward(ctx, g_loss, g_lse, _):
         hidden, lm_head, targets, lse = ctx.saved_tensors
         # (a sum's or a mean's gradient comes as one number broadcast over the rows)
@@ -51,7 +53,8 @@ class _HeadLoss(torch.autograd.Function):
 def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor,
               ignore_index: int = IGNORE):
     """Per-position (loss, lse, status), as ops.head_loss, with gradients for hidden bf16
-    [..., K] and lm_head bf16 [V, K] through loss and lse. targets int32 or int64 [...]."""
+    [..., K] and lm_head bf16 [V, K] through loss and lse (first derivatives: differentiating a
+    gradient raises). targets int32 or int64 [...]."""
     shape = hidden.shape[:-1]
     if targets.shape != shape:
         raise ValueError(f"targets must be {tuple(shape)}, got {tuple(targets.shape)}")

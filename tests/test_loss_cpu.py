@@ -1,0 +1,53 @@
+"""The differentiable loss's own logic, without a GPU: the formulas in plain torch stand in for the
+device calls."""
+import pytest
+import torch
+
+from strim_amd import loss as L
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """head_loss and head_loss_grad by their formulas; the arguments of each gradient call."""
+    seen = []
+
+    def rows(h, w, t, ignore_index):
+        live = (t != ignore_index) & (t >= 0) & (t < w.shape[0])
+        return h.float() @ w.float().T, live, torch.where(live, t, 0).long()[:, None]
+
+    def head_loss(h, w, t, ignore_index=-100):
+        x, live, at = rows(h, w, t, ignore_index)
+        lse = torch.logsumexp(x, 1)
+        return torch.where(live, lse - x.gather(1, at)[:, 0], 0.0), lse, torch.zeros_like(t)
+
+    def head_loss_grad(h, w, t, lse, gl, gz=None, want_hidden=True, want_lm_head=True, ignore_index=-100):
+        seen.append(dict(grad_loss=gl, grad_lse=gz, want_hidden=want_hidden, want_lm_head=want_lm_head))
+        x, live, at = rows(h, w, t, ignore_index)
+        p = torch.exp(x - lse[:, None]) * (gl if gz is None else gl + gz)[:, None]
+        p.scatter_add_(1, at, -gl[:, None])
+        p = torch.where(live[:, None], p, 0.0)
+        return ((p @ w.float()).to(h.dtype) if want_hidden else None,
+                (p.T @ h.float()).to(w.dtype) if want_lm_head else None)
+
+    monkeypatch.setattr(L.ops, "head_loss", head_loss)
+    monkeypatch.setattr(L.ops, "head_loss_grad", head_loss_grad)
+    return seen
+
+
+def inputs(R=6, K=8, V=20):
+    g = torch.Generator().manual_seed(0)
+    h, w = torch.randn(R, K, generator=g), torch.randn(V, K, generator=g)
+    return h.requires_grad_(), w.requires_grad_(), torch.randint(0, V, (R,), generator=g)
+
+
+def test_second_derivatives_raise(calls):
+    """A gradient penalty on the loss is refused: it would add nothing."""
+    h, w, t = inputs()
+    (dh,) = torch.autograd.grad(L.head_cross_entropy(h, w, t), h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dh.square().sum().backward()
+    # first derivatives are what they were
+    ref = torch.autograd.grad(torch.nn.functional.cross_entropy(h @ w.T, t), (h, w))
+    got = torch.autograd.grad(L.head_cross_entropy(h, w, t), (h, w))
+    for a, b in zip(got, ref):
+        assert torch.allclose(a, b, rtol=1e-4, atol=1e-6)
