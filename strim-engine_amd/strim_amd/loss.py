@@ -34,6 +34,7 @@ class _HeadLoss(torch.autograd.Function):
         ctx.save_for_backward(hidden, lm_head, targets, lse)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(status)
+        ctx.set_materialize_grads(False)  # (an output that is not used has no gradient, not zeros)
         return loss, lse, status
 
     @staticmethod

@@ -51,3 +51,18 @@ def test_second_derivatives_raise(calls):
     got = torch.autograd.grad(L.head_cross_entropy(h, w, t), (h, w))
     for a, b in zip(got, ref):
         assert torch.allclose(a, b, rtol=1e-4, atol=1e-6)
+
+
+def test_an_unused_output_takes_no_gradient(calls):
+    """A plain loss hands no gradient of the log-sum-exp to the device (not zeros), and the
+    log-sum-exp alone has zeros for the loss; frozen inputs are not asked for."""
+    h, w, t = inputs()
+    L.head_cross_entropy(h, w, t).backward()
+    assert calls[-1]["grad_lse"] is None and calls[-1]["want_hidden"] and calls[-1]["want_lm_head"]
+    L.head_loss(h, w.detach(), t)[1].sum().backward()
+    assert bool((calls[-1]["grad_loss"] == 0).all()) and bool((calls[-1]["grad_lse"] == 1).all())
+    assert calls[-1]["want_hidden"] and not calls[-1]["want_lm_head"]
+    loss, lse, _ = L.head_loss(h.detach(), w, t)
+    (2 * loss.sum() + 3 * lse.sum()).backward()
+    assert bool((calls[-1]["grad_loss"] == 2).all()) and bool((calls[-1]["grad_lse"] == 3).all())
+    assert not calls[-1]["want_hidden"] and calls[-1]["want_lm_head"]
