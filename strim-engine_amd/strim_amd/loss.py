@@ -18,6 +18,7 @@ IGNORE = -100
 
 def _ids(targets: torch.Tensor, V: int, ignore_index: int) -> torch.Tensor:
     """int32 target ids: an id outside [0, V) stays outside (also one past 32 bits)."""
+    ops.check_ignore_index(ignore_index)
     if targets.dtype == torch.int32:
         return targets.contiguous()
     if targets.dtype != torch.int64:

@@ -383,7 +383,13 @@ def _check_with(device: torch.device, *ts) -> None:
             raise ValueError("tensor arguments must be contiguous")
 
 
-def _loss_args(hidden, lm_head, targets):
+def check_ignore_index(ignore_index: int) -> None:
+    if not -2 ** 31 <= ignore_index < 2 ** 31:
+        raise ValueError(f"ignore_index must be a 32-bit number, got {ignore_index}")
+
+
+def _loss_args(hidden, lm_head, targets, ignore_index):
+    check_ignore_index(ignore_index)
     _check_bf16_rows("hidden", hidden)
     _check_bf16_rows("lm_head", lm_head)
     _check_with(hidden.device, targets)
@@ -437,7 +443,7 @@ def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor
     int32 [N]): minus the targets' log-probabilities, the logits' log-sum-exp, and OK, EINVAL
     (a target outside [0, V) that is not ignore_index) or ENONFINITE. Ignored rows have loss
     0. strim_amd.loss has the differentiable form."""
-    R, K, V = _loss_args(hidden, lm_head, targets)
+    R, K, V = _loss_args(hidden, lm_head, targets, ignore_index)
     dev = hidden.device
     res = []
     with _on(stream, (hidden, lm_head, targets, workspace), res):
@@ -461,7 +467,7 @@ def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.T
     """Gradients of head_loss: (d_hidden bf16 [N, K] or None, d_lm_head bf16 [V, K] or None)
     from lse as head_loss gave it and the float32 [N] gradients of its loss and (optional)
     its lse."""
-    R, K, V = _loss_args(hidden, lm_head, targets)
+    R, K, V = _loss_args(hidden, lm_head, targets, ignore_index)
     dev = hidden.device
     _check_with(dev, lse, grad_loss, grad_lse)
     for t in (lse, grad_loss, grad_lse):

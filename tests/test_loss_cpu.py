@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from strim_amd import loss as L
+from strim_amd import ops
 
 
 @pytest.fixture
@@ -66,3 +67,23 @@ def test_an_unused_output_takes_no_gradient(calls):
     (2 * loss.sum() + 3 * lse.sum()).backward()
     assert bool((calls[-1]["grad_loss"] == 2).all()) and bool((calls[-1]["grad_lse"] == 3).all())
     assert not calls[-1]["want_hidden"] and calls[-1]["want_lm_head"]
+
+
+@pytest.mark.parametrize("ignore", [2 ** 31, -2 ** 31 - 1, 2 ** 40])
+def test_ignore_index_past_32_bits_is_refused(calls, ignore):
+    """It would be cut to 32 bits, 2^40 to token 0."""
+    h, w, t = inputs()
+    for ids in (t, t.int()):
+        with pytest.raises(ValueError, match="ignore_index"):
+            L.head_loss(h, w, ids, ignore_index=ignore)
+        with pytest.raises(ValueError, match="ignore_index"):
+            L.head_cross_entropy(h, w, ids, ignore_index=ignore)
+
+
+@pytest.mark.parametrize("ignore", [2 ** 31, -2 ** 31 - 1])
+def test_device_calls_refuse_it_too(ignore):
+    h, w, t = inputs()
+    with pytest.raises(ValueError, match="ignore_index"):
+        ops.head_loss(h, w, t, ignore)
+    with pytest.raises(ValueError, match="ignore_index"):
+        ops.head_loss_grad(h, w, t, t, t, ignore_index=ignore)
