@@ -17,14 +17,15 @@ IGNORE = -100
 
 
 def _ids(targets: torch.Tensor, V: int, ignore_index: int) -> torch.Tensor:
-    """int32 target ids: an id outside [0, V) stays outside (also one past 32 bits)."""
+    """int32 target ids: an id outside [0, V) that is not ignored stays so (also one past 32 bits)."""
     ops.check_ignore_index(ignore_index)
     if targets.dtype == torch.int32:
         return targets.contiguous()
     if targets.dtype != torch.int64:
         raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
     inside = (targets >= 0) & (targets < V)
-    kept = torch.where(targets == ignore_index, ignore_index, torch.where(inside, targets, V))
+    outside = V if ignore_index != V else -1
+    kept = torch.where(targets == ignore_index, ignore_index, torch.where(inside, targets, outside))
     return kept.to(torch.int32)
 
 

@@ -87,3 +87,16 @@ def test_device_calls_refuse_it_too(ignore):
         ops.head_loss(h, w, t, ignore)
     with pytest.raises(ValueError, match="ignore_index"):
         ops.head_loss_grad(h, w, t, t, t, ignore_index=ignore)
+
+
+@pytest.mark.parametrize("ignore", [-100, 20, 21, -1, 7, 2 ** 31 - 1, -2 ** 31])
+def test_ids_outside_the_vocabulary_stay_outside(ignore):
+    """Whatever the ignored id is, and however large the others are: ids of the vocabulary as they
+    are, the ignored id as it is, any other id neither."""
+    V = 20
+    t = torch.tensor([0, 5, 19, 20, 21, 25, -1, -7, 2 ** 40, 2 ** 40 + 5, -2 ** 40, 2 ** 32 + 7, ignore])
+    got = L._ids(t, V, ignore).long()
+    inside = (t >= 0) & (t < V)
+    assert torch.equal(got[inside], t[inside]) and torch.equal(got == ignore, t == ignore)
+    outside = ~inside & (t != ignore)
+    assert bool(((got < 0) | (got >= V))[outside].all())
