@@ -515,15 +515,15 @@ __global__ __launch_bounds__(256) void k_loss_rows_in(const uint16_t* x, int64_t
 // row, K = 1,024: 6.0 us, one after the other 18.0, sixteen 7.6).
 __global__ __launch_bounds__(256) void k_loss_join(const float* acc, int splits, int N, int K,
                                                    uint16_t* out, int64_t out_stride) {
-  const int64_t total = (int64_t)N * K;
-  const int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
-  if (i >= total) return;
-  lf32x4 s = *(const lf32x4*)(acc + i);
+  const int64_t total = (int64_t)N * K, stride = (int64_t)gridDim.x * 1024;
+  for (int64_t i = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x); i < total; i += stride) {
+    lf32x4 s = *(const lf32x4*)(acc + i);
 #pragma unroll 8
-  for (int q = 1; q < splits; ++q) s += *(const lf32x4*)(acc + q * total + i);
-  const float f[4] = {s[0], s[1], s[2], s[3]};
-  const int64_t n = i / K;
-  *(uint2*)(out + n * out_stride + (i - n * K)) = loss_pack4(f);
+    for (int q = 1; q < splits; ++q) s += *(const lf32x4*)(acc + q * total + i);
+    const float f[4] = {s[0], s[1], s[2], s[3]};
+    const int64_t n = i / K;
+    *(uint2*)(out + n * out_stride + (i - n * K)) = loss_pack4(f);
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------
@@ -665,8 +665,18 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
   return q;
 }
 
+// Rows whose logits' product is one launch: a launch has fewer than 2^32 threads (one of more runs
+// some of its workgroups only, without an error), and this many rows' tiles half of that. The
+// gradients' products take more only beyond what memory holds.
+static int loss_launch_rows(int V) { return (int)(((int64_t)1 << 22) / ceil_div(V, 256) * 256); }
+
 int64_t loss_workspace(int N, int K, int V, bool hid, bool head) {
-  return loss_plan(N, K, V, hid, head).bytes;
+  const int64_t bytes = loss_plan(N, K, V, hid, head).bytes;
+  const int most = loss_launch_rows(V);
+  if (hid || head || N <= most) return bytes;
+  const int64_t full = loss_plan(most, K, V, false, false).bytes;
+  const int64_t last = loss_plan((N - 1) % most + 1, K, V, false, false).bytes;
+  return full > last ? full : last;
 }
 
 template <int MODE, int WM, int WN, int TM, int TN, int R>
@@ -711,9 +721,9 @@ static void loss_gemm_vocab(const LossGemm& g, LossShape s, int64_t v, int64_t o
   loss_gemm<MODE>(t, rest, HEAD ? other : v - main, HEAD ? v - main : other, st);
 }
 
-hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws, int V,
-                       const int32_t* targets, int ignore_index, void* workspace, float* loss,
-                       float* lse, int32_t* status, hipStream_t st) {
+static void loss_rows(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws, int V,
+                      const int32_t* targets, int ignore_index, void* workspace, float* loss,
+                      float* lse, int32_t* status, hipStream_t st) {
   const LossPlan q = loss_plan(N, K, V, false, false);
   uint8_t* w8 = (uint8_t*)workspace;
   LossGemm g{};
@@ -738,6 +748,15 @@ hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void*
   if (N >= 1024) rows(k_loss_rows<16>, 16);
   else if (N >= 256) rows(k_loss_rows<8>, 8);
   else rows(k_loss_rows<2>, 2);
+}
+
+hipError_t launch_loss(const void* hidden, int64_t hs, int N, int K, const void* W, int64_t ws, int V,
+                       const int32_t* targets, int ignore_index, void* workspace, float* loss,
+                       float* lse, int32_t* status, hipStream_t st) {
+  const int most = loss_launch_rows(V);
+  for (int n = 0; n < N; n += most)
+    loss_rows((const uint16_t*)hidden + n * hs, hs, min(most, N - n), K, W, ws, V, targets + n,
+              ignore_index, workspace, loss + n, lse ? lse + n : nullptr, status ? status + n : nullptr, st);
   return hipGetLastError();
 }
 
@@ -808,9 +827,11 @@ hipError_t launch_loss_grad(const void* hidden, int64_t hs, int N, int K, const 
       loss_gemm_vocab<LM_DHEAD>(h, q.head, vn, K, st);
     }
   }
-  if (d_hidden)
-    hipLaunchKernelGGL(k_loss_join, dim3((unsigned)ceil_div((int64_t)N * K, 1024)), dim3(256), 0, st,
+  if (d_hidden) {
+    const int64_t blocks = min(ceil_div((int64_t)N * K, 1024), (int64_t)1 << 22);
+    hipLaunchKernelGGL(k_loss_join, dim3((unsigned)blocks), dim3(256), 0, st,
                        (const float*)(w8 + q.acc), q.splits, N, K, (uint16_t*)d_hidden, dhs);
+  }
   return hipGetLastError();
 }
 

@@ -438,3 +438,43 @@ def test_logits_far_below_zero_in_pieces():
         s = slice(a, a + 410)
         E = Exact(h[s], w, t[s], gl[s])
         within(dh[s], E.dh, E.tol_h, "d_hidden")
+
+
+def test_more_tiles_than_a_launch_has():
+    """As many rows as there may be by a wide vocabulary: 2^23 tiles of 512 threads, more threads
+    than one launch can have. The rows repeat a thousand."""
+    R, K, V, M = 1024, 8, 131_584, 4096
+    print(f"[loss] N={R * M} K={K} V={V}", flush=True)
+    h, w, t, _ = inputs(R, K, V, seed=71)
+    E = Exact(h, w, t)
+    loss, lse, st = ops.head_loss(h.repeat(M, 1), w, t.repeat(M))
+    assert int(st.abs().max()) == N.OK
+    for i in range(0, M, 512):
+        a = slice(i * R, (i + 512) * R)
+        err = (loss[a].double().view(-1, R) - E.loss).abs().amax(0)
+        assert bool((err <= E.tol).all()), (i, float((err / E.tol).max()))
+        err = (lse[a].double().view(-1, R) - E.lse).abs().amax(0)
+        assert bool((err <= E.tol)[E.live].all()), (i, float((err / E.tol)[E.live].max()))
+
+
+def test_more_gradients_than_a_launch_has():
+    """The hidden states' gradients of more elements than 2^34, four of which a thread adds. The
+    rows repeat 64."""
+    R, K, V, M = 64, 4104, 8, 1 << 16
+    print(f"[loss] N={R * M} K={K} V={V}", flush=True)
+    h, w, t, gl = inputs(R, K, V, seed=72)
+    _, lse, _ = ops.head_loss(h, w, t)
+    need = ops.head_loss_workspace(R * M, K, V, True, False) + 5 * R * M * K
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < need:
+        pytest.skip(f"needs {need >> 30} GB of memory")
+    E = Exact(h, w, t, gl)
+    rows = [x.repeat(M, *[1] * (x.dim() - 1)) for x in (h, t, lse, gl)]
+    dh, _ = ops.head_loss_grad(rows[0], w, *rows[1:], want_lm_head=False)
+    for i in range(0, M, 512):
+        got = dh[i * R:(i + 512) * R].float().view(-1, R, K)
+        lo, hi = got.amin(0).double(), got.amax(0).double()
+        within(lo, E.dh, E.tol_h, f"d_hidden, least of rows {i * R} on")
+        within(hi, E.dh, E.tol_h, f"d_hidden, largest of rows {i * R} on")
+    del rows, dh, got
+    torch.cuda.empty_cache()
