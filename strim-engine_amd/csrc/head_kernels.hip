@@ -527,8 +527,11 @@ __global__ __launch_bounds__(HP_T) void k_head_pick(const uint2* tbest, int ntil
 
 void launch_head_norm(const void* hidden, int64_t hidden_stride, int B, int K, const void* norm_w,
                       float eps, void* xn, hipStream_t st) {
-  hipLaunchKernelGGL(k_head_norm, dim3((unsigned)B), dim3(HN_T), 0, st, (const uint16_t*)hidden,
-                     hidden_stride, K, (const uint16_t*)norm_w, eps, (uint16_t*)xn);
+  constexpr int64_t MOST = 1 << 21;  // a launch has fewer than 2^32 threads
+  for (int64_t b = 0; b < B; b += MOST)
+    hipLaunchKernelGGL(k_head_norm, dim3((unsigned)(B - b < MOST ? B - b : MOST)), dim3(HN_T), 0, st,
+                       (const uint16_t*)hidden + b * hidden_stride, hidden_stride, K,
+                       (const uint16_t*)norm_w, eps, (uint16_t*)xn + b * K);
 }
 
 hipError_t launch_head(const void* hidden, int64_t hidden_stride, int B, int K,

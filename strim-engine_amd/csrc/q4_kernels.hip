@@ -1135,15 +1135,15 @@ hipError_t launch_q4_logits(const void* x, int64_t x_stride, int B, int K, const
                             int64_t words_stride, const uint16_t* scales, const uint16_t* biases,
                             int64_t scales_stride, int group, int V, void* workspace, void* out,
                             bool out_f32, int64_t out_stride, hipStream_t st) {
-  for (int b = 0; b < B; b += 64) {  // the weights are read once per 64 rows
+  for (int64_t b = 0; b < B; b += 64) {  // the weights are read once per 64 rows
     Q4Args a{};
     a.w = Q4Weights{words, words_stride, scales, biases, scales_stride, V, K};
-    a.x = (const uint16_t*)x + (int64_t)b * x_stride;
+    a.x = (const uint16_t*)x + b * x_stride;
     a.x_stride = x_stride;
-    a.B = B - b < 64 ? B - b : 64;
+    a.B = B - b < 64 ? (int)(B - b) : 64;
     a.blocks = (uint8_t*)workspace;
     a.part = (float*)(a.blocks + q4_blocks_bytes(B < 64 ? B : 64, K));
-    a.out = (uint8_t*)out + (int64_t)b * out_stride * (out_f32 ? 4 : 2);
+    a.out = (uint8_t*)out + b * out_stride * (out_f32 ? 4 : 2);
     a.out_stride = out_stride;
     a.out_f32 = out_f32;
     if (group == 32) q4_logits<32>(a, st);

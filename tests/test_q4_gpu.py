@@ -334,3 +334,16 @@ def test_several_tiles_a_wave(B, K, V, G):
     q = weight(V, K, G, False, seed=B + K)
     x = torch.randn(B, K, device="cuda", generator=gen(V)).to(torch.bfloat16)
     check_logits(x, q, ops.head_logits_q4(x, q, out_dtype=torch.float32), "f32")
+
+
+def test_norm_of_more_rows_than_a_launch_has():
+    """More rows to normalise than workgroups of 1,024 threads in a launch. The rows repeat 64."""
+    R, K, V, M = 64, 32, 5, 1 << 16
+    B = R * M + 1
+    print(f"[q4] norm B={B}", flush=True)
+    q = weight(V, K, 32, False, seed=8)
+    x = torch.randn(R, K, device="cuda", generator=gen(8)).to(torch.bfloat16)
+    nw = torch.ones(K, dtype=torch.bfloat16, device="cuda")
+    ref = ops.head_logits_q4(x, q, nw)
+    got = ops.head_logits_q4(torch.cat([x.repeat(M, 1), x[:1]]), q, nw)
+    assert bool((got[:-1].view(M, R, V) == ref).all()) and torch.equal(got[-1], ref[0])
