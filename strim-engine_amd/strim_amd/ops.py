@@ -30,9 +30,11 @@ _AS_IS = contextlib.nullcontext()
 
 
 @contextlib.contextmanager
-def _given(stream, tensors, results: list):
+def _given(stream, device: torch.device, tensors, results: list):
     if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(stream.cuda_stream, tensors[0].device)
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device)
+    if stream.device != device:
+        raise ValueError(f"the stream is one of {stream.device}, the tensors are on {device}")
     caller = torch.cuda.current_stream(stream.device)
     for t in tensors:
         if t is not None:
@@ -44,13 +46,16 @@ def _given(stream, tensors, results: list):
             t.record_stream(caller)
 
 
-def _on(stream, tensors, results: list):
-    """The context in which a call allocates and launches. With a given stream that stream is
-    current: temporary memory is taken from it and goes back to it, in the order of its work (taken
-    from the caller's stream it would be handed out again while the kernels still use it).
-    `tensors`, the caller's own, are not handed out again before the stream is done with them, nor
-    `results` before the caller's stream is."""
-    return _AS_IS if stream is None else _given(stream, tensors, results)
+def _on(stream, device: torch.device, tensors, results: list):
+    """The context in which a call on `device` allocates and launches: that device is current (the
+    default stream, and what a kernel is told once, are the current device's). With a given stream
+    that stream is current too: temporary memory is taken from it and goes back to it, in the order
+    of its work (taken from the caller's stream it would be handed out again while the kernels still
+    use it). `tensors`, the caller's own, are not handed out again before the stream is done with
+    them, nor `results` before the caller's stream is."""
+    if stream is not None:
+        return _given(stream, device, tensors, results)
+    return _AS_IS if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -303,7 +308,7 @@ def head_logits(hidden: torch.Tensor, lm_head: torch.Tensor,
     if lm_head.shape[1] != K:
         raise ValueError(f"lm_head is [{lm_head.shape[0]}, {lm_head.shape[1]}], hidden K={K}")
     res = []
-    with _on(stream, (hidden, lm_head, norm_weight, out, xn), res):
+    with _on(stream, hidden.device, (hidden, lm_head, norm_weight, out, xn), res):
         if out is None:
             out = torch.empty(B, V, dtype=torch.bfloat16, device=hidden.device)
             res.append(out)
@@ -336,7 +341,8 @@ def head_greedy(ctx: "Context", hidden: torch.Tensor, lm_head: torch.Tensor,
     if lm_head.shape[1] != K:
         raise ValueError(f"lm_head is [{lm_head.shape[0]}, {lm_head.shape[1]}], hidden K={K}")
     res = []
-    with _on(stream, (hidden, lm_head, norm_weight, out_logits, xn, ids, status), res):
+    mine = (hidden, lm_head, norm_weight, out_logits, xn, ids, status)
+    with _on(stream, hidden.device, mine, res):
         if norm_weight is not None and xn is None:
             xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
         if ids is None:
@@ -446,7 +452,7 @@ def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor
     R, K, V = _loss_args(hidden, lm_head, targets, ignore_index)
     dev = hidden.device
     res = []
-    with _on(stream, (hidden, lm_head, targets, workspace), res):
+    with _on(stream, dev, (hidden, lm_head, targets, workspace), res):
         loss = torch.empty(R, dtype=torch.float32, device=dev)
         lse = torch.empty(R, dtype=torch.float32, device=dev)
         status = torch.empty(R, dtype=torch.int32, device=dev)
@@ -476,7 +482,7 @@ def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.T
     if not (want_hidden or want_lm_head):
         return None, None
     res = []
-    with _on(stream, (hidden, lm_head, targets, lse, grad_loss, grad_lse, workspace), res):
+    with _on(stream, dev, (hidden, lm_head, targets, lse, grad_loss, grad_lse, workspace), res):
         dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
         dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
         res += [dh, dw]
@@ -524,7 +530,7 @@ def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
         raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
     dev = weight.device
     res = []
-    with _on(stream, (weight,), res):
+    with _on(stream, dev, (weight,), res):
         words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
         scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
         biases = None if symmetric else torch.empty_like(scales)
@@ -538,7 +544,7 @@ def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
 def q4_unpack(q: Q4Weight, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """The values [V, K] that a packed projection stands for, as bf16 or float32."""
     dev, res = q.words.device, []
-    with _on(stream, (q.words, q.scales, q.biases), res):
+    with _on(stream, dev, (q.words, q.scales, q.biases), res):
         out = torch.empty(q.V, q.K, dtype=dtype, device=dev)
         res.append(out)
         N.check(N.lib().strim_unpack_weights(_stream_of(stream, dev), _ptr(q.words), q.K // 8,
@@ -572,7 +578,7 @@ def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor 
     if out is not None and out.shape != (B, q.V):
         raise ValueError(f"out must be [{B}, {q.V}]")
     res = []
-    with _on(stream, (hidden, q.words, q.scales, q.biases, norm_weight, out, xn, workspace), res):
+    with _on(stream, dev, (hidden, q.words, q.scales, q.biases, norm_weight, out, xn, workspace), res):
         if norm_weight is not None and xn is None:
             xn = torch.empty(B, K, dtype=torch.bfloat16, device=dev)
         if out is None:
