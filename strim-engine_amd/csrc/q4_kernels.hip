@@ -13,6 +13,8 @@
 // scaling of weights before the product, so T is a bf16 MFMA's sum in float32, and a group
 // costs two multiply-adds a result. The offset 16 (and not 128, which would save one of the
 // four shifts) keeps what cancels between T and 16 X to a few bits.
+#include <atomic>
+
 #include "kernels.hpp"
 
 namespace strim {
@@ -1033,12 +1035,20 @@ int64_t q4_workspace(int B, int K) {
   return q4_blocks_bytes(B, K) + (int64_t)QC_SPLIT * 16 * rows * 4;
 }
 
-// A launch with more than 64 KB of LDS, which a kernel has to be told of once.
+// A launch with more than 64 KB of LDS, which a kernel has to be told of once on each device. (One
+// that cannot be told is not launched; the call ends with that error.)
 template <auto KERNEL, class... More>
 static bool q4_big_lds(dim3 grid, size_t lds, hipStream_t st, const Q4Args& a, int waves, More... more) {
-  static const hipError_t told = hipFuncSetAttribute(
-      (const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize, (int)QS_LDS);
-  (void)told;
+  static std::atomic<uint64_t> told{0};  // a bit a device
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess) return true;
+  const uint64_t bit = (uint64_t)1 << (device & 63);
+  if (!(told.load(std::memory_order_relaxed) & bit)) {
+    if (hipFuncSetAttribute((const void*)KERNEL, hipFuncAttributeMaxDynamicSharedMemorySize,
+                            (int)QS_LDS) != hipSuccess)
+      return true;
+    told.fetch_or(bit, std::memory_order_relaxed);
+  }
   hipLaunchKernelGGL(KERNEL, grid, dim3(waves * WAVE), lds, st, a, more...);
   return true;
 }
