@@ -320,7 +320,8 @@ __global__ __launch_bounds__(WM* WN* WAVE, 2) void k_loss_gemm(const LossGemm g)
     interleave();
     cur = nxt;
   }
-  if (R > 2) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (none left open)
+  // none left open (of two stages: the second one's, where there was no step)
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
   // lane l holds C[row 4 (l / 16) + r][column l % 16] of each 16 x 16 tile
   const int h = lane >> 4, c16 = lane & 15;

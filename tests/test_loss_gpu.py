@@ -478,3 +478,27 @@ def test_more_gradients_than_a_launch_has():
         within(hi, E.dh, E.tol_h, f"d_hidden, largest of rows {i * R} on")
     del rows, dh, got
     torch.cuda.empty_cache()
+
+
+def test_products_without_steps():
+    """Workgroups that have nothing to add (no rows; a part of the vocabulary's last piece that is
+    empty) leave nothing under way for those that have their place next."""
+    h, w, t, gl = inputs(300, 256, 40_000, seed=81)
+    ref = ops.head_loss(h, w, t)
+    grads = ops.head_loss_grad(h, w, t, ref[1], gl)
+    for _ in range(4):
+        _, zero = ops.head_loss_grad(h[:0], w, t[:0], ref[1][:0], gl[:0], want_hidden=False)
+        got = ops.head_loss(h, w, t)
+        assert torch.equal(zero, torch.zeros_like(w))
+        again = ops.head_loss_grad(h, w, t, got[1], gl)
+        for a, b in zip((*got, *again), (*ref, *grads)):
+            assert torch.equal(a, b)
+    # a vocabulary in pieces
+    R, K, V = 2050, 64, 65_536 * 2 + 65
+    h, w, t, gl = inputs(R, K, V, seed=82)
+    _, lse, _ = ops.head_loss(h, w, t)
+    dh, _ = ops.head_loss_grad(h, w, t, lse, gl, want_lm_head=False)
+    for a in range(0, R, 410):
+        s = slice(a, a + 410)
+        E = Exact(h[s], w, t[s], gl[s])
+        within(dh[s], E.dh, E.tol_h, "d_hidden")
