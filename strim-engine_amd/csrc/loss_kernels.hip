@@ -652,10 +652,7 @@ static LossPlan loss_plan(int N, int K, int V, bool hid, bool head) {
   double least = 1e30;
   for (int s = 1; s <= 64 && s <= steps; ++s) {
     const LossShape shape = loss_shape(K, N, s, false);
-    const int64_t turns = ceil_div(K, shape_m(shape)) * ceil_div(N, shape_n(shape)) * s;
-    const double alone = turns <= LG_CUS && shape_m(shape) == 128 ? 0.6 : 1.0;
-    const double us = alone * shape_us(shape) * (double)(ceil_div(turns, shape_round(shape)) * ceil_div(steps, s)) +
-                      8.0 * s * N * (double)K / 4e6;
+    const double us = shape_cost(shape, K, N, s) * (double)ceil_div(steps, s) + 8.0 * s * N * (double)K / 4e6;
     if (us < least) least = us, q.splits = s, q.hid = shape;
   }
   q.scale = take(4);
