@@ -259,7 +259,7 @@ int strim_head_greedy(strim_ctx* ctx, void* stream, const void* hidden, int64_t 
  * strim_head_loss_grad: lse as strim_head_loss wrote it; grad_loss [N] and grad_lse [N] (NULL:
  * none) the gradients with respect to out_loss and out_lse (an ignored row's are not read;
  * its out_lse takes none). It computes the logits again, in pieces of the vocabulary whose
- * probabilities fit 512 MB:
+ * probabilities fit 512 MB (of 256 tokens at least, which take more from N = 2^20 on):
  *   p[n][v] = (grad_loss[n] + grad_lse[n]) exp(x[n][v] - lse[n]) - grad_loss[n] [v = targets[n]]
  *   d_hidden[n] = sum_v p[n][v] lm_head[v],   d_lm_head[v] = sum_n p[n][v] hidden[n]
  * p is rounded to bf16, sums are float32, results bf16; either result may be NULL (a frozen
@@ -293,8 +293,9 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
  * aligned).
  * strim_head_logits_packed is strim_head_logits over such a projection: hidden, norm_weight, eps
  * and xn as there, any B >= 1 (the weights are read once per 64 rows), logits as dtype (bf16 or
- * float32, what strim_sample takes), V up to STRIM_PACKED_MAX_VOCAB, accumulated in float32 from the exact s q + b. words and
- * its stride 16-byte aligned; workspace device, 16-byte aligned, of
+ * float32, what strim_sample takes), V up to STRIM_PACKED_MAX_VOCAB, accumulated in float32 from
+ * the exact s q + b. A hidden row that holds a NaN or an infinity has no finite logits (NaN as a rule).
+ * words and its stride 16-byte aligned; workspace device, 16-byte aligned, of
  * strim_head_logits_packed_workspace's bytes (else STRIM_ECAPACITY). */
 #define STRIM_PACKED_MAX_VOCAB (1 << 24)
 int strim_pack_weights(void* stream, const void* weight, int32_t dtype, int64_t weight_stride, int32_t V,

@@ -10,8 +10,9 @@
 //
 // Four products of 2 N V K operations: the logits twice (once for their row statistics, once
 // more for p), and one for each gradient. What is kept between them is a (max, sum) pair per
-// row and 128-row vocabulary slice, and p of one piece of the vocabulary, rounded to bf16 for
-// the two gradient products (the gradients are bf16 themselves; their sums are float32).
+// row and slice of the vocabulary (the 32, 64 or 128 of its rows that one wave has), and p of one
+// piece of the vocabulary, rounded to bf16 for the two gradient products (the gradients are bf16
+// themselves; their sums are float32).
 //
 // k_loss_gemm is all four: a tile of C = A B^T on v_mfma_f32_16x16x32_bf16, its operands
 // brought by 16-byte loads straight into LDS, one stage of 64 along the reduction ahead of
@@ -529,7 +530,8 @@ __global__ __launch_bounds__(256) void k_loss_join(const float* acc, int splits,
 
 // ---- host --------------------------------------------------------------------------------
 constexpr int LG_CUS = 256;
-constexpr int64_t LOSS_P_BYTES = (int64_t)512 << 20;  // p of one vocabulary piece
+// p of one vocabulary piece (256 of the vocabulary's rows are the least: more from 2^20 rows on)
+constexpr int64_t LOSS_P_BYTES = (int64_t)512 << 20;
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int64_t up256(int64_t b) { return (b + 255) & ~(int64_t)255; }

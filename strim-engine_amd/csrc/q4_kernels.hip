@@ -11,8 +11,9 @@
 // 16 + q is made in place: a code moved to bits 3 .. 6 of a half word under the bits of 16.0
 // in bf16, two codes an instruction pair (the shift, and an AND-OR), exact; no conversion, no
 // scaling of weights before the product, so T is a bf16 MFMA's sum in float32, and a group
-// costs two multiply-adds a result. The offset 16 (and not 128, which would save one of the
-// four shifts) keeps what cancels between T and 16 X to a few bits.
+// costs two multiply-adds a result (one in k_q4_chunk, whose X term is MFMAs as well). The offset
+// 16 (and not 128, which would save one of the four shifts) keeps what cancels between T and 16 X
+// to a few bits. An infinity in a hidden row makes both infinite: its logits are NaN as a rule.
 #include <atomic>
 
 #include "kernels.hpp"

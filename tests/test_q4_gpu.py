@@ -380,3 +380,16 @@ def test_pack_scales_are_the_rounded_quotients(symmetric, dtype):
         assert torch.equal(q.biases[:, 0].double(), base)
     want = ((d.float() - base.float()[:, None]) / s.float()[:, None]).round() + (8 if symmetric else 0)
     assert torch.equal(codes(q)[:, 0], want.clamp(0, 15).double())
+
+
+@pytest.mark.parametrize("B", [2, 8, 16, 64])
+def test_an_infinity_stays_in_its_row(B):
+    """A hidden row that holds an infinity has no finite logit; the other rows keep their bits."""
+    q = weight(300, 512, 64, True, seed=9)
+    x = torch.randn(B, 512, device="cuda", generator=gen(9)).to(torch.bfloat16)
+    ref = ops.head_logits_q4(x, q)
+    x[B // 2, 77] = float("-inf")
+    got = ops.head_logits_q4(x, q)
+    assert not bool(got[B // 2].isfinite().any())
+    keep = torch.arange(B, device="cuda") != B // 2
+    assert torch.equal(got[keep], ref[keep])
