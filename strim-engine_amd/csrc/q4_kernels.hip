@@ -37,8 +37,9 @@ __device__ __forceinline__ uint32_t q4_bf16(float f) {
 // 33).
 //   biased:    s = bf16((max - min) / 15), b = bf16(min), q = clamp(rint((w - b) / s), 0, 15)
 //   symmetric: s = bf16(max|w| / 7),                      q = clamp(rint(w / s) + 8, 0, 15)
-// s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). A group with a NaN or an
-// infinity gets NaN for its scale and its bias.
+// s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). The divisions by 15 and 7
+// are products with their float32 reciprocals. A group with a NaN or an infinity gets NaN for
+// its scale and its bias.
 struct Q4Pack {
   const void* w;
   int64_t w_stride;
@@ -60,17 +61,6 @@ __device__ __forceinline__ float q4_extreme(float v) {
   if constexpr (LANES > 4) with(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, false));
   if constexpr (LANES > 8) with(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x140, 0xF, 0xF, false));
   return v;
-}
-
-// d / D, correctly rounded, for d >= 0: the product with the rounded reciprocal and one correction,
-// as for the codes below (every significand was tried for 7 and 15; the remainder is exact among
-// subnormals too). The product alone takes some quotients that are exactly between two bf16 numbers to
-// the wrong one; a division instead: V = 151,936, K = 5,120, bf16, groups of 32, 458 -> 469 us.
-template <int D>
-__device__ __forceinline__ float q4_over(float d) {
-  constexpr float R = 1.0f / D;
-  const float t = d * R, y = __builtin_fmaf(__builtin_fmaf(-t, (float)D, d), R, t);
-  return t < INFINITY ? y : t;
 }
 
 // The items (row, E elements) that a thread takes: every `stride` of the whole.
@@ -122,7 +112,7 @@ __global__ __launch_bounds__(256) void k_q4_pack(const Q4Pack a) {
     hi = q4_extreme<G / 8, true>(hi);
     if constexpr (!SYM) lo = q4_extreme<G / 8, false>(lo);
     const float nan = hi < INFINITY ? 0.0f : __uint_as_float(0x7FC00000u);
-    const uint32_t s16 = q4_bf16((SYM ? q4_over<7>(hi) : q4_over<15>(hi - lo)) + nan);
+    const uint32_t s16 = q4_bf16((SYM ? hi * (1.0f / 7.0f) : (hi - lo) * (1.0f / 15.0f)) + nan);
     const uint32_t b16 = SYM ? 0u : q4_bf16(lo + nan);
     const float s = __uint_as_float(s16 << 16), b = __uint_as_float(b16 << 16);
     // The correctly rounded quotient from the correctly rounded reciprocal, with one correction
