@@ -35,11 +35,13 @@ __device__ __forceinline__ uint32_t q4_bf16(float f) {
 // groups of 64: bf16 95 us, 4.5 TB/s, float32 153, 5.0 TB/s). The words do not go past the caches:
 // what reads them next finds them there (packed and read back, 8,193 x 2,048 in float32: 28 us, else
 // 33).
-//   biased:    s = bf16((max - min) / 15), b = bf16(min), q = clamp(rint((w - b) / s), 0, 15)
-//   symmetric: s = bf16(max|w| / 7),                      q = clamp(rint(w / s) + 8, 0, 15)
-// s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). The divisions by 15 and 7
-// are products with their float32 reciprocals. A group with a NaN or an infinity gets NaN for
-// its scale and its bias.
+//   biased:    s = bf16((max - min) r), b = bf16(min), q = clamp(rint((w - b) / s), 0, 15)
+//   symmetric: s = bf16(max|w| r),                     q = clamp(rint(w / s) + 8, 0, 15)
+// s and b are the values stored; s = 0 gives q = 0 (symmetric: 8). r is the float32 number next to
+// 1 / 15 (1 / 7) and the product a float32 one, which is what torch's division of a float32 tensor
+// by 15 (7) gives on the GPU: weights packed by elementary operations there have the same scales.
+// The quotient itself may round to the other of two bf16 numbers that it is as good as between. A
+// group with a NaN or an infinity gets NaN for its scale and its bias.
 struct Q4Pack {
   const void* w;
   int64_t w_stride;

@@ -360,3 +360,37 @@ def test_an_infinity_stays_in_its_row(B):
     assert not bool(got[B // 2].isfinite().any())
     keep = torch.arange(B, device="cuda") != B // 2
     assert torch.equal(got[keep], ref[keep])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("symmetric", [False, True])
+def test_pack_scales_are_the_products(symmetric, dtype):
+    """A stored scale is the float32 product of the group's width and the float32 number next to 1 / 15
+    (1 / 7), rounded to bf16, also where the quotient is exactly between two bf16 numbers; its codes
+    are the nearest ones for that scale."""
+    if symmetric and dtype == torch.bfloat16:
+        n = torch.arange(1, 256, device="cuda").double().repeat(2)  # (no 8-bit number is 7 times such a one)
+    else:
+        n = torch.arange(257, 512, 2, device="cuda").double() * (7 if symmetric else 15)
+    n = torch.cat([n * 2.0 ** e for e in (-9, -1, 6)])
+    V, G = n.numel(), 64
+    u = torch.rand(V, G, device="cuda", dtype=torch.float64, generator=gen(12))
+    if symmetric:
+        w = (2 * u - 1) * n[:, None]
+        w[:, 5], w[:, 9] = n, -n
+    else:
+        lo = -torch.remainder(n, 32 * 2.0 ** torch.floor(torch.log2(n) - 12))  # n's bits past the first eight
+        w = lo[:, None] + u * n[:, None]
+        w[:, 5], w[:, 9] = lo, n + lo
+    w = w.to(dtype)
+    q = ops.q4_pack(w, G, symmetric)
+    d = w.double()
+    hi, lo = d.amax(1), d.amin(1)
+    assert torch.equal(hi if symmetric else hi - lo, n)
+    s = (n.float() * torch.full_like(n, 1 / (7 if symmetric else 15), dtype=torch.float32)).to(torch.bfloat16)
+    assert torch.equal(q.scales[:, 0], s)
+    base = torch.zeros_like(lo) if symmetric else lo.to(torch.bfloat16).double()
+    if not symmetric:
+        assert torch.equal(q.biases[:, 0].double(), base)
+    want = ((d.float() - base.float()[:, None]) / s.float()[:, None]).round() + (8 if symmetric else 0)
+    assert torch.equal(codes(q)[:, 0], want.clamp(0, 15).double())
