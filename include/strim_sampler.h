@@ -289,8 +289,8 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
  * strim_pack_weights fills words, scales and biases (contiguous; biases NULL: symmetric) from a
  * bf16 or float32 weight: s = bf16((max - min) r15), b = bf16(min), q = rint((w - b) / s), or
  * s = bf16(max|w| r7), q = rint(w / s) + 8, clamped to [0, 15], with r15 and r7 the float32
- * numbers next to 1 / 15 and 1 / 7 and float32 products; s = 0 gives the group's minimum (0) back. strim_unpack_weights writes s q + b, rounded once, as dtype (rows 16-byte
- * aligned).
+ * numbers next to 1 / 15 and 1 / 7 and float32 products; s = 0 gives the group's minimum (0) back.
+ * strim_unpack_weights writes s q + b, rounded once, as dtype (rows 16-byte aligned).
  * strim_head_logits_packed is strim_head_logits over such a projection: hidden, norm_weight, eps
  * and xn as there, any B >= 1 (the weights are read once per 64 rows), logits as dtype (bf16 or
  * float32, what strim_sample takes), V up to STRIM_PACKED_MAX_VOCAB, accumulated in float32 from
