@@ -487,9 +487,10 @@ __global__ __launch_bounds__(256) void k_loss_rows(const float2* part, int slice
   }
   if (w != 0 || n >= N) return;
   const int t = targets[n];
-  const float lse = m + logf(s);
+  const float ls = logf(s), lse = m + ls;
   const bool known = t >= 0 && t < V, live = known && t != ignore_index;
-  const float loss = live ? lse - tlogit[n] : 0.0f;
+  // (not from lse, which is rounded to the largest logit's spacing)
+  const float loss = live ? (m - tlogit[n]) + ls : 0.0f;
   if (out_lse) out_lse[n] = lse;
   out_loss[n] = loss;
   if (out_status)

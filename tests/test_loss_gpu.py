@@ -502,3 +502,24 @@ def test_products_without_steps():
         s = slice(a, a + 410)
         E = Exact(h[s], w, t[s], gl[s])
         within(dh[s], E.dh, E.tol_h, "d_hidden")
+
+
+@pytest.mark.parametrize("V", [9, 300, 5001])
+def test_small_losses_beside_large_logits(V):
+    """A loss is as exact as its own size allows, and not only to the log-sum-exp's spacing: logits
+    that are exact in bf16 and float32, the target's the largest by d, so that the loss is log(1 +
+    (V - 1) exp(-d)). Bound: some thirty additions of a sum near 1 (2^-24 each), and an exponential's
+    and a logarithm's few 2^-24 of their own."""
+    for top in (40.0, 992.0, -992.0, -30_464.0):
+        for d in (8.0, 16.0) if abs(top) < 1000 else (256.0, 512.0):
+            w = torch.zeros(V, 8, device="cuda")
+            w[:, 0], w[V // 2, 0] = top - d, top
+            h = torch.zeros(2, 8, device="cuda")
+            h[:, 0] = 1.0
+            w, h = w.to(torch.bfloat16), h.to(torch.bfloat16)
+            assert float(w[V // 2, 0]) == top and float(w[0, 0]) == top - d
+            loss, lse, _ = ops.head_loss(h, w, torch.tensor([V // 2, 0], dtype=torch.int32, device="cuda"))
+            ref = np.log1p((V - 1) * np.exp(-d))
+            assert abs(float(loss[0]) - ref) <= 2e-6 + 4e-6 * ref, (top, d)
+            assert abs(float(loss[1]) - (ref + d)) <= 2e-6 + 4e-6 * ref + 2.0 ** -24 * (ref + d), (top, d)
+            assert abs(float(lse[0]) - (top + ref)) <= 2e-6 + 4e-6 * ref + 2.0 ** -24 * abs(top + ref), (top, d)
