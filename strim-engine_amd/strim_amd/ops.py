@@ -7,7 +7,6 @@ uses the results wait for that stream.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from functools import lru_cache
 
@@ -26,36 +25,44 @@ def _stream(stream=None) -> ctypes.c_void_p:
     return ctypes.c_void_p(s.cuda_stream)
 
 
-_AS_IS = contextlib.nullcontext()
+def _tensors(*xs):
+    """The tensors among a call's arguments or results."""
+    for x in xs:
+        if isinstance(x, torch.Tensor):
+            yield x
+        elif isinstance(x, Q4Weight):
+            yield from _tensors(x.words, x.scales, x.biases)
+        elif isinstance(x, tuple):
+            yield from _tensors(*x)
 
 
-@contextlib.contextmanager
-def _given(stream, device: torch.device, tensors, results: list):
+def _elsewhere(stream, device: torch.device) -> bool:
+    """Whether a call on `device` has to be made by _there: on a given stream, or with another
+    device current."""
+    return stream is not None or torch._C._cuda_getDevice() != device.index
+
+
+def _there(fn, stream, device: torch.device, *args):
+    """fn(*args) with `device` current (the default stream, and what a kernel is told once, are the
+    current device's). With a given stream that stream is current too: temporary memory is taken from
+    it and goes back to it, in the order of its work (taken from the caller's stream it would be
+    handed out again while the kernels still use it); the caller's tensors are not handed out again
+    before that stream is done with them, nor the results before the caller's is."""
+    if stream is None:
+        with torch.cuda.device(device):
+            return fn(*args)
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(stream.cuda_stream, device)
     if stream.device != device:
         raise ValueError(f"the stream is one of {stream.device}, the tensors are on {device}")
-    caller = torch.cuda.current_stream(stream.device)
-    for t in tensors:
-        if t is not None:
-            t.record_stream(stream)
+    caller = torch.cuda.current_stream(device)
+    for t in _tensors(*args):
+        t.record_stream(stream)
     with torch.cuda.stream(stream):
-        yield
-    for t in results:
-        if t is not None:
-            t.record_stream(caller)
-
-
-def _on(stream, device: torch.device, tensors, results: list):
-    """The context in which a call on `device` allocates and launches: that device is current (the
-    default stream, and what a kernel is told once, are the current device's). With a given stream
-    that stream is current too: temporary memory is taken from it and goes back to it, in the order
-    of its work (taken from the caller's stream it would be handed out again while the kernels still
-    use it). `tensors`, the caller's own, are not handed out again before the stream is done with
-    them, nor `results` before the caller's stream is."""
-    if stream is not None:
-        return _given(stream, device, tensors, results)
-    return _AS_IS if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+        out = fn(*args)
+    for t in _tensors(out):
+        t.record_stream(caller)
+    return out
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -307,17 +314,16 @@ def head_logits(hidden: torch.Tensor, lm_head: torch.Tensor,
     V = lm_head.shape[0]
     if lm_head.shape[1] != K:
         raise ValueError(f"lm_head is [{lm_head.shape[0]}, {lm_head.shape[1]}], hidden K={K}")
-    res = []
-    with _on(stream, hidden.device, (hidden, lm_head, norm_weight, out, xn), res):
-        if out is None:
-            out = torch.empty(B, V, dtype=torch.bfloat16, device=hidden.device)
-            res.append(out)
-        if norm_weight is not None and xn is None:
-            xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
-        N.check(N.lib().strim_head_logits(_stream(stream), _ptr(hidden), _row_stride(hidden), B, K,
-                                          _ptr(norm_weight), float(eps), _ptr(xn), _ptr(lm_head),
-                                          _row_stride(lm_head), V, _ptr(out), _row_stride(out)),
-                "strim_head_logits")
+    if _elsewhere(stream, hidden.device):
+        return _there(head_logits, stream, hidden.device, hidden, lm_head, norm_weight, eps, out, xn)
+    if out is None:
+        out = torch.empty(B, V, dtype=torch.bfloat16, device=hidden.device)
+    if norm_weight is not None and xn is None:
+        xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
+    N.check(N.lib().strim_head_logits(_stream(), _ptr(hidden), _row_stride(hidden), B, K,
+                                      _ptr(norm_weight), float(eps), _ptr(xn), _ptr(lm_head),
+                                      _row_stride(lm_head), V, _ptr(out), _row_stride(out)),
+            "strim_head_logits")
     return out
 
 
@@ -340,23 +346,22 @@ def head_greedy(ctx: "Context", hidden: torch.Tensor, lm_head: torch.Tensor,
     V = lm_head.shape[0]
     if lm_head.shape[1] != K:
         raise ValueError(f"lm_head is [{lm_head.shape[0]}, {lm_head.shape[1]}], hidden K={K}")
-    res = []
-    mine = (hidden, lm_head, norm_weight, out_logits, xn, ids, status)
-    with _on(stream, hidden.device, mine, res):
-        if norm_weight is not None and xn is None:
-            xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
-        if ids is None:
-            ids = torch.empty(B, dtype=torch.int32, device=hidden.device)
-        if status is None:
-            status = torch.empty(B, dtype=torch.int32, device=hidden.device)
-        res += [ids, status]
-        N.check(N.lib().strim_head_greedy(ctx.handle, _stream(stream), _ptr(hidden),
-                                          _row_stride(hidden), B, K, _ptr(norm_weight), float(eps),
-                                          _ptr(xn), _ptr(lm_head), _row_stride(lm_head), V,
-                                          _ptr(out_logits),
-                                          _row_stride(out_logits) if out_logits is not None else 0,
-                                          _ptr(ids), _ptr(status)),
-                "strim_head_greedy")
+    if _elsewhere(stream, hidden.device):
+        return _there(head_greedy, stream, hidden.device, ctx, hidden, lm_head, norm_weight, eps,
+                      out_logits, xn, ids, status)
+    if norm_weight is not None and xn is None:
+        xn = torch.empty(B, K, dtype=torch.bfloat16, device=hidden.device)
+    if ids is None:
+        ids = torch.empty(B, dtype=torch.int32, device=hidden.device)
+    if status is None:
+        status = torch.empty(B, dtype=torch.int32, device=hidden.device)
+    N.check(N.lib().strim_head_greedy(ctx.handle, _stream(), _ptr(hidden),
+                                      _row_stride(hidden), B, K, _ptr(norm_weight), float(eps),
+                                      _ptr(xn), _ptr(lm_head), _row_stride(lm_head), V,
+                                      _ptr(out_logits),
+                                      _row_stride(out_logits) if out_logits is not None else 0,
+                                      _ptr(ids), _ptr(status)),
+            "strim_head_greedy")
     return ids, status
 
 
@@ -372,10 +377,10 @@ def _check_bf16_rows(name: str, t: torch.Tensor) -> None:
         raise ValueError(f"{name} must be [rows, K] with contiguous rows")
 
 
-def _stream_of(stream, device: torch.device) -> int:
-    """The given stream's handle, or `device`'s current one (without the Stream object that
+def _stream_of(device: torch.device) -> int:
+    """The handle of `device`'s current stream (without the Stream object that
     torch.cuda.current_stream makes, 2.6 us)."""
-    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _check_with(device: torch.device, *ts) -> None:
@@ -451,17 +456,16 @@ def head_loss(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.Tensor
     0. strim_amd.loss has the differentiable form."""
     R, K, V = _loss_args(hidden, lm_head, targets, ignore_index)
     dev = hidden.device
-    res = []
-    with _on(stream, dev, (hidden, lm_head, targets, workspace), res):
-        loss = torch.empty(R, dtype=torch.float32, device=dev)
-        lse = torch.empty(R, dtype=torch.float32, device=dev)
-        status = torch.empty(R, dtype=torch.int32, device=dev)
-        res += [loss, lse, status]
-        ws = _workspace(workspace, head_loss_workspace(R, K, V), dev)
-        N.check(N.lib().strim_head_loss(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), R,
-                                        K, _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
-                                        ignore_index, _ptr(ws), _bytes(ws), _ptr(loss), _ptr(lse),
-                                        _ptr(status)), "strim_head_loss")
+    if _elsewhere(stream, dev):
+        return _there(head_loss, stream, dev, hidden, lm_head, targets, ignore_index, workspace)
+    loss = torch.empty(R, dtype=torch.float32, device=dev)
+    lse = torch.empty(R, dtype=torch.float32, device=dev)
+    status = torch.empty(R, dtype=torch.int32, device=dev)
+    ws = _workspace(workspace, head_loss_workspace(R, K, V), dev)
+    N.check(N.lib().strim_head_loss(_stream_of(dev), _ptr(hidden), _row_stride(hidden), R, K,
+                                    _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
+                                    ignore_index, _ptr(ws), _bytes(ws), _ptr(loss), _ptr(lse),
+                                    _ptr(status)), "strim_head_loss")
     return loss, lse, status
 
 
@@ -481,18 +485,17 @@ def head_loss_grad(hidden: torch.Tensor, lm_head: torch.Tensor, targets: torch.T
             raise ValueError(f"lse and the gradients must be float32 [{R}]")
     if not (want_hidden or want_lm_head):
         return None, None
-    res = []
-    with _on(stream, dev, (hidden, lm_head, targets, lse, grad_loss, grad_lse, workspace), res):
-        dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
-        dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
-        res += [dh, dw]
-        ws = _workspace(workspace, head_loss_workspace(R, K, V, want_hidden, want_lm_head), dev)
-        N.check(N.lib().strim_head_loss_grad(_stream_of(stream, dev), _ptr(hidden), _row_stride(hidden),
-                                             R, K, _ptr(lm_head), _row_stride(lm_head), V,
-                                             _ptr(targets), ignore_index, _ptr(lse), _ptr(grad_loss),
-                                             _ptr(grad_lse), _ptr(ws), _bytes(ws), _ptr(dh), K,
-                                             _ptr(dw), K),
-                "strim_head_loss_grad")
+    if _elsewhere(stream, dev):
+        return _there(head_loss_grad, stream, dev, hidden, lm_head, targets, lse, grad_loss, grad_lse,
+                      want_hidden, want_lm_head, ignore_index, workspace)
+    dh = torch.empty(R, K, dtype=torch.bfloat16, device=dev) if want_hidden else None
+    dw = torch.empty(V, K, dtype=torch.bfloat16, device=dev) if want_lm_head else None
+    ws = _workspace(workspace, head_loss_workspace(R, K, V, want_hidden, want_lm_head), dev)
+    N.check(N.lib().strim_head_loss_grad(_stream_of(dev), _ptr(hidden), _row_stride(hidden), R, K,
+                                         _ptr(lm_head), _row_stride(lm_head), V, _ptr(targets),
+                                         ignore_index, _ptr(lse), _ptr(grad_loss), _ptr(grad_lse),
+                                         _ptr(ws), _bytes(ws), _ptr(dh), K, _ptr(dw), K),
+            "strim_head_loss_grad")
     return dh, dw
 
 
@@ -529,28 +532,27 @@ def q4_pack(weight: torch.Tensor, group: int = 64, symmetric: bool = False,
     if group not in (32, 64, 128) or K % group:
         raise ValueError(f"group must be 32, 64 or 128 and divide K={K}, got {group}")
     dev = weight.device
-    res = []
-    with _on(stream, dev, (weight,), res):
-        words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
-        scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
-        biases = None if symmetric else torch.empty_like(scales)
-        res += [words, scales, biases]
-        N.check(N.lib().strim_pack_weights(_stream_of(stream, dev), _ptr(weight), code,
-                                           _row_stride(weight), V, K, group, _ptr(words), _ptr(scales),
-                                           _ptr(biases)), "strim_pack_weights")
+    if _elsewhere(stream, dev):
+        return _there(q4_pack, stream, dev, weight, group, symmetric)
+    words = torch.empty(V, K // 8, dtype=torch.int32, device=dev)
+    scales = torch.empty(V, K // group, dtype=torch.bfloat16, device=dev)
+    biases = None if symmetric else torch.empty_like(scales)
+    N.check(N.lib().strim_pack_weights(_stream_of(dev), _ptr(weight), code, _row_stride(weight), V,
+                                       K, group, _ptr(words), _ptr(scales), _ptr(biases)),
+            "strim_pack_weights")
     return Q4Weight(words, scales, biases, group)
 
 
 def q4_unpack(q: Q4Weight, dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
     """The values [V, K] that a packed projection stands for, as bf16 or float32."""
-    dev, res = q.words.device, []
-    with _on(stream, dev, (q.words, q.scales, q.biases), res):
-        out = torch.empty(q.V, q.K, dtype=dtype, device=dev)
-        res.append(out)
-        N.check(N.lib().strim_unpack_weights(_stream_of(stream, dev), _ptr(q.words), q.K // 8,
-                                             _ptr(q.scales), _ptr(q.biases), q.K // q.group, q.V, q.K,
-                                             q.group, _ptr(out), _dtype_code(out), q.K),
-                "strim_unpack_weights")
+    dev = q.words.device
+    if _elsewhere(stream, dev):
+        return _there(q4_unpack, stream, dev, q, dtype)
+    out = torch.empty(q.V, q.K, dtype=dtype, device=dev)
+    N.check(N.lib().strim_unpack_weights(_stream_of(dev), _ptr(q.words), q.K // 8, _ptr(q.scales),
+                                         _ptr(q.biases), q.K // q.group, q.V, q.K, q.group,
+                                         _ptr(out), _dtype_code(out), q.K),
+            "strim_unpack_weights")
     return out
 
 
@@ -570,25 +572,24 @@ def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor 
         raise ValueError("every tensor argument must be on the same GPU")
     if K != q.K:
         raise ValueError(f"the projection has K={q.K}, hidden K={K}")
+    if _elsewhere(stream, dev):
+        return _there(head_logits_q4, stream, dev, hidden, q, norm_weight, eps, out, out_dtype, xn, workspace)
     if norm_weight is not None:
         if norm_weight.dtype != torch.bfloat16 or norm_weight.shape != (K,):
             raise ValueError(f"norm_weight must be bfloat16 [{K}]")
-        if xn is not None and (xn.dtype != torch.bfloat16 or xn.shape != (B, K)):
-            raise ValueError(f"xn must be bfloat16 [{B}, {K}]")
-    if out is not None and out.shape != (B, q.V):
-        raise ValueError(f"out must be [{B}, {q.V}]")
-    res = []
-    with _on(stream, dev, (hidden, q.words, q.scales, q.biases, norm_weight, out, xn, workspace), res):
-        if norm_weight is not None and xn is None:
+        if xn is None:
             xn = torch.empty(B, K, dtype=torch.bfloat16, device=dev)
-        if out is None:
-            out = torch.empty(B, q.V, dtype=out_dtype, device=dev)
-            res.append(out)
-        ws = _workspace(workspace, head_logits_q4_workspace(B, K), dev)
-        N.check(N.lib().strim_head_logits_packed(
-            _stream_of(stream, dev), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
-            _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
-            q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
+        elif xn.dtype != torch.bfloat16 or xn.shape != (B, K):
+            raise ValueError(f"xn must be bfloat16 [{B}, {K}]")
+    if out is None:
+        out = torch.empty(B, q.V, dtype=out_dtype, device=dev)
+    elif out.shape != (B, q.V):
+        raise ValueError(f"out must be [{B}, {q.V}]")
+    ws = _workspace(workspace, head_logits_q4_workspace(B, K), dev)
+    N.check(N.lib().strim_head_logits_packed(
+        _stream_of(dev), _ptr(hidden), _row_stride(hidden), B, K, _ptr(norm_weight), eps,
+        _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
+        q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
     return out
 
 

@@ -18,12 +18,9 @@ def test_a_call_runs_with_its_device_current(monkeypatch):
 
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setattr(torch.cuda, "device", device)
-    one = torch.device("cuda:1")
-    with ops._on(None, torch.device("cuda:0"), (), []):
-        pass
-    assert made == []
-    with ops._on(None, one, (), []):
-        assert made == [one]
+    zero, one = torch.device("cuda:0"), torch.device("cuda:1")
+    assert not ops._elsewhere(None, zero) and ops._elsewhere(None, one)
+    assert ops._there(lambda *a: (a, list(made)), None, one, 1, 2) == ((1, 2), [one])
 
 
 @pytest.mark.gpu
