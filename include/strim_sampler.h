@@ -248,7 +248,8 @@ int strim_head_greedy(strim_ctx* ctx, void* stream, const void* hidden, int64_t 
  * head over its truncated vocabulary, and the log-probabilities of given tokens. No
  * counterpart in the reference, which trains nothing.
  *   hidden      bf16 [N][hidden_stride], lm_head bf16 [V][lm_head_stride]: K a multiple of 8,
- *               16-byte aligned, strides multiples of 8 of at most STRIM_LOSS_MAX_STRIDE.
+ *               16-byte aligned, strides multiples of 8; strides, K and V at most
+ *               STRIM_LOSS_MAX_STRIDE, N at most STRIM_LOSS_MAX_ROWS.
  *   targets     device [N]. ignore_index: the row counts for nothing (loss 0, no gradient,
  *               whatever its hidden row holds). Another id outside [0, V): the same, with
  *               STRIM_EINVAL in out_status.
