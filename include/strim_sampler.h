@@ -281,6 +281,114 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
                          int64_t workspace_bytes, void* d_hidden, int64_t d_hidden_stride,
                          void* d_lm_head, int64_t d_lm_head_stride);
 
+/* ---- what a row of logits says about its tokens -----------------------------------------
+ * Over the logits rows that strim_sample reads (bf16 or float32, rows of any stride >= V, aligned as
+ * their type), under its allow-mask and a temperature: with z[v] = x[v] / temperature on allowed ids
+ * and -inf elsewhere, p = exp(z - lse),
+ *   out_lse[r] = log sum_v exp(z[v]),        out_logprobs[r][s] = z[tokens[r][s]] - out_lse[r],
+ *   out_entropy[r] = -sum_v p[v] log p[v],   out_top_ids / out_top_logprobs [r][top] = the `top` first
+ *   ids in token order (logit descending, then id) and their z - out_lse.
+ * A server's log-probabilities with alternatives, a prompt's or a policy's scores, the alternatives a
+ * teacher gives to strim_distill. No counterpart in the reference, which reports no probabilities.
+ *   tokens      device [R][S] (S may be 0: NULL). ignore_index: the token counts for nothing
+ *               (log-probability 0, no gradient). Another id outside [0, V): the same, with STRIM_EINVAL
+ *               in out_status. A token that the mask forbids has log-probability -inf.
+ *   top         only logits above -inf are alternatives; places past the last one have id -1 and
+ *               log-probability -inf.
+ *   workspace   device, 16-byte aligned, of strim_token_scores_workspace's bytes, else
+ *               STRIM_ECAPACITY; free again when the call's work ends.
+ *   out_status  [R] or NULL. STRIM_EEMPTY (no allowed logit above -inf): out_lse -inf, entropy 0,
+ *               log-probabilities -inf. STRIM_ENONFINITE (an allowed NaN or +inf): NaN, ids -1.
+ * strim_token_scores_grad: from lse and entropy as strim_token_scores wrote them (entropy read only with
+ * grad_entropy) and the gradients with respect to out_logprobs [R][S], out_entropy [R] and out_lse [R]
+ * (each may be NULL: none),
+ *   d_logits[v] = 1 / temperature (sum_s g_s ([v = tokens[s]] - p[v])
+ *                                  - g_entropy p[v] (log p[v] + entropy) + g_lse p[v])
+ * for allowed v, else 0, in the logits' type; 0 throughout an empty row, NaN on the allowed ids of one
+ * that is not finite. A token given twice has both gradients. d_logits may be the logits themselves.
+ * R at most STRIM_SCORE_MAX_ROWS, V at most STRIM_SCORE_MAX_VOCAB, S and top at most
+ * STRIM_SCORE_MAX_LIST, temperature finite and > 0. R = 0: nothing is launched. */
+#define STRIM_SCORE_MAX_ROWS (1 << 22)
+#define STRIM_SCORE_MAX_VOCAB (1 << 20)
+#define STRIM_SCORE_MAX_LIST 128
+int64_t strim_token_scores_workspace(int32_t R, int32_t V, int32_t top);
+int strim_token_scores(void* stream, const void* logits, int32_t dtype, int32_t R, int32_t V,
+                       int64_t row_stride, float temperature, const uint32_t* mask_words,
+                       int64_t mask_stride, const int32_t* tokens, int32_t S, int32_t ignore_index,
+                       int32_t top, void* workspace, int64_t workspace_bytes, float* out_logprobs,
+                       float* out_entropy, float* out_lse, int32_t* out_top_ids,
+                       float* out_top_logprobs, int32_t* out_status);
+int strim_token_scores_grad(void* stream, const void* logits, int32_t dtype, int32_t R, int32_t V,
+                            int64_t row_stride, float temperature, const uint32_t* mask_words,
+                            int64_t mask_stride, const int32_t* tokens, int32_t S,
+                            int32_t ignore_index, const float* lse, const float* entropy,
+                            const float* grad_logprobs, const float* grad_entropy,
+                            const float* grad_lse, void* d_logits, int64_t d_stride);
+
+/* ---- distillation from a teacher's top logits -----------------------------------------------
+ * Student logits rows x (as above) against a teacher's alternatives: ids [N][M] and logprobs [N][M],
+ * log-probabilities at the loss's temperature, as strim_token_scores gives them. With q =
+ * softmax(x / temperature) over the whole vocabulary:
+ *   tail 0: p_m = softmax of the row's logprobs (any common shift of them is the same);
+ *           out_loss = sum_m p_m (log p_m - log q[id_m])
+ *   tail 1: p_m = exp(logprobs_m), and the teacher's remaining mass r = max(0, 1 - sum p) is one more
+ *           alternative against q_rest, the student's mass outside the ids:
+ *           out_loss += r (log r - log q_rest)
+ *   d_logits[v] = grad_loss / temperature
+ *                 (q[v] (sum p + r - [v no alternative] r / q_rest) - sum of p_m with id_m = v)
+ * A negative id, or a log-probability of -inf, is no alternative (padding). A row without any, or with
+ * an id of V or more (STRIM_EINVAL), counts for nothing: loss and gradient 0, whatever it holds. An id
+ * given twice counts with both probabilities. A row whose grad_loss is 0 has gradient 0.
+ *   out_lse, out_log_rest  [N] or NULL: log sum exp(x / temperature) and log q_rest (0 without tail),
+ *               what strim_distill_grad takes; 0 in a row that counts for nothing.
+ *   out_status  [N] or NULL: STRIM_OK, STRIM_EINVAL, or STRIM_ENONFINITE (a NaN or infinite loss).
+ *   workspace   as above, of strim_distill_workspace's bytes (step: for strim_distill_step).
+ * strim_distill_step is strim_distill and strim_distill_grad in one, for rows whose weights are known
+ * beforehand (a mean's 1 / count): the logits are read once. d_logits may be the logits themselves.
+ * strim_distill_scale: data *= *factor (device), which writes nothing where the factor is 1: a step's
+ * gradient times the gradient of what the rows' weighted sum went into. */
+int64_t strim_distill_workspace(int32_t N, int32_t V, int32_t M, int32_t step);
+int strim_distill(void* stream, const void* logits, int32_t dtype, int32_t N, int32_t V,
+                  int64_t row_stride, float temperature, const int32_t* ids, const float* logprobs,
+                  int32_t M, int32_t tail, void* workspace, int64_t workspace_bytes, float* out_loss,
+                  float* out_lse, float* out_log_rest, int32_t* out_status);
+int strim_distill_grad(void* stream, const void* logits, int32_t dtype, int32_t N, int32_t V,
+                       int64_t row_stride, float temperature, const int32_t* ids,
+                       const float* logprobs, int32_t M, int32_t tail, const float* lse,
+                       const float* log_rest, const float* grad_loss, void* d_logits,
+                       int64_t d_stride);
+int strim_distill_step(void* stream, const void* logits, int32_t dtype, int32_t N, int32_t V,
+                       int64_t row_stride, float temperature, const int32_t* ids,
+                       const float* logprobs, int32_t M, int32_t tail, const float* weights,
+                       void* workspace, int64_t workspace_bytes, float* out_loss, void* d_logits,
+                       int64_t d_stride, int32_t* out_status);
+int strim_distill_scale(void* stream, void* data, int32_t dtype, int64_t n, const float* factor);
+
+/* ---- norms with gradients ---------------------------------------------------------------------
+ * Rows x [N][x_stride] of K elements (bf16 or float32, any stride >= K, aligned as their type):
+ *   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(sum_k (x - mean)^2 / K + eps)
+ * with mean = sum_k x / K (center 1, out_mean [N]) or 0 (center 0, out_mean NULL: the root mean square
+ * of the projection's final norm, Weights.swift:270-273), in float32, rounded once. weight and bias
+ * [K] of wdtype, or NULL; out_rstd [N] or NULL. Rows whose squares sum past float32 have rstd 0.
+ * strim_norm_grad, with xh = (x - mean) rstd and h = weight grad_y (of x's type):
+ *   d_x = rstd (h - xh mean_k(h xh) [- mean_k(h), where mean is given]),
+ *   d_weight = sum_n grad_y xh,  d_bias = sum_n grad_y   (of wdtype; each of the three may be NULL)
+ * summed in float32 in an order that the sizes alone fix; d_x may be grad_y or x itself. rstd and mean as
+ * strim_norm wrote them (mean NULL: center 0). workspace as above, of strim_norm_workspace's bytes.
+ * K at most STRIM_NORM_MAX_WIDTH, N at most STRIM_NORM_MAX_ROWS. N = 0: nothing is launched but for
+ * d_weight and d_bias, which are zeroed. */
+#define STRIM_NORM_MAX_WIDTH (1 << 16)
+#define STRIM_NORM_MAX_ROWS (1 << 28)
+int strim_norm(void* stream, const void* x, int32_t dtype, int32_t N, int32_t K, int64_t x_stride,
+               const void* weight, const void* bias, int32_t wdtype, float eps, int32_t center,
+               void* y, int64_t y_stride, float* out_rstd, float* out_mean);
+int64_t strim_norm_workspace(int32_t N, int32_t K, int32_t want_weight, int32_t want_bias);
+int strim_norm_grad(void* stream, const void* x, int32_t dtype, int32_t N, int32_t K,
+                    int64_t x_stride, const void* grad_y, int64_t grad_stride, const void* weight,
+                    int32_t wdtype, const float* rstd, const float* mean, void* workspace,
+                    int64_t workspace_bytes, void* d_x, int64_t d_x_stride, void* d_weight,
+                    void* d_bias);
+
 /* ---- projections in 4 bits ----------------------------------------------------------
  * [V, K] as words uint32 [V][K / 8] (eight codes a word, the lowest four bits first), and per
  * group of 32, 64 or 128 elements of a row a bf16 scale s and bias b, [V][K / group]: the

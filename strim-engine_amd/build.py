@@ -43,6 +43,8 @@ UNITS = [
     ("head_kernels.hip", []),
     ("loss_kernels.hip", []),
     ("q4_kernels.hip", []),
+    ("score_kernels.hip", []),
+    ("norm_kernels.hip", []),
     ("grammar_kernels.hip", []),
     ("capi.hip", []),
 ]

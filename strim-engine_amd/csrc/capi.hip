@@ -9,6 +9,7 @@
 
 #include <mutex>
 
+#include "score.hpp"
 #include "stream.hpp"
 
 namespace strim {
@@ -860,6 +861,223 @@ int strim_head_logits_packed(void* stream, const void* hidden, int64_t hidden_st
                                         (const uint16_t*)scales, (const uint16_t*)biases,
                                         scales_stride, group, V, workspace, out_logits,
                                         dtype == STRIM_DTYPE_F32, out_stride, (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+namespace {
+bool aligned_as(const void* p, int32_t dtype) {
+  return ((uintptr_t)p & (dtype == STRIM_DTYPE_BF16 ? 1u : 3u)) == 0;
+}
+// rows of logits for the scores and the distillation loss
+bool score_rows_ok(int32_t dtype, int32_t R, int32_t V, int64_t stride, float T) {
+  return dtype_ok(dtype) && R >= 0 && R <= STRIM_SCORE_MAX_ROWS && V > 0 &&
+         V <= STRIM_SCORE_MAX_VOCAB && stride >= V && T > 0.0f && T < INFINITY;
+}
+bool list_ok(int32_t n) { return n >= 0 && n <= STRIM_SCORE_MAX_LIST; }
+}  // namespace
+
+int64_t strim_token_scores_workspace(int32_t R, int32_t V, int32_t top) {
+  if (!score_rows_ok(STRIM_DTYPE_BF16, R, V, V, 1.0f) || !list_ok(top)) return STRIM_EINVAL;
+  return R == 0 ? 0 : scores_workspace(R, V, top);
+}
+
+int strim_token_scores(void* stream, const void* logits, int32_t dtype, int32_t R, int32_t V,
+                       int64_t row_stride, float temperature, const uint32_t* mask_words,
+                       int64_t mask_stride, const int32_t* tokens, int32_t S, int32_t ignore_index,
+                       int32_t top, void* workspace, int64_t workspace_bytes, float* out_logprobs,
+                       float* out_entropy, float* out_lse, int32_t* out_top_ids,
+                       float* out_top_logprobs, int32_t* out_status) {
+  if (!score_rows_ok(dtype, R, V, row_stride, temperature) || !list_ok(S) || !list_ok(top) ||
+      (mask_words && mask_stride < ((int64_t)V + 31) / 32))
+    return STRIM_EINVAL;
+  if (R == 0) return STRIM_OK;
+  if (!logits || !aligned_as(logits, dtype) || !out_entropy || !out_lse ||
+      (S > 0 && (!tokens || !out_logprobs)) || (top > 0 && (!out_top_ids || !out_top_logprobs)))
+    return STRIM_EINVAL;
+  const int64_t need = scores_workspace(R, V, top);
+  if (need > 0 && (!workspace || !al16(workspace))) return STRIM_EINVAL;
+  if (workspace_bytes < need) return STRIM_ECAPACITY;
+  const ScoreArgs a{logits, row_stride, R, V, temperature, mask_words, mask_stride, tokens, S,
+                    ignore_index, top, out_logprobs, out_entropy, out_lse, out_top_ids,
+                    out_top_logprobs, out_status};
+  const hipError_t e = launch_scores(a, dtype == STRIM_DTYPE_BF16, workspace, (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_token_scores_grad(void* stream, const void* logits, int32_t dtype, int32_t R, int32_t V,
+                            int64_t row_stride, float temperature, const uint32_t* mask_words,
+                            int64_t mask_stride, const int32_t* tokens, int32_t S,
+                            int32_t ignore_index, const float* lse, const float* entropy,
+                            const float* grad_logprobs, const float* grad_entropy,
+                            const float* grad_lse, void* d_logits, int64_t d_stride) {
+  if (!score_rows_ok(dtype, R, V, row_stride, temperature) || !list_ok(S) || d_stride < V ||
+      (mask_words && mask_stride < ((int64_t)V + 31) / 32))
+    return STRIM_EINVAL;
+  if (R == 0) return STRIM_OK;
+  if (!logits || !aligned_as(logits, dtype) || !d_logits || !aligned_as(d_logits, dtype) || !lse ||
+      (grad_entropy && !entropy) || (S > 0 && grad_logprobs && !tokens))
+    return STRIM_EINVAL;
+  if (!grad_logprobs) S = 0;
+  const ScoreGradArgs a{logits, row_stride, R, V, temperature, mask_words, mask_stride, tokens, S,
+                        ignore_index, lse, entropy, grad_logprobs, grad_entropy, grad_lse, d_logits,
+                        d_stride};
+  const hipError_t e = launch_scores_grad(a, dtype == STRIM_DTYPE_BF16, (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int64_t strim_distill_workspace(int32_t N, int32_t V, int32_t M, int32_t step) {
+  if (!score_rows_ok(STRIM_DTYPE_BF16, N, V, V, 1.0f) || !list_ok(M) || M == 0) return STRIM_EINVAL;
+  return N == 0 ? 0 : distill_workspace(N, V, M, step != 0);
+}
+
+namespace {
+// the rows and their alternatives (N = 0: nothing is looked at)
+int distill_args(const void* logits, int32_t dtype, int32_t N, int32_t V, int64_t row_stride,
+                 float temperature, const int32_t* ids, const float* logprobs, int32_t M, int32_t tail,
+                 DistillArgs& a) {
+  if (!score_rows_ok(dtype, N, V, row_stride, temperature) || !list_ok(M) || M == 0) return STRIM_EINVAL;
+  if (N > 0 && (!logits || !aligned_as(logits, dtype) || !ids || !logprobs)) return STRIM_EINVAL;
+  a.logits = logits;
+  a.stride = row_stride;
+  a.N = N;
+  a.V = V;
+  a.T = temperature;
+  a.ids = ids;
+  a.logprobs = logprobs;
+  a.M = M;
+  a.tail = tail != 0;
+  return STRIM_OK;
+}
+int distill_space(int32_t N, int32_t V, int32_t M, bool step, const void* workspace, int64_t bytes) {
+  const int64_t need = distill_workspace(N, V, M, step);
+  if (need > 0 && (!workspace || !al16(workspace))) return STRIM_EINVAL;
+  return bytes < need ? STRIM_ECAPACITY : STRIM_OK;
+}
+}  // namespace
+
+int strim_distill(void* stream, const void* logits, int32_t dtype, int32_t N, int32_t V,
+                  int64_t row_stride, float temperature, const int32_t* ids, const float* logprobs,
+                  int32_t M, int32_t tail, void* workspace, int64_t workspace_bytes, float* out_loss,
+                  float* out_lse, float* out_log_rest, int32_t* out_status) {
+  DistillArgs a{};
+  int rc = distill_args(logits, dtype, N, V, row_stride, temperature, ids, logprobs, M, tail, a);
+  if (rc != STRIM_OK || N == 0) return rc;
+  if (!out_loss) return STRIM_EINVAL;
+  rc = distill_space(N, V, M, false, workspace, workspace_bytes);
+  if (rc != STRIM_OK) return rc;
+  a.loss = out_loss;
+  a.out_lse = out_lse;
+  a.out_log_rest = out_log_rest;
+  a.status = out_status;
+  const hipError_t e = launch_distill(a, dtype == STRIM_DTYPE_BF16, true, false, workspace,
+                                      (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_distill_grad(void* stream, const void* logits, int32_t dtype, int32_t N, int32_t V,
+                       int64_t row_stride, float temperature, const int32_t* ids,
+                       const float* logprobs, int32_t M, int32_t tail, const float* lse,
+                       const float* log_rest, const float* grad_loss, void* d_logits,
+                       int64_t d_stride) {
+  DistillArgs a{};
+  const int rc = distill_args(logits, dtype, N, V, row_stride, temperature, ids, logprobs, M, tail, a);
+  if (rc != STRIM_OK || d_stride < V) return rc != STRIM_OK ? rc : STRIM_EINVAL;
+  if (N == 0) return STRIM_OK;
+  if (!lse || (tail && !log_rest) || !grad_loss || !d_logits || !aligned_as(d_logits, dtype))
+    return STRIM_EINVAL;
+  a.lse = lse;
+  a.log_rest = log_rest;
+  a.weights = grad_loss;
+  a.d_logits = d_logits;
+  a.d_stride = d_stride;
+  const hipError_t e = launch_distill(a, dtype == STRIM_DTYPE_BF16, false, true, nullptr,
+                                      (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_distill_step(void* stream, const void* logits, int32_t dtype, int32_t N, int32_t V,
+                       int64_t row_stride, float temperature, const int32_t* ids,
+                       const float* logprobs, int32_t M, int32_t tail, const float* weights,
+                       void* workspace, int64_t workspace_bytes, float* out_loss, void* d_logits,
+                       int64_t d_stride, int32_t* out_status) {
+  DistillArgs a{};
+  int rc = distill_args(logits, dtype, N, V, row_stride, temperature, ids, logprobs, M, tail, a);
+  if (rc != STRIM_OK || d_stride < V) return rc != STRIM_OK ? rc : STRIM_EINVAL;
+  if (N == 0) return STRIM_OK;
+  if (!out_loss || !weights || !d_logits || !aligned_as(d_logits, dtype)) return STRIM_EINVAL;
+  rc = distill_space(N, V, M, true, workspace, workspace_bytes);
+  if (rc != STRIM_OK) return rc;
+  a.loss = out_loss;
+  a.status = out_status;
+  a.weights = weights;
+  a.d_logits = d_logits;
+  a.d_stride = d_stride;
+  const hipError_t e = launch_distill(a, dtype == STRIM_DTYPE_BF16, true, true, workspace,
+                                      (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int strim_distill_scale(void* stream, void* data, int32_t dtype, int64_t n, const float* factor) {
+  if (!dtype_ok(dtype) || n < 0) return STRIM_EINVAL;
+  if (n == 0) return STRIM_OK;
+  if (!data || !aligned_as(data, dtype) || !factor) return STRIM_EINVAL;
+  const hipError_t e = launch_distill_scale(data, dtype == STRIM_DTYPE_BF16, n, factor,
+                                            (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+namespace {
+bool norm_rows_ok(const void* p, int32_t dtype, int32_t K, int64_t stride) {
+  return p && aligned_as(p, dtype) && stride >= K;
+}
+bool norm_sizes_ok(int32_t dtype, int32_t N, int32_t K, int32_t wdtype) {
+  return dtype_ok(dtype) && dtype_ok(wdtype) && N >= 0 && N <= STRIM_NORM_MAX_ROWS && K > 0 &&
+         K <= STRIM_NORM_MAX_WIDTH;
+}
+}  // namespace
+
+int strim_norm(void* stream, const void* x, int32_t dtype, int32_t N, int32_t K, int64_t x_stride,
+               const void* weight, const void* bias, int32_t wdtype, float eps, int32_t center,
+               void* y, int64_t y_stride, float* out_rstd, float* out_mean) {
+  if (!norm_sizes_ok(dtype, N, K, wdtype) || !(eps >= 0.0f) || (center && N > 0 && !out_mean))
+    return STRIM_EINVAL;
+  if (N == 0) return STRIM_OK;
+  if (!norm_rows_ok(x, dtype, K, x_stride) || !norm_rows_ok(y, dtype, K, y_stride) ||
+      (weight && !aligned_as(weight, wdtype)) || (bias && !aligned_as(bias, wdtype)))
+    return STRIM_EINVAL;
+  const NormArgs a{x, x_stride, N, K, weight, bias, eps, y, y_stride, out_rstd,
+                   center ? out_mean : nullptr};
+  const hipError_t e = launch_norm(a, dtype == STRIM_DTYPE_BF16, wdtype == STRIM_DTYPE_BF16,
+                                   (hipStream_t)stream);
+  return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
+}
+
+int64_t strim_norm_workspace(int32_t N, int32_t K, int32_t want_weight, int32_t want_bias) {
+  if (!norm_sizes_ok(STRIM_DTYPE_F32, N, K, STRIM_DTYPE_F32)) return STRIM_EINVAL;
+  return N == 0 ? 0 : norm_workspace(N, K, want_weight != 0, want_bias != 0);
+}
+
+int strim_norm_grad(void* stream, const void* x, int32_t dtype, int32_t N, int32_t K,
+                    int64_t x_stride, const void* grad_y, int64_t grad_stride, const void* weight,
+                    int32_t wdtype, const float* rstd, const float* mean, void* workspace,
+                    int64_t workspace_bytes, void* d_x, int64_t d_x_stride, void* d_weight,
+                    void* d_bias) {
+  if (!norm_sizes_ok(dtype, N, K, wdtype) || (d_weight && !aligned_as(d_weight, wdtype)) ||
+      (d_bias && !aligned_as(d_bias, wdtype)))
+    return STRIM_EINVAL;
+  if (N > 0) {
+    if (!norm_rows_ok(x, dtype, K, x_stride) || !norm_rows_ok(grad_y, dtype, K, grad_stride) ||
+        (weight && !aligned_as(weight, wdtype)) || !rstd ||
+        (d_x && !norm_rows_ok(d_x, dtype, K, d_x_stride)))
+      return STRIM_EINVAL;
+    const int64_t need = norm_workspace(N, K, d_weight != nullptr, d_bias != nullptr);
+    if (need > 0 && (!workspace || !al16(workspace))) return STRIM_EINVAL;
+    if (workspace_bytes < need) return STRIM_ECAPACITY;
+  }
+  const NormGradArgs a{x, x_stride, grad_y, grad_stride, N, K, weight, rstd, mean, d_x, d_x_stride,
+                       d_weight, d_bias};
+  const hipError_t e = launch_norm_grad(a, dtype == STRIM_DTYPE_BF16, wdtype == STRIM_DTYPE_BF16,
+                                        workspace, (hipStream_t)stream);
   return e == hipSuccess ? STRIM_OK : STRIM_EHIP;
 }
 

@@ -43,6 +43,17 @@ EXPORTS = (
     "strim_unpack_weights",
     "strim_head_logits_packed_workspace",
     "strim_head_logits_packed",
+    "strim_token_scores_workspace",
+    "strim_token_scores",
+    "strim_token_scores_grad",
+    "strim_distill_workspace",
+    "strim_distill",
+    "strim_distill_grad",
+    "strim_distill_step",
+    "strim_distill_scale",
+    "strim_norm",
+    "strim_norm_workspace",
+    "strim_norm_grad",
     "strim_profile_begin",
     "strim_profile_end",
     "strim_kernel_name",
@@ -60,6 +71,8 @@ EXPORTS = (
 )
 KERNEL_COUNT = 8
 LOSS_MAX_ROWS, LOSS_MAX_STRIDE = 1 << 22, 1 << 20  # strim_head_loss limits
+SCORE_MAX_ROWS, SCORE_MAX_VOCAB, SCORE_MAX_LIST = 1 << 22, 1 << 20, 128  # strim_token_scores limits
+NORM_MAX_WIDTH, NORM_MAX_ROWS = 1 << 16, 1 << 28  # strim_norm limits
 NOALLOC_MAX_ROWS, NOALLOC_MAX_VOCAB = 32, 262144  # strim_sample_noalloc limits
 
 
@@ -165,6 +178,32 @@ def lib() -> ctypes.CDLL:
         L.strim_head_logits_packed.restype = ctypes.c_int
         L.strim_head_logits_packed.argtypes = [P, P, I64, I32, I32, P, ctypes.c_float, P, P, I64, P, P,
                                            I64, I32, I32, P, I64, P, I32, I64]
+        F = ctypes.c_float
+        L.strim_token_scores_workspace.restype = I64
+        L.strim_token_scores_workspace.argtypes = [I32, I32, I32]
+        L.strim_token_scores.restype = ctypes.c_int
+        L.strim_token_scores.argtypes = [P, P, I32, I32, I32, I64, F, P, I64, P, I32, I32, I32, P, I64,
+                                         P, P, P, P, P, P]
+        L.strim_token_scores_grad.restype = ctypes.c_int
+        L.strim_token_scores_grad.argtypes = [P, P, I32, I32, I32, I64, F, P, I64, P, I32, I32, P, P, P,
+                                              P, P, P, I64]
+        L.strim_distill_workspace.restype = I64
+        L.strim_distill_workspace.argtypes = [I32, I32, I32, I32]
+        L.strim_distill.restype = ctypes.c_int
+        L.strim_distill.argtypes = [P, P, I32, I32, I32, I64, F, P, P, I32, I32, P, I64, P, P, P, P]
+        L.strim_distill_grad.restype = ctypes.c_int
+        L.strim_distill_grad.argtypes = [P, P, I32, I32, I32, I64, F, P, P, I32, I32, P, P, P, P, I64]
+        L.strim_distill_step.restype = ctypes.c_int
+        L.strim_distill_step.argtypes = [P, P, I32, I32, I32, I64, F, P, P, I32, I32, P, P, I64, P, P,
+                                         I64, P]
+        L.strim_distill_scale.restype = ctypes.c_int
+        L.strim_distill_scale.argtypes = [P, P, I32, I64, P]
+        L.strim_norm.restype = ctypes.c_int
+        L.strim_norm.argtypes = [P, P, I32, I32, I32, I64, P, P, I32, F, I32, P, I64, P, P]
+        L.strim_norm_workspace.restype = I64
+        L.strim_norm_workspace.argtypes = [I32, I32, I32, I32]
+        L.strim_norm_grad.restype = ctypes.c_int
+        L.strim_norm_grad.argtypes = [P, P, I32, I32, I32, I64, P, I64, P, I32, P, P, P, I64, P, I64, P, P]
         L.strim_profile_begin.restype = ctypes.c_int
         L.strim_profile_begin.argtypes = [P, I32]
         L.strim_profile_end.restype = ctypes.c_int

@@ -1,4 +1,5 @@
-"""Training and scoring over the vocabulary: the differentiable form of ops.head_loss.
+"""Training and scoring over the vocabulary: the differentiable forms of ops.head_loss,
+ops.token_scores and ops.distill.
 
 Cross entropy of a vocabulary projection's logits against target ids, over the whole
 vocabulary and without keeping the logits, for training (or distilling) a draft head over its
@@ -86,3 +87,142 @@ def token_logprobs(hidden: torch.Tensor, lm_head: torch.Tensor, tokens: torch.Te
     """log p(token) of each position under its projected distribution (temperature 1, no
     filters), float32; 0 where the token is not an id of the vocabulary."""
     return -head_loss(hidden, lm_head, tokens)[0]
+
+
+class _TokenScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, temperature, mask, ignore_index):
+        out = ops.token_scores(logits, tokens, top, temperature, mask, ignore_index)
+        ctx.save_for_backward(logits, tokens, mask, out.lse, out.entropy)
+        ctx.args = temperature, ignore_index
+        ctx.mark_non_differentiable(*(t for t in (out.top_ids, out.top_logprobs, out.status)
+                                      if t is not None))
+        ctx.set_materialize_grads(False)
+        return tuple(out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logprobs, g_entropy, g_lse, *_):
+        logits, tokens, mask, lse, entropy = ctx.saved_tensors
+        temperature, ignore_index = ctx.args
+        g = [None if t is None else t.float().contiguous() for t in (g_logprobs, g_entropy, g_lse)]
+        d = ops.token_scores_grad(logits, tokens, lse, entropy, *g, temperature=temperature, mask=mask,
+                                  ignore_index=ignore_index)
+        return d, None, None, None, None, None
+
+
+def _rows(logits: torch.Tensor) -> torch.Tensor:
+    """[..., V] as [R, V] with contiguous rows."""
+    rows = logits.reshape(-1, logits.shape[-1])
+    return rows if rows.stride(-1) == 1 else rows.contiguous()
+
+
+def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0,
+                 temperature: float = 1.0, mask: torch.Tensor | None = None,
+                 ignore_index: int = IGNORE) -> ops.TokenScores:
+    """ops.token_scores over logits [..., V], with gradients for the logits through the tokens'
+    log-probabilities, the entropy and the log-sum-exp (first derivatives; the alternatives have none).
+    tokens int32 or int64 [...] or [..., S], mask [..., words]; results have the same leading shape."""
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    given = None
+    if tokens is not None:
+        if tokens.shape[:len(lead)] != lead or tokens.dim() > len(lead) + 1:
+            raise ValueError(f"tokens must be {tuple(lead)} or {tuple(lead)} + (n,), got {tuple(tokens.shape)}")
+        given = tokens.shape
+        R = lead.numel()
+        tokens = _ids(tokens.reshape((R,) if tokens.dim() == len(lead) else (R, tokens.shape[-1])), V,
+                      ignore_index)
+    if mask is not None:
+        if mask.shape[:-1] != lead:
+            raise ValueError(f"mask must be {tuple(lead)} + (words,), got {tuple(mask.shape)}")
+        mask = mask.reshape(-1, mask.shape[-1]).contiguous()
+    out = _TokenScores.apply(_rows(logits), tokens, top, temperature, mask, ignore_index)
+    lp, entropy, lse, ids, ilp, status = out
+    return ops.TokenScores(None if lp is None else lp.reshape(given), entropy.reshape(lead),
+                           lse.reshape(lead), None if ids is None else ids.reshape(*lead, top),
+                           None if ilp is None else ilp.reshape(*lead, top), status.reshape(lead))
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, logprobs, temperature, tail):
+        loss, lse, log_rest, status = ops.distill(logits, ids, logprobs, temperature, tail)
+        ctx.save_for_backward(logits, ids, logprobs, lse, log_rest)
+        ctx.args = temperature, tail
+        ctx.mark_non_differentiable(status)
+        ctx.set_materialize_grads(False)
+        return loss, status
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_loss, _):
+        if g_loss is None:
+            return None, None, None, None, None
+        logits, ids, logprobs, lse, log_rest = ctx.saved_tensors
+        temperature, tail = ctx.args
+        d = ops.distill_grad(logits, ids, logprobs, lse, log_rest, g_loss.float().contiguous(),
+                             temperature, tail)
+        return d, None, None, None, None
+
+
+class _DistillSum(torch.autograd.Function):
+    """The rows' losses times their weights, summed; the gradient comes with the loss, from one pass
+    over the logits."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, logprobs, weights, temperature, tail):
+        if ctx.needs_input_grad[0]:
+            loss, ctx.d, _ = ops.distill_step(logits, ids, logprobs, weights, temperature, tail)
+            ctx.save_for_backward(logits, ids, logprobs, weights)
+            ctx.args = temperature, tail
+        else:
+            loss = ops.distill(logits, ids, logprobs, temperature, tail)[0]
+        # (a row of weight 0 counts for nothing, an infinite or NaN loss included)
+        return torch.where(weights != 0, loss * weights, 0.0).sum()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, ids, logprobs, weights = ctx.saved_tensors
+        d, ctx.d = ctx.d, None
+        if d is None:  # (a second pass over a retained graph: the first one's result is the caller's)
+            d = ops.distill_step(logits, ids, logprobs, weights, *ctx.args)[1]
+        return ops.distill_scale(d, g.float().reshape(1)), None, None, None, None, None
+
+
+def _alternatives(logits, ids, logprobs):
+    lead = logits.shape[:-1]
+    if ids.shape[:-1] != lead or logprobs.shape != ids.shape:
+        raise ValueError(f"ids and logprobs must be {tuple(lead)} + (M,), got {tuple(ids.shape)} and "
+                         f"{tuple(logprobs.shape)}")
+    V, M = logits.shape[-1], ids.shape[-1]
+    if ids.dtype == torch.int64:  # (one past 32 bits stays outside the vocabulary)
+        ids = torch.where(ids < 0, -1, ids.clamp_max(V)).to(torch.int32)
+    if ids.dtype != torch.int32:
+        raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
+    if logprobs.requires_grad:
+        raise ValueError("the teacher's log-probabilities take no gradient: detach them")
+    return ids.reshape(-1, M).contiguous(), logprobs.reshape(-1, M).float().contiguous()
+
+
+def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                 temperature: float = 1.0, tail: bool = False, reduction: str = "mean") -> torch.Tensor:
+    """Divergence of softmax(logits / temperature) from a teacher's alternatives (ids and logprobs
+    [..., M], as token_scores gives them), with gradients for the logits [..., V] (first derivatives):
+    "mean" over the positions that have alternatives (0 if none has), "sum", or "none" (per position).
+    The mean and the sum make their gradient with the loss, in one pass over the logits, and hold it
+    until the backward pass; the gradient is then multiplied by what comes back (and rounded again
+    unless that is a power of two)."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction must be mean, sum or none, got {reduction}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    ids, logprobs = _alternatives(logits, ids, logprobs)
+    rows = _rows(logits)
+    if reduction == "none":
+        return _Distill.apply(rows, ids, logprobs, temperature, tail)[0].reshape(lead)
+    if reduction == "sum":
+        weights = torch.ones(rows.shape[0], dtype=torch.float32, device=rows.device)
+    else:
+        live = ((ids >= 0) & (logprobs != float("-inf"))).any(1) & (ids < V).all(1)
+        weights = live.float() / live.sum().clamp_min(1)
+    return _DistillSum.apply(rows, ids, logprobs, weights, temperature, tail)

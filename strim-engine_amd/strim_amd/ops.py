@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 from functools import lru_cache
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -591,6 +592,345 @@ def head_logits_q4(hidden: torch.Tensor, q: Q4Weight, norm_weight: torch.Tensor 
         _ptr(xn), _ptr(q.words), K // 8, _ptr(q.scales), _ptr(q.biases), K // q.group, q.group,
         q.V, _ptr(ws), _bytes(ws), _ptr(out), _dtype_code(out), q.V), "strim_head_logits_packed")
     return out
+
+
+class TokenScores(NamedTuple):
+    """What token_scores returns: log-probabilities of the given tokens (as tokens is shaped; None
+    without tokens), entropy and log-sum-exp float32 [R], the alternatives' ids int32 and
+    log-probabilities float32 [R, top] (None for top 0), status int32 [R]."""
+
+    logprobs: torch.Tensor | None
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_ids: torch.Tensor | None
+    top_logprobs: torch.Tensor | None
+    status: torch.Tensor
+
+
+def _check_logits(logits: torch.Tensor, temperature: float) -> int:
+    """The dtype code of logits [R, V] with contiguous rows."""
+    code = _dtype_code(logits)
+    if not logits.is_cuda:
+        raise ValueError("logits must be on the GPU")
+    if logits.dim() != 2 or (not logits.is_contiguous() and
+                             (logits.stride(1) != 1 or _row_stride(logits) < logits.shape[1])):
+        raise ValueError("logits must be [R, V] with contiguous rows (row stride >= V)")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be finite and positive, got {temperature}")
+    R, V = logits.shape
+    if R > N.SCORE_MAX_ROWS or not 0 < V <= N.SCORE_MAX_VOCAB:
+        raise ValueError(f"logits must be at most [{N.SCORE_MAX_ROWS}, {N.SCORE_MAX_VOCAB}], got [{R}, {V}]")
+    return code
+
+
+def _check_list(name: str, t: torch.Tensor, dtype: torch.dtype, R: int) -> int:
+    """Entries a row of a list int32 or float32 [R] or [R, S]."""
+    if t.dtype != dtype or t.dim() not in (1, 2) or t.shape[0] != R:
+        raise ValueError(f"{name} must be {dtype} [{R}] or [{R}, n], got {t.dtype} {tuple(t.shape)}")
+    S = 1 if t.dim() == 1 else t.shape[1]
+    if S > N.SCORE_MAX_LIST:
+        raise ValueError(f"{name} may have {N.SCORE_MAX_LIST} entries a row, got {S}")
+    return S
+
+
+def _check_mask(mask: torch.Tensor | None, R: int, V: int) -> int:
+    if mask is None:
+        return 0
+    if mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] != R or 32 * mask.shape[1] < V:
+        raise ValueError(f"mask must be int32 words [{R}, {(V + 31) // 32}], got {mask.dtype} "
+                         f"{tuple(mask.shape)}")
+    return mask.shape[1]
+
+
+def _logits_out(out: torch.Tensor | None, logits: torch.Tensor) -> torch.Tensor:
+    """Where the gradient goes: `out` (logits itself, say), or new memory."""
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if out.dtype != logits.dtype or out.shape != logits.shape or out.device != logits.device:
+        raise ValueError("out must be as the logits are")
+    _check_rows(out)
+    return out
+
+
+@lru_cache(maxsize=256)
+def token_scores_workspace(R: int, V: int, top: int) -> int:
+    """Bytes of workspace that token_scores takes."""
+    need = N.lib().strim_token_scores_workspace(R, V, top)
+    if need < 0:
+        raise N.StrimError(need, "strim_token_scores_workspace")
+    return need
+
+
+def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0,
+                 temperature: float = 1.0, mask: torch.Tensor | None = None,
+                 ignore_index: int = -100, workspace: torch.Tensor | None = None,
+                 stream=None) -> TokenScores:
+    """Log-probabilities of the given tokens (int32 [R] or [R, S]) under softmax(logits /
+    temperature) over the ids that `mask` (int32 words as Context.sample takes them) allows, its
+    entropy and log-sum-exp, and its `top` most probable ids (the lower id first where logits are
+    equal; past the last one -1 and -inf). logits bf16 or float32 [R, V]. Status per row: OK, EINVAL
+    (a token outside [0, V) that is not ignore_index: log-probability 0, as an ignored one's), EEMPTY
+    or ENONFINITE. strim_amd.loss has the differentiable form."""
+    code = _check_logits(logits, temperature)
+    check_ignore_index(ignore_index)
+    R, V = logits.shape
+    dev = logits.device
+    S = 0 if tokens is None else _check_list("tokens", tokens, torch.int32, R)
+    words = _check_mask(mask, R, V)
+    if not 0 <= top <= N.SCORE_MAX_LIST:
+        raise ValueError(f"top must be in [0, {N.SCORE_MAX_LIST}], got {top}")
+    _check_with(dev, tokens, mask)
+    if _elsewhere(stream, dev):
+        return _there(token_scores, stream, dev, logits, tokens, top, temperature, mask, ignore_index,
+                      workspace)
+    lp = None if tokens is None else torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(R, dtype=torch.float32, device=dev)
+    lse = torch.empty(R, dtype=torch.float32, device=dev)
+    ids = torch.empty(R, top, dtype=torch.int32, device=dev) if top else None
+    ilp = torch.empty(R, top, dtype=torch.float32, device=dev) if top else None
+    status = torch.empty(R, dtype=torch.int32, device=dev)
+    ws = _workspace(workspace, token_scores_workspace(R, V, top), dev)
+    N.check(N.lib().strim_token_scores(_stream_of(dev), _ptr(logits), code, R, V, _row_stride(logits),
+                                       temperature, _ptr(mask), words, _ptr(tokens), S, ignore_index,
+                                       top, _ptr(ws), _bytes(ws), _ptr(lp), _ptr(entropy), _ptr(lse),
+                                       _ptr(ids), _ptr(ilp), _ptr(status)), "strim_token_scores")
+    return TokenScores(lp, entropy, lse, ids, ilp, status)
+
+
+def token_scores_grad(logits: torch.Tensor, tokens: torch.Tensor | None, lse: torch.Tensor,
+                      entropy: torch.Tensor | None = None, grad_logprobs: torch.Tensor | None = None,
+                      grad_entropy: torch.Tensor | None = None, grad_lse: torch.Tensor | None = None,
+                      temperature: float = 1.0, mask: torch.Tensor | None = None,
+                      ignore_index: int = -100, out: torch.Tensor | None = None,
+                      stream=None) -> torch.Tensor:
+    """The logits' gradient [R, V] (of their type) from lse and entropy as token_scores gave them and
+    the float32 gradients of its log-probabilities (shaped as tokens), entropy and lse; each may be
+    None. out: where it goes, the logits themselves included."""
+    code = _check_logits(logits, temperature)
+    check_ignore_index(ignore_index)
+    R, V = logits.shape
+    dev = logits.device
+    S = 0
+    if grad_logprobs is not None:
+        if tokens is None or grad_logprobs.shape != tokens.shape:
+            raise ValueError("grad_logprobs must be shaped as the tokens are")
+        S = _check_list("tokens", tokens, torch.int32, R)
+        _check_list("grad_logprobs", grad_logprobs, torch.float32, R)
+    if grad_entropy is not None and entropy is None:
+        raise ValueError("grad_entropy needs the entropy")
+    for t in (lse, entropy, grad_entropy, grad_lse):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (R,)):
+            raise ValueError(f"lse, entropy and their gradients must be float32 [{R}]")
+    words = _check_mask(mask, R, V)
+    _check_with(dev, tokens, mask, lse, entropy, grad_logprobs, grad_entropy, grad_lse)
+    if _elsewhere(stream, dev):
+        return _there(token_scores_grad, stream, dev, logits, tokens, lse, entropy, grad_logprobs,
+                      grad_entropy, grad_lse, temperature, mask, ignore_index, out)
+    d = _logits_out(out, logits)
+    N.check(N.lib().strim_token_scores_grad(
+        _stream_of(dev), _ptr(logits), code, R, V, _row_stride(logits), temperature, _ptr(mask), words,
+        _ptr(tokens), S, ignore_index, _ptr(lse), _ptr(entropy), _ptr(grad_logprobs), _ptr(grad_entropy),
+        _ptr(grad_lse), _ptr(d), _row_stride(d)), "strim_token_scores_grad")
+    return d
+
+
+def _distill_args(logits, ids, logprobs, temperature):
+    """Checks of the distillation calls; (dtype code, N, V, M)."""
+    code = _check_logits(logits, temperature)
+    R, V = logits.shape
+    for t, dt, name in ((ids, torch.int32, "ids"), (logprobs, torch.float32, "logprobs")):
+        if t.dtype != dt or t.dim() != 2 or t.shape[0] != R or t.shape != ids.shape:
+            raise ValueError(f"{name} must be {dt} [{R}, M], got {t.dtype} {tuple(t.shape)}")
+    M = ids.shape[1]
+    if not 0 < M <= N.SCORE_MAX_LIST:
+        raise ValueError(f"a row has 1 to {N.SCORE_MAX_LIST} alternatives, got {M}")
+    _check_with(logits.device, ids, logprobs)
+    return code, R, V, M
+
+
+@lru_cache(maxsize=256)
+def distill_workspace(rows: int, V: int, M: int, step: bool = False) -> int:
+    """Bytes of workspace that distill (or distill_step) takes."""
+    need = N.lib().strim_distill_workspace(rows, V, M, int(step))
+    if need < 0:
+        raise N.StrimError(need, "strim_distill_workspace")
+    return need
+
+
+def distill(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, temperature: float = 1.0,
+            tail: bool = False, workspace: torch.Tensor | None = None, stream=None):
+    """Divergence of softmax(logits / temperature) from a teacher's alternatives: ids int32 and
+    logprobs float32 [N, M] as token_scores gives them (at the same temperature), a negative id or a
+    log-probability of -inf being padding. tail: the teacher's remaining mass is one more alternative,
+    against the student's mass outside the ids; else the alternatives are renormalised. Returns (loss
+    [N], lse [N], log_rest [N], status [N]); a row without alternatives has loss 0, one with an id of V
+    or more 0 and EINVAL. strim_amd.loss has the differentiable form."""
+    code, R, V, M = _distill_args(logits, ids, logprobs, temperature)
+    dev = logits.device
+    if _elsewhere(stream, dev):
+        return _there(distill, stream, dev, logits, ids, logprobs, temperature, tail, workspace)
+    loss = torch.empty(R, dtype=torch.float32, device=dev)
+    lse = torch.empty(R, dtype=torch.float32, device=dev)
+    rest = torch.empty(R, dtype=torch.float32, device=dev)
+    status = torch.empty(R, dtype=torch.int32, device=dev)
+    ws = _workspace(workspace, distill_workspace(R, V, M), dev)
+    N.check(N.lib().strim_distill(_stream_of(dev), _ptr(logits), code, R, V, _row_stride(logits),
+                                  temperature, _ptr(ids), _ptr(logprobs), M, int(tail), _ptr(ws),
+                                  _bytes(ws), _ptr(loss), _ptr(lse), _ptr(rest), _ptr(status)),
+            "strim_distill")
+    return loss, lse, rest, status
+
+
+def distill_grad(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor, lse: torch.Tensor,
+                 log_rest: torch.Tensor, grad_loss: torch.Tensor, temperature: float = 1.0,
+                 tail: bool = False, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """The logits' gradient [N, V] (of their type) from lse and log_rest as distill gave them and the
+    float32 [N] gradient of its loss. out: where it goes, the logits themselves included."""
+    code, R, V, M = _distill_args(logits, ids, logprobs, temperature)
+    dev = logits.device
+    for t in (lse, log_rest, grad_loss):
+        if t.dtype != torch.float32 or t.shape != (R,):
+            raise ValueError(f"lse, log_rest and grad_loss must be float32 [{R}]")
+    _check_with(dev, lse, log_rest, grad_loss)
+    if _elsewhere(stream, dev):
+        return _there(distill_grad, stream, dev, logits, ids, logprobs, lse, log_rest, grad_loss,
+                      temperature, tail, out)
+    d = _logits_out(out, logits)
+    N.check(N.lib().strim_distill_grad(_stream_of(dev), _ptr(logits), code, R, V, _row_stride(logits),
+                                       temperature, _ptr(ids), _ptr(logprobs), M, int(tail), _ptr(lse),
+                                       _ptr(log_rest), _ptr(grad_loss), _ptr(d), _row_stride(d)),
+            "strim_distill_grad")
+    return d
+
+
+def distill_step(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                 weights: torch.Tensor, temperature: float = 1.0, tail: bool = False,
+                 out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
+    """distill and distill_grad in one call, for rows whose weights float32 [N] are known beforehand
+    (a mean's 1 / count): (loss [N], d_logits [N, V], status [N]). The logits are read once."""
+    code, R, V, M = _distill_args(logits, ids, logprobs, temperature)
+    dev = logits.device
+    if weights.dtype != torch.float32 or weights.shape != (R,):
+        raise ValueError(f"weights must be float32 [{R}]")
+    _check_with(dev, weights)
+    if _elsewhere(stream, dev):
+        return _there(distill_step, stream, dev, logits, ids, logprobs, weights, temperature, tail, out,
+                      workspace)
+    loss = torch.empty(R, dtype=torch.float32, device=dev)
+    status = torch.empty(R, dtype=torch.int32, device=dev)
+    d = _logits_out(out, logits)
+    ws = _workspace(workspace, distill_workspace(R, V, M, True), dev)
+    N.check(N.lib().strim_distill_step(_stream_of(dev), _ptr(logits), code, R, V, _row_stride(logits),
+                                       temperature, _ptr(ids), _ptr(logprobs), M, int(tail),
+                                       _ptr(weights), _ptr(ws), _bytes(ws), _ptr(loss), _ptr(d),
+                                       _row_stride(d), _ptr(status)), "strim_distill_step")
+    return loss, d, status
+
+
+def distill_scale(data: torch.Tensor, factor: torch.Tensor, stream=None) -> torch.Tensor:
+    """data *= factor (one float32 on the device), in place; nothing is written where it is 1."""
+    code = _dtype_code(data)
+    if factor.dtype != torch.float32 or factor.numel() != 1:
+        raise ValueError("factor must be one float32 number")
+    if not data.is_cuda:
+        raise ValueError("every tensor argument must be on the GPU")
+    _check_with(data.device, data, factor)
+    if _elsewhere(stream, data.device):
+        return _there(distill_scale, stream, data.device, data, factor)
+    N.check(N.lib().strim_distill_scale(_stream_of(data.device), _ptr(data), code, data.numel(),
+                                        _ptr(factor)), "strim_distill_scale")
+    return data
+
+
+def _norm_args(x, weight, bias):
+    """Checks of the norm calls; (dtype code, weight dtype code, N, K)."""
+    code = _dtype_code(x)
+    if not x.is_cuda:
+        raise ValueError("every tensor argument must be on the GPU")
+    _check_norm_rows("x", x)
+    R, K = x.shape
+    if R > N.NORM_MAX_ROWS or not 0 < K <= N.NORM_MAX_WIDTH:
+        raise ValueError(f"x must be at most [{N.NORM_MAX_ROWS}, {N.NORM_MAX_WIDTH}], got [{R}, {K}]")
+    wcode = N.DTYPE_F32
+    for t in (weight, bias):
+        if t is None:
+            continue
+        wcode = _dtype_code(t)
+        if t.shape != (K,):
+            raise ValueError(f"weight and bias must be [{K}], got {tuple(t.shape)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must be of one type")
+    _check_with(x.device, weight, bias)
+    return code, wcode, R, K
+
+
+def _check_norm_rows(name: str, t: torch.Tensor) -> None:
+    if t.dim() != 2 or (not t.is_contiguous() and
+                        (t.stride(1) != 1 or _row_stride(t) < t.shape[1])):
+        raise ValueError(f"{name} must be [N, K] with contiguous rows (row stride >= K)")
+
+
+def norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+         eps: float = 1e-6, center: bool = False, stream=None):
+    """Rows of x (bf16 or float32 [N, K]) over their root mean square, or (center) less their mean over
+    their standard deviation, times weight plus bias ([K], both of one type or None). Returns (y of x's
+    type, rstd float32 [N], mean float32 [N] or None without center). strim_amd.norm has the
+    differentiable forms."""
+    code, wcode, R, K = _norm_args(x, weight, bias)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    dev = x.device
+    if _elsewhere(stream, dev):
+        return _there(norm, stream, dev, x, weight, bias, eps, center)
+    y = torch.empty(R, K, dtype=x.dtype, device=dev)
+    rstd = torch.empty(R, dtype=torch.float32, device=dev)
+    mean = torch.empty(R, dtype=torch.float32, device=dev) if center else None
+    N.check(N.lib().strim_norm(_stream_of(dev), _ptr(x), code, R, K, _row_stride(x), _ptr(weight),
+                               _ptr(bias), wcode, eps, int(center), _ptr(y), K, _ptr(rstd), _ptr(mean)),
+            "strim_norm")
+    return y, rstd, mean
+
+
+@lru_cache(maxsize=256)
+def norm_workspace(rows: int, K: int, want_weight: bool = False, want_bias: bool = False) -> int:
+    """Bytes of workspace that norm_grad takes."""
+    need = N.lib().strim_norm_workspace(rows, K, int(want_weight), int(want_bias))
+    if need < 0:
+        raise N.StrimError(need, "strim_norm_workspace")
+    return need
+
+
+def norm_grad(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None,
+              grad_y: torch.Tensor, rstd: torch.Tensor, mean: torch.Tensor | None = None,
+              want_x: bool = True, want_weight: bool = True, want_bias: bool = True,
+              workspace: torch.Tensor | None = None, stream=None):
+    """Gradients of norm: (d_x of x's type or None, d_weight, d_bias of their types, or None where there
+    is no weight, no bias, or none wanted) from rstd and mean as norm gave them and grad_y of x's type
+    and shape."""
+    code, wcode, R, K = _norm_args(x, weight, bias)
+    dev = x.device
+    if grad_y.dtype != x.dtype or grad_y.shape != x.shape or grad_y.device != dev:
+        raise ValueError("grad_y must be as x is")
+    _check_norm_rows("grad_y", grad_y)
+    for t in (rstd, mean):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (R,)):
+            raise ValueError(f"rstd and mean must be float32 [{R}]")
+    _check_with(dev, rstd, mean)
+    want_weight, want_bias = want_weight and weight is not None, want_bias and bias is not None
+    if not (want_x or want_weight or want_bias):
+        return None, None, None
+    if _elsewhere(stream, dev):
+        return _there(norm_grad, stream, dev, x, weight, bias, grad_y, rstd, mean, want_x, want_weight,
+                      want_bias, workspace)
+    dx = torch.empty(R, K, dtype=x.dtype, device=dev) if want_x else None
+    dw = torch.empty(K, dtype=weight.dtype, device=dev) if want_weight else None
+    db = torch.empty(K, dtype=bias.dtype, device=dev) if want_bias else None
+    ws = _workspace(workspace, norm_workspace(R, K, want_weight, want_bias), dev)
+    N.check(N.lib().strim_norm_grad(_stream_of(dev), _ptr(x), code, R, K, _row_stride(x), _ptr(grad_y),
+                                    _row_stride(grad_y), _ptr(weight), wcode, _ptr(rstd), _ptr(mean),
+                                    _ptr(ws), _bytes(ws), _ptr(dx), K, _ptr(dw), _ptr(db)),
+            "strim_norm_grad")
+    return dx, dw, db
 
 
 def draft_argmax(draft_logits: torch.Tensor, draft_to_full: torch.Tensor | None = None,
