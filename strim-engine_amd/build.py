@@ -44,6 +44,7 @@ UNITS = [
     ("loss_kernels.hip", []),
     ("q4_kernels.hip", []),
     ("score_kernels.hip", []),
+    ("distill_kernels.hip", []),
     ("norm_kernels.hip", []),
     ("grammar_kernels.hip", []),
     ("capi.hip", []),

@@ -1,0 +1,139 @@
+// rows.hpp — rows of logits as the scores and the distillation read and write them: eight tokens a
+// lane, any alignment; and their softmax statistics.
+#pragma once
+
+#include "common.hpp"
+
+namespace strim {
+
+typedef uint32_t ru32x4 __attribute__((ext_vector_type(4)));
+// (gfx950 takes 16-byte accesses at any address: rows of odd strides need no path of their own)
+typedef ru32x4 ru32x4_any __attribute__((aligned(2)));
+typedef float rf32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 rbf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr uint32_t NINF_BITS = 0xFF800000u;
+
+__device__ __forceinline__ float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float fma_f(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+
+// Eight tokens of a row as they lie in memory.
+template <int DT>
+struct RowVec {
+  static constexpr int WORDS = DT == STRIM_DTYPE_BF16 ? 4 : 8;
+  static constexpr int SIZE = DT == STRIM_DTYPE_BF16 ? 2 : 4;
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (DT == STRIM_DTYPE_BF16)
+      return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
+    else
+      return __uint_as_float(w[j]);
+  }
+  // tokens v .. v + 7, all inside the row
+  __device__ __forceinline__ void load(const char* row, int v) {
+    const char* p = row + (int64_t)v * SIZE;
+#pragma unroll
+    for (int i = 0; i < WORDS / 4; ++i) {
+      const ru32x4 q = ((const ru32x4_any*)p)[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
+    }
+  }
+  // tokens from v on that lie before V; -inf past them
+  __device__ __forceinline__ void load_to(const char* row, int v, int V) {
+    if (v + 8 <= V) return load(row, v);
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = DT == STRIM_DTYPE_BF16 ? 0xFF80FF80u : NINF_BITS;
+    const char* p = row + (int64_t)v * SIZE;
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+      if (v + j < V) {
+        if constexpr (DT == STRIM_DTYPE_BF16) {
+          const uint32_t h = ((const uint16_t*)p)[j];
+          w[j >> 1] = j & 1 ? (w[j >> 1] & 0xFFFFu) | h << 16 : (w[j >> 1] & 0xFFFF0000u) | h;
+        } else {
+          w[j] = ((const uint32_t*)p)[j];
+        }
+      }
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    if constexpr (DT == STRIM_DTYPE_BF16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rf32x2{f[2 * i], f[2 * i + 1]}, rbf16x2));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
+    }
+  }
+  __device__ __forceinline__ void store_to(char* row, int v, int V) const {
+    char* p = row + (int64_t)v * SIZE;
+    if (v + 8 <= V) {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i)
+        ((ru32x4_any*)p)[i] = ru32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 7; ++j)
+      if (v + j < V) {
+        if constexpr (DT == STRIM_DTYPE_BF16) ((uint16_t*)p)[j] = (uint16_t)(w[j >> 1] >> (j & 1 ? 16 : 0));
+        else ((uint32_t*)p)[j] = w[j];
+      }
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ float token_at(const char* row, int v) {
+  return DT == STRIM_DTYPE_BF16 ? bf16_to_f32(((const uint16_t*)row)[v]) : ((const float*)row)[v];
+}
+
+__device__ __forceinline__ float op_add_f(float a, float b) { return a + b; }
+__device__ __forceinline__ float wave_sum_f(float v) {
+  STRIM_WAVE_REDUCE(float, v, dpp_f, rl_f, op_add_f);
+  return v;
+}
+
+// Over some of a row's tokens: m the largest x, s = sum exp((x - m) / T), u = sum (x - m) exp((x - m) / T).
+// Without a token above -inf m is -inf, s = u = 0; a NaN or +inf makes s NaN. c = log2(e) / T throughout.
+struct RowStat {
+  float m, s, u;
+};
+__device__ __forceinline__ float stat_ref(float m) { return m == -INFINITY ? 0.0f : m; }
+// a's sums relative to `top` >= a.m. (The difference is bounded: the type's lowest value lies 3.4e38
+// below zero, and u times a vanishing factor would be an infinity times 0.)
+__device__ __forceinline__ void stat_rebase(RowStat& a, float top, float c) {
+  const float d = a.m - stat_ref(top), f = hw_exp2(d * c), near = fmaxf(d, -1e30f);
+  a.u = a.s == 0.0f ? 0.0f : fma_f(near, a.s, a.u) * f;
+  a.s = a.s == 0.0f ? 0.0f : a.s * f;
+  a.m = top;
+}
+__device__ __forceinline__ void stat_merge(RowStat& a, RowStat b, float c) {
+  const float top = fmaxf(a.m, b.m);
+  stat_rebase(a, top, c);
+  stat_rebase(b, top, c);
+  a.s += b.s;
+  a.u += b.u;
+}
+// A lane's next E tokens; `mx` is their maximum.
+template <int E, bool U>
+__device__ __forceinline__ void stat_add(RowStat& a, const float (&x)[E], float mx, float c) {
+  if (mx > a.m) stat_rebase(a, mx, c);
+  const float ref = stat_ref(a.m);
+#pragma unroll
+  for (int j = 0; j < E; ++j) {
+    const float d = x[j] - ref, e = hw_exp2(d * c);  // (a NaN goes through to s)
+    a.s += e;
+    if (U) a.u = fma_f(fmaxf(d, -1e30f), e, a.u);
+  }
+}
+// The wave's statistics in every lane.
+__device__ __forceinline__ void stat_wave(RowStat& a, float c) {
+  stat_rebase(a, wave_max_f(a.m), c);
+  a.s = wave_sum_f(a.s);
+  a.u = wave_sum_f(a.u);
+}
+
+}  // namespace strim

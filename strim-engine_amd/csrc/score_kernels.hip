@@ -1,311 +1,347 @@
-// score_kernels.hip — what a row of logits says about its tokens, and the gradients that go back
-// into it.
+// score_kernels.hip — what a row of logits says about its tokens, and the gradient that goes back into it.
 //
 //   z[v] = x[v] / T on allowed ids, -inf elsewhere;  lse = log sum_v exp(z[v])
-// Token scores: logprob[t] = z[t] - lse, the entropy -sum p log p with p = exp(z - lse), the largest
-// x in token order; gradient
-//   dx[v] = 1/T (sum_s g[s] ([v = t_s] - p[v]) - gH p[v] (log p[v] + H) + gL p[v]).
-// Distillation from a teacher's alternatives (id_m, log-probability t_m): p_m = softmax of t_m over the
-// alternatives, or exp(t_m) with the remaining mass r as one bucket;
-//   loss = sum_m p_m (log p_m - log q[id_m]) + r (log r - log q_rest),  q = softmax(z)
-//   dx[v] = w/T (q[v] (sum p + r - [v no alternative] r / q_rest) - sum of p_m with id_m = v).
+//   logprob[t] = z[t] - lse,  H = -sum_v p log p with p = exp(z - lse),  the first `top` ids in token order
+//   dx[v] = 1/T (sum_s g[s] ([v = t_s] - p[v]) - gH p[v] (log p[v] + H) + gL p[v])
+//
+// k_scores reads the logits once: per lane the running maximum m, s = sum exp((x - m) / T) and u = sum
+// (x - m) exp((x - m) / T), from which lse = m / T + log s and H = log s - u / (s T), and the row's
+// alternatives (top.hpp). A row is one workgroup's where there are many, else in parts that
+// k_scores_join merges.
+#include <type_traits>
+
 #include "kernels.hpp"
+#include "rows.hpp"
 #include "score.hpp"
+#include "top.hpp"
 
 namespace strim {
 
 namespace {
 
-constexpr int SC_T = 256;  // threads of a row's workgroup
+constexpr int SC_T = TOP_T;                    // threads of a workgroup
+constexpr int SC_U = TOP_STEP * 2 / (8 * SC_T);  // vectors of eight tokens a lane has of a tile
+constexpr int SC_TILE = 8 * SC_U * SC_T;       // tokens a tile
 
-template <int DT>
-__device__ __forceinline__ float row_at(const void* row, int64_t v) {
-  return DT == STRIM_DTYPE_BF16 ? bf16_to_f32(((const uint16_t*)row)[v]) : ((const float*)row)[v];
+// What a part of a row leaves for the join: its statistics and up to ScoreParts::room keys.
+struct ScorePart {
+  RowStat st;
+  int32_t n;
+};
+struct ScoreParts {
+  int32_t parts, tiles;  // parts of a row; tiles of a part
+  int32_t room;
+  ScorePart* part;       // [R][parts]
+  uint64_t* keys;        // [R][parts][room]
+};
+
+__device__ __forceinline__ uint32_t allowed8(const uint32_t* mask, int v, int V) {
+  return !mask ? 0xFFu : v < V ? ((const uint8_t*)mask)[v >> 3] : 0u;
 }
-template <int DT>
-__device__ __forceinline__ const void* row_of(const void* x, int64_t r, int64_t stride) {
-  return (const char*)x + r * stride * (DT == STRIM_DTYPE_BF16 ? 2 : 4);
-}
-template <int DT>
-__device__ __forceinline__ void row_set(void* row, int64_t v, float f) {
-  if (DT == STRIM_DTYPE_BF16) ((uint16_t*)row)[v] = __builtin_bit_cast(uint16_t, (__bf16)f);
-  else ((float*)row)[v] = f;
-}
-__device__ __forceinline__ bool allowed_at(const uint32_t* mask, int64_t v) {
+__device__ __forceinline__ bool allowed_at(const uint32_t* mask, int v) {
   return !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
 }
 
-// Block reductions; every thread gets the result. `op` merges b into a, in a fixed order.
-template <class T, class Op>
-__device__ __forceinline__ T block_all(T v, T* scratch, Op op) {
-  const int t = threadIdx.x;
-  __syncthreads();
-  scratch[t] = v;
-  for (int d = SC_T / 2; d > 0; d >>= 1) {
-    __syncthreads();
-    if (t < d) scratch[t] = op(scratch[t], scratch[t + d]);
-  }
-  __syncthreads();
-  return scratch[0];
-}
-
-// max, sum exp((x - max) / T), sum (x - max) exp((x - max) / T); a max of -inf carries no sums (but
-// keeps a NaN)
-struct Stat {
-  float m, s, u;
-};
-__device__ __forceinline__ Stat stat_merge(Stat a, Stat b, float c) {
-  const float top = fmaxf(a.m, b.m);
-  if (top == -INFINITY) return Stat{top, a.s + b.s, 0.0f};
-  // (a difference that is the lowest value's would make u infinite, and that times 0)
-  const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - top, -1e30f);
-  const float db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - top, -1e30f);
-  const float fa = __builtin_amdgcn_exp2f(da * c), fb = __builtin_amdgcn_exp2f(db * c);
-  return Stat{top, a.s * fa + b.s * fb, (a.u + da * a.s) * fa + (b.u + db * b.s) * fb};
-}
-__device__ __forceinline__ void stat_add(Stat& a, float x, float c) {
-  a = stat_merge(a, Stat{x, x == -INFINITY ? 0.0f : 1.0f + 0.0f * x, 0.0f}, c);
-}
-
+// The row's results from its statistics and the list that holds its first `top` keys.
 template <int DT>
-__global__ __launch_bounds__(SC_T) void k_scores(ScoreArgs a) {
-  __shared__ Stat s_stat[SC_T];
-  __shared__ uint64_t s_key[SC_T];
-  const int64_t r = blockIdx.x;
-  const void* row = row_of<DT>(a.logits, r, a.stride);
+__device__ __forceinline__ void score_finish(const ScoreArgs& a, int64_t r, RowStat st, TopList* l, int n) {
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
   const uint32_t* mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
-  const float c = 1.44269504088896340736f / a.T;
-  Stat st{-INFINITY, 0.0f, 0.0f};
-  for (int v = threadIdx.x; v < a.V; v += SC_T)
-    if (allowed_at(mask, v)) {
-      const float x = row_at<DT>(row, v);
-      stat_add(st, x, c);
-    }
-  st = block_all(st, s_stat, [&](Stat p, Stat q) { return stat_merge(p, q, c); });
+  const float nan = __builtin_nanf("");
   const bool bad = !(st.s < INFINITY), empty = !bad && st.s == 0.0f;
-  const float ls = logf(st.s), nan = __builtin_nanf("");
-  bool known = true;
+  const float ls = logf(st.s);
+  // (not from lse, which is rounded to the largest logit's spacing)
+  auto logprob = [&](float x) { return (x - st.m) / a.T - ls; };
+  bool unknown = false;
   for (int s = threadIdx.x; s < a.S; s += SC_T) {
     const int t = a.tokens[r * a.S + s];
+    const bool given = t != a.ignore_index, inside = t >= 0 && t < a.V;
+    unknown |= given && !inside;
     float lp = 0.0f;
-    if (t != a.ignore_index && t >= 0 && t < a.V) {
-      lp = bad ? nan : empty || !allowed_at(mask, t) ? -INFINITY : (row_at<DT>(row, t) - st.m) / a.T - ls;
-    } else if (t != a.ignore_index) known = false;
+    if (given && inside)
+      lp = bad ? nan : empty || !allowed_at(mask, t) ? -INFINITY : logprob(token_at<DT>(row, t));
     a.logprobs[r * a.S + s] = lp;
   }
-  known = !block_all((uint64_t)!known, s_key, [](uint64_t p, uint64_t q) { return p | q; });
+  unknown = __syncthreads_or(unknown);
   if (threadIdx.x == 0) {
     a.entropy[r] = bad ? nan : empty ? 0.0f : ls - st.u / st.s / a.T;
     a.lse[r] = bad ? nan : empty ? -INFINITY : st.m / a.T + ls;
     if (a.status)
-      a.status[r] = bad ? STRIM_ENONFINITE : empty ? STRIM_EEMPTY : known ? STRIM_OK : STRIM_EINVAL;
+      a.status[r] = bad ? STRIM_ENONFINITE : empty ? STRIM_EEMPTY : unknown ? STRIM_EINVAL : STRIM_OK;
   }
-  // the alternatives one after the other: the least key past the last one's
-  uint64_t last = 0;
-  for (int k = 0; k < a.top; ++k) {
-    uint64_t best = ~0ull;
-    if (!bad)
-      for (int v = threadIdx.x; v < a.V; v += SC_T) {
-        const float x = row_at<DT>(row, v);
-        if (x > -INFINITY && allowed_at(mask, v)) {
-          const uint64_t key = ckey(x, v);
-          if ((k == 0 || key > last) && key < best) best = key;
-        }
+  if (!l) return;
+  int32_t* ids = a.top_ids + r * a.top;
+  float* lps = a.top_logprobs + r * a.top;
+  if (bad) n = 0;
+  for (int k = n + (int)threadIdx.x; k < a.top; k += SC_T) {
+    ids[k] = -1;
+    lps[k] = bad ? nan : -INFINITY;
+  }
+  top_order(*l, n, a.top, [&](int k, uint64_t key) {
+    ids[k] = (int32_t)(uint32_t)key;
+    lps[k] = logprob(fkey_desc_inv((uint32_t)(key >> 32)));
+  });
+}
+
+// The workgroup's statistics in every thread.
+__device__ __forceinline__ RowStat stat_block(RowStat st, float c, RowStat* scratch) {
+  stat_wave(st, c);
+  if ((threadIdx.x & (WAVE - 1)) == 0) scratch[threadIdx.x / WAVE] = st;
+  __syncthreads();
+  st = scratch[0];
+#pragma unroll
+  for (int i = 1; i < SC_T / WAVE; ++i) stat_merge(st, scratch[i], c);
+  return st;
+}
+
+template <int DT, bool MASK, bool TOP>
+__global__ __launch_bounds__(SC_T) void k_scores(const ScoreArgs a, const ScoreParts q) {
+  __shared__ RowStat s_stat[SC_T / WAVE];
+  __shared__ std::conditional_t<TOP, TopList, char> s_list;
+  TopList* const s_top = (TopList*)&s_list;  // (unused without TOP)
+  const int64_t r = blockIdx.x / q.parts;
+  const int p = blockIdx.x - (int)r * q.parts;
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  const uint32_t* mask = MASK ? a.mask + r * a.mask_stride : nullptr;
+  const float c = LOG2E / a.T;
+  const int t0 = p * q.tiles * SC_TILE, t1 = min(a.V, t0 + q.tiles * SC_TILE);
+  RowVec<DT> next[SC_U];
+  uint32_t ok[SC_U];
+  auto request = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < SC_U; ++u) {
+      const int v = t + 8 * (u * SC_T + (int)threadIdx.x);
+      if (t + SC_TILE <= a.V) next[u].load(row, v);
+      else next[u].load_to(row, v, a.V);
+      if (MASK) ok[u] = allowed8(mask, v, a.V);
+    }
+  };
+  request(t0);
+  TopRun top;
+  if constexpr (TOP) top.init(s_top[0], a.top);
+  RowStat st{-INFINITY, 0.0f, 0.0f};
+  for (int t = t0; t < t1; t += SC_TILE) {
+    float x[8 * SC_U], mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < SC_U; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float f = next[u].at(j);
+        if (MASK) f = (ok[u] >> j) & 1u ? f : -INFINITY;
+        x[8 * u + j] = f;
+        mx = fmaxf(mx, f);
       }
-    best = block_all(best, s_key, [](uint64_t p, uint64_t q) { return p < q ? p : q; });
-    last = best;
-    if (threadIdx.x == 0) {
-      const bool none = best == ~0ull;
-      a.top_ids[r * a.top + k] = none ? -1 : (int32_t)(uint32_t)best;
-      a.top_logprobs[r * a.top + k] =
-          bad ? nan : none ? -INFINITY : (fkey_desc_inv((uint32_t)(best >> 32)) - st.m) / a.T - ls;
+    if (t + SC_TILE < t1) request(t + SC_TILE);
+    stat_add<8 * SC_U, true>(st, x, mx, c);
+    if constexpr (TOP) top.add<SC_U>(s_top[0], x, mx, st.m, t + 8 * (int)threadIdx.x);
+  }
+  const float most = st.m;
+  st = stat_block(st, c, s_stat);
+  if constexpr (TOP) {
+    top.trim(s_top[0], most);
+    if (q.parts > 1) {
+      uint32_t unused = 0;
+      if (top.held > q.room) top.held = top_reduce(s_top[0], top.held, a.top, unused);
+      uint64_t* out = q.keys + (r * q.parts + p) * q.room;
+      for (int i = threadIdx.x; i < top.held; i += SC_T) out[i] = s_top[0].key[i];
     }
-    if (best == ~0ull) last = ~0ull;
+  }
+  if (q.parts > 1) {
+    if (threadIdx.x == 0) q.part[r * q.parts + p] = ScorePart{st, TOP ? top.held : 0};
+  } else {
+    score_finish<DT>(a, r, st, TOP ? s_top : nullptr, TOP ? top.held : 0);
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(SC_T) void k_scores_grad(ScoreGradArgs a) {
+template <int DT, bool TOP>
+__global__ __launch_bounds__(SC_T) void k_scores_join(const ScoreArgs a, const ScoreParts q) {
+  __shared__ RowStat s_stat[SC_T / WAVE];
+  __shared__ std::conditional_t<TOP, TopList, char> s_list;
+  TopList* const s_top = (TopList*)&s_list;  // (unused without TOP)
+  __shared__ int s_n[TOP ? SC_T : 1];
   const int64_t r = blockIdx.x;
-  const void* row = row_of<DT>(a.logits, r, a.stride);
-  void* out = (void*)row_of<DT>(a.d_logits, r, a.d_stride);
-  const uint32_t* mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
-  const float lse = a.lse[r];
-  const float gh = a.grad_entropy ? a.grad_entropy[r] : 0.0f, H = a.grad_entropy ? a.entropy[r] : 0.0f;
-  float g = a.grad_lse ? -a.grad_lse[r] : 0.0f;
-  for (int s = 0; s < a.S; ++s) {
-    const int t = a.tokens[r * a.S + s];
-    if (t != a.ignore_index && t >= 0 && t < a.V) g += a.grad_logprobs[r * a.S + s];
+  const float c = LOG2E / a.T;
+  RowStat st{-INFINITY, 0.0f, 0.0f};
+  if constexpr (TOP) s_n[threadIdx.x] = 0;
+  if ((int)threadIdx.x < q.parts) {
+    const ScorePart o = q.part[r * q.parts + threadIdx.x];
+    st = o.st;
+    if constexpr (TOP) s_n[threadIdx.x] = o.n;
   }
-  for (int v = threadIdx.x; v < a.V; v += SC_T) {
-    float d = 0.0f;
-    if (lse != -INFINITY && allowed_at(mask, v)) {
-      const float z = fmaxf(row_at<DT>(row, v) / a.T - lse, -1e30f), x = row_at<DT>(row, v);
-      const float p = x == x ? expf(z) : x;
-      d = -p * (g + gh * (z + H));
-      for (int s = 0; s < a.S; ++s)
-        if (a.tokens[r * a.S + s] == v && v != a.ignore_index) d += a.grad_logprobs[r * a.S + s];
-      if (lse != lse) d = lse;
+  st = stat_block(st, c, s_stat);
+  int n = 0;
+  if constexpr (TOP) {
+    const uint64_t* keys = q.keys + r * q.parts * q.room;
+    const int all = q.parts * q.room;
+    auto key_at = [&](int i) {
+      const int p = i / q.room;
+      return i < all && i - p * q.room < s_n[p] ? keys[i] : ~0ull;
+    };
+    uint64_t best = ~0ull;
+    for (int i = threadIdx.x; i < all; i += SC_T) best = min(best, key_at(i));
+    const uint32_t t = top_threshold(s_top[0], (uint32_t)(best >> 32), a.top);
+    uint64_t limit = (uint64_t)t << 32 | 0xFFFFFFFFu;
+    if (threadIdx.x == 0) s_top[0].n = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < all; i0 += TOP_STEP) {
+      if (n > TOP_T) {  // (lists full of ties)
+        uint32_t unused = 0;
+        n = top_reduce(s_top[0], n, a.top, unused);
+        if (threadIdx.x == 0) s_top[0].n = n;
+        __syncthreads();
+      }
+      for (int i = i0 + (int)threadIdx.x; i < min(all, i0 + TOP_STEP); i += SC_T) {
+        const uint64_t k = key_at(i);
+        if (k <= limit) s_top[0].key[atomicAdd(&s_top[0].n, 1)] = k;
+      }
+      __syncthreads();
+      n = __builtin_amdgcn_readfirstlane(s_top[0].n);
+      __syncthreads();
     }
-    row_set<DT>(out, v, d / a.T);
+  }
+  score_finish<DT>(a, r, st, TOP ? s_top : nullptr, n);
+}
+
+// The gradient: G = sum of the tokens' gradients, then d = p (gL - G - gH (log p + H)) / T everywhere and
+// g / T more at the tokens. A wave finds its 512 tokens' given ones by one ballot of the list, which its
+// lanes hold (two entries each), and hands each to the lane and element that it belongs to.
+constexpr int SG_TILES = 4;  // tiles of eight tokens a thread that a workgroup takes
+
+template <int DT, bool MASK, bool ENT>
+__global__ __launch_bounds__(SC_T) void k_scores_grad(const ScoreGradArgs a, int parts) {
+  const int64_t r = blockIdx.x / parts;
+  const int p = blockIdx.x - (int)r * parts, lane = threadIdx.x & (WAVE - 1);
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  char* out = (char*)a.d_logits + r * a.d_stride * RowVec<DT>::SIZE;
+  const uint32_t* mask = MASK ? a.mask + r * a.mask_stride : nullptr;
+  const int t0 = p * SG_TILES * 8 * SC_T;
+  RowVec<DT> x[SG_TILES];
+  uint32_t ok[SG_TILES];
+#pragma unroll
+  for (int u = 0; u < SG_TILES; ++u) {
+    const int v = t0 + 8 * (u * SC_T + (int)threadIdx.x);
+    if (v < a.V) x[u].load_to(row, v, a.V);
+    if (MASK) ok[u] = allowed8(mask, v, a.V);
+  }
+  const float lse = a.lse[r], c = LOG2E / a.T, inv = 1.0f / a.T;
+  const float gh = ENT ? a.grad_entropy[r] : 0.0f, H = ENT ? a.entropy[r] : 0.0f;
+  int id[2];
+  float g[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int s = lane + i * WAVE;
+    id[i] = s < a.S ? a.tokens[r * a.S + s] : -1;
+    if (id[i] == a.ignore_index || id[i] >= a.V) id[i] = -1;
+    g[i] = id[i] >= 0 ? a.grad_logprobs[r * a.S + s] * inv : 0.0f;
+  }
+  const float G = wave_sum_f(g[0] + g[1]), top = (a.grad_lse ? a.grad_lse[r] * inv : 0.0f) - G;
+  const bool empty = lse == -INFINITY;
+  const float ref = lse * a.T;
+#pragma unroll
+  for (int u = 0; u < SG_TILES; ++u) {
+    const int w0 = __builtin_amdgcn_readfirstlane(t0 + 8 * (u * SC_T + (int)threadIdx.x - lane));
+    if (w0 >= a.V) break;
+    const int v = w0 + 8 * lane;
+    float d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = x[u].at(j) - ref, p = hw_exp2(y * c);
+      d[j] = ENT ? p * (top - gh * inv * (fmaxf(y * inv, -200.0f) + H)) : p * top;
+    }
+    // the given tokens among these 512, in the list's order
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint64_t hit = __ballot(id[i] >= 0 && (uint32_t)(id[i] - w0) < 8u * WAVE);
+      while (hit) {
+        const int l = __builtin_ctzll(hit);
+        hit &= hit - 1;
+        const int off = rl_i(id[i], l) - w0;
+        const float more = rl_f(g[i], l);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) d[j] += lane == off >> 3 && j == (off & 7) ? more : 0.0f;
+      }
+    }
+    if (MASK)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = (ok[u] >> j) & 1u ? d[j] : 0.0f;
+    RowVec<DT> y;
+    y.set(d);
+    if (empty)
+#pragma unroll
+      for (int i = 0; i < RowVec<DT>::WORDS; ++i) y.w[i] = 0;
+    if (v < a.V) y.store_to(out, v, a.V);
   }
 }
 
-// A distillation row's numbers: from the statistics of its tokens (`tail`: of those that are no
-// alternative) and its alternatives.
-struct DistillRow {
-  double lse, log_rest, loss, mass, r;
-  bool has, bad;
-};
+int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
+int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-template <int DT>
-__device__ DistillRow distill_row(const DistillArgs& a, int64_t r, const void* row, bool given) {
-  const int32_t* ids = a.ids + r * a.M;
-  const float* lps = a.logprobs + r * a.M;
-  DistillRow o{0.0, 0.0, 0.0, 0.0, 0.0, false, false};
-  double tmax = -INFINITY;
-  for (int m = 0; m < a.M; ++m) {
-    if (ids[m] >= a.V) o.bad = true;
-    if (ids[m] >= 0 && !(lps[m] == -INFINITY)) {
-      o.has = true;
-      tmax = fmax(tmax, (double)lps[m]);
-    }
-  }
-  if (o.bad || !o.has) {
-    o.has = false;
-    return o;
-  }
-  if (a.tail) tmax = 0.0;
-  double sum = 0.0;
-  for (int m = 0; m < a.M; ++m)
-    if (ids[m] >= 0 && !(lps[m] == -INFINITY)) sum += exp((double)lps[m] - tmax);
-  o.mass = a.tail ? sum : 1.0;
-  o.r = a.tail ? fmax(0.0, 1.0 - sum) : 0.0;
-  if (given) {
-    o.lse = a.lse[r];
-    o.log_rest = a.log_rest ? a.log_rest[r] : 0.0;
-    return o;
-  }
-  // (plain sums: one thread's worth of work per workgroup, repeated by all)
-  __shared__ Stat s_stat[SC_T];
-  const float c = 1.44269504088896340736f / a.T;
-  Stat st{-INFINITY, 0.0f, 0.0f};
-  for (int v = threadIdx.x; v < a.V; v += SC_T) {
-    bool in = false;
-    if (a.tail)
-      for (int m = 0; m < a.M; ++m) in |= ids[m] == v && !(lps[m] == -INFINITY);
-    if (!in) stat_add(st, row_at<DT>(row, v), c);
-  }
-  st = block_all(st, s_stat, [&](Stat p, Stat q) { return stat_merge(p, q, c); });
-  double top = st.m;
-  if (a.tail)
-    for (int m = 0; m < a.M; ++m)
-      if (ids[m] >= 0 && !(lps[m] == -INFINITY)) top = fmax(top, (double)row_at<DT>(row, ids[m]));
-  double rest = st.m == -INFINITY ? st.s : (double)st.s * exp(((double)st.m - top) / a.T), in = 0.0;
-  if (a.tail)
-    for (int m = 0; m < a.M; ++m) {
-      if (ids[m] < 0 || lps[m] == -INFINITY) continue;
-      bool first = true;
-      for (int q = 0; q < m; ++q) first &= !(ids[q] == ids[m] && !(lps[q] == -INFINITY));
-      if (first) in += exp(((double)row_at<DT>(row, ids[m]) - top) / a.T);
-    }
-  const double ls = log(rest + in);
-  o.lse = top / a.T + ls;
-  o.log_rest = a.tail ? log(rest) - ls : 0.0;
-  for (int m = 0; m < a.M; ++m) {
-    if (ids[m] < 0 || lps[m] == -INFINITY) continue;
-    const double lp = (double)lps[m] - tmax - (a.tail ? 0.0 : log(sum)), p = exp(lp);
-    if (p > 0.0 || p != p) o.loss += p * (lp - (((double)row_at<DT>(row, ids[m]) - top) / a.T - ls));
-  }
-  if (o.r > 0.0) o.loss += o.r * (log(o.r) - o.log_rest);
-  return o;
-}
-
-template <int DT, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(SC_T) void k_distill(DistillArgs a) {
-  const int64_t r = blockIdx.x;
-  const void* row = row_of<DT>(a.logits, r, a.stride);
-  const DistillRow o = distill_row<DT>(a, r, row, !LOSS);
-  if (LOSS && threadIdx.x == 0) {
-    const float loss = (float)o.loss;
-    a.loss[r] = loss;
-    if (a.out_lse) a.out_lse[r] = (float)o.lse;
-    if (a.out_log_rest) a.out_log_rest[r] = (float)o.log_rest;
-    if (a.status)
-      a.status[r] = o.bad ? STRIM_EINVAL : fabsf(loss) < INFINITY ? STRIM_OK : STRIM_ENONFINITE;
-  }
-  if (!GRAD) return;
-  void* out = (void*)row_of<DT>(a.d_logits, r, a.d_stride);
-  const int32_t* ids = a.ids + r * a.M;
-  const float* lps = a.logprobs + r * a.M;
-  double tmax = -INFINITY, sum = 0.0;
-  if (a.tail) tmax = 0.0;
-  else
-    for (int m = 0; m < a.M; ++m)
-      if (ids[m] >= 0 && !(lps[m] == -INFINITY)) tmax = fmax(tmax, (double)lps[m]);
-  for (int m = 0; m < a.M; ++m)
-    if (ids[m] >= 0 && !(lps[m] == -INFINITY)) sum += exp((double)lps[m] - tmax);
-  if (a.tail) sum = 1.0;
-  const double w = o.has ? (double)a.weights[r] / a.T : 0.0;
-  const double in = w * (o.mass + o.r);
-  const double other = o.r > 0.0 && o.log_rest > -1e300 ? in - w * o.r * exp(-o.log_rest) : in;
-  for (int v = threadIdx.x; v < a.V; v += SC_T) {
-    double d = 0.0;
-    if (o.has && w != 0.0) {
-      double p = 0.0;
-      bool hit = false;
-      for (int m = 0; m < a.M; ++m)
-        if (ids[m] == v && !(lps[m] == -INFINITY)) {
-          hit = true;
-          p += exp((double)lps[m] - tmax) / sum;
-        }
-      const double q = exp((double)row_at<DT>(row, v) / a.T - o.lse);
-      d = (hit || !a.tail ? in : other) * q - w * p;
-    }
-    row_set<DT>(out, v, (float)d);
-  }
-}
-
-// (a factor of 1, what the last step of a backward pass usually has, costs no pass over the data)
-template <int DT>
-__global__ __launch_bounds__(SC_T) void k_distill_scale(void* data, int64_t n, const float* factor) {
-  const float f = *factor;
-  if (f == 1.0f) return;
-  for (int64_t i = (int64_t)blockIdx.x * SC_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * SC_T)
-    row_set<DT>(data, i, row_at<DT>(data, i) * f);
+// Parts of a row: about eight workgroups a CU in all, one a row where there are that many.
+ScoreParts score_parts(int R, int V, int top) {
+  ScoreParts q{};
+  const int64_t tiles = ceil_of(V, SC_TILE), each = (int64_t)R * tiles / 2048;
+  q.tiles = (int32_t)(each < 1 ? 1 : each > tiles ? tiles : each);
+  q.parts = (int32_t)ceil_of(tiles, q.tiles);
+  q.room = 2 * top;
+  return q;
 }
 
 }  // namespace
 
-int64_t scores_workspace(int, int, int) { return 0; }
+int64_t scores_workspace(int R, int V, int top) {
+  const ScoreParts q = score_parts(R, V, top);
+  if (q.parts == 1) return 0;
+  return up16((int64_t)R * q.parts * (int64_t)sizeof(ScorePart)) + (int64_t)R * q.parts * q.room * 8;
+}
 
-hipError_t launch_scores(const ScoreArgs& a, bool bf16, void*, hipStream_t st) {
-  if (bf16) hipLaunchKernelGGL(k_scores<STRIM_DTYPE_BF16>, dim3((unsigned)a.R), dim3(SC_T), 0, st, a);
-  else hipLaunchKernelGGL(k_scores<STRIM_DTYPE_F32>, dim3((unsigned)a.R), dim3(SC_T), 0, st, a);
+hipError_t launch_scores(const ScoreArgs& a, bool bf16, void* workspace, hipStream_t st) {
+  ScoreParts q = score_parts(a.R, a.V, a.top);
+  if (q.parts > 1) {
+    q.part = (ScorePart*)workspace;
+    q.keys = (uint64_t*)((char*)workspace + up16((int64_t)a.R * q.parts * (int64_t)sizeof(ScorePart)));
+  }
+  const dim3 grid((unsigned)((int64_t)a.R * q.parts)), threads(SC_T);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, threads, 0, st, a, q); };
+  auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)a.R), threads, 0, st, a, q); };
+  auto all = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (a.mask) a.top ? go(k_scores<DT, true, true>) : go(k_scores<DT, true, false>);
+    else a.top ? go(k_scores<DT, false, true>) : go(k_scores<DT, false, false>);
+    if (q.parts > 1) a.top ? join(k_scores_join<DT, true>) : join(k_scores_join<DT, false>);
+  };
+  if (bf16) all(std::integral_constant<int, STRIM_DTYPE_BF16>{});
+  else all(std::integral_constant<int, STRIM_DTYPE_F32>{});
   return hipGetLastError();
 }
+
 hipError_t launch_scores_grad(const ScoreGradArgs& a, bool bf16, hipStream_t st) {
-  if (bf16) hipLaunchKernelGGL(k_scores_grad<STRIM_DTYPE_BF16>, dim3((unsigned)a.R), dim3(SC_T), 0, st, a);
-  else hipLaunchKernelGGL(k_scores_grad<STRIM_DTYPE_F32>, dim3((unsigned)a.R), dim3(SC_T), 0, st, a);
-  return hipGetLastError();
-}
-
-int64_t distill_workspace(int, int, int, bool) { return 0; }
-
-hipError_t launch_distill(const DistillArgs& a, bool bf16, bool loss, bool grad, void*, hipStream_t st) {
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)a.N), dim3(SC_T), 0, st, a); };
-  constexpr int B = STRIM_DTYPE_BF16, F = STRIM_DTYPE_F32;
-  if (loss && grad) bf16 ? go(k_distill<B, true, true>) : go(k_distill<F, true, true>);
-  else if (loss) bf16 ? go(k_distill<B, true, false>) : go(k_distill<F, true, false>);
-  else bf16 ? go(k_distill<B, false, true>) : go(k_distill<F, false, true>);
-  return hipGetLastError();
-}
-
-hipError_t launch_distill_scale(void* data, bool bf16, int64_t n, const float* factor, hipStream_t st) {
-  const int64_t blocks = (n + SC_T - 1) / SC_T;
-  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
-  if (bf16) hipLaunchKernelGGL(k_distill_scale<STRIM_DTYPE_BF16>, grid, dim3(SC_T), 0, st, data, n, factor);
-  else hipLaunchKernelGGL(k_distill_scale<STRIM_DTYPE_F32>, grid, dim3(SC_T), 0, st, data, n, factor);
+  const int parts = (int)ceil_of(a.V, 8 * SC_T * SG_TILES);
+  // (a launch has fewer than 2^32 threads)
+  const int most = (int)(((int64_t)1 << 23) / parts);
+  for (int r0 = 0; r0 < a.R; r0 += most) {
+    ScoreGradArgs b = a;
+    const int64_t at = r0;
+    b.R = a.R - r0 < most ? a.R - r0 : most;
+    b.logits = (const char*)a.logits + at * a.stride * (bf16 ? 2 : 4);
+    b.d_logits = (char*)a.d_logits + at * a.d_stride * (bf16 ? 2 : 4);
+    if (a.mask) b.mask = a.mask + at * a.mask_stride;
+    if (a.tokens) b.tokens = a.tokens + at * a.S;
+    b.lse = a.lse + at;
+    if (a.entropy) b.entropy = a.entropy + at;
+    if (a.grad_logprobs) b.grad_logprobs = a.grad_logprobs + at * a.S;
+    if (a.grad_entropy) b.grad_entropy = a.grad_entropy + at;
+    if (a.grad_lse) b.grad_lse = a.grad_lse + at;
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((int64_t)b.R * parts)), dim3(SC_T), 0, st, b, parts);
+    };
+    auto all = [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      if (a.mask) a.grad_entropy ? go(k_scores_grad<DT, true, true>) : go(k_scores_grad<DT, true, false>);
+      else a.grad_entropy ? go(k_scores_grad<DT, false, true>) : go(k_scores_grad<DT, false, false>);
+    };
+    if (bf16) all(std::integral_constant<int, STRIM_DTYPE_BF16>{});
+    else all(std::integral_constant<int, STRIM_DTYPE_F32>{});
+  }
   return hipGetLastError();
 }
 
