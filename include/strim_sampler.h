@@ -334,6 +334,7 @@ int strim_token_scores_grad(void* stream, const void* logits, int32_t dtype, int
  *   tail 1: p_m = exp(logprobs_m), and the teacher's remaining mass r = max(0, 1 - sum p) is one more
  *           alternative against q_rest, the student's mass outside the ids:
  *           out_loss += r (log r - log q_rest)
+ *           (no token outside the ids: r below 2^-20, which float32 does not tell from 0, is 0)
  *   d_logits[v] = grad_loss / temperature
  *                 (q[v] (sum p + r - [v no alternative] r / q_rest) - sum of p_m with id_m = v)
  * A negative id, or a log-probability of -inf, is no alternative (padding). A row without any, or with

@@ -1,204 +1,622 @@
-// distill_kernels.hip — distillation from a teacher's top logits.
+// distill_kernels.hip — distillation from a teacher's top logits: a student's rows x [V] against the
+// alternatives (id_m, log-probability t_m), m < M.
+//
+//   p_m = softmax of t_m over the alternatives, r = 0; or (tail) p_m = exp(t_m), r = max(0, 1 - sum p)
+//   q = softmax(x / T);  loss = sum_m p_m (log p_m - log q[id_m]) + r (log r - log q_rest)
+//   dx[v] = w / T (q[v] (P + r - [v no alternative] r / q_rest) - sum of p_m with id_m = v),  P = sum p
+//
+// What needs the whole row is one softmax statistic: of all its tokens, or (tail) of those that are no
+// alternative, so that q_rest is no difference of near numbers; the alternatives' own logits are looked
+// up. Those M numbers are in 64 bits: a small loss is the difference of much larger terms.
+//
+// k_distill_step has a row in one workgroup's registers between the statistic and the gradient: read
+// once, written once. Few rows, a loss or a gradient alone: k_distill_stat over parts of the rows,
+// k_distill_join, k_distill_grad.
+#include <type_traits>
+
 #include "kernels.hpp"
+#include "rows.hpp"
 #include "score.hpp"
 
 namespace strim {
 
 namespace {
 
-constexpr int SC_T = 256;  // threads of a row's workgroup
+constexpr int DI_T = 256;                 // threads of the parts' workgroups
+constexpr int DI_U = 4;                   // vectors of eight tokens a thread has of a tile
+constexpr int DI_TILE = 8 * DI_U * DI_T;  // tokens a tile
+constexpr int DI_M = STRIM_SCORE_MAX_LIST;
 
-template <int DT>
-__device__ __forceinline__ float row_at(const void* row, int64_t v) {
-  return DT == STRIM_DTYPE_BF16 ? bf16_to_f32(((const uint16_t*)row)[v]) : ((const float*)row)[v];
-}
-template <int DT>
-__device__ __forceinline__ const void* row_of(const void* x, int64_t r, int64_t stride) {
-  return (const char*)x + r * stride * (DT == STRIM_DTYPE_BF16 ? 2 : 4);
-}
-template <int DT>
-__device__ __forceinline__ void row_set(void* row, int64_t v, float f) {
-  if (DT == STRIM_DTYPE_BF16) ((uint16_t*)row)[v] = __builtin_bit_cast(uint16_t, (__bf16)f);
-  else ((float*)row)[v] = f;
-}
-__device__ __forceinline__ bool allowed_at(const uint32_t* mask, int64_t v) {
-  return !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
-}
-
-// Block reductions; every thread gets the result. `op` merges b into a, in a fixed order.
-template <class T, class Op>
-__device__ __forceinline__ T block_all(T v, T* scratch, Op op) {
-  const int t = threadIdx.x;
-  __syncthreads();
-  scratch[t] = v;
-  for (int d = SC_T / 2; d > 0; d >>= 1) {
-    __syncthreads();
-    if (t < d) scratch[t] = op(scratch[t], scratch[t + d]);
-  }
-  __syncthreads();
-  return scratch[0];
-}
-
-// max, sum exp((x - max) / T), sum (x - max) exp((x - max) / T); a max of -inf carries no sums (but
-// keeps a NaN)
-struct Stat {
-  float m, s, u;
+// A row's alternatives as a wave holds them: entry lane + 64 i in each lane, id -1 where there is none.
+struct Alternatives {
+  int id[2];
+  float lp[2];
+  bool known;  // no id past the vocabulary
+  bool any;    // (and an alternative)
 };
-__device__ __forceinline__ Stat stat_merge(Stat a, Stat b, float c) {
-  const float top = fmaxf(a.m, b.m);
-  if (top == -INFINITY) return Stat{top, a.s + b.s, 0.0f};
-  // (a difference that is the lowest value's would make u infinite, and that times 0)
-  const float da = a.m == -INFINITY ? 0.0f : fmaxf(a.m - top, -1e30f);
-  const float db = b.m == -INFINITY ? 0.0f : fmaxf(b.m - top, -1e30f);
-  const float fa = __builtin_amdgcn_exp2f(da * c), fb = __builtin_amdgcn_exp2f(db * c);
-  return Stat{top, a.s * fa + b.s * fb, (a.u + da * a.s) * fa + (b.u + db * b.s) * fb};
-}
-__device__ __forceinline__ void stat_add(Stat& a, float x, float c) {
-  a = stat_merge(a, Stat{x, x == -INFINITY ? 0.0f : 1.0f + 0.0f * x, 0.0f}, c);
-}
-
-// A distillation row's numbers: from the statistics of its tokens (`tail`: of those that are no
-// alternative) and its alternatives.
-struct DistillRow {
-  double lse, log_rest, loss, mass, r;
-  bool has, bad;
-};
-
-template <int DT>
-__device__ DistillRow distill_row(const DistillArgs& a, int64_t r, const void* row, bool given) {
-  const int32_t* ids = a.ids + r * a.M;
-  const float* lps = a.logprobs + r * a.M;
-  DistillRow o{0.0, 0.0, 0.0, 0.0, 0.0, false, false};
-  double tmax = -INFINITY;
-  for (int m = 0; m < a.M; ++m) {
-    if (ids[m] >= a.V) o.bad = true;
-    if (ids[m] >= 0 && !(lps[m] == -INFINITY)) {
-      o.has = true;
-      tmax = fmax(tmax, (double)lps[m]);
-    }
+__device__ __forceinline__ Alternatives alternatives_of(const DistillArgs& a, int64_t r) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  Alternatives o;
+  bool past = false, any = false;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int m = lane + i * WAVE;
+    o.id[i] = m < a.M ? a.ids[r * a.M + m] : -1;
+    o.lp[i] = m < a.M ? a.logprobs[r * a.M + m] : -INFINITY;
+    past |= o.id[i] >= a.V;
+    if (o.lp[i] == -INFINITY) o.id[i] = -1;
+    any |= o.id[i] >= 0;
   }
-  if (o.bad || !o.has) {
-    o.has = false;
-    return o;
-  }
-  if (a.tail) tmax = 0.0;
-  double sum = 0.0;
-  for (int m = 0; m < a.M; ++m)
-    if (ids[m] >= 0 && !(lps[m] == -INFINITY)) sum += exp((double)lps[m] - tmax);
-  o.mass = a.tail ? sum : 1.0;
-  o.r = a.tail ? fmax(0.0, 1.0 - sum) : 0.0;
-  if (given) {
-    o.lse = a.lse[r];
-    o.log_rest = a.log_rest ? a.log_rest[r] : 0.0;
-    return o;
-  }
-  // (plain sums: one thread's worth of work per workgroup, repeated by all)
-  __shared__ Stat s_stat[SC_T];
-  const float c = 1.44269504088896340736f / a.T;
-  Stat st{-INFINITY, 0.0f, 0.0f};
-  for (int v = threadIdx.x; v < a.V; v += SC_T) {
-    bool in = false;
-    if (a.tail)
-      for (int m = 0; m < a.M; ++m) in |= ids[m] == v && !(lps[m] == -INFINITY);
-    if (!in) stat_add(st, row_at<DT>(row, v), c);
-  }
-  st = block_all(st, s_stat, [&](Stat p, Stat q) { return stat_merge(p, q, c); });
-  double top = st.m;
-  if (a.tail)
-    for (int m = 0; m < a.M; ++m)
-      if (ids[m] >= 0 && !(lps[m] == -INFINITY)) top = fmax(top, (double)row_at<DT>(row, ids[m]));
-  double rest = st.m == -INFINITY ? st.s : (double)st.s * exp(((double)st.m - top) / a.T), in = 0.0;
-  if (a.tail)
-    for (int m = 0; m < a.M; ++m) {
-      if (ids[m] < 0 || lps[m] == -INFINITY) continue;
-      bool first = true;
-      for (int q = 0; q < m; ++q) first &= !(ids[q] == ids[m] && !(lps[q] == -INFINITY));
-      if (first) in += exp(((double)row_at<DT>(row, ids[m]) - top) / a.T);
-    }
-  const double ls = log(rest + in);
-  o.lse = top / a.T + ls;
-  o.log_rest = a.tail ? log(rest) - ls : 0.0;
-  for (int m = 0; m < a.M; ++m) {
-    if (ids[m] < 0 || lps[m] == -INFINITY) continue;
-    const double lp = (double)lps[m] - tmax - (a.tail ? 0.0 : log(sum)), p = exp(lp);
-    if (p > 0.0 || p != p) o.loss += p * (lp - (((double)row_at<DT>(row, ids[m]) - top) / a.T - ls));
-  }
-  if (o.r > 0.0) o.loss += o.r * (log(o.r) - o.log_rest);
+  o.known = __ballot(past) == 0;
+  o.any = o.known && __ballot(any) != 0;
   return o;
 }
 
-template <int DT, bool LOSS, bool GRAD>
-__global__ __launch_bounds__(SC_T) void k_distill(DistillArgs a) {
-  const int64_t r = blockIdx.x;
-  const void* row = row_of<DT>(a.logits, r, a.stride);
-  const DistillRow o = distill_row<DT>(a, r, row, !LOSS);
-  if (LOSS && threadIdx.x == 0) {
-    const float loss = (float)o.loss;
-    a.loss[r] = loss;
-    if (a.out_lse) a.out_lse[r] = (float)o.lse;
-    if (a.out_log_rest) a.out_log_rest[r] = (float)o.log_rest;
-    if (a.status)
-      a.status[r] = o.bad ? STRIM_EINVAL : fabsf(loss) < INFINITY ? STRIM_OK : STRIM_ENONFINITE;
-  }
-  if (!GRAD) return;
-  void* out = (void*)row_of<DT>(a.d_logits, r, a.d_stride);
-  const int32_t* ids = a.ids + r * a.M;
-  const float* lps = a.logprobs + r * a.M;
-  double tmax = -INFINITY, sum = 0.0;
-  if (a.tail) tmax = 0.0;
-  else
-    for (int m = 0; m < a.M; ++m)
-      if (ids[m] >= 0 && !(lps[m] == -INFINITY)) tmax = fmax(tmax, (double)lps[m]);
-  for (int m = 0; m < a.M; ++m)
-    if (ids[m] >= 0 && !(lps[m] == -INFINITY)) sum += exp((double)lps[m] - tmax);
-  if (a.tail) sum = 1.0;
-  const double w = o.has ? (double)a.weights[r] / a.T : 0.0;
-  const double in = w * (o.mass + o.r);
-  const double other = o.r > 0.0 && o.log_rest > -1e300 ? in - w * o.r * exp(-o.log_rest) : in;
-  for (int v = threadIdx.x; v < a.V; v += SC_T) {
-    double d = 0.0;
-    if (o.has && w != 0.0) {
-      double p = 0.0;
-      bool hit = false;
-      for (int m = 0; m < a.M; ++m)
-        if (ids[m] == v && !(lps[m] == -INFINITY)) {
-          hit = true;
-          p += exp((double)lps[m] - tmax) / sum;
-        }
-      const double q = exp((double)row_at<DT>(row, v) / a.T - o.lse);
-      d = (hit || !a.tail ? in : other) * q - w * p;
+// Each entry that is among the wave's 512 tokens from w0 on, in the list's order: f(lane, element, entry's
+// lane, i).
+template <class F>
+__device__ __forceinline__ void each_hit(const int (&id)[2], int w0, F f) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint64_t hit = __ballot((uint32_t)(id[i] - w0) < 8u * WAVE);  // (an id of -1 is never)
+    while (hit) {
+      const int l = __builtin_ctzll(hit);
+      hit &= hit - 1;
+      const int off = rl_i(id[i], l) - w0;
+      f(off >> 3, off & 7, l, i);
     }
-    row_set<DT>(out, v, (float)d);
+  }
+}
+template <int DT>
+__device__ __forceinline__ void without_hits(float (&x)[8], const int (&id)[2], int w0) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  each_hit(id, w0, [&](int at, int e, int, int) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane == at && j == e) x[j] = -INFINITY;
+  });
+}
+
+// A row's teacher: the entries' probabilities (0 where there is none), log p_m = lp_m - shift, P and r. The
+// exponentials are float32 ones, the sums and differences double: an error that the p_m share with r moves
+// a small loss by its product with the loss's own size.
+struct Teacher {
+  float p[2];
+  double shift, mass, r;
+};
+__device__ __forceinline__ Teacher teacher_of(const Alternatives& o, bool tail) {
+  Teacher t;
+  float mx = 0.0f;
+  if (!tail)
+    mx = wave_max_f(fmaxf(o.id[0] >= 0 ? o.lp[0] : -INFINITY, o.id[1] >= 0 ? o.lp[1] : -INFINITY));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) t.p[i] = o.id[i] >= 0 ? expf(o.lp[i] - mx) : 0.0f;
+  const double sum = wave_sum((double)t.p[0] + (double)t.p[1]);
+  t.mass = tail ? sum : 1.0;
+  t.r = tail ? fmax(0.0, 1.0 - sum) : 0.0;
+  t.shift = 0.0;
+  if (!tail) {
+    t.shift = mx + log(sum);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) t.p[i] = (float)(t.p[i] / sum);
+  }
+  return t;
+}
+
+// Which entries are the first with their id, and those entries' p with the later ones' added. One wave.
+__device__ __forceinline__ void merge_repeats(const Alternatives& o, int M, bool (&first)[2], float (&p)[2]) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  float sum[2] = {0.0f, 0.0f};
+  first[0] = o.id[0] >= 0;
+  first[1] = o.id[1] >= 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    for (int l = 0; l < min(WAVE, M - h * WAVE); ++l) {
+      const int id = rl_i(o.id[h], l);
+      const float more = rl_f(p[h], l);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (id == o.id[i]) {
+          sum[i] += more;
+          if (h < i || (h == i && l < lane)) first[i] = false;
+        }
+    }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) p[i] = sum[i];
+}
+
+// The teacher's remaining mass: where nothing lies outside the ids, one that float32 log-probabilities do not
+// tell from none is none.
+__device__ __forceinline__ double bucket_of(double r, bool empty) { return empty && r < 0x1p-20 ? 0.0 : r; }
+
+// A row's numbers from the statistic: the loss; `ls` = log sum exp((x - top) / T) and log q_rest. x: the
+// entries' logits. By one wave, every lane the same.
+struct RowNumbers {
+  double loss, top, ls, log_rest;
+};
+__device__ __forceinline__ RowNumbers numbers_of(const Alternatives& o, const Teacher& t, const bool (&first)[2],
+                                                 const float (&x)[2], RowStat st, float T, bool tail) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  RowNumbers n;
+  n.top = st.m;
+  double all = st.s, far = 0.0;
+  if (tail) {
+    n.top = wave_max_f(fmaxf(st.m, fmaxf(first[0] ? x[0] : -INFINITY, first[1] ? x[1] : -INFINITY)));
+    const float ref = stat_ref((float)n.top);
+    double in = 0.0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) in += first[i] ? (double)expf((x[i] - ref) / T) : 0.0;
+    in = wave_sum(in);
+    far = ((double)st.m - ref) / T;
+    all = (st.m == -INFINITY ? (double)st.s : (double)st.s * exp(far)) + in;
+  }
+  // the three logarithms by three lanes
+  const double l = log(lane == 0 ? all : lane == 1 ? (double)st.s : t.r);
+  n.ls = rl_d(l, 0);
+  // (a rest whose share vanishes in 64 bits keeps its logarithm)
+  n.log_rest = !tail ? 0.0 : st.m == -INFINITY ? -(double)INFINITY : far + rl_d(l, 1) - n.ls;
+  double loss = 0.0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (o.id[i] >= 0 && !(t.p[i] == 0.0f))
+      loss += t.p[i] * (((double)o.lp[i] - t.shift) - (((double)x[i] - n.top) / T - n.ls));
+  n.loss = wave_sum(loss);
+  if (bucket_of(t.r, st.m == -INFINITY) > 0.0) n.loss += t.r * (rl_d(l, 2) - n.log_rest);
+  return n;
+}
+
+// What the gradient takes of a row: sign exp2((x - ref) c + k) at every token, but at the alternatives
+// in exp2((x - ref) c + kq) - p.
+struct GradRow {
+  float ref, k, kq, in;
+  uint32_t sign;  // 0 or 0x80008000
+  int32_t dead;   // the row has no gradient
+};
+// lse = ref / T + ls; w = weight / T
+__device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, float ref, double ls, double log_rest,
+                                            double w) {
+  constexpr double L2E = 1.4426950408889634074;
+  GradRow g;
+  g.dead = !any || w == 0.0;
+  const double in = w * (t.mass + bucket_of(t.r, log_rest == -INFINITY));
+  double all = in, more = 0.0;
+  if (t.r > 0.0 && log_rest > -INFINITY) {  // (nothing lies outside where q_rest is 0)
+    if (log_rest > -600.0) {
+      all = in - w * t.r * exp(-log_rest);
+    } else {
+      all = -w * t.r;
+      more = -log_rest;
+    }
+  }
+  g.ref = ref;
+  g.kq = (float)(-ls * L2E);
+  g.k = (float)(log2(fabs(all)) + (more - ls) * L2E);
+  g.in = (float)in;
+  g.sign = all < 0.0 ? 0x80008000u : 0u;
+  return g;
+}
+
+// Eight tokens' gradients; id, p: the wave's alternatives (each id once) and w / T p_m; hits: whether any
+// is among the wave's tokens, which begin at w0.
+template <int DT>
+__device__ __forceinline__ RowVec<DT> grad_of(const RowVec<DT>& x, const GradRow& g, float c,
+                                              const int (&id)[2], const float (&p)[2], int w0, bool hits) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  float d[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) d[j] = hw_exp2(fma_f(x.at(j) - g.ref, c, g.k));
+  RowVec<DT> y;
+  y.set(d);
+#pragma unroll
+  for (int i = 0; i < RowVec<DT>::WORDS; ++i)
+    y.w[i] ^= DT == STRIM_DTYPE_BF16 ? g.sign : g.sign & 0x80000000u;
+  if (hits)
+    each_hit(id, w0, [&](int at, int e, int l, int i) {
+      const float less = rl_f(p[i], l);
+      // (masks, not an index: words that are indexed at run time are put into memory)
+      const int word = DT == STRIM_DTYPE_BF16 ? e >> 1 : e;
+      const uint32_t half = DT == STRIM_DTYPE_F32 ? ~0u : e & 1 ? 0xFFFF0000u : 0xFFFFu;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int q = 0; q < RowVec<DT>::WORDS; ++q) bits |= x.w[q] & (q == word ? half : 0u);
+      if (DT == STRIM_DTYPE_BF16 && !(e & 1)) bits <<= 16;
+      const float f = g.in * hw_exp2(fma_f(__uint_as_float(bits) - g.ref, c, g.kq)) - less;
+      const float two[8] = {f, f};
+      RowVec<DT> z;
+      z.set(two);
+      const uint32_t mine = lane == at ? half : 0u;
+#pragma unroll
+      for (int q = 0; q < RowVec<DT>::WORDS; ++q) {
+        const uint32_t m = q == word ? mine : 0u;
+        y.w[q] = (y.w[q] & ~m) | (z.w[0] & m);
+      }
+    });
+  if (g.dead)
+#pragma unroll
+    for (int i = 0; i < RowVec<DT>::WORDS; ++i) y.w[i] = 0;
+  return y;
+}
+
+// The row's alternatives for the gradient in LDS, each id once: what a workgroup's waves read.
+struct GradList {
+  int id[DI_M];
+  float p[DI_M];
+  int repeats;  // whether an id stands twice
+};
+// Looks for repeated ids, all threads: entry e against a part of those before it. (Two barriers' worth:
+// the caller's before reading l.repeats.)
+template <int T>
+__device__ __forceinline__ void find_repeats(GradList& l, const Alternatives& o) {
+  if (threadIdx.x < WAVE) {
+    l.id[threadIdx.x] = o.id[0];
+    l.id[threadIdx.x + WAVE] = o.id[1];
+    if (threadIdx.x == 0) l.repeats = 0;
+  }
+  __syncthreads();
+  constexpr int SEG = DI_M * DI_M / T;
+  const int e = threadIdx.x % DI_M, from = (int)threadIdx.x / DI_M * SEG, id = l.id[e];
+  bool twice = false;
+#pragma unroll 4
+  for (int j = from; j < from + SEG; ++j) twice |= j < e && l.id[j] == id;
+  if (twice && id >= 0) l.repeats = 1;
+}
+// The wave's entries as GradList has them: w / T p_m, each id once.
+__device__ __forceinline__ void list_out(GradList& l, const Alternatives& o, const Teacher& t, int M, double w,
+                                         bool (&first)[2], bool repeats) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  float p[2] = {t.p[0], t.p[1]};
+  if (repeats) merge_repeats(o, M, first, p);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l.id[lane + i * WAVE] = first[i] ? o.id[i] : -1;
+    l.p[lane + i * WAVE] = (float)(w * p[i]);
+  }
+}
+
+struct DistillParts {
+  int32_t parts, tiles;  // parts of a row; tiles of a part
+  RowStat* part;         // [N][parts]
+};
+
+// The tokens' statistic of a part of a row; TAIL: without the alternatives'.
+template <int DT, bool TAIL>
+__global__ __launch_bounds__(DI_T) void k_distill_stat(const DistillArgs a, const DistillParts q) {
+  __shared__ RowStat s_stat[DI_T / WAVE];
+  const int64_t r = blockIdx.x / q.parts;
+  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1);
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  const float c = LOG2E / a.T;
+  const int t0 = p * q.tiles * DI_TILE, t1 = min(a.V, t0 + q.tiles * DI_TILE);
+  RowVec<DT> next[DI_U];
+  auto request = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < DI_U; ++u) {
+      const int v = t + 8 * (u * DI_T + (int)threadIdx.x);
+      if (t + DI_TILE <= a.V) next[u].load(row, v);
+      else next[u].load_to(row, v, a.V);
+    }
+  };
+  request(t0);
+  Alternatives o;
+  if constexpr (TAIL) o = alternatives_of(a, r);
+  RowStat st{-INFINITY, 0.0f, 0.0f};
+  for (int t = t0; t < t1; t += DI_TILE) {
+    float x[8 * DI_U];
+#pragma unroll
+    for (int u = 0; u < DI_U; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[8 * u + j] = next[u].at(j);
+    if (t + DI_TILE < t1) request(t + DI_TILE);
+    if constexpr (TAIL)
+#pragma unroll
+      for (int u = 0; u < DI_U; ++u)
+        each_hit(o.id, t + 8 * (u * DI_T + (int)threadIdx.x - lane), [&](int at, int e, int, int) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (lane == at && j == e) x[8 * u + j] = -INFINITY;
+        });
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8 * DI_U; ++j) mx = fmaxf(mx, x[j]);
+    stat_add<8 * DI_U, false>(st, x, mx, c);
+  }
+  stat_wave(st, c);
+  if (lane == 0) s_stat[threadIdx.x / WAVE] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < DI_T / WAVE; ++i) stat_merge(st, s_stat[i], c);
+    q.part[r * q.parts + p] = st;
+  }
+}
+
+// The rows' results; a wave a row.
+template <int DT>
+__global__ __launch_bounds__(DI_T) void k_distill_join(const DistillArgs a, const DistillParts q) {
+  const int64_t r = (int64_t)blockIdx.x * (DI_T / WAVE) + wave_id();
+  if (r >= a.N) return;
+  const int lane = threadIdx.x & (WAVE - 1);
+  const float c = LOG2E / a.T;
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  RowStat st{-INFINITY, 0.0f, 0.0f};
+  for (int p = lane; p < q.parts; p += WAVE) stat_merge(st, q.part[r * q.parts + p], c);
+  stat_wave(st, c);
+  const Alternatives o = alternatives_of(a, r);
+  RowNumbers n{0.0, 0.0, 0.0, 0.0};
+  if (o.any) {
+    float x[2], p[2] = {0.0f, 0.0f};
+    bool first[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
+    if (a.tail) merge_repeats(o, a.M, first, p);
+    n = numbers_of(o, teacher_of(o, a.tail), first, x, st, a.T, a.tail);
+  }
+  if (lane != 0) return;
+  const float loss = (float)n.loss;
+  a.loss[r] = loss;
+  if (a.out_lse) a.out_lse[r] = (float)(n.top / a.T + n.ls);
+  if (a.out_log_rest) a.out_log_rest[r] = (float)n.log_rest;
+  if (a.status)
+    a.status[r] = !o.known ? STRIM_EINVAL : fabsf(loss) < INFINITY ? STRIM_OK : STRIM_ENONFINITE;
+}
+
+// A part of a row's gradient from its lse and log q_rest.
+template <int DT>
+__global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, const DistillParts q) {
+  __shared__ GradList s_list;
+  __shared__ GradRow s_grad;
+  const int64_t r = blockIdx.x / q.parts;
+  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1);
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  char* out = (char*)a.d_logits + r * a.d_stride * RowVec<DT>::SIZE;
+  const float c = LOG2E / a.T;
+  const int t0 = p * q.tiles * DI_TILE, t1 = min(a.V, t0 + q.tiles * DI_TILE);
+  RowVec<DT> next[DI_U];
+  auto request = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < DI_U; ++u) {
+      const int v = t + 8 * (u * DI_T + (int)threadIdx.x);
+      if (v < a.V) next[u].load_to(row, v, a.V);
+    }
+  };
+  request(t0);
+  const Alternatives o = alternatives_of(a, r);
+  find_repeats<DI_T>(s_list, o);
+  __syncthreads();
+  if (wave_id() == 0) {
+    const Teacher t = teacher_of(o, a.tail);
+    const double w = (double)a.weights[r] / a.T, lse = a.lse[r];
+    const float ref = (float)(lse * a.T);
+    bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};
+    list_out(s_list, o, t, a.M, w, first, s_list.repeats != 0);
+    const GradRow g = grad_row(o.any, t, ref, lse - (double)ref / a.T, a.tail ? (double)a.log_rest[r] : 0.0, w);
+    if (lane == 0) s_grad = g;
+  }
+  __syncthreads();
+  const GradRow g = s_grad;
+  const int id[2] = {s_list.id[lane], s_list.id[lane + WAVE]};
+  const float less[2] = {s_list.p[lane], s_list.p[lane + WAVE]};
+  for (int s = t0; s < t1; s += DI_TILE) {
+    RowVec<DT> x[DI_U];
+#pragma unroll
+    for (int u = 0; u < DI_U; ++u) x[u] = next[u];
+    if (s + DI_TILE < t1) request(s + DI_TILE);
+#pragma unroll
+    for (int u = 0; u < DI_U; ++u) {
+      const int w0 = __builtin_amdgcn_readfirstlane(s + 8 * (u * DI_T + (int)threadIdx.x - lane));
+      if (w0 >= a.V) break;
+      const RowVec<DT> y = grad_of<DT>(x[u], g, c, id, less, w0, true);
+      if (w0 + 8 * lane < a.V) y.store_to(out, w0 + 8 * lane, a.V);
+    }
+  }
+}
+
+// A row whole: NV vectors of eight tokens a thread in registers; what is past them is read again for the
+// gradient.
+template <int DT, int T, int NV, bool TAIL>
+__global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
+  constexpr int NWAVES = T / WAVE;
+  __shared__ RowStat s_stat[NWAVES];
+  __shared__ GradList s_list;
+  __shared__ GradRow s_grad;
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x & (WAVE - 1), wave = wave_id();
+  const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  char* out = (char*)a.d_logits + r * a.d_stride * RowVec<DT>::SIZE;
+  const float c = LOG2E / a.T;
+  RowVec<DT> x[NV];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) x[u].load_to(row, 8 * (u * T + (int)threadIdx.x), a.V);
+  const Alternatives o = alternatives_of(a, r);
+  find_repeats<T>(s_list, o);
+  // the vectors among which the wave's alternatives are
+  uint64_t hits = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    for (uint64_t b = __ballot(o.id[i] >= 0 && (o.id[i] / (8 * WAVE)) % NWAVES == wave); b; b &= b - 1)
+      hits |= 1ull << min(63, rl_i(o.id[i], __builtin_ctzll(b)) / (8 * T));
+  RowStat st{-INFINITY, 0.0f, 0.0f};
+  auto add = [&](const RowVec<DT>& q, int w0, bool hit) {
+    float f[8], mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = q.at(j);
+    if (TAIL && hit) without_hits<DT>(f, o.id, w0);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, f[j]);
+    stat_add<8, false>(st, f, mx, c);
+  };
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    add(x[u], 8 * WAVE * (u * NWAVES + wave), (hits >> u) & 1u);
+    // (else the tokens as floats are kept for the gradient, beside the words: 568 bytes a lane spilled)
+#pragma unroll
+    for (int i = 0; i < RowVec<DT>::WORDS; ++i) asm volatile("" : "+v"(x[u].w[i]));
+  }
+  for (int v0 = 8 * NV * T; v0 < a.V; v0 += 8 * T) {
+    RowVec<DT> q;
+    q.load_to(row, v0 + 8 * (int)threadIdx.x, a.V);
+    add(q, v0 + 8 * WAVE * wave, true);
+  }
+  stat_wave(st, c);
+  if (lane == 0) s_stat[wave] = st;
+  __syncthreads();
+  if (wave == 0) {
+    st = lane < NWAVES ? s_stat[lane] : RowStat{-INFINITY, 0.0f, 0.0f};
+    stat_wave(st, c);
+    const Teacher t = teacher_of(o, TAIL);
+    const double w = (double)a.weights[r] / a.T;
+    bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};
+    list_out(s_list, o, t, a.M, w, first, s_list.repeats != 0);
+    RowNumbers n{0.0, 0.0, 0.0, 0.0};
+    if (o.any) {
+      float xa[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) xa[i] = o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
+      n = numbers_of(o, t, first, xa, st, a.T, TAIL);
+    }
+    const GradRow g = grad_row(o.any, t, (float)n.top, n.ls, n.log_rest, w);
+    if (lane == 0) {
+      s_grad = g;
+      const float loss = (float)n.loss;
+      a.loss[r] = loss;
+      if (a.status)
+        a.status[r] = !o.known ? STRIM_EINVAL : fabsf(loss) < INFINITY ? STRIM_OK : STRIM_ENONFINITE;
+    }
+  }
+  __syncthreads();
+  const GradRow g = s_grad;
+  const int id[2] = {s_list.id[lane], s_list.id[lane + WAVE]};
+  const float less[2] = {s_list.p[lane], s_list.p[lane + WAVE]};
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int w0 = 8 * WAVE * (u * NWAVES + wave);
+    if (w0 < a.V) {
+      const RowVec<DT> y = grad_of<DT>(x[u], g, c, id, less, w0, (hits >> u) & 1u);
+      if (w0 + 8 * lane < a.V) y.store_to(out, w0 + 8 * lane, a.V);
+    }
+  }
+  for (int w0 = 8 * (NV * T + WAVE * wave); w0 < a.V; w0 += 8 * T) {
+    RowVec<DT> q;
+    q.load_to(row, w0 + 8 * lane, a.V);
+    const RowVec<DT> y = grad_of<DT>(q, g, c, id, less, w0, true);
+    if (w0 + 8 * lane < a.V) y.store_to(out, w0 + 8 * lane, a.V);
   }
 }
 
 // (a factor of 1, what the last step of a backward pass usually has, costs no pass over the data)
 template <int DT>
-__global__ __launch_bounds__(SC_T) void k_distill_scale(void* data, int64_t n, const float* factor) {
+__global__ __launch_bounds__(DI_T) void k_distill_scale(char* data, int64_t n, const float* factor) {
   const float f = *factor;
   if (f == 1.0f) return;
-  for (int64_t i = (int64_t)blockIdx.x * SC_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * SC_T)
-    row_set<DT>(data, i, row_at<DT>(data, i) * f);
+  for (int64_t i = (int64_t)blockIdx.x * DI_T + threadIdx.x; i < n; i += (int64_t)gridDim.x * DI_T) {
+    if constexpr (DT == STRIM_DTYPE_BF16) {
+      uint16_t* p = (uint16_t*)data + i;
+      *p = __builtin_bit_cast(uint16_t, (__bf16)(bf16_to_f32(*p) * f));
+    } else {
+      ((float*)data)[i] *= f;
+    }
+  }
+}
+
+int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
+int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Parts of a row: about eight workgroups a CU in all, one a row where there are that many.
+DistillParts distill_parts(int N, int V) {
+  DistillParts q{};
+  const int64_t tiles = ceil_of(V, DI_TILE), each = (int64_t)N * tiles / 2048;
+  q.tiles = (int32_t)(each < 1 ? 1 : each > tiles ? tiles : each);
+  q.parts = (int32_t)ceil_of(tiles, q.tiles);
+  return q;
+}
+// Rows from which a step keeps each in a workgroup.
+constexpr int DI_WHOLE = 192;
+
+template <class F>
+void with_dtype(bool bf16, F f) {
+  if (bf16) f(std::integral_constant<int, STRIM_DTYPE_BF16>{});
+  else f(std::integral_constant<int, STRIM_DTYPE_F32>{});
+}
+
+void launch_grad(const DistillArgs& a, bool bf16, hipStream_t st) {
+  // (a launch has fewer than 2^32 threads)
+  const DistillParts q = distill_parts(a.N, a.V);
+  with_dtype(bf16, [&](auto dt) {
+    hipLaunchKernelGGL((k_distill_grad<decltype(dt)::value>), dim3((unsigned)((int64_t)a.N * q.parts)), dim3(DI_T), 0,
+                       st, a, q);
+  });
+}
+
+template <int DT, bool TAIL>
+void launch_whole(const DistillArgs& a, hipStream_t st) {
+  constexpr int WIDE = DT == STRIM_DTYPE_BF16 ? 19 : 9;
+  constexpr int MOST = 1 << 21;  // (a launch has fewer than 2^32 threads)
+  for (int r0 = 0; r0 < a.N; r0 += MOST) {
+    DistillArgs b = a;
+    const int64_t at = r0;
+    b.N = a.N - r0 < MOST ? a.N - r0 : MOST;
+    b.logits = (const char*)a.logits + at * a.stride * RowVec<DT>::SIZE;
+    b.d_logits = (char*)a.d_logits + at * a.d_stride * RowVec<DT>::SIZE;
+    b.ids = a.ids + at * a.M;
+    b.logprobs = a.logprobs + at * a.M;
+    b.weights = a.weights + at;
+    b.loss = a.loss + at;
+    if (a.status) b.status = a.status + at;
+    auto go = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)b.N), dim3(threads), 0, st, b);
+    };
+    if (a.V <= 8 * 256 * 4) go(k_distill_step<DT, 256, 4, TAIL>, 256);
+    else if (a.V <= 8 * 1024 * 4) go(k_distill_step<DT, 1024, 4, TAIL>, 1024);
+    else go(k_distill_step<DT, 1024, WIDE, TAIL>, 1024);
+  }
 }
 
 }  // namespace
 
-int64_t distill_workspace(int, int, int, bool) { return 0; }
+int64_t distill_workspace(int N, int V, int M, bool step) {
+  (void)M;
+  if (step && N >= DI_WHOLE) return 0;
+  const int64_t part = up16((int64_t)N * distill_parts(N, V).parts * (int64_t)sizeof(RowStat));
+  return part + (step ? 2 * up16(4 * (int64_t)N) : 0);
+}
 
-hipError_t launch_distill(const DistillArgs& a, bool bf16, bool loss, bool grad, void*, hipStream_t st) {
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)a.N), dim3(SC_T), 0, st, a); };
-  constexpr int B = STRIM_DTYPE_BF16, F = STRIM_DTYPE_F32;
-  if (loss && grad) bf16 ? go(k_distill<B, true, true>) : go(k_distill<F, true, true>);
-  else if (loss) bf16 ? go(k_distill<B, true, false>) : go(k_distill<F, true, false>);
-  else bf16 ? go(k_distill<B, false, true>) : go(k_distill<F, false, true>);
+hipError_t launch_distill(const DistillArgs& given, bool bf16, bool loss, bool grad, void* workspace,
+                          hipStream_t st) {
+  DistillArgs a = given;
+  if (loss && grad && a.N >= DI_WHOLE) {
+    with_dtype(bf16, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      a.tail ? launch_whole<DT, true>(a, st) : launch_whole<DT, false>(a, st);
+    });
+    return hipGetLastError();
+  }
+  if (loss) {
+    DistillParts q = distill_parts(a.N, a.V);
+    q.part = (RowStat*)workspace;
+    if (grad) {
+      char* rows = (char*)workspace + up16((int64_t)a.N * q.parts * (int64_t)sizeof(RowStat));
+      a.out_lse = (float*)rows;
+      a.out_log_rest = (float*)(rows + up16(4 * (int64_t)a.N));
+      a.lse = a.out_lse;
+      a.log_rest = a.out_log_rest;
+    }
+    with_dtype(bf16, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      const dim3 grid((unsigned)((int64_t)a.N * q.parts));
+      if (a.tail) hipLaunchKernelGGL((k_distill_stat<DT, true>), grid, dim3(DI_T), 0, st, a, q);
+      else hipLaunchKernelGGL((k_distill_stat<DT, false>), grid, dim3(DI_T), 0, st, a, q);
+      hipLaunchKernelGGL(k_distill_join<DT>, dim3((unsigned)ceil_of(a.N, DI_T / WAVE)), dim3(DI_T), 0, st, a, q);
+    });
+  }
+  if (grad) launch_grad(a, bf16, st);
   return hipGetLastError();
 }
 
 hipError_t launch_distill_scale(void* data, bool bf16, int64_t n, const float* factor, hipStream_t st) {
-  const int64_t blocks = (n + SC_T - 1) / SC_T;
-  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
-  if (bf16) hipLaunchKernelGGL(k_distill_scale<STRIM_DTYPE_BF16>, grid, dim3(SC_T), 0, st, data, n, factor);
-  else hipLaunchKernelGGL(k_distill_scale<STRIM_DTYPE_F32>, grid, dim3(SC_T), 0, st, data, n, factor);
+  const int64_t blocks = ceil_of(n, DI_T);
+  with_dtype(bf16, [&](auto dt) {
+    hipLaunchKernelGGL(k_distill_scale<decltype(dt)::value>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(DI_T), 0,
+                       st, (char*)data, n, factor);
+  });
   return hipGetLastError();
 }
 
