@@ -447,9 +447,7 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     add(x[u], 8 * WAVE * (u * NWAVES + wave), (hits >> u) & 1u);
-    // (else the tokens as floats are kept for the gradient, beside the words: 568 bytes a lane spilled)
-#pragma unroll
-    for (int i = 0; i < RowVec<DT>::WORDS; ++i) asm volatile("" : "+v"(x[u].w[i]));
+    x[u].renew();  // (568 bytes a lane spilled without)
   }
   for (int v0 = 8 * NV * T; v0 < a.V; v0 += 8 * T) {
     RowVec<DT> q;

@@ -4,106 +4,435 @@
 //   y = (x - mu) rstd w + b,  rstd = 1 / sqrt(mean (x - mu)^2 + eps),  mu = mean x or 0
 //   with xh = (x - mu) rstd, h = w dy:
 //   dx = rstd (h - xh mean(h xh) [- mean h]),  dw = sum_n dy xh,  db = sum_n dy
+//
+// A row is held in the registers of L threads, NV vectors of eight elements each: 16 lanes, a wave or a
+// workgroup of 256 or 1,024, the fewest that hold it. The variance is taken of x - mu, not from the squares'
+// mean. The weights' gradients are sums over the rows: each thread adds those of its own columns over the
+// rows that its workgroup takes one after the other (the next row is requested before this one's sums are
+// met), a workgroup leaves one float32 row of them, and k_norm_join adds those in order.
+#include <type_traits>
+
 #include "kernels.hpp"
+#include "rows.hpp"
 #include "score.hpp"
 
 namespace strim {
 
 namespace {
 
-constexpr int NO_T = 256;
-
-__device__ __forceinline__ float norm_at(const void* p, int64_t i, bool bf16) {
-  return bf16 ? bf16_to_f32(((const uint16_t*)p)[i]) : ((const float*)p)[i];
-}
-__device__ __forceinline__ void norm_set(void* p, int64_t i, float f, bool bf16) {
-  if (bf16) ((uint16_t*)p)[i] = __builtin_bit_cast(uint16_t, (__bf16)f);
-  else ((float*)p)[i] = f;
-}
-__device__ __forceinline__ float norm_sum(float v, float* scratch) {
-  __syncthreads();
-  scratch[threadIdx.x] = v;
-  for (int d = NO_T / 2; d > 0; d >>= 1) {
-    __syncthreads();
-    if ((int)threadIdx.x < d) scratch[threadIdx.x] += scratch[threadIdx.x + d];
-  }
-  __syncthreads();
-  return scratch[0];
-}
-
-__global__ __launch_bounds__(NO_T) void k_norm(NormArgs a, bool bf16, bool wbf16) {
-  __shared__ float s_sum[NO_T];
-  const int64_t n = blockIdx.x;
-  float mu = 0.0f;
-  if (a.mean) {
-    float s = 0.0f;
-    for (int k = threadIdx.x; k < a.K; k += NO_T) s += norm_at(a.x, n * a.x_stride + k, bf16);
-    mu = norm_sum(s, s_sum) / (float)a.K;
-  }
-  float q = 0.0f;
-  for (int k = threadIdx.x; k < a.K; k += NO_T) {
-    const float c = norm_at(a.x, n * a.x_stride + k, bf16) - mu;
-    q += c * c;
-  }
-  const float rstd = 1.0f / sqrtf(norm_sum(q, s_sum) / (float)a.K + a.eps);
-  for (int k = threadIdx.x; k < a.K; k += NO_T) {
-    float y = (norm_at(a.x, n * a.x_stride + k, bf16) - mu) * rstd;
-    if (a.weight) y *= norm_at(a.weight, k, wbf16);
-    if (a.bias) y += norm_at(a.bias, k, wbf16);
-    norm_set(a.y, n * a.y_stride + k, y, bf16);
-  }
-  if (threadIdx.x == 0) {
-    if (a.rstd) a.rstd[n] = rstd;
-    if (a.mean) a.mean[n] = mu;
+// Elements k .. k + 7 of a weight or bias of either type; `none` where there is no tensor, 0 past K.
+__device__ __forceinline__ void param8(const void* p, bool bf16, int k, int K, float none, float (&f)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = none;
+  if (!p) return;
+  if (bf16) {
+    RowVec<STRIM_DTYPE_BF16> v;
+    v.load_to<true>((const char*)p, k, K);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = v.at(j);
+  } else {
+    RowVec<STRIM_DTYPE_F32> v;
+    v.load_to<true>((const char*)p, k, K);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = v.at(j);
   }
 }
 
-__global__ __launch_bounds__(NO_T) void k_norm_dx(NormGradArgs a, bool bf16, bool wbf16) {
-  __shared__ float s_sum[NO_T];
-  const int64_t n = blockIdx.x;
-  const float rstd = a.rstd[n], mu = a.mean ? a.mean[n] : 0.0f;
-  float c1 = 0.0f, c2 = 0.0f;
-  for (int k = threadIdx.x; k < a.K; k += NO_T) {
-    const float h = norm_at(a.dy, n * a.dy_stride + k, bf16) * (a.weight ? norm_at(a.weight, k, wbf16) : 1.0f);
-    c1 += h * ((norm_at(a.x, n * a.x_stride + k, bf16) - mu) * rstd);
-    c2 += h;
-  }
-  c1 = norm_sum(c1, s_sum) / (float)a.K;
-  c2 = a.mean ? norm_sum(c2, s_sum) / (float)a.K : 0.0f;
-  for (int k = threadIdx.x; k < a.K; k += NO_T) {
-    const float h = norm_at(a.dy, n * a.dy_stride + k, bf16) * (a.weight ? norm_at(a.weight, k, wbf16) : 1.0f);
-    const float xh = (norm_at(a.x, n * a.x_stride + k, bf16) - mu) * rstd;
-    norm_set(a.dx, n * a.dx_stride + k, rstd * (h - xh * c1 - c2), bf16);
+// The sum of v over the row's L threads, in each of them. `scratch` (L > 64: a wave's place each) is free
+// again after the next call's barrier, so two take turns.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float* scratch) {
+  if constexpr (L == 16) {
+    v += dpp_f<DPP_XOR1>(v);
+    v += dpp_f<DPP_XOR2>(v);
+    v += dpp_f<DPP_HALF_MIRROR>(v);
+    v += dpp_f<DPP_MIRROR>(v);
+    return v;
+  } else {
+    v = wave_sum_f(v);
+    if constexpr (L > WAVE) {
+      if ((threadIdx.x & (WAVE - 1)) == 0) scratch[threadIdx.x / WAVE] = v;
+      __syncthreads();
+      v = scratch[0];
+#pragma unroll
+      for (int i = 1; i < L / WAVE; ++i) v += scratch[i];
+    }
+    return v;
   }
 }
 
-__global__ __launch_bounds__(NO_T) void k_norm_dw(NormGradArgs a, bool bf16, bool wbf16) {
-  const int64_t k = (int64_t)blockIdx.x * NO_T + threadIdx.x;
+template <int L>
+struct NormShape {
+  static constexpr int T = L < 256 ? 256 : L;  // threads of a workgroup
+  static constexpr int ROWS = T / L;           // rows it has at once
+};
+
+template <int DT, int L, int NV, bool CENTER>
+__global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool wbf16) {
+  constexpr int ROWS = NormShape<L>::ROWS;
+  __shared__ float s_sum[2][16];
+  const int l = threadIdx.x % L;
+  const float inv = 1.0f / (float)a.K;
+  for (int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L; n < a.N; n += (int64_t)gridDim.x * ROWS) {
+    const char* row = (const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE;
+    RowVec<DT> x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i].template load_to<true>(row, 8 * (i * L + l), a.K);
+    float mu = 0.0f;
+    if constexpr (CENTER) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += x[i].at(j);
+      mu = row_sum<L>(s, s_sum[0]) * inv;
+    }
+    float q = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int left = a.K - 8 * (i * L + l);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = !CENTER ? x[i].at(j) : j < left ? x[i].at(j) - mu : 0.0f;
+        q = fma_f(c, c, q);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i].renew();
+    const float rstd = 1.0f / sqrtf(row_sum<L>(q, s_sum[1]) * inv + a.eps);
+    char* out = (char*)a.y + n * a.y_stride * RowVec<DT>::SIZE;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = 8 * (i * L + l);
+      float f[8], w[8], b[8];
+      param8(a.weight, wbf16, k, a.K, 1.0f, w);
+      param8(a.bias, wbf16, k, a.K, 0.0f, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = fma_f((x[i].at(j) - mu) * rstd, w[j], b[j]);
+      RowVec<DT> y;
+      y.set(f);
+      if (k < a.K) y.store_to(out, k, a.K);
+    }
+    if (l == 0) {
+      if (a.rstd) a.rstd[n] = rstd;
+      if (CENTER) a.mean[n] = mu;
+    }
+    if (!CENTER && L > WAVE) __syncthreads();  // (one place for the sums alone)
+  }
+}
+
+// PARAM 1: also the workgroup's sums of dy xh, to row blockIdx.x of `part` [grid][PARAM][K]; 2: of dy too.
+// (Past K dy is 0, so that nothing there counts.)
+template <int DT, int L, int NV, bool CENTER, int PARAM>
+__global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArgs a, bool wbf16, float* part) {
+  constexpr int ROWS = NormShape<L>::ROWS;
+  __shared__ float s_sum[2][2][16];
+  const int l = threadIdx.x % L;
+  const float inv = 1.0f / (float)a.K;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  RowVec<DT> nx[NV], ng[NV];
+  float nr = 0.0f, nm = 0.0f;
+  auto request = [&](int64_t n) {
+    const char* x = (const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE;
+    const char* g = (const char*)a.dy + n * a.dy_stride * RowVec<DT>::SIZE;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      nx[i].template load_to<true>(x, 8 * (i * L + l), a.K);
+      ng[i].template load_to<true>(g, 8 * (i * L + l), a.K);
+    }
+    nr = a.rstd[n];
+    if (CENTER) nm = a.mean[n];
+  };
+  int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
+  if (PARAM && n < a.N) request(n);
+  // (a row of its own for each workgroup: the weights are read where they are used)
+  float held[PARAM ? NV : 1][8], dw[PARAM > 0 ? NV : 1][8], db[PARAM > 1 ? NV : 1][8];
+  auto weight = [&](int i, float (&w)[8]) {
+    if constexpr (PARAM > 0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = held[i][j];
+    } else {
+      param8(a.weight, wbf16, 8 * (i * L + l), a.K, 1.0f, w);
+    }
+  };
+  if constexpr (PARAM > 0)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      param8(a.weight, wbf16, 8 * (i * L + l), a.K, 1.0f, held[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        dw[i][j] = 0.0f;
+        if (PARAM > 1) db[i][j] = 0.0f;
+      }
+    }
+  for (int turn = 0; n < a.N; n += step, turn ^= 1) {
+    if (!PARAM) request(n);
+    RowVec<DT> x[NV], g[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      g[i] = ng[i];
+    }
+    const float rstd = nr, mu = nm;
+    if (PARAM && n + step < a.N) request(n + step);
+    float c1 = 0.0f, c2 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float w[8];
+      weight(i, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float d = g[i].at(j), xh = (x[i].at(j) - mu) * rstd, h = d * w[j];
+        c1 = fma_f(h, xh, c1);
+        if (CENTER) c2 += h;
+        if constexpr (PARAM > 0) dw[i][j] = fma_f(d, xh, dw[i][j]);
+        if constexpr (PARAM > 1) db[i][j] += d;
+      }
+    }
+    if (!a.dx) continue;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i].renew();
+      g[i].renew();
+    }
+    // (both sums at one barrier)
+    if constexpr (L > WAVE) {
+      c1 = wave_sum_f(c1);
+      if (CENTER) c2 = wave_sum_f(c2);
+      float* s = s_sum[turn][0];
+      if ((threadIdx.x & (WAVE - 1)) == 0) {
+        s[threadIdx.x / WAVE] = c1;
+        s[16 + threadIdx.x / WAVE] = c2;
+      }
+      __syncthreads();
+      c1 = s[0];
+      c2 = s[16];
+#pragma unroll
+      for (int i = 1; i < L / WAVE; ++i) {
+        c1 += s[i];
+        c2 += s[16 + i];
+      }
+    } else {
+      c1 = row_sum<L>(c1, nullptr);
+      if (CENTER) c2 = row_sum<L>(c2, nullptr);
+    }
+    c1 *= inv;
+    c2 = CENTER ? c2 * inv : 0.0f;
+    char* out = (char*)a.dx + n * a.dx_stride * RowVec<DT>::SIZE;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int k = 8 * (i * L + l);
+      float w[8], d[8];
+      weight(i, w);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float xh = (x[i].at(j) - mu) * rstd, h = g[i].at(j) * w[j];
+        d[j] = rstd * (fma_f(-xh, c1, h) - c2);
+      }
+      RowVec<DT> y;
+      y.set(d);
+      if (k < a.K) y.store_to(out, k, a.K);
+    }
+  }
+  if constexpr (PARAM > 0) {
+    float* out = part + (int64_t)blockIdx.x * PARAM * a.K;
+    if constexpr (ROWS > 1) {
+      // the workgroup's rows first
+      __shared__ float s_acc[PARAM][ROWS][8 * L * NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          s_acc[0][threadIdx.x / L][8 * (i * L + l) + j] = dw[i][j];
+          if constexpr (PARAM > 1) s_acc[1][threadIdx.x / L][8 * (i * L + l) + j] = db[i][j];
+        }
+      __syncthreads();
+      for (int k = threadIdx.x; k < a.K; k += NormShape<L>::T)
+#pragma unroll
+        for (int h = 0; h < PARAM; ++h) {
+          float s = 0.0f;
+#pragma unroll
+          for (int q = 0; q < ROWS; ++q) s += s_acc[h][q][k];
+          out[h * a.K + k] = s;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int k = 8 * (i * L + l);
+        RowVec<STRIM_DTYPE_F32> v;
+        if (k >= a.K) continue;
+        v.set(dw[i]);
+        v.store_to((char*)out, k, a.K);
+        if constexpr (PARAM > 1) {
+          v.set(db[i]);
+          v.store_to((char*)(out + a.K), k, a.K);
+        }
+      }
+    }
+  }
+}
+
+// The weights' gradients alone, where a row is too wide to hold them beside it: eight columns a thread, the
+// rows dealt to gridDim.y parts.
+template <int DT, bool CENTER, int PARAM>
+__global__ __launch_bounds__(256) void k_norm_columns(const NormGradArgs a, float* part) {
+  const int k = 8 * (int)(blockIdx.x * 256 + threadIdx.x);
   if (k >= a.K) return;
-  float w = 0.0f, b = 0.0f;
-  for (int64_t n = 0; n < a.N; ++n) {
-    const float g = norm_at(a.dy, n * a.dy_stride + k, bf16);
-    w += g * ((norm_at(a.x, n * a.x_stride + k, bf16) - (a.mean ? a.mean[n] : 0.0f)) * a.rstd[n]);
-    b += g;
+  float dw[8] = {}, db[8] = {};
+#pragma unroll 4
+  for (int64_t n = blockIdx.y; n < a.N; n += gridDim.y) {
+    RowVec<DT> x, g;
+    x.template load_to<true>((const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE, k, a.K);
+    g.template load_to<true>((const char*)a.dy + n * a.dy_stride * RowVec<DT>::SIZE, k, a.K);
+    const float rstd = a.rstd[n], mu = CENTER ? a.mean[n] : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      dw[j] = fma_f(g.at(j), (x.at(j) - mu) * rstd, dw[j]);
+      if (PARAM > 1) db[j] += g.at(j);
+    }
   }
-  if (a.dw) norm_set(a.dw, k, w, wbf16);
-  if (a.db) norm_set(a.db, k, b, wbf16);
+  float* out = part + (int64_t)blockIdx.y * PARAM * a.K;
+  RowVec<STRIM_DTYPE_F32> v;
+  v.set(dw);
+  v.store_to((char*)out, k, a.K);
+  if constexpr (PARAM > 1) {
+    v.set(db);
+    v.store_to((char*)(out + a.K), k, a.K);
+  }
+}
+
+// dw and db from the workgroups' rows of `width` sums (K of dw, then K of db), added in order: 64 columns a
+// workgroup, its waves a part of the rows each.
+constexpr int NJ_T = 1024;
+__global__ __launch_bounds__(NJ_T) void k_norm_join(const float* part, int parts, int width, int K, void* dw,
+                                                    void* db, bool wbf16) {
+  __shared__ float s_sum[NJ_T / WAVE][WAVE];
+  const int lane = threadIdx.x & (WAVE - 1), wave = wave_id();
+  const int at = blockIdx.x * WAVE + lane;
+  float s = 0.0f;
+  if (at < width) {
+    const int each = (parts + NJ_T / WAVE - 1) / (NJ_T / WAVE);
+    const int end = min(parts, (wave + 1) * each);
+#pragma unroll 8
+    for (int p = wave * each; p < end; ++p) s += part[(int64_t)p * width + at];
+  }
+  s_sum[wave][lane] = s;
+  __syncthreads();
+  if (wave != 0 || at >= width) return;
+#pragma unroll
+  for (int i = 1; i < NJ_T / WAVE; ++i) s += s_sum[i][lane];
+  void* out = at < K ? dw : db;
+  const int k = at < K ? at : at - K;
+  if (!out) return;
+  if (wbf16) ((uint16_t*)out)[k] = __builtin_bit_cast(uint16_t, (__bf16)s);
+  else ((float*)out)[k] = s;
+}
+
+__global__ __launch_bounds__(256) void k_norm_zero(int K, void* dw, void* db, bool wbf16) {
+  const int k = blockIdx.x * 256 + threadIdx.x;
+  if (k >= K) return;
+  for (void* p : {dw, db})
+    if (p) {
+      if (wbf16) ((uint16_t*)p)[k] = 0;
+      else ((float*)p)[k] = 0.0f;
+    }
+}
+
+int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The threads that hold a row, and their vectors: f(L, NV).
+template <class F>
+void with_shape(int K, F f) {
+  using std::integral_constant;
+  auto go = [&](auto l, auto nv) { f(l, nv); };
+#define STRIM_SHAPE(L, NV) \
+  if (K <= 8 * L * NV) return go(integral_constant<int, L>{}, integral_constant<int, NV>{})
+  STRIM_SHAPE(16, 1);
+  STRIM_SHAPE(64, 1);
+  STRIM_SHAPE(256, 1);
+  STRIM_SHAPE(256, 2);
+  STRIM_SHAPE(256, 3);
+  STRIM_SHAPE(256, 4);
+  STRIM_SHAPE(1024, 2);
+  STRIM_SHAPE(1024, 4);
+  STRIM_SHAPE(1024, 8);
+#undef STRIM_SHAPE
+}
+constexpr int NO_WIDE = 8 * 256 * 4;  // columns past which the weights' gradients have a pass of their own
+int rows_at_once(int K) { return K <= 8 * 16 ? 16 : K <= 8 * 64 ? 4 : 1; }
+
+// Workgroups of the gradient's pass with the weights' sums: two a CU, or fewer with four rows each.
+int norm_parts(int N, int K) {
+  const int64_t groups = ceil_of(N, rows_at_once(K));
+  if (K > NO_WIDE) return (int)(groups < 64 ? groups : 64);
+  const int64_t most = rows_at_once(K) > 1 ? 1024 : 512;
+  int64_t g = ceil_of(groups, 4);
+  if (g < 128) g = groups < 128 ? groups : 128;
+  return (int)(g < most ? g : most);
+}
+
+template <class F>
+void with_dtype(bool bf16, F f) {
+  if (bf16) f(std::integral_constant<int, STRIM_DTYPE_BF16>{});
+  else f(std::integral_constant<int, STRIM_DTYPE_F32>{});
 }
 
 }  // namespace
 
 hipError_t launch_norm(const NormArgs& a, bool bf16, bool wbf16, hipStream_t st) {
-  hipLaunchKernelGGL(k_norm, dim3((unsigned)a.N), dim3(NO_T), 0, st, a, bf16, wbf16);
+  with_dtype(bf16, [&](auto dt) {
+    with_shape(a.K, [&](auto l, auto nv) {
+      constexpr int DT = decltype(dt)::value, L = decltype(l)::value, NV = decltype(nv)::value;
+      int64_t grid = ceil_of(a.N, NormShape<L>::ROWS);
+      if (grid > 1 << 20) grid = 1 << 20;
+      const dim3 g((unsigned)grid), t(NormShape<L>::T);
+      if (a.mean) hipLaunchKernelGGL((k_norm<DT, L, NV, true>), g, t, 0, st, a, wbf16);
+      else hipLaunchKernelGGL((k_norm<DT, L, NV, false>), g, t, 0, st, a, wbf16);
+    });
+  });
   return hipGetLastError();
 }
 
-int64_t norm_workspace(int, int, bool, bool) { return 0; }
+int64_t norm_workspace(int N, int K, bool want_w, bool want_b) {
+  return (int64_t)norm_parts(N, K) * (want_b ? 2 : want_w ? 1 : 0) * K * 4;
+}
 
-hipError_t launch_norm_grad(const NormGradArgs& a, bool bf16, bool wbf16, void*, hipStream_t st) {
-  if (a.dw || a.db)
-    hipLaunchKernelGGL(k_norm_dw, dim3((unsigned)((a.K + NO_T - 1) / NO_T)), dim3(NO_T), 0, st, a, bf16, wbf16);
-  if (a.dx && a.N > 0)
-    hipLaunchKernelGGL(k_norm_dx, dim3((unsigned)a.N), dim3(NO_T), 0, st, a, bf16, wbf16);
+hipError_t launch_norm_grad(const NormGradArgs& a, bool bf16, bool wbf16, void* workspace, hipStream_t st) {
+  const int param = a.db ? 2 : a.dw ? 1 : 0;  // rows of sums
+  if (a.N == 0) {
+    if (param)
+      hipLaunchKernelGGL(k_norm_zero, dim3((unsigned)ceil_of(a.K, 256)), dim3(256), 0, st, a.K, a.dw, a.db, wbf16);
+    return hipGetLastError();
+  }
+  float* part = (float*)workspace;
+  const int parts = norm_parts(a.N, a.K);
+  const bool wide = a.K > NO_WIDE;
+  with_dtype(bf16, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (param && wide) {  // (before dx: it may go where x or dy is)
+      const dim3 g((unsigned)ceil_of(a.K, 2048), (unsigned)parts);
+      auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, g, dim3(256), 0, st, a, part); };
+      if (a.mean) param > 1 ? go(k_norm_columns<DT, true, 2>) : go(k_norm_columns<DT, true, 1>);
+      else param > 1 ? go(k_norm_columns<DT, false, 2>) : go(k_norm_columns<DT, false, 1>);
+    }
+    if (wide && !a.dx) return;
+    with_shape(a.K, [&](auto l, auto nv) {
+      constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
+      const dim3 t(NormShape<L>::T);
+      auto go = [&](auto kernel, int64_t grid) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(grid < 1 << 20 ? grid : 1 << 20)), t, 0, st, a, wbf16, part);
+      };
+      if constexpr (L < 1024) {
+        if (param == 2) return a.mean ? go(k_norm_grad<DT, L, NV, true, 2>, parts) : go(k_norm_grad<DT, L, NV, false, 2>, parts);
+        if (param == 1) return a.mean ? go(k_norm_grad<DT, L, NV, true, 1>, parts) : go(k_norm_grad<DT, L, NV, false, 1>, parts);
+      }
+      const int64_t grid = ceil_of(a.N, NormShape<L>::ROWS);
+      a.mean ? go(k_norm_grad<DT, L, NV, true, 0>, grid) : go(k_norm_grad<DT, L, NV, false, 0>, grid);
+    });
+  });
+  if (param)
+    hipLaunchKernelGGL(k_norm_join, dim3((unsigned)ceil_of((int64_t)param * a.K, WAVE)), dim3(NJ_T), 0, st, part, parts,
+                       param * a.K, a.K, a.dw, a.db, wbf16);
   return hipGetLastError();
 }
 

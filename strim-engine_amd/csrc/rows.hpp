@@ -41,11 +41,12 @@ struct RowVec {
       for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
     }
   }
-  // tokens from v on that lie before V; -inf past them
+  // tokens from v on that lie before V; past them -inf, or 0
+  template <bool ZERO = false>
   __device__ __forceinline__ void load_to(const char* row, int v, int V) {
     if (v + 8 <= V) return load(row, v);
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) w[i] = DT == STRIM_DTYPE_BF16 ? 0xFF80FF80u : NINF_BITS;
+    for (int i = 0; i < WORDS; ++i) w[i] = ZERO ? 0u : DT == STRIM_DTYPE_BF16 ? 0xFF80FF80u : NINF_BITS;
     const char* p = row + (int64_t)v * SIZE;
 #pragma unroll
     for (int j = 0; j < 7; ++j)
@@ -57,6 +58,12 @@ struct RowVec {
           w[j] = ((const uint32_t*)p)[j];
         }
       }
+  }
+  // What was made of the words before is made anew after this (else the compiler keeps the tokens as floats
+  // from one pass over a row to the next, beside the words, until registers spill).
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
     if constexpr (DT == STRIM_DTYPE_BF16) {
