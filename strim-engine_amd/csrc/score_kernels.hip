@@ -23,15 +23,12 @@ constexpr int SC_T = TOP_T;                    // threads of a workgroup
 constexpr int SC_U = TOP_STEP * 2 / (8 * SC_T);  // vectors of eight tokens a lane has of a tile
 constexpr int SC_TILE = 8 * SC_U * SC_T;       // tokens a tile
 
-// What a part of a row leaves for the join: its statistics and up to ScoreParts::room keys.
-struct ScorePart {
-  RowStat st;
-  int32_t n;
-};
+// What a part of a row leaves for the join: its statistics and ScoreParts::room entries of its alternatives
+// (TOP_NONE past the last).
 struct ScoreParts {
   int32_t parts, tiles;  // parts of a row; tiles of a part
   int32_t room;
-  ScorePart* part;       // [R][parts]
+  RowStat* part;         // [R][parts]
   uint64_t* keys;        // [R][parts][room]
 };
 
@@ -42,27 +39,36 @@ __device__ __forceinline__ bool allowed_at(const uint32_t* mask, int v) {
   return !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
 }
 
-// The row's results from its statistics and the list that holds its first `top` keys.
+// A given token and its logit, -inf where the mask forbids it; the thread's own (S <= SC_T). Asked for before
+// the row's statistics are known.
+struct Given {
+  float x;
+  bool given, inside;
+};
 template <int DT>
-__device__ __forceinline__ void score_finish(const ScoreArgs& a, int64_t r, RowStat st, TopList* l, int n) {
+__device__ __forceinline__ Given given_of(const ScoreArgs& a, int64_t r) {
   const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
   const uint32_t* mask = a.mask ? a.mask + r * a.mask_stride : nullptr;
+  Given o{-INFINITY, false, false};
+  if ((int)threadIdx.x < a.S) {
+    const int t = a.tokens[r * a.S + threadIdx.x];
+    o.given = t != a.ignore_index;
+    o.inside = t >= 0 && t < a.V;
+    if (o.given && o.inside && allowed_at(mask, t)) o.x = token_at<DT>(row, t);
+  }
+  return o;
+}
+
+// The row's results from its statistics and the list that holds its first `top` keys.
+__device__ __forceinline__ void score_finish(const ScoreArgs& a, int64_t r, RowStat st, Given t, TopList* l, int n) {
   const float nan = __builtin_nanf("");
   const bool bad = !(st.s < INFINITY), empty = !bad && st.s == 0.0f;
   const float ls = logf(st.s);
   // (not from lse, which is rounded to the largest logit's spacing)
   auto logprob = [&](float x) { return (x - st.m) / a.T - ls; };
-  bool unknown = false;
-  for (int s = threadIdx.x; s < a.S; s += SC_T) {
-    const int t = a.tokens[r * a.S + s];
-    const bool given = t != a.ignore_index, inside = t >= 0 && t < a.V;
-    unknown |= given && !inside;
-    float lp = 0.0f;
-    if (given && inside)
-      lp = bad ? nan : empty || !allowed_at(mask, t) ? -INFINITY : logprob(token_at<DT>(row, t));
-    a.logprobs[r * a.S + s] = lp;
-  }
-  unknown = __syncthreads_or(unknown);
+  if ((int)threadIdx.x < a.S)
+    a.logprobs[r * a.S + threadIdx.x] = !(t.given && t.inside) ? 0.0f : bad ? nan : empty ? -INFINITY : logprob(t.x);
+  const bool unknown = a.status && __syncthreads_or(t.given && !t.inside);
   if (threadIdx.x == 0) {
     a.entropy[r] = bad ? nan : empty ? 0.0f : ls - st.u / st.s / a.T;
     a.lse[r] = bad ? nan : empty ? -INFINITY : st.m / a.T + ls;
@@ -95,7 +101,7 @@ __device__ __forceinline__ RowStat stat_block(RowStat st, float c, RowStat* scra
 }
 
 template <int DT, bool MASK, bool TOP>
-__global__ __launch_bounds__(SC_T) void k_scores(const ScoreArgs a, const ScoreParts q) {
+__global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores(const ScoreArgs a, const ScoreParts q) {
   __shared__ RowStat s_stat[SC_T / WAVE];
   __shared__ std::conditional_t<TOP, TopList, char> s_list;
   TopList* const s_top = (TopList*)&s_list;  // (unused without TOP)
@@ -120,36 +126,56 @@ __global__ __launch_bounds__(SC_T) void k_scores(const ScoreArgs a, const ScoreP
   TopRun top;
   if constexpr (TOP) top.init(s_top[0], a.top);
   RowStat st{-INFINITY, 0.0f, 0.0f};
-  for (int t = t0; t < t1; t += SC_TILE) {
-    float x[8 * SC_U], mx = -INFINITY;
+  for (int t = t0; t < t1;) {
+    bool fits = true;
+    for (; fits && t < t1; t += SC_TILE) {
+      float x[8 * SC_U], mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < SC_U; ++u)
+      for (int u = 0; u < SC_U; ++u)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        float f = next[u].at(j);
-        if (MASK) f = (ok[u] >> j) & 1u ? f : -INFINITY;
-        x[8 * u + j] = f;
-        mx = fmaxf(mx, f);
+        for (int j = 0; j < 8; ++j) {
+          float f = next[u].at(j);
+          if (MASK) f = (ok[u] >> j) & 1u ? f : -INFINITY;
+          x[8 * u + j] = f;
+          mx = fmaxf(mx, f);
+        }
+      if (t + SC_TILE < t1) request(t + SC_TILE);
+      stat_add<8 * SC_U, true>(st, x, mx, c);
+      if constexpr (TOP) fits = top.add<SC_U>(s_top[0], x, mx, st.m, t + 8 * (int)threadIdx.x);
+    }
+    if constexpr (TOP)
+      if (!fits) {  // the last tile again, slot by slot (out of the loop, for its registers' sake)
+        const int s = t - SC_TILE;
+        top_slots<SC_U>(s_top[0], top, s + 8 * (int)threadIdx.x, [&](int u, float (&x)[8]) {
+          const int v = s + 8 * (u * SC_T + (int)threadIdx.x);
+          RowVec<DT> q;
+          uint32_t in = 0;
+          if (v < a.V) {
+            q.load_to(row, v, a.V);
+            in = MASK ? allowed8(mask, v, a.V) : 0xFFu;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = (in >> j) & 1u ? q.at(j) : -INFINITY;
+        });
       }
-    if (t + SC_TILE < t1) request(t + SC_TILE);
-    stat_add<8 * SC_U, true>(st, x, mx, c);
-    if constexpr (TOP) top.add<SC_U>(s_top[0], x, mx, st.m, t + 8 * (int)threadIdx.x);
   }
   const float most = st.m;
+  Given given{};
+  if (q.parts == 1) given = given_of<DT>(a, r);
   st = stat_block(st, c, s_stat);
+  if constexpr (TOP) top.trim(s_top[0], most);
+  if (q.parts == 1) return score_finish(a, r, st, given, TOP ? s_top : nullptr, TOP ? top.held : 0);
+  if (threadIdx.x == 0) q.part[r * q.parts + p] = st;
   if constexpr (TOP) {
-    top.trim(s_top[0], most);
-    if (q.parts > 1) {
-      uint32_t unused = 0;
-      if (top.held > q.room) top.held = top_reduce(s_top[0], top.held, a.top, unused);
-      uint64_t* out = q.keys + (r * q.parts + p) * q.room;
-      for (int i = threadIdx.x; i < top.held; i += SC_T) out[i] = s_top[0].key[i];
-    }
-  }
-  if (q.parts > 1) {
-    if (threadIdx.x == 0) q.part[r * q.parts + p] = ScorePart{st, TOP ? top.held : 0};
-  } else {
-    score_finish<DT>(a, r, st, TOP ? s_top : nullptr, TOP ? top.held : 0);
+    uint64_t* out = q.keys + (r * q.parts + p) * q.room;
+    const int n = min(top.held, q.room);
+    if (top.held <= q.room)
+      for (int i = threadIdx.x; i < n; i += SC_T) out[i] = s_top[0].e[i];
+    else
+      top_order(s_top[0], top.held, q.room, [&](int k, uint64_t key) {
+        out[k] = top_entry(fkey_desc_inv((uint32_t)(key >> 32)), (int32_t)(uint32_t)key);
+      });
+    for (int i = n + (int)threadIdx.x; i < q.room; i += SC_T) out[i] = TOP_NONE;
   }
 }
 
@@ -158,48 +184,53 @@ __global__ __launch_bounds__(SC_T) void k_scores_join(const ScoreArgs a, const S
   __shared__ RowStat s_stat[SC_T / WAVE];
   __shared__ std::conditional_t<TOP, TopList, char> s_list;
   TopList* const s_top = (TopList*)&s_list;  // (unused without TOP)
-  __shared__ int s_n[TOP ? SC_T : 1];
+  constexpr int Q = TOP_STEP / SC_T;         // entries a thread takes at a time
   const int64_t r = blockIdx.x;
   const float c = LOG2E / a.T;
   RowStat st{-INFINITY, 0.0f, 0.0f};
-  if constexpr (TOP) s_n[threadIdx.x] = 0;
-  if ((int)threadIdx.x < q.parts) {
-    const ScorePart o = q.part[r * q.parts + threadIdx.x];
-    st = o.st;
-    if constexpr (TOP) s_n[threadIdx.x] = o.n;
-  }
+  if ((int)threadIdx.x < q.parts) st = q.part[r * q.parts + threadIdx.x];
+  const uint64_t* keys = q.keys + r * q.parts * q.room;
+  const int all = TOP ? q.parts * q.room : 0;
+  uint64_t k[Q];
+  auto request = [&](int i0) {
+#pragma unroll
+    for (int i = 0; i < Q; ++i) {
+      const int at = i0 + i * SC_T + (int)threadIdx.x;
+      k[i] = at < all ? keys[at] : TOP_NONE;
+    }
+  };
+  if constexpr (TOP) request(0);
+  const Given given = given_of<DT>(a, r);
   st = stat_block(st, c, s_stat);
   int n = 0;
   if constexpr (TOP) {
-    const uint64_t* keys = q.keys + r * q.parts * q.room;
-    const int all = q.parts * q.room;
-    auto key_at = [&](int i) {
-      const int p = i / q.room;
-      return i < all && i - p * q.room < s_n[p] ? keys[i] : ~0ull;
-    };
-    uint64_t best = ~0ull;
-    for (int i = threadIdx.x; i < all; i += SC_T) best = min(best, key_at(i));
-    const uint32_t t = top_threshold(s_top[0], (uint32_t)(best >> 32), a.top);
-    uint64_t limit = (uint64_t)t << 32 | 0xFFFFFFFFu;
+    uint32_t best = ~0u;
+    for (int i0 = 0; i0 < all; i0 += TOP_STEP) {
+      if (i0 > 0) request(i0);
+#pragma unroll
+      for (int i = 0; i < Q; ++i) best = min(best, fkey_desc(__uint_as_float((uint32_t)(k[i] >> 32))));
+    }
+    const uint32_t t = top_threshold(s_top[0], best, TOP_ALL, a.top, 0);
+    const float floor = fkey_desc_inv(t);
     if (threadIdx.x == 0) s_top[0].n = 0;
     __syncthreads();
     for (int i0 = 0; i0 < all; i0 += TOP_STEP) {
+      if (all > TOP_STEP) request(i0);
       if (n > TOP_T) {  // (lists full of ties)
         uint32_t unused = 0;
         n = top_reduce(s_top[0], n, a.top, unused);
         if (threadIdx.x == 0) s_top[0].n = n;
         __syncthreads();
       }
-      for (int i = i0 + (int)threadIdx.x; i < min(all, i0 + TOP_STEP); i += SC_T) {
-        const uint64_t k = key_at(i);
-        if (k <= limit) s_top[0].key[atomicAdd(&s_top[0].n, 1)] = k;
-      }
+#pragma unroll
+      for (int i = 0; i < Q; ++i)
+        if (__uint_as_float((uint32_t)(k[i] >> 32)) >= floor) s_top[0].e[atomicAdd(&s_top[0].n, 1)] = k[i];
       __syncthreads();
       n = __builtin_amdgcn_readfirstlane(s_top[0].n);
       __syncthreads();
     }
   }
-  score_finish<DT>(a, r, st, TOP ? s_top : nullptr, n);
+  score_finish(a, r, st, given, TOP ? s_top : nullptr, n);
 }
 
 // The gradient: G = sum of the tokens' gradients, then d = p (gL - G - gH (log p + H)) / T everywhere and
@@ -276,13 +307,14 @@ __global__ __launch_bounds__(SC_T) void k_scores_grad(const ScoreGradArgs a, int
 int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Parts of a row: about eight workgroups a CU in all, one a row where there are that many.
+// Parts of a row: as many workgroups in all as the chip holds at once (eight a CU), one a row where there
+// are that many rows.
 ScoreParts score_parts(int R, int V, int top) {
   ScoreParts q{};
-  const int64_t tiles = ceil_of(V, SC_TILE), each = (int64_t)R * tiles / 2048;
-  q.tiles = (int32_t)(each < 1 ? 1 : each > tiles ? tiles : each);
+  const int64_t tiles = ceil_of(V, SC_TILE), each = ceil_of((int64_t)R * tiles, 2048);
+  q.tiles = (int32_t)(each > tiles ? tiles : each);
   q.parts = (int32_t)ceil_of(tiles, q.tiles);
-  q.room = 2 * top;
+  q.room = top == 0 ? 0 : 2 * top > 32 ? 2 * top : 32;
   return q;
 }
 
@@ -291,14 +323,14 @@ ScoreParts score_parts(int R, int V, int top) {
 int64_t scores_workspace(int R, int V, int top) {
   const ScoreParts q = score_parts(R, V, top);
   if (q.parts == 1) return 0;
-  return up16((int64_t)R * q.parts * (int64_t)sizeof(ScorePart)) + (int64_t)R * q.parts * q.room * 8;
+  return up16((int64_t)R * q.parts * (int64_t)sizeof(RowStat)) + (int64_t)R * q.parts * q.room * 8;
 }
 
 hipError_t launch_scores(const ScoreArgs& a, bool bf16, void* workspace, hipStream_t st) {
   ScoreParts q = score_parts(a.R, a.V, a.top);
   if (q.parts > 1) {
-    q.part = (ScorePart*)workspace;
-    q.keys = (uint64_t*)((char*)workspace + up16((int64_t)a.R * q.parts * (int64_t)sizeof(ScorePart)));
+    q.part = (RowStat*)workspace;
+    q.keys = (uint64_t*)((char*)workspace + up16((int64_t)a.R * q.parts * (int64_t)sizeof(RowStat)));
   }
   const dim3 grid((unsigned)((int64_t)a.R * q.parts)), threads(SC_T);
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, threads, 0, st, a, q); };
