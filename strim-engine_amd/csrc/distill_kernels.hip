@@ -340,6 +340,7 @@ __global__ __launch_bounds__(DI_T) void k_distill_join(const DistillArgs a, cons
   RowStat st{-INFINITY, 0.0f, 0.0f};
   for (int p = lane; p < q.parts; p += WAVE) stat_merge(st, q.part[r * q.parts + p], c);
   stat_wave(st, c);
+  stat_exact(st, c);
   const Alternatives o = alternatives_of(a, r);
   RowNumbers n{0.0, 0.0, 0.0, 0.0};
   if (o.any) {
@@ -460,6 +461,7 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
   if (wave == 0) {
     st = lane < NWAVES ? s_stat[lane] : RowStat{-INFINITY, 0.0f, 0.0f};
     stat_wave(st, c);
+    stat_exact(st, c);
     const Teacher t = teacher_of(o, TAIL);
     const double w = (double)a.weights[r] / a.T;
     bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};

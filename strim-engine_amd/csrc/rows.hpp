@@ -103,17 +103,22 @@ __device__ __forceinline__ float wave_sum_f(float v) {
   return v;
 }
 
-// Over some of a row's tokens: m the largest x, s = sum exp((x - m) / T), u = sum (x - m) exp((x - m) / T).
-// Without a token above -inf m is -inf, s = u = 0; a NaN or +inf makes s NaN. c = log2(e) / T throughout.
+// Over some of a row's tokens: m the largest x, s = sum 2^y, u = sum y 2^y, with y = x c - b and c = log2(e) /
+// T throughout. While tokens are added b is m c as it is rounded, so that a token costs one fused multiply-add;
+// the rounding is the same for all of them, and stat_exact takes it out again (then y = (x - m) c). Without a
+// token above -inf m is -inf, s = u = 0; a NaN or +inf makes s NaN.
 struct RowStat {
   float m, s, u;
 };
 __device__ __forceinline__ float stat_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-// a's sums relative to `top` >= a.m. (The difference is bounded: the type's lowest value lies 3.4e38
-// below zero, and u times a vanishing factor would be an infinity times 0.)
+// (past this m c or its difference to x c may be infinite: there y = (x - m) c from the start)
+__device__ __forceinline__ bool stat_far(float ref) { return !(fabsf(ref) <= 1e30f); }
+// a's sums for the maximum `top` >= a.m. (y is bounded: the type's lowest value lies 3.4e38 below zero, and u
+// times a vanishing factor would be an infinity times 0.)
 __device__ __forceinline__ void stat_rebase(RowStat& a, float top, float c) {
-  const float d = a.m - stat_ref(top), f = hw_exp2(d * c), near = fmaxf(d, -1e30f);
-  a.u = a.s == 0.0f ? 0.0f : fma_f(near, a.s, a.u) * f;
+  const float ref = stat_ref(top);
+  const float d = stat_far(ref) ? (a.m - ref) * c : a.m * c - ref * c, f = hw_exp2(d);
+  a.u = a.s == 0.0f ? 0.0f : fma_f(fmaxf(d, -1e30f), a.s, a.u) * f;
   a.s = a.s == 0.0f ? 0.0f : a.s * f;
   a.m = top;
 }
@@ -129,11 +134,18 @@ template <int E, bool U>
 __device__ __forceinline__ void stat_add(RowStat& a, const float (&x)[E], float mx, float c) {
   if (mx > a.m) stat_rebase(a, mx, c);
   const float ref = stat_ref(a.m);
-#pragma unroll
-  for (int j = 0; j < E; ++j) {
-    const float d = x[j] - ref, e = hw_exp2(d * c);  // (a NaN goes through to s)
+  auto one = [&](float y) {
+    const float e = hw_exp2(y);  // (a NaN goes through to s)
     a.s += e;
-    if (U) a.u = fma_f(fmaxf(d, -1e30f), e, a.u);
+    if (U) a.u = fma_f(fmaxf(y, -1e30f), e, a.u);
+  };
+  if (!stat_far(ref)) {
+    const float b = -(ref * c);
+#pragma unroll
+    for (int j = 0; j < E; ++j) one(fma_f(x[j], c, b));
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j) one((x[j] - ref) * c);
   }
 }
 // The wave's statistics in every lane.
@@ -141,6 +153,15 @@ __device__ __forceinline__ void stat_wave(RowStat& a, float c) {
   stat_rebase(a, wave_max_f(a.m), c);
   a.s = wave_sum_f(a.s);
   a.u = wave_sum_f(a.u);
+}
+// After the last merge.
+__device__ __forceinline__ void stat_exact(RowStat& a, float c) {
+  const float ref = stat_ref(a.m);
+  if (stat_far(ref)) return;
+  const float off = fma_f(ref, c, -(ref * c));  // m c past its rounding
+  const float f = hw_exp2(-off);
+  a.u = (a.u - off * a.s) * f;
+  a.s *= f;
 }
 
 }  // namespace strim

@@ -4,8 +4,8 @@
 //   logprob[t] = z[t] - lse,  H = -sum_v p log p with p = exp(z - lse),  the first `top` ids in token order
 //   dx[v] = 1/T (sum_s g[s] ([v = t_s] - p[v]) - gH p[v] (log p[v] + H) + gL p[v])
 //
-// k_scores reads the logits once: per lane the running maximum m, s = sum exp((x - m) / T) and u = sum
-// (x - m) exp((x - m) / T), from which lse = m / T + log s and H = log s - u / (s T), and the row's
+// k_scores reads the logits once: per lane the running maximum m, s = sum 2^y and u = sum y 2^y with y =
+// (x - m) log2(e) / T, from which lse = m / T + log s and H = log s - log(2) u / s, and the row's
 // alternatives (top.hpp). A row is one workgroup's where there are many, else in parts that
 // k_scores_join merges.
 #include <type_traits>
@@ -70,7 +70,7 @@ __device__ __forceinline__ void score_finish(const ScoreArgs& a, int64_t r, RowS
     a.logprobs[r * a.S + threadIdx.x] = !(t.given && t.inside) ? 0.0f : bad ? nan : empty ? -INFINITY : logprob(t.x);
   const bool unknown = a.status && __syncthreads_or(t.given && !t.inside);
   if (threadIdx.x == 0) {
-    a.entropy[r] = bad ? nan : empty ? 0.0f : ls - st.u / st.s / a.T;
+    a.entropy[r] = bad ? nan : empty ? 0.0f : ls - 0.69314718055994531f * (st.u / st.s);
     a.lse[r] = bad ? nan : empty ? -INFINITY : st.m / a.T + ls;
     if (a.status)
       a.status[r] = bad ? STRIM_ENONFINITE : empty ? STRIM_EEMPTY : unknown ? STRIM_EINVAL : STRIM_OK;
@@ -129,19 +129,25 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
   for (int t = t0; t < t1;) {
     bool fits = true;
     for (; fits && t < t1; t += SC_TILE) {
-      float x[8 * SC_U], mx = -INFINITY;
+      float x[8 * SC_U], mv[SC_U], mx = -INFINITY;
 #pragma unroll
-      for (int u = 0; u < SC_U; ++u)
+      for (int u = 0; u < SC_U; ++u) {
+        mv[u] = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float f = next[u].at(j);
           if (MASK) f = (ok[u] >> j) & 1u ? f : -INFINITY;
           x[8 * u + j] = f;
-          mx = fmaxf(mx, f);
+          mv[u] = fmaxf(mv[u], f);
         }
+        mx = fmaxf(mx, mv[u]);
+      }
+      // (requested into the registers that the tokens leave)
+#pragma unroll
+      for (int j = 0; j < 8 * SC_U; ++j) asm volatile("" : "+v"(x[j]));
       if (t + SC_TILE < t1) request(t + SC_TILE);
       stat_add<8 * SC_U, true>(st, x, mx, c);
-      if constexpr (TOP) fits = top.add<SC_U>(s_top[0], x, mx, st.m, t + 8 * (int)threadIdx.x);
+      if constexpr (TOP) fits = top.add<SC_U>(s_top[0], x, mv, st.m, t + 8 * (int)threadIdx.x);
     }
     if constexpr (TOP)
       if (!fits) {  // the last tile again, slot by slot (out of the loop, for its registers' sake)
@@ -164,7 +170,10 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
   if (q.parts == 1) given = given_of<DT>(a, r);
   st = stat_block(st, c, s_stat);
   if constexpr (TOP) top.trim(s_top[0], most);
-  if (q.parts == 1) return score_finish(a, r, st, given, TOP ? s_top : nullptr, TOP ? top.held : 0);
+  if (q.parts == 1) {
+    stat_exact(st, c);
+    return score_finish(a, r, st, given, TOP ? s_top : nullptr, TOP ? top.held : 0);
+  }
   if (threadIdx.x == 0) q.part[r * q.parts + p] = st;
   if constexpr (TOP) {
     uint64_t* out = q.keys + (r * q.parts + p) * q.room;
@@ -230,6 +239,7 @@ __global__ __launch_bounds__(SC_T) void k_scores_join(const ScoreArgs a, const S
       __syncthreads();
     }
   }
+  stat_exact(st, c);
   score_finish(a, r, st, given, TOP ? s_top : nullptr, n);
 }
 

@@ -152,36 +152,38 @@ struct TopRun {
   }
 
   // A tile of U slots of TOP_STEP tokens, eight a thread: x[8 u ..] are the thread's of slot u, from id
-  // first + u TOP_STEP on; mx is their maximum, `most` the largest that the thread has met. False where more
-  // were to be appended than the list holds: the tile is then given to top_slots.
+  // first + u TOP_STEP on; mv[u] is their maximum, `most` the largest that the thread has met. False where
+  // more were to be appended than the list holds: the tile is then given to top_slots.
   template <int U>
-  __device__ __forceinline__ bool add(TopList& l, const float (&x)[8 * U], float mx, float most, int first) {
+  __device__ __forceinline__ bool add(TopList& l, const float (&x)[8 * U], const float (&mv)[U], float most, int first) {
     const bool raise = ((tile + 1) & tile) == 0;
     before = limit;
     if (raise) limit = top_threshold(l, fkey_desc(most), limit, M, by);
     const float floor = fkey_desc_inv(limit);
     int* added = &l.added[tile % 3];
     if (threadIdx.x == 0) l.added[(tile + 1) % 3] = 0;
-    if (__ballot(mx >= floor)) {
-      // one atomic a wave: its lanes' places follow from the ballots
-      uint64_t m[8 * U];
-      int n = 0;
 #pragma unroll
-      for (int j = 0; j < 8 * U; ++j) {
-        m[j] = __ballot(x[j] >= floor);
-        n += __popcll(m[j]);
-      }
-      int at = 0;
-      if ((threadIdx.x & (WAVE - 1)) == 0) at = atomicAdd(added, n);
-      at = held + __builtin_amdgcn_readfirstlane(at);
+    for (int u = 0; u < U; ++u)
+      if (__ballot(mv[u] >= floor)) {
+        // one atomic for the wave's tokens: its lanes' places follow from the ballots
+        uint64_t m[8];
+        int n = 0;
 #pragma unroll
-      for (int j = 0; j < 8 * U; ++j)
-        if (m[j]) {
-          const int to = at + lanes_below(m[j]);
-          if (x[j] >= floor && to < TOP_CAP) l.e[to] = top_entry(x[j], first + (j >> 3) * TOP_STEP + (j & 7));
-          at += __popcll(m[j]);
+        for (int j = 0; j < 8; ++j) {
+          m[j] = __ballot(x[8 * u + j] >= floor);
+          n += __popcll(m[j]);
         }
-    }
+        int at = 0;
+        if ((threadIdx.x & (WAVE - 1)) == 0) at = atomicAdd(added, n);
+        at = held + __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (m[j]) {
+            const int to = at + lanes_below(m[j]);
+            if (x[8 * u + j] >= floor && to < TOP_CAP) l.e[to] = top_entry(x[8 * u + j], first + u * TOP_STEP + j);
+            at += __popcll(m[j]);
+          }
+      }
     __syncthreads();
     const int more = __builtin_amdgcn_readfirstlane(*added);
     ++tile;
