@@ -54,7 +54,7 @@ __device__ __forceinline__ Alternatives alternatives_of(const DistillArgs& a, in
 
 // Each entry that is among the wave's 512 tokens from w0 on, in the list's order: f(lane, element, entry's
 // lane, i).
-template <class F>
+template <int DT, class F>
 __device__ __forceinline__ void each_hit(const int (&id)[2], int w0, F f) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -63,14 +63,14 @@ __device__ __forceinline__ void each_hit(const int (&id)[2], int w0, F f) {
       const int l = __builtin_ctzll(hit);
       hit &= hit - 1;
       const int off = rl_i(id[i], l) - w0;
-      f(off >> 3, off & 7, l, i);
+      f(RowVec<DT>::lane_of(off), RowVec<DT>::element_of(off), l, i);
     }
   }
 }
 template <int DT>
 __device__ __forceinline__ void without_hits(float (&x)[8], const int (&id)[2], int w0) {
   const int lane = threadIdx.x & (WAVE - 1);
-  each_hit(id, w0, [&](int at, int e, int, int) {
+  each_hit<DT>(id, w0, [&](int at, int e, int, int) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (lane == at && j == e) x[j] = -INFINITY;
@@ -211,7 +211,7 @@ __device__ __forceinline__ RowVec<DT> grad_of(const RowVec<DT>& x, const GradRow
   for (int i = 0; i < RowVec<DT>::WORDS; ++i)
     y.w[i] ^= DT == STRIM_DTYPE_BF16 ? g.sign : g.sign & 0x80000000u;
   if (hits)
-    each_hit(id, w0, [&](int at, int e, int l, int i) {
+    each_hit<DT>(id, w0, [&](int at, int e, int l, int i) {
       const float less = rl_f(p[i], l);
       // (masks, not an index: words that are indexed at run time are put into memory)
       const int word = DT == STRIM_DTYPE_BF16 ? e >> 1 : e;
@@ -283,7 +283,7 @@ template <int DT, bool TAIL>
 __global__ __launch_bounds__(DI_T) void k_distill_stat(const DistillArgs a, const DistillParts q) {
   __shared__ RowStat s_stat[DI_T / WAVE];
   const int64_t r = blockIdx.x / q.parts;
-  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1);
+  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1), wave = wave_id();
   const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
   const float c = LOG2E / a.T;
   const int t0 = p * q.tiles * DI_TILE, t1 = min(a.V, t0 + q.tiles * DI_TILE);
@@ -291,9 +291,9 @@ __global__ __launch_bounds__(DI_T) void k_distill_stat(const DistillArgs a, cons
   auto request = [&](int t) {
 #pragma unroll
     for (int u = 0; u < DI_U; ++u) {
-      const int v = t + 8 * (u * DI_T + (int)threadIdx.x);
-      if (t + DI_TILE <= a.V) next[u].load(row, v);
-      else next[u].load_to(row, v, a.V);
+      const int w0 = t + 8 * WAVE * (u * (DI_T / WAVE) + wave);
+      if (t + DI_TILE <= a.V) next[u].template load<true>(row, w0, lane);
+      else next[u].load_to(row, w0, lane, a.V);
     }
   };
   request(t0);
@@ -310,7 +310,7 @@ __global__ __launch_bounds__(DI_T) void k_distill_stat(const DistillArgs a, cons
     if constexpr (TAIL)
 #pragma unroll
       for (int u = 0; u < DI_U; ++u)
-        each_hit(o.id, t + 8 * (u * DI_T + (int)threadIdx.x - lane), [&](int at, int e, int, int) {
+        each_hit<DT>(o.id, t + 8 * WAVE * (u * (DI_T / WAVE) + wave), [&](int at, int e, int, int) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (lane == at && j == e) x[8 * u + j] = -INFINITY;
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
   __shared__ GradList s_list;
   __shared__ GradRow s_grad;
   const int64_t r = blockIdx.x / q.parts;
-  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1);
+  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1), wave = wave_id();
   const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
   char* out = (char*)a.d_logits + r * a.d_stride * RowVec<DT>::SIZE;
   const float c = LOG2E / a.T;
@@ -375,8 +375,7 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
   auto request = [&](int t) {
 #pragma unroll
     for (int u = 0; u < DI_U; ++u) {
-      const int v = t + 8 * (u * DI_T + (int)threadIdx.x);
-      if (v < a.V) next[u].load_to(row, v, a.V);
+      next[u].template load_to<false, true>(row, t + 8 * WAVE * (u * (DI_T / WAVE) + wave), lane, a.V);
     }
   };
   request(t0);
@@ -403,10 +402,9 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
     if (s + DI_TILE < t1) request(s + DI_TILE);
 #pragma unroll
     for (int u = 0; u < DI_U; ++u) {
-      const int w0 = __builtin_amdgcn_readfirstlane(s + 8 * (u * DI_T + (int)threadIdx.x - lane));
+      const int w0 = s + 8 * WAVE * (u * (DI_T / WAVE) + wave);
       if (w0 >= a.V) break;
-      const RowVec<DT> y = grad_of<DT>(x[u], g, c, id, less, w0, true);
-      if (w0 + 8 * lane < a.V) y.store_to(out, w0 + 8 * lane, a.V);
+      grad_of<DT>(x[u], g, c, id, less, w0, true).store_to(out, w0, lane, a.V, a.stream);
     }
   }
 }
@@ -426,7 +424,7 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
   const float c = LOG2E / a.T;
   RowVec<DT> x[NV];
 #pragma unroll
-  for (int u = 0; u < NV; ++u) x[u].load_to(row, 8 * (u * T + (int)threadIdx.x), a.V);
+  for (int u = 0; u < NV; ++u) x[u].template load_to<false, true>(row, 8 * WAVE * (u * NWAVES + wave), lane, a.V);
   const Alternatives o = alternatives_of(a, r);
   find_repeats<T>(s_list, o);
   // the vectors among which the wave's alternatives are
@@ -452,7 +450,7 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
   }
   for (int v0 = 8 * NV * T; v0 < a.V; v0 += 8 * T) {
     RowVec<DT> q;
-    q.load_to(row, v0 + 8 * (int)threadIdx.x, a.V);
+    q.load_to(row, v0 + 8 * WAVE * wave, lane, a.V);
     add(q, v0 + 8 * WAVE * wave, true);
   }
   stat_wave(st, c);
@@ -489,16 +487,13 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     const int w0 = 8 * WAVE * (u * NWAVES + wave);
-    if (w0 < a.V) {
-      const RowVec<DT> y = grad_of<DT>(x[u], g, c, id, less, w0, (hits >> u) & 1u);
-      if (w0 + 8 * lane < a.V) y.store_to(out, w0 + 8 * lane, a.V);
-    }
+    if (w0 < a.V)
+      grad_of<DT>(x[u], g, c, id, less, w0, (hits >> u) & 1u).store_to(out, w0, lane, a.V, a.stream);
   }
   for (int w0 = 8 * (NV * T + WAVE * wave); w0 < a.V; w0 += 8 * T) {
     RowVec<DT> q;
-    q.load_to(row, w0 + 8 * lane, a.V);
-    const RowVec<DT> y = grad_of<DT>(q, g, c, id, less, w0, true);
-    if (w0 + 8 * lane < a.V) y.store_to(out, w0 + 8 * lane, a.V);
+    q.load_to(row, w0, lane, a.V);
+    grad_of<DT>(q, g, c, id, less, w0, true).store_to(out, w0, lane, a.V, a.stream);
   }
 }
 
@@ -582,6 +577,7 @@ int64_t distill_workspace(int N, int V, int M, bool step) {
 hipError_t launch_distill(const DistillArgs& given, bool bf16, bool loss, bool grad, void* workspace,
                           hipStream_t st) {
   DistillArgs a = given;
+  a.stream = grad && (int64_t)a.N * a.V * (bf16 ? 2 : 4) > ROWS_CACHED;
   if (loss && grad && a.N >= DI_WHOLE) {
     with_dtype(bf16, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;

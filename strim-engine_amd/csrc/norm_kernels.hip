@@ -20,21 +20,66 @@ namespace strim {
 
 namespace {
 
-// Elements k .. k + 7 of a weight or bias of either type; `none` where there is no tensor, 0 past K.
-__device__ __forceinline__ void param8(const void* p, bool bf16, int k, int K, float none, float (&f)[8]) {
+// A lane's eight columns from k0 on, as RowVec<DT, G> has a row's: of a weight or bias of either type (`none`
+// where there is no tensor, 0 past K), and of a float32 row of sums.
+template <int DT, int G>
+__device__ __forceinline__ void param8(const void* p, bool bf16, int k0, int lane, int K, float none, float (&f)[8]) {
+  typedef RowVec<DT, G> X;
 #pragma unroll
   for (int j = 0; j < 8; ++j) f[j] = none;
   if (!p) return;
-  if (bf16) {
-    RowVec<STRIM_DTYPE_BF16> v;
-    v.load_to<true>((const char*)p, k, K);
+  if (bf16 == X::BF16) {
+    X v;
+    v.template load_to<true>((const char*)p, k0, lane, K);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = v.at(j);
+    return;
+  }
+  const int k = k0 + X::first(lane);
+  if (k + X::step(7) < K) {
+    if constexpr (X::BF16) {  // float32 weights beside bf16 rows
+      const ru32x4_any* a = (const ru32x4_any*)((const float*)p + k);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(a[j >> 2][j & 3]);
+    } else {  // bf16 weights beside float32 rows
+      typedef uint32_t pair_any __attribute__((ext_vector_type(2), aligned(2)));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const pair_any q = *(const pair_any*)((const uint16_t*)p + k + X::step(4 * i));
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          f[4 * i + j] = __uint_as_float(j & 1 ? q[j >> 1] & 0xFFFF0000u : q[j >> 1] << 16);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    f[j] = 0.0f;
+    const int at = k + X::step(j);
+    if (at < K) f[j] = bf16 ? bf16_to_f32(((const uint16_t*)p)[at]) : ((const float*)p)[at];
+  }
+}
+template <int DT, int G>
+__device__ __forceinline__ void sums8(float* out, int k0, int lane, int K, const float (&f)[8]) {
+  typedef RowVec<DT, G> X;
+  if constexpr (!X::BF16) {
+    X v;
+    v.set(f);
+    v.store_to((char*)out, k0, lane, K);
   } else {
-    RowVec<STRIM_DTYPE_F32> v;
-    v.load_to<true>((const char*)p, k, K);
+    const int k = k0 + 8 * lane;
+    if (k + 8 <= K) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = v.at(j);
+      for (int i = 0; i < 2; ++i)
+        *(ru32x4_any*)(out + k + 4 * i) =
+            ru32x4{__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]),
+                   __float_as_uint(f[4 * i + 3])};
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < K) out[k + j] = f[j];
   }
 }
 
@@ -65,19 +110,21 @@ template <int L>
 struct NormShape {
   static constexpr int T = L < 256 ? 256 : L;  // threads of a workgroup
   static constexpr int ROWS = T / L;           // rows it has at once
+  static constexpr int G = L < WAVE ? L : WAVE;  // lanes that share a vector's columns
 };
 
 template <int DT, int L, int NV, bool CENTER>
 __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool wbf16) {
-  constexpr int ROWS = NormShape<L>::ROWS;
+  constexpr int ROWS = NormShape<L>::ROWS, G = NormShape<L>::G;
+  typedef RowVec<DT, G> X;
   __shared__ float s_sum[2][16];
-  const int l = threadIdx.x % L;
+  const int l = threadIdx.x % L, lane = l % G, g0 = 8 * (l - lane);  // (of the row, of its group; the group's)
   const float inv = 1.0f / (float)a.K;
   for (int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L; n < a.N; n += (int64_t)gridDim.x * ROWS) {
-    const char* row = (const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE;
-    RowVec<DT> x[NV];
+    const char* row = (const char*)a.x + n * a.x_stride * X::SIZE;
+    X x[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i].template load_to<true>(row, 8 * (i * L + l), a.K);
+    for (int i = 0; i < NV; ++i) x[i].template load_to<true>(row, 8 * L * i + g0, lane, a.K);
     float mu = 0.0f;
     if constexpr (CENTER) {
       float s = 0.0f;
@@ -90,28 +137,28 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool
     float q = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int left = a.K - 8 * (i * L + l);
+      const int left = a.K - 8 * L * i - g0 - X::first(lane);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = !CENTER ? x[i].at(j) : j < left ? x[i].at(j) - mu : 0.0f;
+        const float c = !CENTER ? x[i].at(j) : X::step(j) < left ? x[i].at(j) - mu : 0.0f;
         q = fma_f(c, c, q);
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i].renew();
     const float rstd = 1.0f / sqrtf(row_sum<L>(q, s_sum[1]) * inv + a.eps);
-    char* out = (char*)a.y + n * a.y_stride * RowVec<DT>::SIZE;
+    char* out = (char*)a.y + n * a.y_stride * X::SIZE;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int k = 8 * (i * L + l);
+      const int k0 = 8 * L * i + g0;
       float f[8], w[8], b[8];
-      param8(a.weight, wbf16, k, a.K, 1.0f, w);
-      param8(a.bias, wbf16, k, a.K, 0.0f, b);
+      param8<DT, G>(a.weight, wbf16, k0, lane, a.K, 1.0f, w);
+      param8<DT, G>(a.bias, wbf16, k0, lane, a.K, 0.0f, b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = fma_f((x[i].at(j) - mu) * rstd, w[j], b[j]);
-      RowVec<DT> y;
+      X y;
       y.set(f);
-      if (k < a.K) y.store_to(out, k, a.K);
+      y.store_to(out, k0, lane, a.K);
     }
     if (l == 0) {
       if (a.rstd) a.rstd[n] = rstd;
@@ -125,20 +172,21 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool
 // (Past K dy is 0, so that nothing there counts.)
 template <int DT, int L, int NV, bool CENTER, int PARAM>
 __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArgs a, bool wbf16, float* part) {
-  constexpr int ROWS = NormShape<L>::ROWS;
+  constexpr int ROWS = NormShape<L>::ROWS, G = NormShape<L>::G;
+  typedef RowVec<DT, G> X;
   __shared__ float s_sum[2][2][16];
-  const int l = threadIdx.x % L;
+  const int l = threadIdx.x % L, lane = l % G, g0 = 8 * (l - lane);
   const float inv = 1.0f / (float)a.K;
   const int64_t step = (int64_t)gridDim.x * ROWS;
-  RowVec<DT> nx[NV], ng[NV];
+  X nx[NV], ng[NV];
   float nr = 0.0f, nm = 0.0f;
   auto request = [&](int64_t n) {
-    const char* x = (const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE;
-    const char* g = (const char*)a.dy + n * a.dy_stride * RowVec<DT>::SIZE;
+    const char* x = (const char*)a.x + n * a.x_stride * X::SIZE;
+    const char* g = (const char*)a.dy + n * a.dy_stride * X::SIZE;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      nx[i].template load_to<true>(x, 8 * (i * L + l), a.K);
-      ng[i].template load_to<true>(g, 8 * (i * L + l), a.K);
+      nx[i].template load_to<true>(x, 8 * L * i + g0, lane, a.K);
+      ng[i].template load_to<true>(g, 8 * L * i + g0, lane, a.K);
     }
     nr = a.rstd[n];
     if (CENTER) nm = a.mean[n];
@@ -152,13 +200,13 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = held[i][j];
     } else {
-      param8(a.weight, wbf16, 8 * (i * L + l), a.K, 1.0f, w);
+      param8<DT, G>(a.weight, wbf16, 8 * L * i + g0, lane, a.K, 1.0f, w);
     }
   };
   if constexpr (PARAM > 0)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      param8(a.weight, wbf16, 8 * (i * L + l), a.K, 1.0f, held[i]);
+      param8<DT, G>(a.weight, wbf16, 8 * L * i + g0, lane, a.K, 1.0f, held[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         dw[i][j] = 0.0f;
@@ -167,7 +215,7 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
     }
   for (int turn = 0; n < a.N; n += step, turn ^= 1) {
     if (!PARAM) request(n);
-    RowVec<DT> x[NV], g[NV];
+    X x[NV], g[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       x[i] = nx[i];
@@ -218,10 +266,9 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
     }
     c1 *= inv;
     c2 = CENTER ? c2 * inv : 0.0f;
-    char* out = (char*)a.dx + n * a.dx_stride * RowVec<DT>::SIZE;
+    char* out = (char*)a.dx + n * a.dx_stride * X::SIZE;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int k = 8 * (i * L + l);
       float w[8], d[8];
       weight(i, w);
 #pragma unroll
@@ -229,9 +276,9 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
         const float xh = (x[i].at(j) - mu) * rstd, h = g[i].at(j) * w[j];
         d[j] = rstd * (fma_f(-xh, c1, h) - c2);
       }
-      RowVec<DT> y;
+      X y;
       y.set(d);
-      if (k < a.K) y.store_to(out, k, a.K);
+      y.store_to(out, 8 * L * i + g0, lane, a.K);
     }
   }
   if constexpr (PARAM > 0) {
@@ -243,8 +290,9 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          s_acc[0][threadIdx.x / L][8 * (i * L + l) + j] = dw[i][j];
-          if constexpr (PARAM > 1) s_acc[1][threadIdx.x / L][8 * (i * L + l) + j] = db[i][j];
+          const int k = 8 * L * i + g0 + X::first(lane) + X::step(j);
+          s_acc[0][threadIdx.x / L][k] = dw[i][j];
+          if constexpr (PARAM > 1) s_acc[1][threadIdx.x / L][k] = db[i][j];
         }
       __syncthreads();
       for (int k = threadIdx.x; k < a.K; k += NormShape<L>::T)
@@ -258,15 +306,8 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int k = 8 * (i * L + l);
-        RowVec<STRIM_DTYPE_F32> v;
-        if (k >= a.K) continue;
-        v.set(dw[i]);
-        v.store_to((char*)out, k, a.K);
-        if constexpr (PARAM > 1) {
-          v.set(db[i]);
-          v.store_to((char*)(out + a.K), k, a.K);
-        }
+        sums8<DT, G>(out, 8 * L * i + g0, lane, a.K, dw[i]);
+        if constexpr (PARAM > 1) sums8<DT, G>(out + a.K, 8 * L * i + g0, lane, a.K, db[i]);
       }
     }
   }
@@ -276,14 +317,14 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
 // rows dealt to gridDim.y parts.
 template <int DT, bool CENTER, int PARAM>
 __global__ __launch_bounds__(256) void k_norm_columns(const NormGradArgs a, float* part) {
-  const int k = 8 * (int)(blockIdx.x * 256 + threadIdx.x);
-  if (k >= a.K) return;
+  const int lane = threadIdx.x & (WAVE - 1), k0 = 8 * WAVE * ((int)blockIdx.x * (256 / WAVE) + wave_id());
+  if (k0 >= a.K) return;
   float dw[8] = {}, db[8] = {};
 #pragma unroll 4
   for (int64_t n = blockIdx.y; n < a.N; n += gridDim.y) {
     RowVec<DT> x, g;
-    x.template load_to<true>((const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE, k, a.K);
-    g.template load_to<true>((const char*)a.dy + n * a.dy_stride * RowVec<DT>::SIZE, k, a.K);
+    x.template load_to<true>((const char*)a.x + n * a.x_stride * RowVec<DT>::SIZE, k0, lane, a.K);
+    g.template load_to<true>((const char*)a.dy + n * a.dy_stride * RowVec<DT>::SIZE, k0, lane, a.K);
     const float rstd = a.rstd[n], mu = CENTER ? a.mean[n] : 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -292,13 +333,8 @@ __global__ __launch_bounds__(256) void k_norm_columns(const NormGradArgs a, floa
     }
   }
   float* out = part + (int64_t)blockIdx.y * PARAM * a.K;
-  RowVec<STRIM_DTYPE_F32> v;
-  v.set(dw);
-  v.store_to((char*)out, k, a.K);
-  if constexpr (PARAM > 1) {
-    v.set(db);
-    v.store_to((char*)(out + a.K), k, a.K);
-  }
+  sums8<DT, WAVE>(out, k0, lane, a.K, dw);
+  if constexpr (PARAM > 1) sums8<DT, WAVE>(out + a.K, k0, lane, a.K, db);
 }
 
 // dw and db from the workgroups' rows of `width` sums (K of dw, then K of db), added in order: 64 columns a

@@ -1,5 +1,5 @@
-// rows.hpp — rows of logits as the scores and the distillation read and write them: eight tokens a
-// lane, any alignment; and their softmax statistics.
+// rows.hpp — rows of logits (and of hidden states) as the scores, the distillation and the norms read and
+// write them: eight tokens a lane, any alignment; and their softmax statistics.
 #pragma once
 
 #include "common.hpp"
@@ -18,44 +18,57 @@ constexpr uint32_t NINF_BITS = 0xFF800000u;
 __device__ __forceinline__ float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float fma_f(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 
-// Eight tokens of a row as they lie in memory.
-template <int DT>
+// Eight tokens a lane of the 8 G that G neighbouring lanes share, as they lie in memory: bf16, eight in a row;
+// float32, two runs of four, 4 G tokens apart, so that the lanes' 16 bytes of one load are in a row as well
+// (a lane's own 32 bytes by two loads: 4.6 TB/s past the caches, this 6.6).
+template <int DT, int G = WAVE>
 struct RowVec {
-  static constexpr int WORDS = DT == STRIM_DTYPE_BF16 ? 4 : 8;
-  static constexpr int SIZE = DT == STRIM_DTYPE_BF16 ? 2 : 4;
+  static constexpr bool BF16 = DT == STRIM_DTYPE_BF16;
+  static constexpr int WORDS = BF16 ? 4 : 8;
+  static constexpr int SIZE = BF16 ? 2 : 4;
+  static constexpr int RUN = BF16 ? 8 : 4;  // tokens in a row
   uint32_t w[WORDS];
 
+  // where the lane's element j lies among the 8 G: first(lane) + step(j); and whose token `off` is
+  static __device__ __forceinline__ int first(int lane) { return RUN * lane; }
+  static constexpr __device__ __forceinline__ int step(int j) { return BF16 ? j : (j & 3) + (j >> 2) * 4 * G; }
+  static __device__ __forceinline__ int lane_of(int off) { return BF16 ? off >> 3 : (off & (4 * G - 1)) >> 2; }
+  static __device__ __forceinline__ int element_of(int off) { return BF16 ? off & 7 : (off & 3) + (off / (4 * G)) * 4; }
+
   __device__ __forceinline__ float at(int j) const {
-    if constexpr (DT == STRIM_DTYPE_BF16)
+    if constexpr (BF16)
       return __uint_as_float(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
     else
       return __uint_as_float(w[j]);
   }
-  // tokens v .. v + 7, all inside the row
-  __device__ __forceinline__ void load(const char* row, int v) {
-    const char* p = row + (int64_t)v * SIZE;
+  // The lane's of the tokens from v0 on, all inside the row. NT: past the caches.
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const char* row, int v0, int lane) {
+    const char* p = row + (int64_t)(v0 + first(lane)) * SIZE;
 #pragma unroll
     for (int i = 0; i < WORDS / 4; ++i) {
-      const ru32x4 q = ((const ru32x4_any*)p)[i];
+      const ru32x4_any* a = (const ru32x4_any*)(p + i * 4 * G * SIZE);
+      const ru32x4 q = NT ? __builtin_nontemporal_load(a) : *a;
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
     }
   }
-  // tokens from v on that lie before V; past them -inf, or 0
-  template <bool ZERO = false>
-  __device__ __forceinline__ void load_to(const char* row, int v, int V) {
-    if (v + 8 <= V) return load(row, v);
+  // Those that lie before V; past them -inf, or 0.
+  template <bool ZERO = false, bool NT = false>
+  __device__ __forceinline__ void load_to(const char* row, int v0, int lane, int V) {
+    const int v = v0 + first(lane);
+    if (v + step(7) < V) return load<NT>(row, v0, lane);
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) w[i] = ZERO ? 0u : DT == STRIM_DTYPE_BF16 ? 0xFF80FF80u : NINF_BITS;
+    for (int i = 0; i < WORDS; ++i) w[i] = ZERO ? 0u : BF16 ? 0xFF80FF80u : NINF_BITS;
     const char* p = row + (int64_t)v * SIZE;
 #pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (v + j < V) {
-        if constexpr (DT == STRIM_DTYPE_BF16) {
+    for (int j = 0; j < 8; ++j)
+      if (v + step(j) < V) {
+        if constexpr (BF16) {
           const uint32_t h = ((const uint16_t*)p)[j];
           w[j >> 1] = j & 1 ? (w[j >> 1] & 0xFFFFu) | h << 16 : (w[j >> 1] & 0xFFFF0000u) | h;
         } else {
-          w[j] = ((const uint32_t*)p)[j];
+          w[j] = ((const uint32_t*)p)[step(j)];
         }
       }
   }
@@ -66,7 +79,7 @@ struct RowVec {
     for (int i = 0; i < WORDS; ++i) asm volatile("" : "+v"(w[i]));
   }
   __device__ __forceinline__ void set(const float (&f)[8]) {
-    if constexpr (DT == STRIM_DTYPE_BF16) {
+    if constexpr (BF16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rf32x2{f[2 * i], f[2 * i + 1]}, rbf16x2));
@@ -75,22 +88,44 @@ struct RowVec {
       for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
     }
   }
-  __device__ __forceinline__ void store_to(char* row, int v, int V) const {
+  __device__ __forceinline__ void store_to(char* row, int v0, int lane, int V, bool nt = false) const {
+    const int v = v0 + first(lane);
     char* p = row + (int64_t)v * SIZE;
-    if (v + 8 <= V) {
+    if (v + step(7) < V) {
 #pragma unroll
-      for (int i = 0; i < WORDS / 4; ++i)
-        ((ru32x4_any*)p)[i] = ru32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const ru32x4 q{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        ru32x4_any* a = (ru32x4_any*)(p + i * 4 * G * SIZE);
+        if (nt) __builtin_nontemporal_store(q, a);
+        else *a = q;
+      }
       return;
     }
 #pragma unroll
-    for (int j = 0; j < 7; ++j)
-      if (v + j < V) {
-        if constexpr (DT == STRIM_DTYPE_BF16) ((uint16_t*)p)[j] = (uint16_t)(w[j >> 1] >> (j & 1 ? 16 : 0));
-        else ((uint32_t*)p)[j] = w[j];
+    for (int j = 0; j < 8; ++j)
+      if (v + step(j) < V) {
+        if constexpr (BF16) ((uint16_t*)p)[j] = (uint16_t)(w[j >> 1] >> (j & 1 ? 16 : 0));
+        else ((uint32_t*)p)[step(j)] = w[j];
       }
   }
 };
+
+// The allow-mask's bits of a lane's eight tokens from v0 on (0 past V).
+template <int DT>
+__device__ __forceinline__ uint32_t allowed8(const uint32_t* mask, int v0, int lane, int V) {
+  const uint8_t* b = (const uint8_t*)mask;
+  const int v = v0 + RowVec<DT>::first(lane);
+  if constexpr (DT == STRIM_DTYPE_BF16) {
+    return v < V ? b[v >> 3] : 0u;
+  } else {
+    const int v2 = v + RowVec<DT>::step(4);
+    const uint32_t lo = v < V ? b[v >> 3] >> (v & 4) : 0u, hi = v2 < V ? b[v2 >> 3] >> (v2 & 4) : 0u;
+    return (lo & 15u) | (hi & 15u) << 4;
+  }
+}
+
+// Stores of results larger than the memory-side cache go past the caches: nobody finds them there.
+constexpr int64_t ROWS_CACHED = (int64_t)256 << 20;
 
 template <int DT>
 __device__ __forceinline__ float token_at(const char* row, int v) {

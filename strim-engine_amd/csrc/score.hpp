@@ -33,6 +33,7 @@ struct ScoreGradArgs {
   const float *lse, *entropy, *grad_logprobs, *grad_entropy, *grad_lse;
   void* d_logits;
   int64_t d_stride;
+  bool stream;  // the launcher's: stores past the caches
 };
 
 struct DistillArgs {
@@ -50,6 +51,7 @@ struct DistillArgs {
   const float* weights;  // the loss's gradient per row
   void* d_logits;
   int64_t d_stride;
+  bool stream;  // the launcher's: stores past the caches
 };
 
 struct NormArgs {

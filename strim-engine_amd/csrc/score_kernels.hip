@@ -32,9 +32,6 @@ struct ScoreParts {
   uint64_t* keys;        // [R][parts][room]
 };
 
-__device__ __forceinline__ uint32_t allowed8(const uint32_t* mask, int v, int V) {
-  return !mask ? 0xFFu : v < V ? ((const uint8_t*)mask)[v >> 3] : 0u;
-}
 __device__ __forceinline__ bool allowed_at(const uint32_t* mask, int v) {
   return !mask || ((mask[v >> 5] >> (v & 31)) & 1u);
 }
@@ -106,7 +103,7 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
   __shared__ std::conditional_t<TOP, TopList, char> s_list;
   TopList* const s_top = (TopList*)&s_list;  // (unused without TOP)
   const int64_t r = blockIdx.x / q.parts;
-  const int p = blockIdx.x - (int)r * q.parts;
+  const int p = blockIdx.x - (int)r * q.parts, lane = threadIdx.x & (WAVE - 1), wave = wave_id();
   const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
   const uint32_t* mask = MASK ? a.mask + r * a.mask_stride : nullptr;
   const float c = LOG2E / a.T;
@@ -116,10 +113,10 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
   auto request = [&](int t) {
 #pragma unroll
     for (int u = 0; u < SC_U; ++u) {
-      const int v = t + 8 * (u * SC_T + (int)threadIdx.x);
-      if (t + SC_TILE <= a.V) next[u].load(row, v);
-      else next[u].load_to(row, v, a.V);
-      if (MASK) ok[u] = allowed8(mask, v, a.V);
+      const int v0 = t + 8 * WAVE * (u * (SC_T / WAVE) + wave);
+      if (t + SC_TILE <= a.V) next[u].template load<true>(row, v0, lane);
+      else next[u].load_to(row, v0, lane, a.V);
+      if (MASK) ok[u] = allowed8<DT>(mask, v0, lane, a.V);
     }
   };
   request(t0);
@@ -147,22 +144,21 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
       for (int j = 0; j < 8 * SC_U; ++j) asm volatile("" : "+v"(x[j]));
       if (t + SC_TILE < t1) request(t + SC_TILE);
       stat_add<8 * SC_U, true>(st, x, mx, c);
-      if constexpr (TOP) fits = top.add<SC_U>(s_top[0], x, mv, st.m, t + 8 * (int)threadIdx.x);
+      if constexpr (TOP)
+        fits = top.add<SC_U>(s_top[0], x, mv, st.m, t + 8 * WAVE * wave + RowVec<DT>::first(lane), RowVec<DT>::step);
     }
     if constexpr (TOP)
       if (!fits) {  // the last tile again, slot by slot (out of the loop, for its registers' sake)
         const int s = t - SC_TILE;
-        top_slots<SC_U>(s_top[0], top, s + 8 * (int)threadIdx.x, [&](int u, float (&x)[8]) {
-          const int v = s + 8 * (u * SC_T + (int)threadIdx.x);
+        auto load = [&](int u, float (&x)[8]) {
+          const int v0 = s + 8 * WAVE * (u * (SC_T / WAVE) + wave);
           RowVec<DT> q;
-          uint32_t in = 0;
-          if (v < a.V) {
-            q.load_to(row, v, a.V);
-            in = MASK ? allowed8(mask, v, a.V) : 0xFFu;
-          }
+          q.load_to(row, v0, lane, a.V);
+          const uint32_t in = MASK ? allowed8<DT>(mask, v0, lane, a.V) : 0xFFu;
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = (in >> j) & 1u ? q.at(j) : -INFINITY;
-        });
+        };
+        top_slots<SC_U>(s_top[0], top, s + 8 * WAVE * wave + RowVec<DT>::first(lane), load, RowVec<DT>::step);
       }
   }
   const float most = st.m;
@@ -255,14 +251,14 @@ __global__ __launch_bounds__(SC_T) void k_scores_grad(const ScoreGradArgs a, int
   const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
   char* out = (char*)a.d_logits + r * a.d_stride * RowVec<DT>::SIZE;
   const uint32_t* mask = MASK ? a.mask + r * a.mask_stride : nullptr;
-  const int t0 = p * SG_TILES * 8 * SC_T;
+  const int t0 = p * SG_TILES * 8 * SC_T, wave = wave_id();
   RowVec<DT> x[SG_TILES];
   uint32_t ok[SG_TILES];
 #pragma unroll
   for (int u = 0; u < SG_TILES; ++u) {
-    const int v = t0 + 8 * (u * SC_T + (int)threadIdx.x);
-    if (v < a.V) x[u].load_to(row, v, a.V);
-    if (MASK) ok[u] = allowed8(mask, v, a.V);
+    const int w0 = t0 + 8 * WAVE * (u * (SC_T / WAVE) + wave);
+    x[u].template load_to<false, true>(row, w0, lane, a.V);
+    if (MASK) ok[u] = allowed8<DT>(mask, w0, lane, a.V);
   }
   const float lse = a.lse[r], c = LOG2E / a.T, inv = 1.0f / a.T;
   const float gh = ENT ? a.grad_entropy[r] : 0.0f, H = ENT ? a.entropy[r] : 0.0f;
@@ -280,9 +276,8 @@ __global__ __launch_bounds__(SC_T) void k_scores_grad(const ScoreGradArgs a, int
   const float ref = lse * a.T;
 #pragma unroll
   for (int u = 0; u < SG_TILES; ++u) {
-    const int w0 = __builtin_amdgcn_readfirstlane(t0 + 8 * (u * SC_T + (int)threadIdx.x - lane));
+    const int w0 = t0 + 8 * WAVE * (u * (SC_T / WAVE) + wave);
     if (w0 >= a.V) break;
-    const int v = w0 + 8 * lane;
     float d[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -299,7 +294,8 @@ __global__ __launch_bounds__(SC_T) void k_scores_grad(const ScoreGradArgs a, int
         const int off = rl_i(id[i], l) - w0;
         const float more = rl_f(g[i], l);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] += lane == off >> 3 && j == (off & 7) ? more : 0.0f;
+        for (int j = 0; j < 8; ++j)
+          d[j] += lane == RowVec<DT>::lane_of(off) && j == RowVec<DT>::element_of(off) ? more : 0.0f;
       }
     }
     if (MASK)
@@ -310,7 +306,7 @@ __global__ __launch_bounds__(SC_T) void k_scores_grad(const ScoreGradArgs a, int
     if (empty)
 #pragma unroll
       for (int i = 0; i < RowVec<DT>::WORDS; ++i) y.w[i] = 0;
-    if (v < a.V) y.store_to(out, v, a.V);
+    y.store_to(out, w0, lane, a.V, a.stream);
   }
 }
 
@@ -362,6 +358,7 @@ hipError_t launch_scores_grad(const ScoreGradArgs& a, bool bf16, hipStream_t st)
   const int most = (int)(((int64_t)1 << 23) / parts);
   for (int r0 = 0; r0 < a.R; r0 += most) {
     ScoreGradArgs b = a;
+    b.stream = (int64_t)a.R * a.V * (bf16 ? 2 : 4) > ROWS_CACHED;
     const int64_t at = r0;
     b.R = a.R - r0 < most ? a.R - r0 : most;
     b.logits = (const char*)a.logits + at * a.stride * (bf16 ? 2 : 4);

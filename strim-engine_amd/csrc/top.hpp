@@ -151,11 +151,12 @@ struct TopRun {
     __syncthreads();
   }
 
-  // A tile of U slots of TOP_STEP tokens, eight a thread: x[8 u ..] are the thread's of slot u, from id
-  // first + u TOP_STEP on; mv[u] is their maximum, `most` the largest that the thread has met. False where
+  // A tile of U slots of TOP_STEP tokens, eight a thread: x[8 u ..] are the thread's of slot u, with ids
+  // first + u TOP_STEP + step(j); mv[u] is their maximum, `most` the largest that the thread has met. False where
   // more were to be appended than the list holds: the tile is then given to top_slots.
-  template <int U>
-  __device__ __forceinline__ bool add(TopList& l, const float (&x)[8 * U], const float (&mv)[U], float most, int first) {
+  template <int U, class S>
+  __device__ __forceinline__ bool add(TopList& l, const float (&x)[8 * U], const float (&mv)[U], float most, int first,
+                                      S step) {
     const bool raise = ((tile + 1) & tile) == 0;
     before = limit;
     if (raise) limit = top_threshold(l, fkey_desc(most), limit, M, by);
@@ -180,7 +181,7 @@ struct TopRun {
         for (int j = 0; j < 8; ++j)
           if (m[j]) {
             const int to = at + lanes_below(m[j]);
-            if (x[8 * u + j] >= floor && to < TOP_CAP) l.e[to] = top_entry(x[8 * u + j], first + u * TOP_STEP + j);
+            if (x[8 * u + j] >= floor && to < TOP_CAP) l.e[to] = top_entry(x[8 * u + j], first + u * TOP_STEP + step(j));
             at += __popcll(m[j]);
           }
       }
@@ -207,8 +208,8 @@ struct TopRun {
 
 // A tile of which too many tokens at once reach the threshold (ties, or a run of large ones): slot by slot,
 // the list cut in between. load(slot, x): the thread's eight tokens of a slot.
-template <int U, class F>
-__device__ __forceinline__ void top_slots(TopList& l, TopRun& r, int first, F load) {
+template <int U, class F, class S>
+__device__ __forceinline__ void top_slots(TopList& l, TopRun& r, int first, F load, S step) {
 #pragma unroll 1
   for (int u = 0; u < U; ++u) {
     if (r.held > TOP_T) r.held = top_reduce(l, r.held, r.M, r.limit);
@@ -220,7 +221,7 @@ __device__ __forceinline__ void top_slots(TopList& l, TopRun& r, int first, F lo
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (x[j] >= floor) l.e[atomicAdd(&l.n, 1)] = top_entry(x[j], first + u * TOP_STEP + j);
+      if (x[j] >= floor) l.e[atomicAdd(&l.n, 1)] = top_entry(x[j], first + u * TOP_STEP + step(j));
     __syncthreads();
     r.held = __builtin_amdgcn_readfirstlane(l.n);
     __syncthreads();
