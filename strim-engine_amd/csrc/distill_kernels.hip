@@ -165,16 +165,18 @@ __device__ __forceinline__ RowNumbers numbers_of(const Alternatives& o, const Te
   return n;
 }
 
-// What the gradient takes of a row: sign exp2((x - ref) c + k) at every token, but at the alternatives
-// in exp2((x - ref) c + kq) - p.
+// What the gradient takes of a row: sign 2^y with y = (x - ref) c + k at every token, but at the alternatives
+// in 2^y' - p, y' = (x - ref) c + kq. Where (x - ref) c + k may be taken as x c + (k - ref c) without an
+// infinity (`near`), bf16 results are: the rounding of k - ref c, 2^-20 of a result, is far below theirs.
 struct GradRow {
-  float ref, k, kq, in;
+  float ref, k, kq, in, b;
   uint32_t sign;  // 0 or 0x80008000
+  int32_t near;
   int32_t dead;   // the row has no gradient
 };
 // lse = ref / T + ls; w = weight / T
 __device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, float ref, double ls, double log_rest,
-                                            double w) {
+                                            double w, float c) {
   constexpr double L2E = 1.4426950408889634074;
   GradRow g;
   g.dead = !any || w == 0.0;
@@ -188,60 +190,64 @@ __device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, float re
       more = -log_rest;
     }
   }
+  const double k = log2(fabs(all)) + (more - ls) * L2E;
   g.ref = ref;
   g.kq = (float)(-ls * L2E);
-  g.k = (float)(log2(fabs(all)) + (more - ls) * L2E);
+  g.k = (float)k;
   g.in = (float)in;
+  g.b = (float)(k - (double)ref * c);
+  g.near = !stat_far(ref);
   g.sign = all < 0.0 ? 0x80008000u : 0u;
   return g;
 }
 
-// Eight tokens' gradients; id, p: the wave's alternatives (each id once) and w / T p_m; hits: whether any
-// is among the wave's tokens, which begin at w0.
+// Eight tokens' gradients, as of no alternatives.
 template <int DT>
-__device__ __forceinline__ RowVec<DT> grad_of(const RowVec<DT>& x, const GradRow& g, float c,
-                                              const int (&id)[2], const float (&p)[2], int w0, bool hits) {
-  const int lane = threadIdx.x & (WAVE - 1);
+__device__ __forceinline__ RowVec<DT> grad_of(const RowVec<DT>& x, const GradRow& g, float c) {
   float d[8];
+  if (DT == STRIM_DTYPE_BF16 && g.near) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) d[j] = hw_exp2(fma_f(x.at(j) - g.ref, c, g.k));
+    for (int j = 0; j < 8; ++j) d[j] = hw_exp2(fma_f(x.at(j), c, g.b));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) d[j] = hw_exp2(fma_f(x.at(j) - g.ref, c, g.k));
+  }
   RowVec<DT> y;
   y.set(d);
+  if (g.sign)
 #pragma unroll
-  for (int i = 0; i < RowVec<DT>::WORDS; ++i)
-    y.w[i] ^= DT == STRIM_DTYPE_BF16 ? g.sign : g.sign & 0x80000000u;
-  if (hits)
-    each_hit<DT>(id, w0, [&](int at, int e, int l, int i) {
-      const float less = rl_f(p[i], l);
-      // (masks, not an index: words that are indexed at run time are put into memory)
-      const int word = DT == STRIM_DTYPE_BF16 ? e >> 1 : e;
-      const uint32_t half = DT == STRIM_DTYPE_F32 ? ~0u : e & 1 ? 0xFFFF0000u : 0xFFFFu;
-      uint32_t bits = 0;
-#pragma unroll
-      for (int q = 0; q < RowVec<DT>::WORDS; ++q) bits |= x.w[q] & (q == word ? half : 0u);
-      if (DT == STRIM_DTYPE_BF16 && !(e & 1)) bits <<= 16;
-      const float f = g.in * hw_exp2(fma_f(__uint_as_float(bits) - g.ref, c, g.kq)) - less;
-      const float two[8] = {f, f};
-      RowVec<DT> z;
-      z.set(two);
-      const uint32_t mine = lane == at ? half : 0u;
-#pragma unroll
-      for (int q = 0; q < RowVec<DT>::WORDS; ++q) {
-        const uint32_t m = q == word ? mine : 0u;
-        y.w[q] = (y.w[q] & ~m) | (z.w[0] & m);
-      }
-    });
+    for (int i = 0; i < RowVec<DT>::WORDS; ++i) y.w[i] ^= DT == STRIM_DTYPE_BF16 ? g.sign : 0x80000000u;
   if (g.dead)
 #pragma unroll
     for (int i = 0; i < RowVec<DT>::WORDS; ++i) y.w[i] = 0;
   return y;
 }
+// The gradients of the wave's own alternatives among its tokens, a lane each, over what the wave stored there
+// before: a wave's stores to one address keep their order. id -1: none.
+template <int DT>
+__device__ __forceinline__ void grad_alternatives(char* out, const GradRow& g, float c, const int (&id)[2],
+                                                  const float (&x)[2], const float (&p)[2]) {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  if (g.dead) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (id[i] >= 0) {
+      const float f = g.in * hw_exp2(fma_f(x[i] - g.ref, c, g.kq)) - p[i];
+      if constexpr (DT == STRIM_DTYPE_BF16) ((uint16_t*)out)[id[i]] = __builtin_bit_cast(uint16_t, (__bf16)f);
+      else ((float*)out)[id[i]] = f;
+    }
+}
 
-// The row's alternatives for the gradient in LDS, each id once: what a workgroup's waves read.
+// The row's alternatives for the gradient, each id once: what the waves read, in LDS or from memory.
 struct GradList {
   int id[DI_M];
-  float p[DI_M];
-  int repeats;  // whether an id stands twice
+  float x[DI_M], p[DI_M];  // its logit, and w / T p_m
+  int repeats;             // whether an id stands twice
+};
+// What k_distill_join leaves for the gradient of a step.
+struct GradRecord {
+  GradRow row;
+  GradList list;
 };
 // Looks for repeated ids, all threads: entry e against a part of those before it. (Two barriers' worth:
 // the caller's before reading l.repeats.)
@@ -260,15 +266,16 @@ __device__ __forceinline__ void find_repeats(GradList& l, const Alternatives& o)
   for (int j = from; j < from + SEG; ++j) twice |= j < e && l.id[j] == id;
   if (twice && id >= 0) l.repeats = 1;
 }
-// The wave's entries as GradList has them: w / T p_m, each id once.
+// The wave's entries as GradList has them, each id once. x: their logits.
 __device__ __forceinline__ void list_out(GradList& l, const Alternatives& o, const Teacher& t, int M, double w,
-                                         bool (&first)[2], bool repeats) {
+                                         const float (&x)[2], bool (&first)[2], bool repeats) {
   const int lane = threadIdx.x & (WAVE - 1);
   float p[2] = {t.p[0], t.p[1]};
   if (repeats) merge_repeats(o, M, first, p);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l.id[lane + i * WAVE] = first[i] ? o.id[i] : -1;
+    l.x[lane + i * WAVE] = x[i];
     l.p[lane + i * WAVE] = (float)(w * p[i]);
   }
 }
@@ -276,6 +283,7 @@ __device__ __forceinline__ void list_out(GradList& l, const Alternatives& o, con
 struct DistillParts {
   int32_t parts, tiles;  // parts of a row; tiles of a part
   RowStat* part;         // [N][parts]
+  GradRecord* record;    // a step's: [N]
 };
 
 // The tokens' statistic of a part of a row; TAIL: without the alternatives'.
@@ -329,27 +337,41 @@ __global__ __launch_bounds__(DI_T) void k_distill_stat(const DistillArgs a, cons
   }
 }
 
-// The rows' results; a wave a row.
-template <int DT>
-__global__ __launch_bounds__(DI_T) void k_distill_join(const DistillArgs a, const DistillParts q) {
-  const int64_t r = (int64_t)blockIdx.x * (DI_T / WAVE) + wave_id();
-  if (r >= a.N) return;
-  const int lane = threadIdx.x & (WAVE - 1);
+// The rows' results; a wave a row. STEP: and what the gradient takes of them.
+template <int DT, bool STEP>
+__global__ __launch_bounds__(WAVE) void k_distill_join(const DistillArgs a, const DistillParts q) {
+  const int64_t r = blockIdx.x;
+  const int lane = threadIdx.x;
   const float c = LOG2E / a.T;
   const char* row = (const char*)a.logits + r * a.stride * RowVec<DT>::SIZE;
+  const Alternatives o = alternatives_of(a, r);
   RowStat st{-INFINITY, 0.0f, 0.0f};
   for (int p = lane; p < q.parts; p += WAVE) stat_merge(st, q.part[r * q.parts + p], c);
+  const double w = STEP ? (double)a.weights[r] / a.T : 0.0;
+  float x[2], merged[2] = {0.0f, 0.0f};
+  bool first[2] = {true, true};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) x[i] = o.any && o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
   stat_wave(st, c);
   stat_exact(st, c);
-  const Alternatives o = alternatives_of(a, r);
-  RowNumbers n{0.0, 0.0, 0.0, 0.0};
-  if (o.any) {
-    float x[2], p[2] = {0.0f, 0.0f};
-    bool first[2];
+  const Teacher t = teacher_of(o, a.tail);
+  if (a.tail || STEP) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
-    if (a.tail) merge_repeats(o, a.M, first, p);
-    n = numbers_of(o, teacher_of(o, a.tail), first, x, st, a.T, a.tail);
+    for (int i = 0; i < 2; ++i) merged[i] = t.p[i];
+    merge_repeats(o, a.M, first, merged);
+  }
+  RowNumbers n{0.0, 0.0, 0.0, 0.0};
+  if (o.any) n = numbers_of(o, t, first, x, st, a.T, a.tail);
+  if constexpr (STEP) {
+    GradRecord* rec = q.record + r;
+    const GradRow g = grad_row(o.any, t, (float)n.top, n.ls, n.log_rest, w, c);
+    if (lane == 0) rec->row = g;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      rec->list.id[lane + i * WAVE] = first[i] ? o.id[i] : -1;
+      rec->list.x[lane + i * WAVE] = x[i];
+      rec->list.p[lane + i * WAVE] = (float)(w * merged[i]);
+    }
   }
   if (lane != 0) return;
   const float loss = (float)n.loss;
@@ -360,8 +382,8 @@ __global__ __launch_bounds__(DI_T) void k_distill_join(const DistillArgs a, cons
     a.status[r] = !o.known ? STRIM_EINVAL : fabsf(loss) < INFINITY ? STRIM_OK : STRIM_ENONFINITE;
 }
 
-// A part of a row's gradient from its lse and log q_rest.
-template <int DT>
+// A part of a row's gradient: from its lse and log q_rest, or (STEP) from its record.
+template <int DT, bool STEP>
 __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, const DistillParts q) {
   __shared__ GradList s_list;
   __shared__ GradRow s_grad;
@@ -374,39 +396,57 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
   RowVec<DT> next[DI_U];
   auto request = [&](int t) {
 #pragma unroll
-    for (int u = 0; u < DI_U; ++u) {
+    for (int u = 0; u < DI_U; ++u)
       next[u].template load_to<false, true>(row, t + 8 * WAVE * (u * (DI_T / WAVE) + wave), lane, a.V);
-    }
   };
   request(t0);
-  const Alternatives o = alternatives_of(a, r);
-  find_repeats<DI_T>(s_list, o);
-  __syncthreads();
-  if (wave_id() == 0) {
-    const Teacher t = teacher_of(o, a.tail);
-    const double w = (double)a.weights[r] / a.T, lse = a.lse[r];
-    const float ref = (float)(lse * a.T);
-    bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};
-    list_out(s_list, o, t, a.M, w, first, s_list.repeats != 0);
-    const GradRow g = grad_row(o.any, t, ref, lse - (double)ref / a.T, a.tail ? (double)a.log_rest[r] : 0.0, w);
-    if (lane == 0) s_grad = g;
-  }
-  __syncthreads();
-  const GradRow g = s_grad;
-  const int id[2] = {s_list.id[lane], s_list.id[lane + WAVE]};
-  const float less[2] = {s_list.p[lane], s_list.p[lane + WAVE]};
-  for (int s = t0; s < t1; s += DI_TILE) {
-    RowVec<DT> x[DI_U];
+  const GradList* list = &s_list;
+  GradRow g;
+  if constexpr (STEP) {
+    list = &q.record[r].list;
+    g = q.record[r].row;
+  } else {
+    const Alternatives o = alternatives_of(a, r);
+    find_repeats<DI_T>(s_list, o);
+    __syncthreads();
+    if (wave == 0) {
+      const Teacher t = teacher_of(o, a.tail);
+      const double w = (double)a.weights[r] / a.T, lse = a.lse[r];
+      const float ref = (float)(lse * a.T);
+      bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};
+      float x[2];
 #pragma unroll
-    for (int u = 0; u < DI_U; ++u) x[u] = next[u];
+      for (int i = 0; i < 2; ++i) x[i] = o.any && o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
+      list_out(s_list, o, t, a.M, w, x, first, s_list.repeats != 0);
+      g = grad_row(o.any, t, ref, lse - (double)ref / a.T, a.tail ? (double)a.log_rest[r] : 0.0, w, c);
+      if (lane == 0) s_grad = g;
+    }
+    __syncthreads();
+    g = s_grad;
+  }
+  // the wave's own alternatives
+  int id[2];
+  float x[2], less[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    id[i] = list->id[lane + i * WAVE];
+    x[i] = list->x[lane + i * WAVE];
+    less[i] = list->p[lane + i * WAVE];
+    if (id[i] < t0 || id[i] >= t1 || id[i] / (8 * WAVE) % (DI_T / WAVE) != wave) id[i] = -1;
+  }
+  for (int s = t0; s < t1; s += DI_TILE) {
+    RowVec<DT> now[DI_U];
+#pragma unroll
+    for (int u = 0; u < DI_U; ++u) now[u] = next[u];
     if (s + DI_TILE < t1) request(s + DI_TILE);
 #pragma unroll
     for (int u = 0; u < DI_U; ++u) {
       const int w0 = s + 8 * WAVE * (u * (DI_T / WAVE) + wave);
       if (w0 >= a.V) break;
-      grad_of<DT>(x[u], g, c, id, less, w0, true).store_to(out, w0, lane, a.V, a.stream);
+      grad_of<DT>(now[u], g, c).store_to(out, w0, lane, a.V, a.stream);
     }
   }
+  grad_alternatives<DT>(out, g, c, id, x, less);
 }
 
 // A row whole: NV vectors of eight tokens a thread in registers; what is past them is read again for the
@@ -429,29 +469,44 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
   find_repeats<T>(s_list, o);
   // the vectors among which the wave's alternatives are
   uint64_t hits = 0;
+  if constexpr (TAIL)
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    for (uint64_t b = __ballot(o.id[i] >= 0 && (o.id[i] / (8 * WAVE)) % NWAVES == wave); b; b &= b - 1)
-      hits |= 1ull << min(63, rl_i(o.id[i], __builtin_ctzll(b)) / (8 * T));
+    for (int i = 0; i < 2; ++i)
+      for (uint64_t b = __ballot(o.id[i] >= 0 && (o.id[i] / (8 * WAVE)) % NWAVES == wave); b; b &= b - 1)
+        hits |= 1ull << min(63, rl_i(o.id[i], __builtin_ctzll(b)) / (8 * T));
   RowStat st{-INFINITY, 0.0f, 0.0f};
-  auto add = [&](const RowVec<DT>& q, int w0, bool hit) {
-    float f[8], mx = -INFINITY;
+  // two vectors at a time
+  auto add = [&](const RowVec<DT>& q0, const RowVec<DT>& q1, int w0, int w1, bool hit0, bool hit1) {
+    float f[16], mx = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = q.at(j);
-    if (TAIL && hit) without_hits<DT>(f, o.id, w0);
+    for (int j = 0; j < 8; ++j) {
+      f[j] = q0.at(j);
+      f[8 + j] = q1.at(j);
+    }
+    if constexpr (TAIL) {
+      if (hit0) without_hits<DT>(*(float(*)[8])&f[0], o.id, w0);
+      if (hit1) without_hits<DT>(*(float(*)[8])&f[8], o.id, w1);
+    }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, f[j]);
-    stat_add<8, false>(st, f, mx, c);
+    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, f[j]);
+    stat_add<16, false>(st, f, mx, c);
   };
+  RowVec<DT> none;
 #pragma unroll
-  for (int u = 0; u < NV; ++u) {
-    add(x[u], 8 * WAVE * (u * NWAVES + wave), (hits >> u) & 1u);
+  for (int i = 0; i < RowVec<DT>::WORDS; ++i) none.w[i] = DT == STRIM_DTYPE_BF16 ? 0xFF80FF80u : NINF_BITS;
+#pragma unroll
+  for (int u = 0; u < NV; u += 2) {
+    const int w0 = 8 * WAVE * (u * NWAVES + wave), w1 = w0 + 8 * T;
+    add(x[u], u + 1 < NV ? x[u + 1] : none, w0, w1, (hits >> u) & 1u, u + 1 < NV && ((hits >> (u + 1)) & 1u));
     x[u].renew();  // (568 bytes a lane spilled without)
+    if (u + 1 < NV) x[u + 1].renew();
   }
-  for (int v0 = 8 * NV * T; v0 < a.V; v0 += 8 * T) {
-    RowVec<DT> q;
-    q.load_to(row, v0 + 8 * WAVE * wave, lane, a.V);
-    add(q, v0 + 8 * WAVE * wave, true);
+  for (int v0 = 8 * NV * T; v0 < a.V; v0 += 16 * T) {
+    const int w0 = v0 + 8 * WAVE * wave, w1 = w0 + 8 * T;
+    RowVec<DT> q0, q1;
+    q0.load_to(row, w0, lane, a.V);
+    q1.load_to(row, w1, lane, a.V);
+    add(q0, q1, w0, w1, true, true);
   }
   stat_wave(st, c);
   if (lane == 0) s_stat[wave] = st;
@@ -463,15 +518,13 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
     const Teacher t = teacher_of(o, TAIL);
     const double w = (double)a.weights[r] / a.T;
     bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};
-    list_out(s_list, o, t, a.M, w, first, s_list.repeats != 0);
-    RowNumbers n{0.0, 0.0, 0.0, 0.0};
-    if (o.any) {
-      float xa[2];
+    float xa[2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) xa[i] = o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
-      n = numbers_of(o, t, first, xa, st, a.T, TAIL);
-    }
-    const GradRow g = grad_row(o.any, t, (float)n.top, n.ls, n.log_rest, w);
+    for (int i = 0; i < 2; ++i) xa[i] = o.any && o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
+    list_out(s_list, o, t, a.M, w, xa, first, s_list.repeats != 0);
+    RowNumbers n{0.0, 0.0, 0.0, 0.0};
+    if (o.any) n = numbers_of(o, t, first, xa, st, a.T, TAIL);
+    const GradRow g = grad_row(o.any, t, (float)n.top, n.ls, n.log_rest, w, c);
     if (lane == 0) {
       s_grad = g;
       const float loss = (float)n.loss;
@@ -482,19 +535,26 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
   }
   __syncthreads();
   const GradRow g = s_grad;
-  const int id[2] = {s_list.id[lane], s_list.id[lane + WAVE]};
-  const float less[2] = {s_list.p[lane], s_list.p[lane + WAVE]};
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     const int w0 = 8 * WAVE * (u * NWAVES + wave);
-    if (w0 < a.V)
-      grad_of<DT>(x[u], g, c, id, less, w0, (hits >> u) & 1u).store_to(out, w0, lane, a.V, a.stream);
+    if (w0 < a.V) grad_of<DT>(x[u], g, c).store_to(out, w0, lane, a.V, a.stream);
   }
   for (int w0 = 8 * (NV * T + WAVE * wave); w0 < a.V; w0 += 8 * T) {
     RowVec<DT> q;
     q.load_to(row, w0, lane, a.V);
-    grad_of<DT>(q, g, c, id, less, w0, true).store_to(out, w0, lane, a.V, a.stream);
+    grad_of<DT>(q, g, c).store_to(out, w0, lane, a.V, a.stream);
   }
+  int id[2];
+  float xa[2], less[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    id[i] = s_list.id[lane + i * WAVE];
+    xa[i] = s_list.x[lane + i * WAVE];
+    less[i] = s_list.p[lane + i * WAVE];
+    if (id[i] >= 0 && id[i] / (8 * WAVE) % NWAVES != wave) id[i] = -1;
+  }
+  grad_alternatives<DT>(out, g, c, id, xa, less);
 }
 
 // (a factor of 1, what the last step of a backward pass usually has, costs no pass over the data)
@@ -515,16 +575,19 @@ __global__ __launch_bounds__(DI_T) void k_distill_scale(char* data, int64_t n, c
 int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Parts of a row: about eight workgroups a CU in all, one a row where there are that many.
-DistillParts distill_parts(int N, int V) {
+// Parts of a row: a round of workgroups over the chip (eight a CU), one a row where there are that many rows;
+// float32 rows, whose kernels hold fewer, in two rounds (N = 500, V = 50,021: 29.0 -> 26.4 us).
+DistillParts distill_parts(int N, int V, bool bf16) {
   DistillParts q{};
-  const int64_t tiles = ceil_of(V, DI_TILE), each = (int64_t)N * tiles / 2048;
-  q.tiles = (int32_t)(each < 1 ? 1 : each > tiles ? tiles : each);
+  const int64_t tiles = ceil_of(V, DI_TILE), each = ceil_of((int64_t)N * tiles, bf16 ? 2048 : 4096);
+  q.tiles = (int32_t)(each > tiles ? tiles : each);
   q.parts = (int32_t)ceil_of(tiles, q.tiles);
   return q;
 }
-// Rows from which a step keeps each in a workgroup.
-constexpr int DI_WHOLE = 192;
+// Whether a step keeps each row in a workgroup: always where four vectors a thread hold it (N = 1, V = 32,768:
+// 7.9 us, in parts 14.2), else from half a round of rows on (V = 151,936: N = 128 35.1 us, in parts 37.1; N =
+// 64 about 35, in parts 25.4).
+bool whole_rows(int N, int V) { return N >= 128 || V <= 8 * 1024 * 4; }
 
 template <class F>
 void with_dtype(bool bf16, F f) {
@@ -532,18 +595,8 @@ void with_dtype(bool bf16, F f) {
   else f(std::integral_constant<int, STRIM_DTYPE_F32>{});
 }
 
-void launch_grad(const DistillArgs& a, bool bf16, hipStream_t st) {
-  // (a launch has fewer than 2^32 threads)
-  const DistillParts q = distill_parts(a.N, a.V);
-  with_dtype(bf16, [&](auto dt) {
-    hipLaunchKernelGGL((k_distill_grad<decltype(dt)::value>), dim3((unsigned)((int64_t)a.N * q.parts)), dim3(DI_T), 0,
-                       st, a, q);
-  });
-}
-
 template <int DT, bool TAIL>
 void launch_whole(const DistillArgs& a, hipStream_t st) {
-  constexpr int WIDE = DT == STRIM_DTYPE_BF16 ? 19 : 9;
   constexpr int MOST = 1 << 21;  // (a launch has fewer than 2^32 threads)
   for (int r0 = 0; r0 < a.N; r0 += MOST) {
     DistillArgs b = a;
@@ -559,9 +612,13 @@ void launch_whole(const DistillArgs& a, hipStream_t st) {
     auto go = [&](auto kernel, int threads) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)b.N), dim3(threads), 0, st, b);
     };
+    // The whole row in registers, or, where there are rows for it, half of it with two workgroups a CU, one
+    // of which reads while the other writes (V = 151,936, 2 GB read and written, N = 4,096: 587 -> 570 us; N =
+    // 128 35 -> 43; V = 248,320, N = 1,024, where only a third would be held: 254 -> 286).
     if (a.V <= 8 * 256 * 4) go(k_distill_step<DT, 256, 4, TAIL>, 256);
     else if (a.V <= 8 * 1024 * 4) go(k_distill_step<DT, 1024, 4, TAIL>, 1024);
-    else go(k_distill_step<DT, 1024, WIDE, TAIL>, 1024);
+    else if (DT == STRIM_DTYPE_BF16 && a.N > 256 && a.V <= 8 * 1024 * 19) go(k_distill_step<DT, 512, 19, TAIL>, 512);
+    else go(k_distill_step<DT, 1024, DT == STRIM_DTYPE_BF16 ? 19 : 9, TAIL>, 1024);
   }
 }
 
@@ -569,41 +626,42 @@ void launch_whole(const DistillArgs& a, hipStream_t st) {
 
 int64_t distill_workspace(int N, int V, int M, bool step) {
   (void)M;
-  if (step && N >= DI_WHOLE) return 0;
-  const int64_t part = up16((int64_t)N * distill_parts(N, V).parts * (int64_t)sizeof(RowStat));
-  return part + (step ? 2 * up16(4 * (int64_t)N) : 0);
+  if (step && whole_rows(N, V)) return 0;
+  // (the parts of the type that has more)
+  const int64_t parts = distill_parts(N, V, true).parts, most = distill_parts(N, V, false).parts;
+  return up16((int64_t)N * (parts > most ? parts : most) * (int64_t)sizeof(RowStat)) +
+         (step ? (int64_t)N * (int64_t)sizeof(GradRecord) : 0);
 }
 
 hipError_t launch_distill(const DistillArgs& given, bool bf16, bool loss, bool grad, void* workspace,
                           hipStream_t st) {
   DistillArgs a = given;
   a.stream = grad && (int64_t)a.N * a.V * (bf16 ? 2 : 4) > ROWS_CACHED;
-  if (loss && grad && a.N >= DI_WHOLE) {
+  const bool step = loss && grad;
+  if (step && whole_rows(a.N, a.V)) {
     with_dtype(bf16, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       a.tail ? launch_whole<DT, true>(a, st) : launch_whole<DT, false>(a, st);
     });
     return hipGetLastError();
   }
+  DistillParts q = distill_parts(a.N, a.V, bf16);
   if (loss) {
-    DistillParts q = distill_parts(a.N, a.V);
-    q.part = (RowStat*)workspace;
-    if (grad) {
-      char* rows = (char*)workspace + up16((int64_t)a.N * q.parts * (int64_t)sizeof(RowStat));
-      a.out_lse = (float*)rows;
-      a.out_log_rest = (float*)(rows + up16(4 * (int64_t)a.N));
-      a.lse = a.out_lse;
-      a.log_rest = a.out_log_rest;
-    }
-    with_dtype(bf16, [&](auto dt) {
-      constexpr int DT = decltype(dt)::value;
-      const dim3 grid((unsigned)((int64_t)a.N * q.parts));
-      if (a.tail) hipLaunchKernelGGL((k_distill_stat<DT, true>), grid, dim3(DI_T), 0, st, a, q);
-      else hipLaunchKernelGGL((k_distill_stat<DT, false>), grid, dim3(DI_T), 0, st, a, q);
-      hipLaunchKernelGGL(k_distill_join<DT>, dim3((unsigned)ceil_of(a.N, DI_T / WAVE)), dim3(DI_T), 0, st, a, q);
-    });
+    q.record = (GradRecord*)workspace;
+    q.part = (RowStat*)(step ? (void*)(q.record + a.N) : workspace);
   }
-  if (grad) launch_grad(a, bf16, st);
+  const dim3 grid((unsigned)((int64_t)a.N * q.parts)), threads(DI_T), rows((unsigned)a.N);
+  with_dtype(bf16, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (loss) {
+      if (a.tail) hipLaunchKernelGGL((k_distill_stat<DT, true>), grid, threads, 0, st, a, q);
+      else hipLaunchKernelGGL((k_distill_stat<DT, false>), grid, threads, 0, st, a, q);
+      if (step) hipLaunchKernelGGL((k_distill_join<DT, true>), rows, dim3(WAVE), 0, st, a, q);
+      else hipLaunchKernelGGL((k_distill_join<DT, false>), rows, dim3(WAVE), 0, st, a, q);
+    }
+    if (step) hipLaunchKernelGGL((k_distill_grad<DT, true>), grid, threads, 0, st, a, q);
+    else if (grad) hipLaunchKernelGGL((k_distill_grad<DT, false>), grid, threads, 0, st, a, q);
+  });
   return hipGetLastError();
 }
 
