@@ -22,7 +22,7 @@ namespace {
 
 // A lane's eight columns from k0 on, as RowVec<DT, G> has a row's: of a weight or bias of either type (`none`
 // where there is no tensor, 0 past K), and of a float32 row of sums.
-template <int DT, int G>
+template <int DT, int G, bool EVEN>
 __device__ __forceinline__ void param8(const void* p, bool bf16, int k0, int lane, int K, float none, float (&f)[8]) {
   typedef RowVec<DT, G> X;
 #pragma unroll
@@ -30,7 +30,7 @@ __device__ __forceinline__ void param8(const void* p, bool bf16, int k0, int lan
   if (!p) return;
   if (bf16 == X::BF16) {
     X v;
-    v.template load_to<true>((const char*)p, k0, lane, K);
+    v.template load_to<true, false, EVEN>((const char*)p, k0, lane, K);
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = v.at(j);
     return;
@@ -60,13 +60,13 @@ __device__ __forceinline__ void param8(const void* p, bool bf16, int k0, int lan
     if (at < K) f[j] = bf16 ? bf16_to_f32(((const uint16_t*)p)[at]) : ((const float*)p)[at];
   }
 }
-template <int DT, int G>
+template <int DT, int G, bool EVEN>
 __device__ __forceinline__ void sums8(float* out, int k0, int lane, int K, const float (&f)[8]) {
   typedef RowVec<DT, G> X;
   if constexpr (!X::BF16) {
     X v;
     v.set(f);
-    v.store_to((char*)out, k0, lane, K);
+    v.template store_to<EVEN>((char*)out, k0, lane, K);
   } else {
     const int k = k0 + 8 * lane;
     if (k + 8 <= K) {
@@ -77,6 +77,7 @@ __device__ __forceinline__ void sums8(float* out, int k0, int lane, int K, const
                    __float_as_uint(f[4 * i + 3])};
       return;
     }
+    if (EVEN) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (k + j < K) out[k + j] = f[j];
@@ -113,18 +114,32 @@ struct NormShape {
   static constexpr int G = L < WAVE ? L : WAVE;  // lanes that share a vector's columns
 };
 
-template <int DT, int L, int NV, bool CENTER>
+// The weights as the rows' lanes hold them where both are of one type (`same`), asked for beside the row and
+// not after its sums (N = 4,096, K = 5,120: 25.1 -> 23.0 us). With four vectors a lane they would cost the
+// waves that hide the loads (K = 8,192: 33.4 us without, 38.2 with).
+template <class X, int L, int NV, bool EVEN>
+__device__ __forceinline__ void held_params(X (&w)[NV], const void* p, bool same, int g0, int lane, int K) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (p && same) w[i].template load_to<true, false, EVEN>((const char*)p, 8 * L * i + g0, lane, K);
+}
+
+template <int DT, int L, int NV, bool CENTER, bool EVEN>
 __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool wbf16) {
   constexpr int ROWS = NormShape<L>::ROWS, G = NormShape<L>::G;
   typedef RowVec<DT, G> X;
-  __shared__ float s_sum[2][16];
+  __shared__ float s_sum[2][2][16];
   const int l = threadIdx.x % L, lane = l % G, g0 = 8 * (l - lane);  // (of the row, of its group; the group's)
   const float inv = 1.0f / (float)a.K;
-  for (int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L; n < a.N; n += (int64_t)gridDim.x * ROWS) {
+  const bool same = NV < 4 && wbf16 == X::BF16;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
+  for (int turn = 0; n < a.N; n += step, turn ^= 1) {
+    X x[NV], wv[NV];
     const char* row = (const char*)a.x + n * a.x_stride * X::SIZE;
-    X x[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i].template load_to<true>(row, 8 * L * i + g0, lane, a.K);
+    for (int i = 0; i < NV; ++i) x[i].template load_to<true, false, EVEN>(row, 8 * L * i + g0, lane, a.K);
+    held_params<X, L, NV, EVEN>(wv, a.weight, same, g0, lane, a.K);  // (beside the row, not after its sums)
     float mu = 0.0f;
     if constexpr (CENTER) {
       float s = 0.0f;
@@ -132,7 +147,7 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) s += x[i].at(j);
-      mu = row_sum<L>(s, s_sum[0]) * inv;
+      mu = row_sum<L>(s, s_sum[turn][0]) * inv;
     }
     float q = 0.0f;
 #pragma unroll
@@ -140,37 +155,150 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool
       const int left = a.K - 8 * L * i - g0 - X::first(lane);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float c = !CENTER ? x[i].at(j) : X::step(j) < left ? x[i].at(j) - mu : 0.0f;
+        const float c = !CENTER ? x[i].at(j) : (EVEN ? X::step(j & ~3) : X::step(j)) < left ? x[i].at(j) - mu : 0.0f;
         q = fma_f(c, c, q);
       }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) x[i].renew();
-    const float rstd = 1.0f / sqrtf(row_sum<L>(q, s_sum[1]) * inv + a.eps);
+    const float rstd = 1.0f / sqrtf(row_sum<L>(q, s_sum[turn][1]) * inv + a.eps);
     char* out = (char*)a.y + n * a.y_stride * X::SIZE;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int k0 = 8 * L * i + g0;
       float f[8], w[8], b[8];
-      param8<DT, G>(a.weight, wbf16, k0, lane, a.K, 1.0f, w);
-      param8<DT, G>(a.bias, wbf16, k0, lane, a.K, 0.0f, b);
+      if (same) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = fma_f((x[i].at(j) - mu) * rstd, w[j], b[j]);
+        for (int j = 0; j < 8; ++j) w[j] = a.weight ? wv[i].at(j) : 1.0f;
+      } else {
+        param8<DT, G, EVEN>(a.weight, wbf16, k0, lane, a.K, 1.0f, w);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = (x[i].at(j) - mu) * rstd;
+      if (a.bias) {
+        param8<DT, G, EVEN>(a.bias, wbf16, k0, lane, a.K, 0.0f, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = fma_f(f[j], w[j], b[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= w[j];
+      }
       X y;
       y.set(f);
-      y.store_to(out, k0, lane, a.K);
+      y.template store_to<EVEN>(out, k0, lane, a.K);
     }
     if (l == 0) {
       if (a.rstd) a.rstd[n] = rstd;
       if (CENTER) a.mean[n] = mu;
     }
-    if (!CENTER && L > WAVE) __syncthreads();  // (one place for the sums alone)
+  }
+}
+
+// Rows too wide for registers: read again (from the caches) for each step. A workgroup of 1,024 a row.
+template <int DT, bool CENTER>
+__global__ __launch_bounds__(1024) void k_norm_wide(const NormArgs a, bool wbf16) {
+  constexpr int T = 1024;
+  typedef RowVec<DT> X;
+  __shared__ float s_sum[2][2][16];
+  const int lane = threadIdx.x & (WAVE - 1), g0 = 8 * WAVE * wave_id();
+  const float inv = 1.0f / (float)a.K;
+  int turn = 0;
+  for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x, turn ^= 1) {
+    const char* row = (const char*)a.x + n * a.x_stride * X::SIZE;
+    float mu = 0.0f, q = 0.0f;
+    if constexpr (CENTER) {
+      float s = 0.0f;
+#pragma unroll 2
+      for (int k0 = g0; k0 < a.K; k0 += 8 * T) {
+        X x;
+        x.template load_to<true>(row, k0, lane, a.K);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += x.at(j);
+      }
+      mu = row_sum<T>(s, s_sum[turn][0]) * inv;
+    }
+#pragma unroll 2
+    for (int k0 = g0; k0 < a.K; k0 += 8 * T) {
+      X x;
+      x.template load_to<true>(row, k0, lane, a.K);
+      const int left = a.K - k0 - X::first(lane);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float c = !CENTER ? x.at(j) : X::step(j) < left ? x.at(j) - mu : 0.0f;
+        q = fma_f(c, c, q);
+      }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<T>(q, s_sum[turn][1]) * inv + a.eps);
+    char* out = (char*)a.y + n * a.y_stride * X::SIZE;
+    for (int k0 = g0; k0 < a.K; k0 += 8 * T) {
+      X x;
+      x.template load_to<true>(row, k0, lane, a.K);
+      float f[8], w[8], b[8];
+      param8<DT, WAVE, false>(a.weight, wbf16, k0, lane, a.K, 1.0f, w);
+      param8<DT, WAVE, false>(a.bias, wbf16, k0, lane, a.K, 0.0f, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = fma_f((x.at(j) - mu) * rstd, w[j], b[j]);
+      x.set(f);
+      x.store_to(out, k0, lane, a.K);
+    }
+    if (threadIdx.x == 0) {
+      if (a.rstd) a.rstd[n] = rstd;
+      if (CENTER) a.mean[n] = mu;
+    }
+  }
+}
+template <int DT, bool CENTER>
+__global__ __launch_bounds__(1024) void k_norm_grad_wide(const NormGradArgs a, bool wbf16) {
+  constexpr int T = 1024;
+  typedef RowVec<DT> X;
+  __shared__ float s_sum[2][2][16];
+  const int lane = threadIdx.x & (WAVE - 1), g0 = 8 * WAVE * wave_id();
+  const float inv = 1.0f / (float)a.K;
+  int turn = 0;
+  for (int64_t n = blockIdx.x; n < a.N; n += gridDim.x, turn ^= 1) {
+    const char* xr = (const char*)a.x + n * a.x_stride * X::SIZE;
+    const char* gr = (const char*)a.dy + n * a.dy_stride * X::SIZE;
+    char* out = (char*)a.dx + n * a.dx_stride * X::SIZE;
+    const float rstd = a.rstd[n], mu = CENTER ? a.mean[n] : 0.0f;
+    // xh, h of eight columns
+    auto each = [&](int k0, float (&xh)[8], float (&h)[8]) {
+      X x, g;
+      x.template load_to<true>(xr, k0, lane, a.K);
+      g.template load_to<true>(gr, k0, lane, a.K);
+      param8<DT, WAVE, false>(a.weight, wbf16, k0, lane, a.K, 1.0f, h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        xh[j] = (x.at(j) - mu) * rstd;
+        h[j] *= g.at(j);
+      }
+    };
+    float c1 = 0.0f, c2 = 0.0f;
+    for (int k0 = g0; k0 < a.K; k0 += 8 * T) {
+      float xh[8], h[8];
+      each(k0, xh, h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        c1 = fma_f(h[j], xh[j], c1);
+        c2 += h[j];
+      }
+    }
+    c1 = row_sum<T>(c1, s_sum[turn][0]) * inv;
+    c2 = CENTER ? row_sum<T>(c2, s_sum[turn][1]) * inv : 0.0f;
+    for (int k0 = g0; k0 < a.K; k0 += 8 * T) {
+      float xh[8], h[8];
+      each(k0, xh, h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] = rstd * (fma_f(-xh[j], c1, h[j]) - c2);
+      X y;
+      y.set(h);
+      y.store_to(out, k0, lane, a.K);
+    }
   }
 }
 
 // PARAM 1: also the workgroup's sums of dy xh, to row blockIdx.x of `part` [grid][PARAM][K]; 2: of dy too.
 // (Past K dy is 0, so that nothing there counts.)
-template <int DT, int L, int NV, bool CENTER, int PARAM>
+template <int DT, int L, int NV, bool CENTER, int PARAM, bool EVEN>
 __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArgs a, bool wbf16, float* part) {
   constexpr int ROWS = NormShape<L>::ROWS, G = NormShape<L>::G;
   typedef RowVec<DT, G> X;
@@ -185,34 +313,35 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
     const char* g = (const char*)a.dy + n * a.dy_stride * X::SIZE;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      nx[i].template load_to<true>(x, 8 * L * i + g0, lane, a.K);
-      ng[i].template load_to<true>(g, 8 * L * i + g0, lane, a.K);
+      nx[i].template load_to<true, false, EVEN>(x, 8 * L * i + g0, lane, a.K);
+      ng[i].template load_to<true, false, EVEN>(g, 8 * L * i + g0, lane, a.K);
     }
     nr = a.rstd[n];
     if (CENTER) nm = a.mean[n];
   };
   int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
   if (PARAM && n < a.N) request(n);
-  // (a row of its own for each workgroup: the weights are read where they are used)
+  // (without the sums each workgroup has a row of its own: the weights are read where they are used)
   float held[PARAM ? NV : 1][8], dw[PARAM > 0 ? NV : 1][8], db[PARAM > 1 ? NV : 1][8];
   auto weight = [&](int i, float (&w)[8]) {
     if constexpr (PARAM > 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = held[i][j];
     } else {
-      param8<DT, G>(a.weight, wbf16, 8 * L * i + g0, lane, a.K, 1.0f, w);
+      param8<DT, G, EVEN>(a.weight, wbf16, 8 * L * i + g0, lane, a.K, 1.0f, w);
     }
   };
-  if constexpr (PARAM > 0)
+  if constexpr (PARAM > 0) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      param8<DT, G>(a.weight, wbf16, 8 * L * i + g0, lane, a.K, 1.0f, held[i]);
+      param8<DT, G, EVEN>(a.weight, wbf16, 8 * L * i + g0, lane, a.K, 1.0f, held[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         dw[i][j] = 0.0f;
         if (PARAM > 1) db[i][j] = 0.0f;
       }
     }
+  }
   for (int turn = 0; n < a.N; n += step, turn ^= 1) {
     if (!PARAM) request(n);
     X x[NV], g[NV];
@@ -278,36 +407,35 @@ __global__ __launch_bounds__(NormShape<L>::T) void k_norm_grad(const NormGradArg
       }
       X y;
       y.set(d);
-      y.store_to(out, 8 * L * i + g0, lane, a.K);
+      y.template store_to<EVEN>(out, 8 * L * i + g0, lane, a.K);
     }
   }
   if constexpr (PARAM > 0) {
     float* out = part + (int64_t)blockIdx.x * PARAM * a.K;
     if constexpr (ROWS > 1) {
       // the workgroup's rows first
-      __shared__ float s_acc[PARAM][ROWS][8 * L * NV];
+      __shared__ float s_acc[ROWS][8 * L * NV];
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
+      for (int h = 0; h < PARAM; ++h) {
+        if (h) __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int k = 8 * L * i + g0 + X::first(lane) + X::step(j);
-          s_acc[0][threadIdx.x / L][k] = dw[i][j];
-          if constexpr (PARAM > 1) s_acc[1][threadIdx.x / L][k] = db[i][j];
-        }
-      __syncthreads();
-      for (int k = threadIdx.x; k < a.K; k += NormShape<L>::T)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int h = 0; h < PARAM; ++h) {
+          for (int j = 0; j < 8; ++j)
+            s_acc[threadIdx.x / L][8 * L * i + g0 + X::first(lane) + X::step(j)] = h == 0 ? dw[i][j] : db[PARAM > 1 ? i : 0][j];
+        __syncthreads();
+        for (int k = threadIdx.x; k < a.K; k += NormShape<L>::T) {
           float s = 0.0f;
 #pragma unroll
-          for (int q = 0; q < ROWS; ++q) s += s_acc[h][q][k];
+          for (int q = 0; q < ROWS; ++q) s += s_acc[q][k];
           out[h * a.K + k] = s;
         }
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        sums8<DT, G>(out, 8 * L * i + g0, lane, a.K, dw[i]);
-        if constexpr (PARAM > 1) sums8<DT, G>(out + a.K, 8 * L * i + g0, lane, a.K, db[i]);
+        sums8<DT, G, EVEN>(out, 8 * L * i + g0, lane, a.K, dw[i]);
+        if constexpr (PARAM > 1) sums8<DT, G, EVEN>(out + a.K, 8 * L * i + g0, lane, a.K, db[i]);
       }
     }
   }
@@ -333,8 +461,8 @@ __global__ __launch_bounds__(256) void k_norm_columns(const NormGradArgs a, floa
     }
   }
   float* out = part + (int64_t)blockIdx.y * PARAM * a.K;
-  sums8<DT, WAVE>(out, k0, lane, a.K, dw);
-  if constexpr (PARAM > 1) sums8<DT, WAVE>(out + a.K, k0, lane, a.K, db);
+  sums8<DT, WAVE, false>(out, k0, lane, a.K, dw);
+  if constexpr (PARAM > 1) sums8<DT, WAVE, false>(out + a.K, k0, lane, a.K, db);
 }
 
 // dw and db from the workgroups' rows of `width` sums (K of dw, then K of db), added in order: 64 columns a
@@ -376,35 +504,42 @@ __global__ __launch_bounds__(256) void k_norm_zero(int K, void* dw, void* db, bo
 
 int64_t ceil_of(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// The threads that hold a row, and their vectors: f(L, NV).
+// The threads that hold a row, and their vectors, f(L, NV). False past what registers hold. Forward and
+// backward in us at N = 20,000 with 4 vectors or fewer a lane of a wave a row, and with a workgroup a row:
+// K = 1,024 19.6, 29.8 and 25.5, 40.6 (N = 1,100: 3.3, 7.7 and 3.6, 8.7), K = 2,048 37.8, 53.8 and 32.0, 52.5.
 template <class F>
-void with_shape(int K, F f) {
+bool with_shape(int K, F f) {
   using std::integral_constant;
-  auto go = [&](auto l, auto nv) { f(l, nv); };
-#define STRIM_SHAPE(L, NV) \
-  if (K <= 8 * L * NV) return go(integral_constant<int, L>{}, integral_constant<int, NV>{})
-  STRIM_SHAPE(16, 1);
-  STRIM_SHAPE(64, 1);
-  STRIM_SHAPE(256, 1);
-  STRIM_SHAPE(256, 2);
-  STRIM_SHAPE(256, 3);
-  STRIM_SHAPE(256, 4);
-  STRIM_SHAPE(1024, 2);
-  STRIM_SHAPE(1024, 4);
-  STRIM_SHAPE(1024, 8);
+#define STRIM_SHAPE(L, NV)                                             \
+  if (K <= 8 * L * NV) {                                               \
+    f(integral_constant<int, L>{}, integral_constant<int, NV>{});      \
+    return true;                                                       \
+  }
+  STRIM_SHAPE(16, 1)
+  STRIM_SHAPE(64, 1)
+  STRIM_SHAPE(64, 2)
+  STRIM_SHAPE(256, 1)
+  STRIM_SHAPE(256, 2)
+  STRIM_SHAPE(256, 3)
+  STRIM_SHAPE(256, 4)
+  STRIM_SHAPE(1024, 2)
 #undef STRIM_SHAPE
+  return false;
 }
 constexpr int NO_WIDE = 8 * 256 * 4;  // columns past which the weights' gradients have a pass of their own
-int rows_at_once(int K) { return K <= 8 * 16 ? 16 : K <= 8 * 64 ? 4 : 1; }
+int rows_at_once(int K) {
+  int rows = 1;
+  with_shape(K, [&](auto l, auto) { rows = NormShape<decltype(l)::value>::ROWS; });
+  return rows;
+}
 
 // Workgroups of the gradient's pass with the weights' sums: two a CU, or fewer with four rows each.
 int norm_parts(int N, int K) {
   const int64_t groups = ceil_of(N, rows_at_once(K));
   if (K > NO_WIDE) return (int)(groups < 64 ? groups : 64);
-  const int64_t most = rows_at_once(K) > 1 ? 1024 : 512;
   int64_t g = ceil_of(groups, 4);
   if (g < 128) g = groups < 128 ? groups : 128;
-  return (int)(g < most ? g : most);
+  return (int)(g < 512 ? g : 512);
 }
 
 template <class F>
@@ -417,14 +552,20 @@ void with_dtype(bool bf16, F f) {
 
 hipError_t launch_norm(const NormArgs& a, bool bf16, bool wbf16, hipStream_t st) {
   with_dtype(bf16, [&](auto dt) {
-    with_shape(a.K, [&](auto l, auto nv) {
-      constexpr int DT = decltype(dt)::value, L = decltype(l)::value, NV = decltype(nv)::value;
-      int64_t grid = ceil_of(a.N, NormShape<L>::ROWS);
-      if (grid > 1 << 20) grid = 1 << 20;
-      const dim3 g((unsigned)grid), t(NormShape<L>::T);
-      if (a.mean) hipLaunchKernelGGL((k_norm<DT, L, NV, true>), g, t, 0, st, a, wbf16);
-      else hipLaunchKernelGGL((k_norm<DT, L, NV, false>), g, t, 0, st, a, wbf16);
+    constexpr int DT = decltype(dt)::value;
+    auto go = [&](auto kernel, int64_t groups, int64_t most, int threads) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < most ? groups : most)), dim3(threads), 0, st, a, wbf16);
+    };
+    const bool held = with_shape(a.K, [&](auto l, auto nv) {
+      constexpr int L = decltype(l)::value, NV = decltype(nv)::value, T = NormShape<L>::T;
+      const int64_t groups = ceil_of(a.N, NormShape<L>::ROWS);
+      constexpr int64_t MOST = 1 << 20;
+      if (a.K % RowVec<DT>::RUN == 0)
+        a.mean ? go(k_norm<DT, L, NV, true, true>, groups, MOST, T) : go(k_norm<DT, L, NV, false, true>, groups, MOST, T);
+      else
+        a.mean ? go(k_norm<DT, L, NV, true, false>, groups, MOST, T) : go(k_norm<DT, L, NV, false, false>, groups, MOST, T);
     });
+    if (!held) a.mean ? go(k_norm_wide<DT, true>, a.N, 512, 1024) : go(k_norm_wide<DT, false>, a.N, 512, 1024);
   });
   return hipGetLastError();
 }
@@ -452,19 +593,25 @@ hipError_t launch_norm_grad(const NormGradArgs& a, bool bf16, bool wbf16, void* 
       else param > 1 ? go(k_norm_columns<DT, false, 2>) : go(k_norm_columns<DT, false, 1>);
     }
     if (wide && !a.dx) return;
-    with_shape(a.K, [&](auto l, auto nv) {
-      constexpr int L = decltype(l)::value, NV = decltype(nv)::value;
-      const dim3 t(NormShape<L>::T);
-      auto go = [&](auto kernel, int64_t grid) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(grid < 1 << 20 ? grid : 1 << 20)), t, 0, st, a, wbf16, part);
+    auto go = [&](auto kernel, int64_t groups, int threads, auto... more) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(groups < 1 << 20 ? groups : 1 << 20)), dim3(threads), 0, st, a, wbf16,
+                         more...);
+    };
+    const bool held = with_shape(a.K, [&](auto l, auto nv) {
+      constexpr int L = decltype(l)::value, NV = decltype(nv)::value, T = NormShape<L>::T;
+      auto as = [&](auto center, auto even) {
+        constexpr bool C = decltype(center)::value, E = decltype(even)::value;
+        if constexpr (L < 1024) {
+          if (param == 2) return go(k_norm_grad<DT, L, NV, C, 2, E>, parts, T, part);
+          if (param == 1) return go(k_norm_grad<DT, L, NV, C, 1, E>, parts, T, part);
+        }
+        go(k_norm_grad<DT, L, NV, C, 0, E>, ceil_of(a.N, NormShape<L>::ROWS), T, part);
       };
-      if constexpr (L < 1024) {
-        if (param == 2) return a.mean ? go(k_norm_grad<DT, L, NV, true, 2>, parts) : go(k_norm_grad<DT, L, NV, false, 2>, parts);
-        if (param == 1) return a.mean ? go(k_norm_grad<DT, L, NV, true, 1>, parts) : go(k_norm_grad<DT, L, NV, false, 1>, parts);
-      }
-      const int64_t grid = ceil_of(a.N, NormShape<L>::ROWS);
-      a.mean ? go(k_norm_grad<DT, L, NV, true, 0>, grid) : go(k_norm_grad<DT, L, NV, false, 0>, grid);
+      const bool even = a.K % RowVec<DT>::RUN == 0;
+      if (a.mean) even ? as(std::true_type{}, std::true_type{}) : as(std::true_type{}, std::false_type{});
+      else even ? as(std::false_type{}, std::true_type{}) : as(std::false_type{}, std::false_type{});
     });
+    if (!held) a.mean ? go(k_norm_grad_wide<DT, true>, a.N, 1024) : go(k_norm_grad_wide<DT, false>, a.N, 1024);
   });
   if (param)
     hipLaunchKernelGGL(k_norm_join, dim3((unsigned)ceil_of((int64_t)param * a.K, WAVE)), dim3(NJ_T), 0, st, part, parts,

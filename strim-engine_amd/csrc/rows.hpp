@@ -53,14 +53,26 @@ struct RowVec {
       for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
     }
   }
-  // Those that lie before V; past them -inf, or 0.
-  template <bool ZERO = false, bool NT = false>
+  // Those that lie before V; past them -inf, or 0. EVEN: V is a multiple of RUN (less code, fewer registers).
+  template <bool ZERO = false, bool NT = false, bool EVEN = false>
   __device__ __forceinline__ void load_to(const char* row, int v0, int lane, int V) {
     const int v = v0 + first(lane);
+    const char* p = row + (int64_t)v * SIZE;
+    if constexpr (EVEN) {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i) {
+        constexpr uint32_t FILL = ZERO ? 0u : BF16 ? 0xFF80FF80u : NINF_BITS;
+        ru32x4 q{FILL, FILL, FILL, FILL};
+        const ru32x4_any* a = (const ru32x4_any*)(p + i * 4 * G * SIZE);
+        if (v + step(4 * i) < V) q = NT ? __builtin_nontemporal_load(a) : *a;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * i + j] = q[j];
+      }
+      return;
+    }
     if (v + step(7) < V) return load<NT>(row, v0, lane);
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) w[i] = ZERO ? 0u : BF16 ? 0xFF80FF80u : NINF_BITS;
-    const char* p = row + (int64_t)v * SIZE;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (v + step(j) < V) {
@@ -88,12 +100,14 @@ struct RowVec {
       for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(f[i]);
     }
   }
+  template <bool EVEN = false>
   __device__ __forceinline__ void store_to(char* row, int v0, int lane, int V, bool nt = false) const {
     const int v = v0 + first(lane);
     char* p = row + (int64_t)v * SIZE;
-    if (v + step(7) < V) {
+    if (EVEN || v + step(7) < V) {
 #pragma unroll
       for (int i = 0; i < WORDS / 4; ++i) {
+        if (EVEN && v + step(4 * i) >= V) continue;
         const ru32x4 q{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
         ru32x4_any* a = (ru32x4_any*)(p + i * 4 * G * SIZE);
         if (nt) __builtin_nontemporal_store(q, a);
