@@ -165,7 +165,7 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
   Given given{};
   if (q.parts == 1) given = given_of<DT>(a, r);
   st = stat_block(st, c, s_stat);
-  if constexpr (TOP) top.trim(s_top[0], most);
+  if constexpr (TOP) top.trim(s_top[0], most, q.parts == 1 ? a.top : q.room);
   if (q.parts == 1) {
     stat_exact(st, c);
     return score_finish(a, r, st, given, TOP ? s_top : nullptr, TOP ? top.held : 0);

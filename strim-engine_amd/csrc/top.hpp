@@ -198,9 +198,10 @@ struct TopRun {
     if (limit != before) --limit;
   }
 
-  // The list without what the threads' maxima show to be past the M-th.
-  __device__ __forceinline__ void trim(TopList& l, float most) {
-    if (held <= M || tile == 1) return;  // (after one tile the list is at its threshold)
+  // The list without what the threads' maxima show to be past the M-th, if longer than `few` (R = 64,
+  // V = 151,936, M = 5: 20.3 us with every list trimmed, 18.1 where longer than the join takes).
+  __device__ __forceinline__ void trim(TopList& l, float most, int few) {
+    if (held <= few || tile == 1) return;  // (after one tile the list is at its threshold)
     const uint32_t t = top_threshold(l, fkey_desc(most), TOP_ALL, M, by);
     held = top_cut(l, held, (uint64_t)t << 32 | 0xFFFFFFFFu);
   }
