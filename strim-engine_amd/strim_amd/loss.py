@@ -114,7 +114,9 @@ class _TokenScores(torch.autograd.Function):
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """[..., V] as [R, V] with contiguous rows."""
     rows = logits.reshape(-1, logits.shape[-1])
-    return rows if rows.stride(-1) == 1 else rows.contiguous()
+    # (one row broadcast over several has a stride of 0)
+    apart = rows.stride(1) == 1 and (rows.shape[0] < 2 or rows.stride(0) >= rows.shape[1])
+    return rows if apart else rows.contiguous()
 
 
 def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: int = 0,
@@ -165,6 +167,14 @@ class _Distill(torch.autograd.Function):
         return d, None, None, None, None
 
 
+def _sum(t: torch.Tensor) -> torch.Tensor:
+    """The sum of [N] numbers by one workgroup a time: over many numbers at once the library's sum
+    clears a counter, which is not safe to replay from a captured graph."""
+    while t.shape[0] > 4096:
+        t = torch.nn.functional.pad(t, (0, -t.shape[0] % 1024)).view(-1, 1024).sum(1)
+    return t.sum()
+
+
 class _DistillSum(torch.autograd.Function):
     """The rows' losses times their weights, summed; the gradient comes with the loss, from one pass
     over the logits."""
@@ -178,7 +188,7 @@ class _DistillSum(torch.autograd.Function):
         else:
             loss = ops.distill(logits, ids, logprobs, temperature, tail)[0]
         # (a row of weight 0 counts for nothing, an infinite or NaN loss included)
-        return torch.where(weights != 0, loss * weights, 0.0).sum()
+        return _sum(torch.where(weights != 0, loss * weights, 0.0))
 
     @staticmethod
     @once_differentiable
@@ -224,5 +234,6 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
         weights = torch.ones(rows.shape[0], dtype=torch.float32, device=rows.device)
     else:
         live = ((ids >= 0) & (logprobs != float("-inf"))).any(1) & (ids < V).all(1)
-        weights = live.float() / live.sum().clamp_min(1)
+        weights = live.float()
+        weights = weights / _sum(weights).clamp_min(1.0)  # (counts are exact in float32 up to 2^24)
     return _DistillSum.apply(rows, ids, logprobs, weights, temperature, tail)

@@ -179,3 +179,56 @@ def test_second_device():
     ref = step(*x, weights, M)
     got = step(*(t.to("cuda:1") for t in x), weights.to("cuda:1"), M)
     same([t.cpu() for t in got], [t.cpu() for t in ref])
+
+
+def test_a_row_broadcast_over_several():
+    """Expanded rows (stride 0) through the differentiable forms: the gradient is the rows' sum."""
+    V, M, R = 700, 8, 5
+    teacher, *_ = inputs(R, 16, V, M, torch.float32)
+    t = ops.token_scores(teacher, top=M)
+    row = torch.randn(V, device="cuda", generator=gen(1))
+    grads = []
+    for wide in (lambda r: r.expand(R, V), lambda r: r.repeat(R, 1)):
+        leaf = row.clone().requires_grad_()
+        x = wide(leaf)
+        s = loss.token_scores(x, t.top_ids[:, 0].contiguous(), top=2)
+        value = (loss.distill_loss(x, t.top_ids, t.top_logprobs) + s.logprobs.sum() + s.entropy.sum()
+                 + (norm.layer_norm(x) * teacher).sum())
+        grads.append(torch.autograd.grad(value, leaf)[0])
+    assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("R", [130, 20_011])
+def test_captured_loss_with_its_backward(R):
+    """The mean over many rows, forward and backward in a graph, replayed over changed inputs."""
+    V, M = 90, 6
+    teacher, *_ = inputs(R, 16, V, M, torch.float32)
+    x = torch.randn(R, V, device="cuda", generator=gen(1)).requires_grad_()
+    t = ops.token_scores(teacher, top=M)
+    ids, lps = t.top_ids.clone(), t.top_logprobs.clone()
+
+    def both():
+        value = loss.distill_loss(x, ids, lps, tail=True)
+        return [value.detach(), *torch.autograd.grad(value, x)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = both()
+    for turn in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(R, V, device="cuda", generator=gen(turn)))
+            lps[turn::7] = float("-inf")  # (rows without alternatives: the mean's count changes)
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        same(got, both())
+        live = (lps > float("-inf")).any(1)
+        rows = loss.distill_loss(x.detach(), ids, lps, tail=True, reduction="none")
+        # (N float32 sums in a tree of depth below 20: 20 2^-24 relative, the weights' rounding as well)
+        want = rows.double()[live].mean()
+        assert abs(got[0].double() - want) <= 2e-6 * rows.double()[live].abs().mean()

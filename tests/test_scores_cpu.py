@@ -141,8 +141,8 @@ def test_workspaces():
         for st in (False, True):
             need = ops.distill_workspace(R, V, max(1, top), st)
             if need:
-                a = dict(N=R, V=V, stride=V, M=max(1, top))
-                assert (step if st else distill)(**a, wsb=need - 1) == N.ECAPACITY
+                a = dict(N=R, V=V, stride=V, M=max(1, top), wsb=need - 1)
+                assert (step(**a, d_stride=V) if st else distill(**a)) == N.ECAPACITY
     for R, K in ((1, 1), (5000, 5120), (1 << 28, 64)):
         need = ops.norm_workspace(R, K, True, True)
         if need:
