@@ -216,6 +216,22 @@ def test_rows_of_every_kind(V, top, copies, dtype):
     check(x, torch.full((x.shape[0],), V - 1, dtype=torch.int32, device="cuda"), top, label=f"V={V}")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,top,copies", [(33_000, 5, 1), (151_936, 128, 1), (20_480, 128, 110), (70_001, 1, 40)])
+def test_rows_whose_waves_differ(V, top, copies, dtype):
+    """Plateaus and runs that fill some waves' lists and not others', ties across them."""
+    at = torch.arange(V)
+    part = at // 512 % 4  # (which wave of a workgroup meets a token)
+    base = torch.randn(V, generator=torch.Generator().manual_seed(3))
+    rows = [(at // 1500).float() / 8, -(at // 1500).float() / 8, torch.where(part == 0, at.float() / V * 40, base),
+            torch.where(part == 2, (at // 4096).float(), base.round()), torch.where(part == 1, 3.0, 2.5 + 0 * base),
+            torch.where(part == 3, base.round() + at // 16384, base.round() + (at // 16384).flip(0)),
+            torch.where(at // 2048 % 9 == 4, 7.0, base), (base * 4).round() / 4 + (at // 8192) * 0.25]
+    x = torch.stack(rows).to("cuda", dtype).repeat(copies, 1)
+    print(f"[scores] waves V={V} top={top} {dtype}", flush=True)
+    check(x, torch.full((x.shape[0],), 0, dtype=torch.int32, device="cuda"), top, label=f"V={V}")
+
+
 def test_statuses():
     """Empty rows, NaN and infinities in allowed and forbidden places, unknown and ignored tokens; what
     the others in the batch give is not touched."""
