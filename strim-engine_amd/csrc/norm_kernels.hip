@@ -114,9 +114,18 @@ struct NormShape {
   static constexpr int G = L < WAVE ? L : WAVE;  // lanes that share a vector's columns
 };
 
+// How many workgroups of k_norm take the rows, as many as the chip holds at once, each the next row's loads on
+// their way while it finishes one (N = 4,096, bf16: K = 5,120 23.0 -> 20.5 us, 8,192 33.7 -> 30.4, with mean 47.2 ->
+// 36.3, 16,384 61.9 -> 52.5; 131,072 rows of 128 14.9 -> 13.8). 0: a workgroup for every row or four, for the
+// shapes where that was as fast or faster (K = 1,024 with mean, N = 20,000: 20.6 us, against 22.4; float32, K =
+// 6,000, N = 3,000: 30.1 against 33.4; 131,072 float32 rows of 128 25.4 against 26.9).
+constexpr int norm_resident(int dt, int L, int NV) {
+  const bool bf16 = dt == STRIM_DTYPE_BF16;
+  return L == 1024 ? 256 : NV == 4 ? 512 : NV == 3 && bf16 ? 768 : NV == 1 && L <= WAVE && bf16 ? 2048 : 0;
+}
+
 // The weights as the rows' lanes hold them where both are of one type (`same`), asked for beside the row and
-// not after its sums (N = 4,096, K = 5,120: 25.1 -> 23.0 us). With four vectors a lane they would cost the
-// waves that hide the loads (K = 8,192: 33.4 us without, 38.2 with).
+// not after its sums (N = 4,096, K = 5,120: 25.1 -> 23.0 us).
 template <class X, int L, int NV, bool EVEN>
 __device__ __forceinline__ void held_params(X (&w)[NV], const void* p, bool same, int g0, int lane, int K) {
 #pragma unroll
@@ -127,19 +136,31 @@ __device__ __forceinline__ void held_params(X (&w)[NV], const void* p, bool same
 template <int DT, int L, int NV, bool CENTER, bool EVEN>
 __global__ __launch_bounds__(NormShape<L>::T) void k_norm(const NormArgs a, bool wbf16) {
   constexpr int ROWS = NormShape<L>::ROWS, G = NormShape<L>::G;
+  constexpr bool AHEAD = norm_resident(DT, L, NV) > 0;
   typedef RowVec<DT, G> X;
   __shared__ float s_sum[2][2][16];
   const int l = threadIdx.x % L, lane = l % G, g0 = 8 * (l - lane);  // (of the row, of its group; the group's)
   const float inv = 1.0f / (float)a.K;
-  const bool same = NV < 4 && wbf16 == X::BF16;
+  const bool same = wbf16 == X::BF16;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   int64_t n = (int64_t)blockIdx.x * ROWS + threadIdx.x / L;
-  for (int turn = 0; n < a.N; n += step, turn ^= 1) {
-    X x[NV], wv[NV];
+  X next[NV], wv[NV];
+  auto request = [&](int64_t n) {
     const char* row = (const char*)a.x + n * a.x_stride * X::SIZE;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x[i].template load_to<true, false, EVEN>(row, 8 * L * i + g0, lane, a.K);
-    held_params<X, L, NV, EVEN>(wv, a.weight, same, g0, lane, a.K);  // (beside the row, not after its sums)
+    for (int i = 0; i < NV; ++i) next[i].template load_to<true, false, EVEN>(row, 8 * L * i + g0, lane, a.K);
+  };
+  if (AHEAD && n < a.N) request(n);
+  if (AHEAD) held_params<X, L, NV, EVEN>(wv, a.weight, same, g0, lane, a.K);
+  for (int turn = 0; n < a.N; n += step, turn ^= 1) {
+    if (!AHEAD) {
+      request(n);
+      held_params<X, L, NV, EVEN>(wv, a.weight, same, g0, lane, a.K);  // (beside the row, not after its sums)
+    }
+    X x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = next[i];
+    if (AHEAD && n + step < a.N) request(n + step);
     float mu = 0.0f;
     if constexpr (CENTER) {
       float s = 0.0f;
@@ -559,7 +580,7 @@ hipError_t launch_norm(const NormArgs& a, bool bf16, bool wbf16, hipStream_t st)
     const bool held = with_shape(a.K, [&](auto l, auto nv) {
       constexpr int L = decltype(l)::value, NV = decltype(nv)::value, T = NormShape<L>::T;
       const int64_t groups = ceil_of(a.N, NormShape<L>::ROWS);
-      constexpr int64_t MOST = 1 << 20;
+      constexpr int64_t MOST = norm_resident(DT, L, NV) > 0 ? norm_resident(DT, L, NV) : 1 << 20;
       if (a.K % RowVec<DT>::RUN == 0)
         a.mean ? go(k_norm<DT, L, NV, true, true>, groups, MOST, T) : go(k_norm<DT, L, NV, false, true>, groups, MOST, T);
       else

@@ -98,7 +98,8 @@ def check(x, w, b, center, dy, eps=1e-5, label=""):
 SIZES = [(1, 1), (3, 1), (1, 7), (2, 8), (5, 33), (17, 64), (64, 128), (1000, 128), (33, 130), (7, 1003),
          (1, 5120), (130, 1024), (300, 2051), (2049, 512), (40, 5120), (600, 5120), (9, 8192), (5, 9001),
          (3, 20_000), (2, 65_536), (70_000, 16), (1, 256), (4099, 72), (1030, 1000), (2500, 514), (1025, 2047),
-         (513, 1500), (300, 6144), (30, 16_384), (30, 16_381)]
+         (513, 1500), (300, 6144), (30, 16_384), (30, 16_381), (800, 5120), (1600, 4100), (530, 8190), (530, 8192),
+         (270, 9001), (530, 16_384), (9000, 200), (9001, 260)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
