@@ -142,9 +142,6 @@ __global__ __launch_bounds__(SC_T, DT == STRIM_DTYPE_BF16 ? 8 : 6) void k_scores
         }
         mx = fmaxf(mx, mv[u]);
       }
-      // (requested into the registers that the tokens leave)
-#pragma unroll
-      for (int j = 0; j < 8 * SC_U; ++j) asm volatile("" : "+v"(x[j]));
       if (t + SC_TILE < t1) request(t + SC_TILE);
       stat_add<8 * SC_U, true>(st, x, mx, c);
       if constexpr (TOP)
