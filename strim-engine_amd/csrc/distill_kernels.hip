@@ -10,7 +10,7 @@
 // up. Those M numbers are in 64 bits: a small loss is the difference of much larger terms.
 //
 // k_distill_step has a row in one workgroup's registers between the statistic and the gradient: read
-// once, written once; bound by HBM (V = 151,936, N = 4,096, bf16: 570 us for 2.5 GB, 4.4 TB/s, a copy's 527; N = 96, V =
+// once, written once; bound by HBM (V = 151,936, N = 4,096, bf16: 553 us for 2.5 GB, 4.5 TB/s, a copy's 527; N = 96, V =
 // 32,768: 10.3 us, a load, a store and the alternatives' chain of about 3 us between). Few rows over a long
 // vocabulary, a loss or a gradient alone: k_distill_stat over parts of the rows (N = 500, V = 50,021, float32: 18.6
 // us, 5.4 TB/s), k_distill_join, k_distill_grad.
@@ -451,11 +451,20 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
   grad_alternatives<DT>(out, g, c, id, x, less);
 }
 
-// A row whole: NV vectors of eight tokens a thread in registers; what is past them is read again for the
-// gradient.
+// A row whole: NV vectors of eight tokens a thread in registers, KEEP more in LDS (one workgroup a CU, or two; bf16,
+// V = 151,936, N = 4,096 572 us without, 553 with; float32, N = 1,024 297 and 283); what is past them is read again for
+// the gradient.
 template <int DT, int T, int NV, bool TAIL>
 __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
-  constexpr int NWAVES = T / WAVE;
+  constexpr int NWAVES = T / WAVE, WORDS = RowVec<DT>::WORDS;
+  constexpr int KEEP = NV <= 4 ? 0 : (T == 512 ? 72 : 136) * 1024 / (T * WORDS * 4);
+  __shared__ uint32_t s_keep[KEEP > 0 ? KEEP : 1][KEEP > 0 ? WORDS / 4 : 1][KEEP > 0 ? 4 * T : 4];
+  auto keep = [&](int k, RowVec<DT>& q) -> void {
+    if constexpr (KEEP > 0)
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i)
+        *(ru32x4*)&s_keep[k][i][4 * threadIdx.x] = ru32x4{q.w[4 * i], q.w[4 * i + 1], q.w[4 * i + 2], q.w[4 * i + 3]};
+  };
   __shared__ RowStat s_stat[NWAVES];
   __shared__ GradList s_list;
   __shared__ GradRow s_grad;
@@ -509,6 +518,9 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
     q0.load_to(row, w0, lane, a.V);
     q1.load_to(row, w1, lane, a.V);
     add(q0, q1, w0, w1, true, true);
+    const int k = v0 / (8 * T) - NV;
+    if (k < KEEP) keep(k, q0);
+    if (k + 1 < KEEP) keep(k + 1, q1);
   }
   stat_wave(st, c);
   if (lane == 0) s_stat[wave] = st;
@@ -542,9 +554,19 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
     const int w0 = 8 * WAVE * (u * NWAVES + wave);
     if (w0 < a.V) grad_of<DT>(x[u], g, c).store_to(out, w0, lane, a.V, a.stream);
   }
-  for (int w0 = 8 * (NV * T + WAVE * wave); w0 < a.V; w0 += 8 * T) {
+  int k = 0;
+  for (int w0 = 8 * (NV * T + WAVE * wave); w0 < a.V; w0 += 8 * T, ++k) {
     RowVec<DT> q;
-    q.load_to(row, w0, lane, a.V);
+    if (k < KEEP) {
+#pragma unroll
+      for (int i = 0; i < (KEEP > 0 ? WORDS / 4 : 0); ++i) {
+        const ru32x4 v = *(const ru32x4*)&s_keep[k][i][4 * threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q.w[4 * i + j] = v[j];
+      }
+    } else {
+      q.load_to(row, w0, lane, a.V);
+    }
     grad_of<DT>(q, g, c).store_to(out, w0, lane, a.V, a.stream);
   }
   int id[2];
@@ -615,12 +637,18 @@ void launch_whole(const DistillArgs& a, hipStream_t st) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)b.N), dim3(threads), 0, st, b);
     };
     // The whole row in registers, or, where there are rows for it, half of it with two workgroups a CU, one
-    // of which reads while the other writes (V = 151,936, 2.5 GB read and written, N = 4,096: 587 -> 570 us; N =
+    // of which reads while the other writes (V = 151,936, 2.5 GB read and written, N = 4,096: 587 -> 570 us, with KEEP 553; N =
     // 128 35 -> 43; V = 248,320, N = 1,024, where only a third would be held: 254 -> 286).
-    if (a.V <= 8 * 256 * 4) go(k_distill_step<DT, 256, 4, TAIL>, 256);
-    else if (a.V <= 8 * 1024 * 4) go(k_distill_step<DT, 1024, 4, TAIL>, 1024);
-    else if (DT == STRIM_DTYPE_BF16 && a.N > 256 && a.V <= 8 * 1024 * 19) go(k_distill_step<DT, 512, 19, TAIL>, 512);
-    else go(k_distill_step<DT, 1024, DT == STRIM_DTYPE_BF16 ? 19 : 9, TAIL>, 1024);
+    if (a.V <= 8 * 256 * 4) {
+      go(k_distill_step<DT, 256, 4, TAIL>, 256);
+    } else if (a.V <= 8 * 1024 * 4) {
+      go(k_distill_step<DT, 1024, 4, TAIL>, 1024);
+    } else if constexpr (DT == STRIM_DTYPE_BF16) {
+      if (a.N > 256 && a.V <= 8 * 1024 * 19) go(k_distill_step<DT, 512, 19, TAIL>, 512);
+      else go(k_distill_step<DT, 1024, 19, TAIL>, 1024);
+    } else {
+      go(k_distill_step<DT, 1024, 9, TAIL>, 1024);
+    }
   }
 }
 

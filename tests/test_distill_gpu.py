@@ -109,7 +109,7 @@ def check(x, ids, lp, w, T=1.0, tail=False, label=""):
 
 SIZES = [(1, 1, 1), (1, 5, 3), (2, 64, 64), (3, 257, 7), (5, 4_095, 33), (4, 4_097, 128), (17, 9_001, 1),
          (96, 32_768, 16), (300, 1_500, 20), (700, 5_003, 64), (1, 151_936, 64), (3, 248_320, 50),
-         (300, 155_650, 64), (260, 160_001, 20)]
+         (300, 155_650, 64), (260, 160_001, 20), (258, 90_001, 20), (258, 150_001, 64), (130, 230_001, 33)]
 
 
 @pytest.mark.parametrize("tail", [False, True])
