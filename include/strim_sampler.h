@@ -305,7 +305,9 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
  *   d_logits[v] = 1 / temperature (sum_s g_s ([v = tokens[s]] - p[v])
  *                                  - g_entropy p[v] (log p[v] + entropy) + g_lse p[v])
  * for allowed v, else 0, in the logits' type; 0 throughout an empty row, NaN on the allowed ids of one
- * that is not finite. A token given twice has both gradients. d_logits may be the logits themselves.
+ * that is not finite. A token given twice has both gradients. d_logits may be the logits themselves. p is
+ * taken from lse as it is held, in float32: relative to itself it is off by lse's rounding (2^-24 |lse|, far
+ * below 1 unless the temperature is far below the logits' range).
  * R at most STRIM_SCORE_MAX_ROWS, V at most STRIM_SCORE_MAX_VOCAB, S and top at most
  * STRIM_SCORE_MAX_LIST, temperature finite and > 0. R = 0: nothing is launched. */
 #define STRIM_SCORE_MAX_ROWS (1 << 22)

@@ -270,3 +270,19 @@ def test_refusals():
             call()
     with pytest.raises(TypeError):
         ops.norm(x.half(), w)
+
+
+def test_past_32_bits():
+    """Rows that begin past 2^31 elements: the same bits as of their copies."""
+    print("[norm] rows past 2^31 elements", flush=True)
+    R, K, stride = 5, 1_030, 600_000_001
+    buf = torch.empty((R - 1) * stride + K, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((R, K), (stride, 1))
+    x.copy_(rows(R, K, torch.bfloat16, 1))
+    dy, w = rows(R, K, torch.bfloat16, 2), weights(K, torch.bfloat16, 3)
+    y, rstd, mean = ops.norm(x, w, w, center=True)
+    got = [y, rstd, mean, *ops.norm_grad(x, w, w, dy, rstd, mean)]
+    c = x.contiguous()
+    y, rstd, mean = ops.norm(c, w, w, center=True)
+    for a, b in zip(got, [y, rstd, mean, *ops.norm_grad(c, w, w, dy, rstd, mean)]):
+        assert torch.equal(a, b)
