@@ -198,7 +198,7 @@ __device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, float re
   g.k = (float)k;
   g.in = (float)in;
   g.b = (float)(k - (double)ref * c);
-  g.near = !stat_far(ref);
+  g.near = !stat_far(ref * c);
   g.sign = all < 0.0 ? 0x80008000u : 0u;
   return g;
 }

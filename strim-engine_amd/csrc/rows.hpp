@@ -154,19 +154,24 @@ __device__ __forceinline__ float wave_sum_f(float v) {
 
 // Over some of a row's tokens: m the largest x, s = sum 2^y, u = sum y 2^y, with y = x c - b and c = log2(e) /
 // T throughout. While tokens are added b is m c as it is rounded, so that a token costs one fused multiply-add;
-// the rounding is the same for all of them, and stat_exact takes it out again (then y = (x - m) c). Without a
-// token above -inf m is -inf, s = u = 0; a NaN or +inf makes s NaN.
+// the rounding is the same for all of them, and stat_exact takes it out again (then y = (x - m) c). That holds
+// while the rounding is small: it is half of m c's spacing, and from |m c| = 2^31 on it alone may pass 2^y's
+// range. Past 2^20 (where it is 2^-5) y = (x - m) c from the start. Without a token above -inf m is -inf, s = u =
+// 0; a NaN or +inf makes s NaN.
 struct RowStat {
   float m, s, u;
 };
 __device__ __forceinline__ float stat_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-// (past this m c or its difference to x c may be infinite: there y = (x - m) c from the start)
-__device__ __forceinline__ bool stat_far(float ref) { return !(fabsf(ref) <= 1e30f); }
+// (of m c: an infinite product or a NaN is far)
+__device__ __forceinline__ bool stat_far(float mc) { return !(fabsf(mc) <= 0x1p20f); }
 // a's sums for the maximum `top` >= a.m. (y is bounded: the type's lowest value lies 3.4e38 below zero, and u
 // times a vanishing factor would be an infinity times 0.)
 __device__ __forceinline__ void stat_rebase(RowStat& a, float top, float c) {
-  const float ref = stat_ref(top);
-  const float d = stat_far(ref) ? (a.m - ref) * c : a.m * c - ref * c, f = hw_exp2(d);
+  const float ref = stat_ref(top), from = a.m * c, to = ref * c;
+  float d;  // the old b less the new one, each as rounded or (far) exact
+  if (stat_far(to)) d = stat_far(from) ? (a.m - ref) * c : fma_f(-ref, c, from);
+  else d = stat_far(from) ? fma_f(a.m, c, -to) : from - to;
+  const float f = hw_exp2(d);
   a.u = a.s == 0.0f ? 0.0f : fma_f(fmaxf(d, -1e30f), a.s, a.u) * f;
   a.s = a.s == 0.0f ? 0.0f : a.s * f;
   a.m = top;
@@ -182,16 +187,15 @@ __device__ __forceinline__ void stat_merge(RowStat& a, RowStat b, float c) {
 template <int E, bool U>
 __device__ __forceinline__ void stat_add(RowStat& a, const float (&x)[E], float mx, float c) {
   if (mx > a.m) stat_rebase(a, mx, c);
-  const float ref = stat_ref(a.m);
+  const float ref = stat_ref(a.m), mc = ref * c;
   auto one = [&](float y) {
     const float e = hw_exp2(y);  // (a NaN goes through to s)
     a.s += e;
     if (U) a.u = fma_f(fmaxf(y, -1e30f), e, a.u);
   };
-  if (!stat_far(ref)) {
-    const float b = -(ref * c);
+  if (!stat_far(mc)) {
 #pragma unroll
-    for (int j = 0; j < E; ++j) one(fma_f(x[j], c, b));
+    for (int j = 0; j < E; ++j) one(fma_f(x[j], c, -mc));
   } else {
 #pragma unroll
     for (int j = 0; j < E; ++j) one((x[j] - ref) * c);
@@ -205,9 +209,9 @@ __device__ __forceinline__ void stat_wave(RowStat& a, float c) {
 }
 // After the last merge.
 __device__ __forceinline__ void stat_exact(RowStat& a, float c) {
-  const float ref = stat_ref(a.m);
-  if (stat_far(ref)) return;
-  const float off = fma_f(ref, c, -(ref * c));  // m c past its rounding
+  const float ref = stat_ref(a.m), mc = ref * c;
+  if (stat_far(mc)) return;
+  const float off = fma_f(ref, c, -mc);  // m c past its rounding
   const float f = hw_exp2(-off);
   a.u = (a.u - off * a.s) * f;
   a.s *= f;
