@@ -168,9 +168,11 @@ __device__ __forceinline__ bool stat_far(float mc) { return !(fabsf(mc) <= 0x1p2
 // times a vanishing factor would be an infinity times 0.)
 __device__ __forceinline__ void stat_rebase(RowStat& a, float top, float c) {
   const float ref = stat_ref(top), from = a.m * c, to = ref * c;
-  float d;  // the old b less the new one, each as rounded or (far) exact
-  if (stat_far(to)) d = stat_far(from) ? (a.m - ref) * c : fma_f(-ref, c, from);
-  else d = stat_far(from) ? fma_f(a.m, c, -to) : from - to;
+  float d = from - to;  // the old b less the new one, each as rounded or (far) exact
+  if (stat_far(fmaxf(fabsf(from), fabsf(to)))) {
+    if (!stat_far(to)) d = fma_f(a.m, c, -to);
+    else d = stat_far(from) ? (a.m - ref) * c : fma_f(-ref, c, from);
+  }
   const float f = hw_exp2(d);
   a.u = a.s == 0.0f ? 0.0f : fma_f(fmaxf(d, -1e30f), a.s, a.u) * f;
   a.s = a.s == 0.0f ? 0.0f : a.s * f;
