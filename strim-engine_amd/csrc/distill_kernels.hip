@@ -168,8 +168,9 @@ __device__ __forceinline__ RowNumbers numbers_of(const Alternatives& o, const Te
 }
 
 // What the gradient takes of a row: sign 2^y with y = (x - ref) c + k at every token, but at the alternatives
-// in 2^y' - p, y' = (x - ref) c + kq. Where (x - ref) c + k may be taken as x c + (k - ref c) without an
-// infinity (`near`), bf16 results are: the rounding of k - ref c, 2^-20 of a result, is far below theirs.
+// in 2^y' - p, y' = (x - ref) c + kq. bf16 results are taken as 2^(x c + b), b = k - ref c, where |b| is below
+// 2^11 (`near`): b's rounding is then at most 2^-14 of an exponent, 2^-14.5 of a result, theirs 2^-9. It grows
+// with b, and so with the largest logit over T.
 struct GradRow {
   float ref, k, kq, in, b;
   uint32_t sign;  // 0 or 0x80008000
@@ -198,7 +199,7 @@ __device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, float re
   g.k = (float)k;
   g.in = (float)in;
   g.b = (float)(k - (double)ref * c);
-  g.near = !stat_far(ref * c);
+  g.near = fabsf(g.b) < 0x1p11f;  // (not where it is a NaN)
   g.sign = all < 0.0 ? 0x80008000u : 0u;
   return g;
 }
