@@ -131,10 +131,11 @@ __device__ __forceinline__ void merge_repeats(const Alternatives& o, int M, bool
 // tell from none is none.
 __device__ __forceinline__ double bucket_of(double r, bool empty) { return empty && r < 0x1p-20 ? 0.0 : r; }
 
-// A row's numbers from the statistic: the loss; `ls` = log sum exp((x - top) / T) and log q_rest. x: the
-// entries' logits. By one wave, every lane the same.
+// A row's numbers from the statistic: the loss; `ls` = log sum exp((x - top) / T) and log q_rest; for the tokens'
+// gradients the same against their own largest logit `ref` (with a tail the rest's): `ls_ref` of all, `ls_rest` of
+// the rest. x: the entries' logits. By one wave, every lane the same.
 struct RowNumbers {
-  double loss, top, ls, log_rest;
+  double loss, top, ls, log_rest, ref, ls_ref, ls_rest;
 };
 __device__ __forceinline__ RowNumbers numbers_of(const Alternatives& o, const Teacher& t, const bool (&first)[2],
                                                  const float (&x)[2], RowStat st, float T, bool tail) {
@@ -157,6 +158,9 @@ __device__ __forceinline__ RowNumbers numbers_of(const Alternatives& o, const Te
   n.ls = rl_d(l, 0);
   // (a rest whose share vanishes in 64 bits keeps its logarithm)
   n.log_rest = !tail ? 0.0 : st.m == -INFINITY ? -(double)INFINITY : far + rl_d(l, 1) - n.ls;
+  n.ref = tail ? (double)stat_ref(st.m) : n.top;
+  n.ls_ref = tail && st.m == -INFINITY ? 0.0 : n.ls - far;  // (no rest: no token that takes it)
+  n.ls_rest = rl_d(l, 1);
   double loss = 0.0;
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -168,40 +172,55 @@ __device__ __forceinline__ RowNumbers numbers_of(const Alternatives& o, const Te
 }
 
 // What the gradient takes of a row: sign 2^y with y = (x - ref) c + k at every token, but at the alternatives
-// in 2^y' - p, y' = (x - ref) c + kq. bf16 results are taken as 2^(x c + b), b = k - ref c, where |b| is below
-// 2^11 (`near`): b's rounding is then at most 2^-14 of an exponent, 2^-14.5 of a result, theirs 2^-9. It grows
-// with b, and so with the largest logit over T.
+// in 2^y' - p, y' = (x - top) c + kq. (k and kq are rounded to float32 and have to be small: each goes with the largest
+// logit of its own tokens.) bf16 results are taken as 2^(x c + b), b = k - ref c, where |b| is below 2^11 (`near`): b's
+// rounding is then at most 2^-14 of an exponent, 2^-14.5 of a result, theirs 2^-9. It grows with b, and so with the
+// largest logit over T.
 struct GradRow {
-  float ref, k, kq, in, b;
+  float top, ref, k, kq, in, b;
   uint32_t sign;  // 0 or 0x80008000
-  int32_t near;
-  int32_t dead;   // the row has no gradient
+  int16_t near;
+  int16_t dead;   // the row has no gradient
 };
-// lse = ref / T + ls; w = weight / T
-__device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, float ref, double ls, double log_rest,
-                                            double w, float c) {
+// w = weight / T
+__device__ __forceinline__ GradRow grad_row(bool any, const Teacher& t, const RowNumbers& n, double w, float c) {
   constexpr double L2E = 1.4426950408889634074;
   GradRow g;
   g.dead = !any || w == 0.0;
-  const double in = w * (t.mass + bucket_of(t.r, log_rest == -INFINITY));
-  double all = in, more = 0.0;
-  if (t.r > 0.0 && log_rest > -INFINITY) {  // (nothing lies outside where q_rest is 0)
-    if (log_rest > -600.0) {
-      all = in - w * t.r * exp(-log_rest);
+  const double in = w * (t.mass + bucket_of(t.r, n.log_rest == -INFINITY));
+  double all = in, ls = n.ls_ref;
+  if (t.r > 0.0 && n.log_rest > -INFINITY) {  // (nothing lies outside where q_rest is 0)
+    if (n.log_rest > -600.0) {
+      all = in - w * t.r * exp(-n.log_rest);
     } else {
       all = -w * t.r;
-      more = -log_rest;
+      ls = n.ls_rest;
     }
   }
-  const double k = log2(fabs(all)) + (more - ls) * L2E;
-  g.ref = ref;
-  g.kq = (float)(-ls * L2E);
+  const double k = log2(fabs(all)) - ls * L2E;
+  g.top = (float)n.top;
+  g.ref = (float)n.ref;
+  g.kq = (float)(-n.ls * L2E);
   g.k = (float)k;
   g.in = (float)in;
-  g.b = (float)(k - (double)ref * c);
+  g.b = (float)(k - n.ref * c);
   g.near = fabsf(g.b) < 0x1p11f;  // (not where it is a NaN)
   g.sign = all < 0.0 ? 0x80008000u : 0u;
   return g;
+}
+// The numbers that the gradient takes from lse and log q_rest as float32 holds them.
+__device__ __forceinline__ RowNumbers numbers_from(double lse, double log_rest, bool tail, float T) {
+  constexpr double MOST = 3.40282346638528859812e38;
+  auto near_to = [&](double z) { return (double)(float)fmax(-MOST, fmin(MOST, z * T)); };
+  RowNumbers n{};
+  n.log_rest = tail ? log_rest : 0.0;
+  const double rest = log_rest > -INFINITY ? lse + log_rest : lse;
+  n.top = near_to(lse);
+  n.ls = lse - n.top / T;
+  n.ref = tail ? near_to(rest) : n.top;
+  n.ls_ref = lse - n.ref / T;
+  n.ls_rest = rest - n.ref / T;
+  return n;
 }
 
 // Eight tokens' gradients, as of no alternatives.
@@ -235,7 +254,7 @@ __device__ __forceinline__ void grad_alternatives(char* out, const GradRow& g, f
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     if (id[i] >= 0) {
-      const float f = g.in * hw_exp2(fma_f(x[i] - g.ref, c, g.kq)) - p[i];
+      const float f = g.in * hw_exp2(fma_f(x[i] - g.top, c, g.kq)) - p[i];
       if constexpr (DT == STRIM_DTYPE_BF16) ((uint16_t*)out)[id[i]] = __builtin_bit_cast(uint16_t, (__bf16)f);
       else ((float*)out)[id[i]] = f;
     }
@@ -363,11 +382,11 @@ __global__ __launch_bounds__(WAVE) void k_distill_join(const DistillArgs a, cons
     for (int i = 0; i < 2; ++i) merged[i] = t.p[i];
     merge_repeats(o, a.M, first, merged);
   }
-  RowNumbers n{0.0, 0.0, 0.0, 0.0};
+  RowNumbers n{};
   if (o.any) n = numbers_of(o, t, first, x, st, a.T, a.tail);
   if constexpr (STEP) {
     GradRecord* rec = q.record + r;
-    const GradRow g = grad_row(o.any, t, (float)n.top, n.ls, n.log_rest, w, c);
+    const GradRow g = grad_row(o.any, t, n, w, c);
     if (lane == 0) rec->row = g;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -414,14 +433,13 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
     __syncthreads();
     if (wave == 0) {
       const Teacher t = teacher_of(o, a.tail);
-      const double w = (double)a.weights[r] / a.T, lse = a.lse[r];
-      const float ref = (float)(lse * a.T);
+      const double w = (double)a.weights[r] / a.T;
       bool first[2] = {o.id[0] >= 0, o.id[1] >= 0};
       float x[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) x[i] = o.any && o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
       list_out(s_list, o, t, a.M, w, x, first, s_list.repeats != 0);
-      g = grad_row(o.any, t, ref, lse - (double)ref / a.T, a.tail ? (double)a.log_rest[r] : 0.0, w, c);
+      g = grad_row(o.any, t, numbers_from(a.lse[r], a.tail ? (double)a.log_rest[r] : 0.0, a.tail, a.T), w, c);
       if (lane == 0) s_grad = g;
     }
     __syncthreads();
@@ -537,9 +555,9 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) xa[i] = o.any && o.id[i] >= 0 ? token_at<DT>(row, o.id[i]) : -INFINITY;
     list_out(s_list, o, t, a.M, w, xa, first, s_list.repeats != 0);
-    RowNumbers n{0.0, 0.0, 0.0, 0.0};
+    RowNumbers n{};
     if (o.any) n = numbers_of(o, t, first, xa, st, a.T, TAIL);
-    const GradRow g = grad_row(o.any, t, (float)n.top, n.ls, n.log_rest, w, c);
+    const GradRow g = grad_row(o.any, t, n, w, c);
     if (lane == 0) {
       s_grad = g;
       const float loss = (float)n.loss;

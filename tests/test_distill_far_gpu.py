@@ -18,9 +18,9 @@ NINF = float("-inf")
 BF16, F32 = torch.bfloat16, torch.float32
 
 
-def exact(x, ids, lp, w, T, tail, rest_bound):
+def exact(x, ids, lp, w, T, tail, rest_bound, held=0.0):
     """(gradient, bound) in 64 bits. rest_bound: the rest's tokens by their distance to the rest's largest logit,
-    else to the row's."""
+    else to the row's. held: what each probability is off by besides."""
     R, V = x.shape
     half, bf16 = torch.finfo(x.dtype).eps / 2, x.dtype == BF16
     x, live = x.double(), ids >= 0
@@ -38,7 +38,7 @@ def exact(x, ids, lp, w, T, tail, rest_bound):
     target = torch.zeros_like(x).scatter_add_(1, at, p * live)
     soft = q * (mass + r)
     e = (V / 256 + 40) * 2.0 ** -24 + 2.0 ** -22 * (8 + (q * -z).sum(1, keepdim=True))
-    rel = 2 * e + 2.0 ** -21 * 8 + (2.0 ** -14 if bf16 else 0.0)
+    rel = 2 * e + 2.0 ** -21 * 8 + (2.0 ** -14 if bf16 else 0.0) + held
     far = (-zr).nan_to_num(posinf=0.0) if tail and rest_bound else -z
     w = w.double()[:, None] / T
     tol = soft * (rel - 2.0 ** -21 * z) + bucket * (rel + 2.0 ** -21 * far + 2.0 ** -22 * mass / r.clamp_min(1e-9))
@@ -73,3 +73,50 @@ def test_step(V, copies, T, dtype, tail):
     # into the logits themselves: the same bits
     y = x.clone()
     assert torch.equal(ops.distill_step(y, ids, lp, w, T, tail, out=y)[1], d)
+
+
+BELOW = [0.0, 30.0, 300.0, 700.0, 1e4, 1e6, 1e8, 1e10, 1e20, 1e30]
+
+
+def apart(V, copies, dtype, seed, lift=1.0):
+    """Rows whose alternatives are far above the rest (lift 1) or far below it (-1)."""
+    g = gen(seed)
+    R = len(BELOW) * copies
+    ids, lp = teacher(R, V, 11, V)
+    x = 2.0 * torch.randn(R, V, device="cuda", generator=g) - lift * torch.tensor(BELOW * copies, device="cuda")[:, None]
+    at = torch.where(ids < 0, ids[:, :1], ids).long()
+    x.scatter_(1, at, 3.0 * torch.randn(R, 1, device="cuda", generator=g).expand(R, 11))
+    return x.to(dtype), ids, lp, torch.randn(R, device="cuda", generator=g)
+
+
+SHAPES = [(2_500, 1), (20_000, 1), (60_001, 1), (60_001, 13), (60_001, 27)]
+
+
+@pytest.mark.parametrize("lift", [1.0, -1.0])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [1.0, 0.3, 2.0])
+@pytest.mark.parametrize("V,copies", SHAPES)
+def test_step_with_the_rest_apart(V, copies, T, dtype, lift):
+    """The teacher's remaining mass goes to a rest that the student all but excludes (a masked vocabulary), and
+    the reverse: the rest's gradients sum to that mass, whatever its distance."""
+    print(f"[far] apart V={V} copies={copies} T={T} {dtype} lift={lift}", flush=True)
+    T = f32(T)
+    x, ids, lp, w = apart(V, copies, dtype, V + copies, lift)
+    ref, tol = exact(x, ids, lp, w, T, True, True)
+    loss, d, st = ops.distill_step(x, ids, lp, w, T, True)
+    assert bool((st == N.OK).all())
+    within(d, ref, tol, "gradient")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V,copies", SHAPES)
+def test_gradient_alone_with_the_rest_apart(V, copies, dtype):
+    """From lse and log_rest as float32 holds them: 2^-23 of either, no more, in each probability."""
+    print(f"[far] apart, the gradient alone V={V} copies={copies} {dtype}", flush=True)
+    x, ids, lp, w = apart(V, copies, dtype, V + copies)
+    near = (torch.tensor(BELOW * copies) <= 1e4).nonzero()[:, 0].cuda()
+    x, ids, lp, w = x[near].contiguous(), ids[near].contiguous(), lp[near].contiguous(), w[near].contiguous()
+    _, lse, rest, _ = ops.distill(x, ids, lp, 1.0, True)
+    held = 2.0 ** -23 * (lse.abs() + rest.abs()).double()[:, None]
+    d = ops.distill_grad(x, ids, lp, lse, rest, w, 1.0, True)
+    within(d, *exact(x, ids, lp, w, 1.0, True, True, held), "gradient")
