@@ -236,4 +236,6 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
         live = ((ids >= 0) & (logprobs != float("-inf"))).any(1) & (ids < V).all(1)
         weights = live.float()
         weights = weights / _sum(weights).clamp_min(1.0)  # (counts are exact in float32 up to 2^24)
+    if not torch.is_grad_enabled():  # (nothing is recorded, though the logits may ask for a gradient)
+        rows = rows.detach()
     return _DistillSum.apply(rows, ids, logprobs, weights, temperature, tail)
