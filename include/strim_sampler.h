@@ -309,10 +309,12 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
  * taken from lse as it is held, in float32: relative to itself it is off by lse's rounding (2^-24 |lse|, far
  * below 1 unless the temperature is far below the logits' range).
  * R at most STRIM_SCORE_MAX_ROWS, V at most STRIM_SCORE_MAX_VOCAB, S and top at most
- * STRIM_SCORE_MAX_LIST, temperature finite and > 0. R = 0: nothing is launched. */
+ * STRIM_SCORE_MAX_LIST, temperature finite and at least STRIM_SCORE_MIN_TEMPERATURE (the least normal number:
+ * below it its reciprocal is infinite). R = 0: nothing is launched. */
 #define STRIM_SCORE_MAX_ROWS (1 << 22)
 #define STRIM_SCORE_MAX_VOCAB (1 << 20)
 #define STRIM_SCORE_MAX_LIST 128
+#define STRIM_SCORE_MIN_TEMPERATURE 1.17549435e-38f /* 2^-126 */
 int64_t strim_token_scores_workspace(int32_t R, int32_t V, int32_t top);
 int strim_token_scores(void* stream, const void* logits, int32_t dtype, int32_t R, int32_t V,
                        int64_t row_stride, float temperature, const uint32_t* mask_words,

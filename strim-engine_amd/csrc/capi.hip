@@ -871,7 +871,7 @@ bool aligned_as(const void* p, int32_t dtype) {
 // rows of logits for the scores and the distillation loss
 bool score_rows_ok(int32_t dtype, int32_t R, int32_t V, int64_t stride, float T) {
   return dtype_ok(dtype) && R >= 0 && R <= STRIM_SCORE_MAX_ROWS && V > 0 &&
-         V <= STRIM_SCORE_MAX_VOCAB && stride >= V && T > 0.0f && T < INFINITY;
+         V <= STRIM_SCORE_MAX_VOCAB && stride >= V && T >= STRIM_SCORE_MIN_TEMPERATURE && T < INFINITY;
 }
 bool list_ok(int32_t n) { return n >= 0 && n <= STRIM_SCORE_MAX_LIST; }
 }  // namespace

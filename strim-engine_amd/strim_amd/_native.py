@@ -72,6 +72,7 @@ EXPORTS = (
 KERNEL_COUNT = 8
 LOSS_MAX_ROWS, LOSS_MAX_STRIDE = 1 << 22, 1 << 20  # strim_head_loss limits
 SCORE_MAX_ROWS, SCORE_MAX_VOCAB, SCORE_MAX_LIST = 1 << 22, 1 << 20, 128  # strim_token_scores limits
+SCORE_MIN_TEMPERATURE = 2.0 ** -126
 NORM_MAX_WIDTH, NORM_MAX_ROWS = 1 << 16, 1 << 28  # strim_norm limits
 NOALLOC_MAX_ROWS, NOALLOC_MAX_VOCAB = 32, 262144  # strim_sample_noalloc limits
 

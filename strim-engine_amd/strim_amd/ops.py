@@ -615,8 +615,8 @@ def _check_logits(logits: torch.Tensor, temperature: float) -> int:
     if logits.dim() != 2 or (not logits.is_contiguous() and
                              (logits.stride(1) != 1 or _row_stride(logits) < logits.shape[1])):
         raise ValueError("logits must be [R, V] with contiguous rows (row stride >= V)")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be finite and positive, got {temperature}")
+    if not N.SCORE_MIN_TEMPERATURE <= temperature < float("inf"):
+        raise ValueError(f"temperature must be finite and at least {N.SCORE_MIN_TEMPERATURE}, got {temperature}")
     R, V = logits.shape
     if R > N.SCORE_MAX_ROWS or not 0 < V <= N.SCORE_MAX_VOCAB:
         raise ValueError(f"logits must be at most [{N.SCORE_MAX_ROWS}, {N.SCORE_MAX_VOCAB}], got [{R}, {V}]")

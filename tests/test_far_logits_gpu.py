@@ -182,3 +182,17 @@ def test_a_filled_tail_through_the_differentiable_forms():
     assert abs(float(out[0][0] - out[1][0])) <= 1e-5 * abs(float(out[0][0]))
     assert bool((out[1][1][:, V:] == 0).all())
     assert float((out[0][1] - out[1][1][:, :V]).abs().max()) <= 4e-5
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [2.0 ** -126, 1e20, 1e38, 3.4e38])
+def test_the_ends_of_the_temperature(T, dtype):
+    print(f"[far] T={T} {dtype}", flush=True)
+    x = (4.0 * torch.randn(5, 9_001, device="cuda", generator=gen(6))).to(dtype)
+    x[1, ::2] = -1e30
+    check(x, T, 20, label=f"T={T}")
+    for bad in (2.0 ** -127, 1e-45, 0.0, -1.0, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_scores(x, temperature=bad)
+        with pytest.raises(ValueError, match="temperature"):
+            ops.distill(x, torch.zeros(5, 1, dtype=torch.int32, device="cuda"), torch.zeros(5, 1, device="cuda"), bad)
