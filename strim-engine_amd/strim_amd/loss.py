@@ -113,7 +113,7 @@ class _TokenScores(torch.autograd.Function):
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """[..., V] as [R, V] with contiguous rows."""
-    rows = logits.reshape(-1, logits.shape[-1])
+    rows = ops.as_rows(logits)
     # (one row broadcast over several has a stride of 0)
     apart = rows.stride(1) == 1 and (rows.shape[0] < 2 or rows.stride(0) >= rows.shape[1])
     return rows if apart else rows.contiguous()
@@ -137,7 +137,7 @@ def token_scores(logits: torch.Tensor, tokens: torch.Tensor | None = None, top: 
     if mask is not None:
         if mask.shape[:-1] != lead:
             raise ValueError(f"mask must be {tuple(lead)} + (words,), got {tuple(mask.shape)}")
-        mask = mask.reshape(-1, mask.shape[-1]).contiguous()
+        mask = ops.as_rows(mask).contiguous()
     out = _TokenScores.apply(_rows(logits), tokens, top, temperature, mask, ignore_index)
     lp, entropy, lse, ids, ilp, status = out
     return ops.TokenScores(None if lp is None else lp.reshape(given), entropy.reshape(lead),
@@ -205,14 +205,14 @@ def _alternatives(logits, ids, logprobs):
     if ids.shape[:-1] != lead or logprobs.shape != ids.shape:
         raise ValueError(f"ids and logprobs must be {tuple(lead)} + (M,), got {tuple(ids.shape)} and "
                          f"{tuple(logprobs.shape)}")
-    V, M = logits.shape[-1], ids.shape[-1]
+    V = logits.shape[-1]
     if ids.dtype == torch.int64:  # (one past 32 bits stays outside the vocabulary)
         ids = torch.where(ids < 0, -1, ids.clamp_max(V)).to(torch.int32)
     if ids.dtype != torch.int32:
         raise TypeError(f"ids must be int32 or int64, got {ids.dtype}")
     if logprobs.requires_grad:
         raise ValueError("the teacher's log-probabilities take no gradient: detach them")
-    return ids.reshape(-1, M).contiguous(), logprobs.reshape(-1, M).float().contiguous()
+    return ops.as_rows(ids).contiguous(), ops.as_rows(logprobs).float().contiguous()
 
 
 def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,

@@ -32,7 +32,7 @@ class _Norm(torch.autograd.Function):
 
 
 def _norm(x, weight, bias, eps, center):
-    rows = x.reshape(-1, x.shape[-1])
+    rows = ops.as_rows(x)
     if rows.stride(1) != 1 or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
         rows = rows.contiguous()  # (one row broadcast over several has a stride of 0)
     return _Norm.apply(rows, weight, bias, eps, center).reshape(x.shape)

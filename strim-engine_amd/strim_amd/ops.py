@@ -92,6 +92,11 @@ def _check_cuda(*ts):
             raise ValueError("tensor arguments must be contiguous")
 
 
+def as_rows(t: torch.Tensor) -> torch.Tensor:
+    """[..., n] as [R, n], also where R or n is 0."""
+    return t.unsqueeze(0) if t.dim() == 1 else t.flatten(0, -2)
+
+
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between rows (a single row may carry any stride, e.g. 0 from a
     broadcast view: its own length is passed)."""

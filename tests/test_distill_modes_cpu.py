@@ -24,3 +24,17 @@ def test_no_gradient_is_made_where_none_is_recorded(plain, mode, reduction):  # 
     assert plain == ["step"] and torch.equal(again.detach(), value.clone())
     again.backward()
     assert x.grad is not None
+
+
+def test_nothing_to_lay_out_is_refused_by_the_call_itself():
+    """Empty vocabularies, lists and widths get the calls' own errors, with and without rows."""
+    from strim_amd import norm
+
+    for lead in ((3,), (2, 3), (0,), ()):
+        none = torch.empty(*lead, 0)
+        for call in (lambda: L.token_scores(none), lambda: L.distill_loss(none, none.int(), none),
+                     lambda: L.distill_loss(torch.zeros(*lead, 8), none.int(), none),
+                     lambda: L.distill_loss(torch.zeros(*lead, 8), none.int(), none, reduction="none"),
+                     lambda: norm.rms_norm(none)):
+            with pytest.raises(ValueError):
+                call()
