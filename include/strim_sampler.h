@@ -306,8 +306,10 @@ int strim_head_loss_grad(void* stream, const void* hidden, int64_t hidden_stride
  *                                  - g_entropy p[v] (log p[v] + entropy) + g_lse p[v])
  * for allowed v, else 0, in the logits' type; 0 throughout an empty row, NaN on the allowed ids of one
  * that is not finite. A token given twice has both gradients. d_logits may be the logits themselves. p is
- * taken from lse as it is held, in float32: relative to itself it is off by lse's rounding (2^-24 |lse|, far
- * below 1 unless the temperature is far below the logits' range).
+ * taken from lse as it is held, in float32: relative to itself it is off by lse's rounding, 2^-24 |lse| or so, which
+ * is small while the largest logit over the temperature is (1e-3 of p at 1e4, all of p at 1e7; where that
+ * quotient passes float32 lse is infinite and p 0). Logits far below the largest one, as a mask by a large
+ * negative number has them, cost no accuracy.
  * R at most STRIM_SCORE_MAX_ROWS, V at most STRIM_SCORE_MAX_VOCAB, S and top at most
  * STRIM_SCORE_MAX_LIST, temperature finite and at least STRIM_SCORE_MIN_TEMPERATURE (the least normal number:
  * below it its reciprocal is infinite). R = 0: nothing is launched. */
@@ -345,11 +347,15 @@ int strim_token_scores_grad(void* stream, const void* logits, int32_t dtype, int
  * an id of V or more (STRIM_EINVAL), counts for nothing: loss and gradient 0, whatever it holds. An id
  * given twice counts with both probabilities. A row whose grad_loss is 0 has gradient 0.
  *   out_lse, out_log_rest  [N] or NULL: log sum exp(x / temperature) and log q_rest (0 without tail),
- *               what strim_distill_grad takes; 0 in a row that counts for nothing.
+ *               what strim_distill_grad takes; 0 in a row that counts for nothing. It has them as float32 holds
+ *               them: its q is off by 2^-24 |lse| of itself or so, the rest's term by 2^-24 |log_rest| more
+ *               (strim_distill_step holds both in 64 bits and is not).
  *   out_status  [N] or NULL: STRIM_OK, STRIM_EINVAL, or STRIM_ENONFINITE (a NaN or infinite loss).
  *   workspace   as above, of strim_distill_workspace's bytes (step: for strim_distill_step).
  * strim_distill_step is strim_distill and strim_distill_grad in one, for rows whose weights are known
- * beforehand (a mean's 1 / count): the logits are read once. d_logits may be the logits themselves.
+ * beforehand (a mean's 1 / count): what a workgroup holds of a row is read once (all of 32,768 tokens, three
+ * quarters of 151,936 in bf16), the rest twice, and all of it where fewer than 128 longer rows are split over
+ * workgroups. d_logits may be the logits themselves.
  * strim_distill_scale: data *= *factor (device), which writes nothing where the factor is 1: a step's
  * gradient times the gradient of what the rows' weighted sum went into. */
 int64_t strim_distill_workspace(int32_t N, int32_t V, int32_t M, int32_t step);
@@ -374,7 +380,8 @@ int strim_distill_scale(void* stream, void* data, int32_t dtype, int64_t n, cons
  *   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(sum_k (x - mean)^2 / K + eps)
  * with mean = sum_k x / K (center 1, out_mean [N]) or 0 (center 0, out_mean NULL: the root mean square
  * of the projection's final norm, Weights.swift:270-273), in float32, rounded once. weight and bias
- * [K] of wdtype, or NULL; out_rstd [N] or NULL. Rows whose squares sum past float32 have rstd 0.
+ * [K] of wdtype, or NULL; out_rstd [N] or NULL. Rows whose squares sum past float32 have rstd 0 (with eps 0,
+ * rows whose squares vanish in it have rstd infinite).
  * strim_norm_grad, with xh = (x - mean) rstd and h = weight grad_y (of x's type):
  *   d_x = rstd (h - xh mean_k(h xh) [- mean_k(h), where mean is given]),
  *   d_weight = sum_n grad_y xh,  d_bias = sum_n grad_y   (of wdtype; each of the three may be NULL)

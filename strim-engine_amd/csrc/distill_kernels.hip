@@ -9,11 +9,13 @@
 // alternative, so that q_rest is no difference of near numbers; the alternatives' own logits are looked
 // up. Those M numbers are in 64 bits: a small loss is the difference of much larger terms.
 //
-// k_distill_step has a row in one workgroup's registers between the statistic and the gradient: read
-// once, written once; bound by HBM (V = 151,936, N = 4,096, bf16: 553 us for 2.5 GB, 4.5 TB/s, a copy's 527; N = 96, V =
-// 32,768: 10.3 us, a load, a store and the alternatives' chain of about 3 us between). Few rows over a long
-// vocabulary, a loss or a gradient alone: k_distill_stat over parts of the rows (N = 500, V = 50,021, float32: 18.6
-// us, 5.4 TB/s), k_distill_join, k_distill_grad.
+// k_distill_step has a row in one workgroup between the statistic and the gradient: what registers and LDS hold
+// of it is read once (all of 32,768 tokens; of 151,936 three quarters in bf16), the rest twice, all written once.
+// Bound by HBM (V = 151,936, N = 4,096, bf16: 547 us for the 2.5 GB of one read and one write, 4.6 TB/s, a copy's
+// 527; N = 96, V = 32,768: 10.3 us, a load, a store and the alternatives' chain of about 3 us between). Few rows over
+// a long vocabulary, a loss or a gradient alone: k_distill_stat over parts of the rows (N = 500, V = 50,021, float32:
+// 18.6 us, 5.4 TB/s), k_distill_join, k_distill_grad; a step so reads the logits twice (N = 64, V = 151,936, bf16: 8.9
+// + 8.1 + 7.4 us; the gradient alone 14.6).
 #include <type_traits>
 
 #include "kernels.hpp"
@@ -471,7 +473,7 @@ __global__ __launch_bounds__(DI_T) void k_distill_grad(const DistillArgs a, cons
 }
 
 // A row whole: NV vectors of eight tokens a thread in registers, KEEP more in LDS (one workgroup a CU, or two; bf16,
-// V = 151,936, N = 4,096 572 us without, 553 with; float32, N = 1,024 297 and 283); what is past them is read again for
+// V = 151,936, N = 4,096 571 us without, 547 with; float32, N = 1,024 297 and 283); what is past them is read again for
 // the gradient.
 template <int DT, int T, int NV, bool TAIL>
 __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
@@ -600,7 +602,8 @@ __global__ __launch_bounds__(T) void k_distill_step(const DistillArgs a) {
   grad_alternatives<DT>(out, g, c, id, xa, less);
 }
 
-// (a factor of 1, what the last step of a backward pass usually has, costs no pass over the data)
+// (a factor of 1, what the last step of a backward pass usually has, costs no pass over the data; another a pass of
+// one element a lane: N = 4,096, V = 151,936 in bf16 854 us, 2.9 TB/s)
 template <int DT>
 __global__ __launch_bounds__(DI_T) void k_distill_scale(char* data, int64_t n, const float* factor) {
   const float f = *factor;
@@ -627,9 +630,15 @@ DistillParts distill_parts(int N, int V, bool bf16) {
   q.parts = (int32_t)ceil_of(tiles, q.tiles);
   return q;
 }
-// Whether a step keeps each row in a workgroup: always where four vectors a thread hold it (N = 1, V = 32,768:
-// 7.9 us, in parts 14.2), else from half a round of rows on (V = 151,936: N = 128 35.1 us, in parts 37.1; N =
-// 64 about 35, in parts 25.4).
+// Whether a step keeps each row in a workgroup: always where four vectors a thread hold it, else from half a round
+// of rows on. Replayed steps of N = 1, 64, 96, 127, 200, whole and in parts, us:
+//   bf16     V = 32,768   8.9, 10.4, 10.4, 11.2, 12.3   13.5, 14.8, 15.8, 16.1, 18.5
+//            V = 40,000   18, 19, 20, 20, 21            14, 16, 16, 17, 20
+//            V = 100,003  19, 28, 29, 30, 33            14, 20, 22, 27, 36
+//            V = 151,936  21, 27, 28, 29, 33            13, 21, 26, 33, 43
+//   float32  V = 40,000   13, 15, 16, 18, 21            13, 17, 18, 20, 24
+//            V = 151,936  23, 32, 34, 38, 49            13, 29, 38, 48, 66
+// (float32 rows of 40,000 and 65,536 tokens would be as fast or faster whole from one row on.)
 bool whole_rows(int N, int V) { return N >= 128 || V <= 8 * 1024 * 4; }
 
 template <class F>
@@ -656,7 +665,7 @@ void launch_whole(const DistillArgs& a, hipStream_t st) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)b.N), dim3(threads), 0, st, b);
     };
     // The whole row in registers, or, where there are rows for it, half of it with two workgroups a CU, one
-    // of which reads while the other writes (V = 151,936, 2.5 GB read and written, N = 4,096: 587 -> 570 us, with KEEP 553; N =
+    // of which reads while the other writes (V = 151,936, 2.5 GB read and written, N = 4,096: 587 -> 571 us, with KEEP 547; N =
     // 128 35 -> 43; V = 248,320, N = 1,024, where only a third would be held: 254 -> 286).
     if (a.V <= 8 * 256 * 4) {
       go(k_distill_step<DT, 256, 4, TAIL>, 256);

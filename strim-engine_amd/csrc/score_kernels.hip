@@ -7,8 +7,8 @@
 // k_scores reads the logits once: per lane the running maximum m, s = sum 2^y and u = sum y 2^y with y =
 // (x - m) log2(e) / T, from which lse = m / T + log s and H = log s - log(2) u / s, and the row's
 // alternatives (top.hpp). A row is one workgroup's where there are many, else in parts that
-// k_scores_join merges. Bound by the reading where rows are many (V = 151,936, bf16, R = 2,048: 113 us, 5.5 TB/s, with
-// 64 alternatives 123; float32, R = 1,003, V = 100,003: 76 us, 5.3), by two launches' round trips where they are few
+// k_scores_join merges. Bound by the reading where rows are many (V = 151,936, bf16, R = 2,048: 105 us, 5.9 TB/s, with
+// 64 alternatives 124; float32, R = 1,003, V = 100,003: 76 us, 5.3), by two launches' round trips where they are few
 // (one row with 20 alternatives 11.3 us, 64 rows with five 16.9). The join is a launch of its own: a last part that
 // waited for the others' results would need a device-scope release, which costs more.
 #include <type_traits>

@@ -176,8 +176,7 @@ def _sum(t: torch.Tensor) -> torch.Tensor:
 
 
 class _DistillSum(torch.autograd.Function):
-    """The rows' losses times their weights, summed; the gradient comes with the loss, from one pass
-    over the logits."""
+    """The rows' losses times their weights, summed; the gradient comes with the loss, from one step."""
 
     @staticmethod
     def forward(ctx, logits, ids, logprobs, weights, temperature, tail):
@@ -220,9 +219,10 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
     """Divergence of softmax(logits / temperature) from a teacher's alternatives (ids and logprobs
     [..., M], as token_scores gives them), with gradients for the logits [..., V] (first derivatives):
     "mean" over the positions that have alternatives (0 if none has), "sum", or "none" (per position).
-    The mean and the sum make their gradient with the loss, in one pass over the logits, and hold it
-    until the backward pass; the gradient is then multiplied by what comes back (and rounded again
-    unless that is a power of two)."""
+    The mean and the sum make their gradient with the loss (ops.distill_step) and hold it until the
+    backward pass; the gradient is then multiplied by what comes back, in a pass of its own unless that
+    is 1 (and rounded again unless that is a power of two). "none" takes it from lse and log_rest as
+    float32 holds them (ops.distill_grad)."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean, sum or none, got {reduction}")
     lead, V = logits.shape[:-1], logits.shape[-1]

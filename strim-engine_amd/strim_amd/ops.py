@@ -790,7 +790,9 @@ def distill_grad(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
                  log_rest: torch.Tensor, grad_loss: torch.Tensor, temperature: float = 1.0,
                  tail: bool = False, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """The logits' gradient [N, V] (of their type) from lse and log_rest as distill gave them and the
-    float32 [N] gradient of its loss. out: where it goes, the logits themselves included."""
+    float32 [N] gradient of its loss. out: where it goes, the logits themselves included. (Probabilities
+    are off by the rounding of lse and log_rest, 2^-24 of either: small unless the largest logit over the
+    temperature is large, or the rest is all but excluded. distill_step's are not.)"""
     code, R, V, M = _distill_args(logits, ids, logprobs, temperature)
     dev = logits.device
     for t in (lse, log_rest, grad_loss):
@@ -812,7 +814,8 @@ def distill_step(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
                  weights: torch.Tensor, temperature: float = 1.0, tail: bool = False,
                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None):
     """distill and distill_grad in one call, for rows whose weights float32 [N] are known beforehand
-    (a mean's 1 / count): (loss [N], d_logits [N, V], status [N]). The logits are read once."""
+    (a mean's 1 / count): (loss [N], d_logits [N, V], status [N]). What a workgroup holds of a row is
+    read once; few rows over a long vocabulary are read twice."""
     code, R, V, M = _distill_args(logits, ids, logprobs, temperature)
     dev = logits.device
     if weights.dtype != torch.float32 or weights.shape != (R,):
